@@ -1,0 +1,508 @@
+"""The 8-bit key/value cache (written, read back, attended) and the log
+probabilities of tokens, as cases that can be timed and compared.
+
+A speech program that generates long text holds the keys and values of its
+prompts, reference voices and finished chunks instead of computing them again:
+in a pool of blocks of 16, 32 or 64 tokens, 8 bits a value, with one power-of-two
+scale per block, key/value head and half (keys or values). New tokens (one
+each for a batch, the frames of a chunk, whole prompts) are quantised as they
+are written, and attend what their sequence holds. Logits then rate the tokens
+that were drawn: their log probabilities, the entropy, the alternatives.
+
+The pool's layout, which every form here reads and writes:
+data uint8 [blocks][kv heads][keys, values][block_tokens * head_dim], e4m3
+codes in groups of 16 tokens; a group of keys is [dim / 16][token][dim % 16],
+a group of values [dim / 64][token / 4][dim % 16][dim / 16 % 4][token % 4].
+scales float32 [blocks][kv heads][keys, values]. A sequence's blocks are the
+entries of its row of `tables`; `lengths` counts its tokens, the rows
+begins[i] .. begins[i + 1] of this call's tensors being its last ones.
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+MOST_BYTES = 600e6  # what a drawn case reads and writes at most
+MOST_PAIRS = 20e6  # and its pairs of a query and a key
+MOST_SCORES = 8e8  # and the scores of its plain form
+
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+SIZE = {"f16": 2, "bf16": 2, "f32": 4}
+
+
+def listed():
+    return [
+        # 64 streams each add the token they just drew: launches and latency count.
+        dict(name="write a token each", kind="write", count=64, new=1, length=2000, ragged=True,
+             kv_heads=8, dim=128, block=32, type="f16"),
+        # The prompts of 16 new streams, ragged, up to 2048 tokens.
+        dict(name="write prompts", kind="write", count=16, new=2048, length=2048, ragged=True,
+             kv_heads=8, dim=128, block=32, type="f16"),
+        # One reference voice of 15 s (375 frames) taken out of the cache.
+        dict(name="read a voice", kind="read", count=1, new=375, length=425, ragged=False,
+             kv_heads=8, dim=128, block=16, type="f16"),
+        # 32 long streams moved out at once.
+        dict(name="read streams", kind="read", count=32, new=4096, length=4096, ragged=True,
+             kv_heads=8, dim=128, block=64, type="bf16"),
+        # One stream's next token over a short prompt: the smallest call.
+        dict(name="attend short", kind="attend", count=1, new=1, length=430, ragged=False,
+             kv_heads=8, group=2, dim=128, block=32, type="f16", causal=True),
+        # The next tokens of 48 streams of up to 8192 tokens: the serving step.
+        dict(name="attend streams", kind="attend", count=48, new=1, length=8192, ragged=True,
+             kv_heads=8, group=2, dim=128, block=32, type="f16", causal=True),
+        # One stream's next token over an hour of context (25 frames a second).
+        dict(name="attend long", kind="attend", count=1, new=1, length=90001, ragged=False,
+             kv_heads=8, group=2, dim=128, block=64, type="bf16", causal=True),
+        # 20 streams' 6 drafted tokens each, 8 query heads a key head of 64.
+        dict(name="attend drafts", kind="attend", count=20, new=6, length=3001, ragged=True,
+             kv_heads=4, group=8, dim=64, block=16, type="bf16", causal=True),
+        # Four chunks of up to 375 frames being unmasked over a held voice and text.
+        dict(name="attend chunks", kind="attend", count=4, new=375, length=1800, ragged=True,
+             kv_heads=8, group=2, dim=128, block=32, type="f16", causal=False),
+        # Two long prompts taken in whole.
+        dict(name="attend prompts", kind="attend", count=2, new=5000, length=5000, ragged=True,
+             kv_heads=8, group=2, dim=128, block=32, type="bf16", causal=True),
+        # The codes of a 10 s utterance (250 frames of 8 codebooks) under guidance.
+        dict(name="logprobs codes", kind="logprobs", rows=2000, vocab=1025, top=5, guided=True,
+             type="f32"),
+        # A text of 1000 tokens over the text vocabulary.
+        dict(name="logprobs text", kind="logprobs", rows=1000, vocab=151936, top=4, guided=False,
+             type="bf16"),
+    ]
+
+
+def _log(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    kind = rng.choice(["write", "read", "attend", "attend", "attend", "logprobs", "logprobs"])
+    while True:
+        if kind == "logprobs":
+            case = dict(kind=kind, rows=_log(rng, 1, 20000), vocab=_log(rng, 60, 200000),
+                        top=rng.randint(1, 20), guided=rng.random() < 0.4,
+                        type=rng.choice(["f16", "bf16", "f32"]))
+        else:
+            new = rng.choice([1, _log(rng, 2, 16), _log(rng, 17, 400), _log(rng, 400, 4096)])
+            case = dict(kind=kind, count=_log(rng, 1, 64), new=new,
+                        length=new + _log(rng, 1, 40000), ragged=rng.random() < 0.7,
+                        kv_heads=rng.choice([1, 2, 4, 8, 8, 16]), dim=rng.choice([64, 128, 128]),
+                        block=rng.choice([16, 32, 64]), type=rng.choice(["f16", "bf16"]))
+            if kind == "attend":
+                case.update(group=rng.choice([1, 2, 2, 4, 8]), causal=rng.random() < 0.6)
+            elif case["type"] == "bf16" and rng.random() < 0.3:
+                case.update(type="f32")
+            if kind == "write" and rng.random() < 0.4:
+                case.update(length=new)
+        held = 0 if kind == "logprobs" else 8.0 * case["count"] * case["length"] * case["kv_heads"] * case["dim"]
+        if _fits(case) and held <= 4e9:
+            return case
+
+
+def _fits(case):
+    w = work(case)
+    if w["bytes"] > MOST_BYTES:
+        return False
+    if case["kind"] != "attend":
+        return True
+    scores = case["count"] * case["new"] * case["length"] * case["kv_heads"] * case["group"]
+    return w["flops"] <= 4.0 * MOST_PAIRS * 2048 and scores <= MOST_SCORES
+
+
+# ------------------------------------------------------------------ sizes
+
+def _sizes(case):
+    """New tokens and length of every sequence: the case's own where it is not
+    ragged, else from a half (new tokens) or a fifth (held ones) of them up."""
+    rng = random.Random("%d %d %d" % (case["count"], case["new"], case["length"]))
+    new, lengths = [], []
+    for i in range(case["count"]):
+        n, held = case["new"], case["length"] - case["new"]
+        if case["ragged"] and i:  # the first one has the full size
+            n = max(1, round(n * rng.uniform(0.5, 1.0)))
+            held = round(held * rng.uniform(0.2, 1.0))
+        new.append(n)
+        lengths.append(n + held)
+    return new, lengths
+
+
+def work(case):
+    size = SIZE[case["type"]]
+    if case["kind"] == "logprobs":
+        values = float(case["rows"]) * case["vocab"]
+        return dict(bytes=values * size * (2 if case["guided"] else 1) +
+                    case["rows"] * (12.0 + 8.0 * case["top"]), flops=4.0 * values)
+    new, lengths = _sizes(case)
+    token = 2.0 * case["kv_heads"] * case["dim"]  # values of a token's keys and values
+    scales = 8.0 * case["kv_heads"] / case["block"]
+    if case["kind"] in ("write", "read"):
+        return dict(bytes=sum(new) * (token * (size + 1) + scales), flops=2.0 * sum(new) * token)
+    if case["causal"]:
+        pairs = sum(n * (l - n) + n * (n + 1) / 2 for n, l in zip(new, lengths))
+    else:
+        pairs = sum(float(n) * l for n, l in zip(new, lengths))
+    heads = case["kv_heads"] * case["group"]
+    return dict(bytes=sum(lengths) * (token + scales) + 2.0 * sum(new) * heads * case["dim"] * size,
+                flops=4.0 * pairs * heads * case["dim"])
+
+
+# ------------------------------------------------------------------ what a program holds
+
+def _keys(x):
+    """[..., token, dim] of whole blocks -> the pool's order of keys."""
+    b, d = x.shape[-2:]
+    y = x.reshape(x.shape[:-2] + (b // 16, 16, d // 16, 16))
+    return y.transpose(-3, -2).reshape(x.shape[:-2] + (b * d,))
+
+
+def _values(x):
+    """[..., token, dim] of whole blocks -> the pool's order of values."""
+    b, d = x.shape[-2:]
+    y = x.reshape(x.shape[:-2] + (b // 16, 4, 4, d // 64, 4, 16))
+    n = y.dim() - 6
+    order = list(range(n)) + [n + k for k in (0, 3, 1, 5, 4, 2)]
+    return y.permute(order).reshape(x.shape[:-2] + (b * d,))
+
+
+def _tokens(data, dim):
+    """The pool's codes [..., 2, block * dim] -> float32 keys and values [..., token, dim]."""
+    lead, b = data.shape[:-2], data.shape[-1] // dim
+    codes = data.view(torch.float8_e4m3fn)
+    k = codes[..., 0, :].reshape(lead + (b // 16, dim // 16, 16, 16)).float()
+    k = k.transpose(-3, -2).reshape(lead + (b, dim))
+    v = codes[..., 1, :].reshape(lead + (b // 16, dim // 64, 4, 16, 4, 4)).float()
+    n = len(lead)
+    v = v.permute(list(range(n)) + [n + i for i in (0, 2, 5, 1, 4, 3)]).reshape(lead + (b, dim))
+    return k, v
+
+
+def _scale(amax):
+    """The smallest power of two, 2^-100 or more, that takes amax into +-448."""
+    m, e = torch.frexp(amax)
+    e = e - 9 + (m > 0.875).to(e.dtype)
+    return ((e.clamp(min=-100) + 127) << 23).view(torch.float32)
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    host = random.Random(seed)
+    dtype = TYPES[case["type"]]
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device="cuda")
+
+    state = dict(case=case)
+    if case["kind"] == "logprobs":
+        rows, vocab, top = case["rows"], case["vocab"], case["top"]
+        # Peaked as a trained model's are: a few entries stand out of each row.
+        logits = normal(rows, vocab).mul_(2.0)
+        best = torch.randint(0, vocab, (rows, 4), generator=gen, device="cuda")
+        logits.scatter_add_(1, best, normal(rows, 4).mul_(3.0).add_(8.0))
+        state.update(logits=logits.to(dtype), uncond=None, mask=None)
+        if case["guided"]:
+            state.update(uncond=(logits + normal(rows, vocab)).to(dtype), mask=vocab - 1)
+        state.update(tokens=best[:, 0].to(torch.int32).contiguous(),
+                     logprob=torch.zeros(rows, device="cuda"),
+                     entropy=torch.zeros(rows, device="cuda"),
+                     top_ids=torch.zeros(rows, top, dtype=torch.int32, device="cuda"),
+                     top_logprobs=torch.zeros(rows, top, device="cuda"))
+        return state
+    new, lengths = _sizes(case)
+    block, dim, heads = case["block"], case["dim"], case["kv_heads"]
+    held = [-(-l // block) for l in lengths]
+    blocks = sum(held) + 8
+    # Keys after their norm (a few loud channels), values of a different loudness per head.
+    loud = 1.0 + 3.0 * (torch.rand(heads, 1, dim, generator=gen, device="cuda") > 0.95)
+    level = torch.exp(normal(heads, 1, 1) * 0.7) * 0.3
+    pool = torch.empty(blocks, heads, 2, block * dim, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(blocks, heads, 2, device="cuda")
+    for half, (shape, order) in enumerate(((loud, _keys), (level, _values))):
+        x = normal(blocks, heads, block, dim) * shape
+        s = _scale(x.abs().amax((-1, -2)))
+        scales[:, :, half] = s
+        pool[:, :, half] = order((x / s[..., None, None]).to(torch.float8_e4m3fn).view(torch.uint8))
+        del x
+    ids = list(range(blocks))
+    host.shuffle(ids)
+    table = np.zeros((len(new), max(held)), dtype=np.int32)
+    for i, n in enumerate(held):
+        table[i, :n] = ids[sum(held[:i]):sum(held[:i]) + n]
+    begins = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    rows = int(begins[-1])
+    state.update(data=pool, scales=scales, tables=torch.from_numpy(table).cuda(),
+                 lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+                 begins=torch.from_numpy(begins).cuda(), longest=max(new), most=max(lengths),
+                 rows=rows)
+    if case["kind"] == "write":
+        state.update(k=(normal(rows, heads, dim) * loud[:, 0]).to(dtype),
+                     v=(normal(rows, heads, dim) * level[:, 0]).to(dtype))
+    elif case["kind"] == "read":
+        state.update(k=torch.zeros(rows, heads, dim, dtype=dtype, device="cuda"),
+                     v=torch.zeros(rows, heads, dim, dtype=dtype, device="cuda"))
+    else:
+        q = normal(rows, heads * case["group"], dim).to(dtype)
+        state.update(q=q, out=torch.zeros_like(q))
+    return state
+
+
+# ------------------------------------------------------------------ a pass
+
+def run(state):
+    if own:
+        return _run_own(state)
+    return PLAIN[state["case"]["kind"]](state)
+
+
+def _run_own(state):
+    import omnivoice_amd as ov
+    case = state["case"]
+    if case["kind"] == "logprobs":
+        ov.op_token_logprobs(state["logits"], state["tokens"], state["logprob"], state["entropy"],
+                             state["top_ids"], state["top_logprobs"], uncond=state["uncond"],
+                             guidance=2.0 if case["guided"] else 0.0, mask_id=state["mask"])
+        return [state[n] for n in ("logprob", "entropy", "top_ids", "top_logprobs")]
+    if "cache" not in state:  # the program's view of its own pool and tables
+        state["cache"] = ov.KVCache(state["data"], state["scales"], case["block"], case["dim"])
+        state["sequences"] = ov.KVSequences(state["tables"], state["lengths"], state["begins"])
+    if case["kind"] == "write":
+        ov.op_cache_write(state["cache"], state["sequences"], state["k"], state["v"])
+        return [state["data"].view(torch.float8_e4m3fn), state["scales"]]
+    if case["kind"] == "read":
+        ov.op_cache_read(state["cache"], state["sequences"], state["k"], state["v"])
+        return [state["k"], state["v"]]
+    ov.op_cache_attention(state["cache"], state["sequences"], state["q"], state["out"],
+                          scale=case["dim"] ** -0.5, causal=case["causal"])
+    return state["out"]
+
+
+def _positions(state):
+    """Sequence and cache position of every row of the call's tensors."""
+    begins, lengths = state["begins"].long(), state["lengths"].long()
+    rows = torch.arange(state["rows"], device="cuda")
+    seq = torch.searchsorted(begins, rows, right=True) - 1
+    return seq, lengths[seq] - begins[seq + 1] + rows
+
+
+def _plain_write(state):
+    block, dim, heads = (state["case"][n] for n in ("block", "dim", "kv_heads"))
+    data, scales = state["data"], state["scales"]
+    seq, pos = _positions(state)
+    # Every (sequence, block) that takes new tokens, and its block of the pool.
+    width = state["tables"].shape[1]
+    touched, item = torch.unique(seq * width + pos // block, return_inverse=True)
+    where = state["tables"].flatten()[touched].long()
+    start = state["lengths"] - state["begins"].diff()
+    first = start.long()[touched // width] - touched % width * block  # tokens that stay
+    last = state["lengths"].long()[touched // width] - touched % width * block
+    at = torch.arange(block, device="cuda")
+    kept = (at < first[:, None])[:, None, :, None]
+    live = (at < last[:, None])[:, None, :, None]
+    old = _tokens(data[where], dim)
+    for half, x in enumerate((state["k"], state["v"])):
+        fresh = torch.zeros(len(where), block, heads, dim, device="cuda")
+        fresh[item, pos % block] = x.float()
+        fresh = fresh.transpose(1, 2)
+        s_old = scales[where, :, half]
+        s = _scale(fresh.abs().amax((-1, -2)))
+        s = torch.where((first > 0)[:, None], torch.maximum(s, s_old), s)
+        y = torch.where(kept, old[half] * (s_old / s)[..., None, None],
+                        fresh / s[..., None, None])
+        y = torch.where(live, y, 0.0)
+        codes = y.to(torch.float8_e4m3fn).view(torch.uint8)
+        data[where, :, half] = (_keys if half == 0 else _values)(codes)
+        scales[where, :, half] = s
+    return [data.view(torch.float8_e4m3fn), scales]
+
+
+def _gathered(state):
+    """Float32 keys and values [sequence][kv head][position][dim] of whole tables."""
+    t = state["tables"].long()
+    k, v = _tokens(state["data"][t], state["case"]["dim"])
+    s = state["scales"][t][..., None, None]
+    heads = state["case"]["kv_heads"]
+    k, v = k * s[..., 0, :, :], v * s[..., 1, :, :]
+    return (x.transpose(1, 2).reshape(t.shape[0], heads, -1, x.shape[-1]) for x in (k, v))
+
+
+def _plain_read(state):
+    seq, pos = _positions(state)
+    block = state["case"]["block"]
+    where = state["tables"][seq, pos // block].long()
+    # Only the blocks that the rows lie in are taken apart.
+    used, item = torch.unique(where, return_inverse=True)
+    k, v = _tokens(state["data"][used], state["case"]["dim"])
+    s = state["scales"][used][..., None, None]
+    dtype = state["k"].dtype
+    k = (k * s[:, :, 0])[item, :, pos % block].to(dtype)
+    v = (v * s[:, :, 1])[item, :, pos % block].to(dtype)
+    return [k, v]
+
+
+def _plain_attend(state):
+    case = state["case"]
+    heads, group, dim = case["kv_heads"], case["group"], case["dim"]
+    k, v = _gathered(state)
+    begins, lengths = state["begins"].long(), state["lengths"].long()
+    t = torch.arange(state["longest"], device="cuda")
+    n = begins.diff()
+    there = t < n[:, None]
+    rows = (begins[:-1, None] + t).clamp(max=state["rows"] - 1)
+    q = state["q"][rows].float()  # [sequence][t][head][dim]
+    q = q.reshape(len(n), len(t), heads, group, dim).permute(0, 2, 3, 1, 4)
+    q = q.reshape(len(n), heads, group * len(t), dim)
+    s = q @ k.transpose(-1, -2) * dim ** -0.5
+    s = s.reshape(len(n), heads, group, len(t), -1)
+    limit = (lengths - n)[:, None] + t + 1 if case["causal"] else lengths[:, None].expand(-1, len(t))
+    seen = torch.arange(s.shape[-1], device="cuda") < limit[..., None]  # [sequence][t][key]
+    s = s.masked_fill(~seen[:, None, None], -math.inf)
+    s = (s - s.amax(-1, keepdim=True)).exp()
+    s = s / s.sum(-1, keepdim=True)
+    o = s.reshape(len(n), heads, group * len(t), -1) @ v
+    o = o.reshape(len(n), heads, group, len(t), dim).permute(0, 3, 1, 2, 4)
+    return o[there].reshape(state["rows"], heads * group, dim).to(state["q"].dtype)
+
+
+def _plain_logprobs(state):
+    z = state["logits"].float()
+    if state["uncond"] is not None:
+        z = z + (z - state["uncond"].float()) * 2.0
+    m = z.amax(-1, keepdim=True)
+    d = z - m
+    e = d.exp()
+    total = e.sum(-1, keepdim=True)
+    log_total = total.log()
+    logp = d - log_total
+    entropy = log_total[:, 0] - (e * d).sum(-1) / total[:, 0]
+    order = z
+    if state["mask"] is not None:
+        order = z.clone()
+        order[:, state["mask"]] = -math.inf
+    ids = torch.sort(order, dim=-1, descending=True, stable=True)[1][:, : state["case"]["top"]]
+    return [logp.gather(1, state["tokens"].long()[:, None])[:, 0], entropy, ids.to(torch.int32),
+            logp.gather(1, ids)]
+
+
+PLAIN = dict(write=_plain_write, read=_plain_read, attend=_plain_attend, logprobs=_plain_logprobs)
+
+
+# ------------------------------------------------------------------ the definitions in 64 bits
+
+def _e4m3_table():
+    """The 256 values of e4m3: sign, four exponent bits of bias 7, three of mantissa."""
+    c = np.arange(256)
+    e, m = (c >> 3) & 15, c & 7
+    x = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0))
+    x = np.where((c & 127) == 127, np.nan, x)
+    return torch.from_numpy(np.where(c >= 128, -x, x)).cuda()
+
+
+def _code_index(block, dim):
+    """Index in a block's codes of (token, dim), for keys and for values."""
+    t, d = torch.arange(block, device="cuda")[:, None], torch.arange(dim, device="cuda")
+    g, t = t // 16 * 16 * dim, t % 16
+    return (g + d // 16 * 256 + t * 16 + d % 16,
+            g + d // 64 * 1024 + t // 4 * 256 + d % 16 * 16 + d // 16 % 4 * 4 + t % 4)
+
+
+def _power(e):
+    """2^e in 64 bits, to the bit (a device's pow is not)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def _round_e4m3(x):
+    """x (|x| <= 448) to the nearest e4m3 value, ties to even, in 64 bits."""
+    step = _power((torch.frexp(x)[1] - 4).clamp(min=-9))
+    return torch.round(x / step) * step
+
+
+def _exact_held(state, i, half):
+    """Sequence i's keys or values, [kv head][token][dim], in 64 bits."""
+    case = state["case"]
+    ids = state["tables"][i].long()
+    index = _code_index(case["block"], case["dim"])[half]
+    x = _e4m3_table()[state["data"][ids, :, half].long()][:, :, index]
+    x = x * state["scales"][ids, :, half].double()[..., None, None]
+    return x.transpose(0, 1).reshape(x.shape[1], -1, case["dim"])
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    if case["kind"] == "logprobs":
+        return _exact_logprobs(state)
+    begins, lengths = state["begins"].tolist(), state["lengths"].tolist()
+    if case["kind"] == "write":
+        return _exact_write(state, begins, lengths)
+    out = []
+    for i, length in enumerate(lengths):
+        n = begins[i + 1] - begins[i]
+        k, v = (_exact_held(state, i, half)[:, :length] for half in (0, 1))
+        if case["kind"] == "read":
+            out.append((k[:, length - n:].transpose(0, 1), v[:, length - n:].transpose(0, 1)))
+            continue
+        q = state["q"][begins[i]:begins[i + 1]].double().transpose(0, 1)
+        seen = torch.full((n, length), True, device="cuda")
+        if case["causal"]:
+            seen = seen.tril(length - n)
+        heads = []
+        for h in range(q.shape[0]):
+            p = torch.softmax((q[h] @ k[h // case["group"]].t() / math.sqrt(case["dim"]))
+                              .masked_fill(~seen, -math.inf), -1)
+            heads.append(p @ v[h // case["group"]])
+        out.append(torch.stack(heads, 1))
+    if case["kind"] == "read":
+        return [torch.cat([o[half] for o in out]) for half in (0, 1)]
+    return torch.cat(out)
+
+
+def _exact_write(state, begins, lengths):
+    case = state["case"]
+    block = case["block"]
+    data = _e4m3_table()[state["data"].long()]
+    scales = state["scales"].double()
+    index = _code_index(block, case["dim"])
+    for i, length in enumerate(lengths):
+        start = length - (begins[i + 1] - begins[i])
+        for b in range(start // block, (length - 1) // block + 1):
+            page = int(state["tables"][i, b])
+            lo, hi = max(start, b * block), min(length, (b + 1) * block)
+            rows = slice(begins[i] + lo - start, begins[i] + hi - start)
+            for half, name in ((0, "k"), (1, "v")):
+                x = state[name][rows].double().transpose(0, 1)
+                amax = x.abs().amax((1, 2))
+                s = _power(torch.ceil(torch.log2(amax / 448)).clamp(min=-100))
+                held = data[page, :, half][:, index[half]]
+                if lo > b * block:
+                    old = scales[page, :, half]
+                    s = torch.maximum(s, old)
+                    held = _round_e4m3(held * (old / s)[:, None, None])
+                held[:, lo - b * block:hi - b * block] = _round_e4m3(x / s[:, None, None])
+                held[:, hi - b * block:] = 0.0
+                data[page, :, half] = torch.zeros_like(data[page, :, half]).scatter(
+                    1, index[half].reshape(1, -1).expand(len(s), -1), held.reshape(len(s), -1))
+                scales[page, :, half] = s
+    return [data, scales]
+
+
+def _exact_logprobs(state):
+    """The guided logits are float32 by definition (a difference, a product and
+    a sum, each rounded); everything after them is in 64 bits. Rows a few at a
+    time, for memory."""
+    got = [[], [], [], []]
+    for a in range(0, len(state["tokens"]), 256):
+        z = state["logits"][a:a + 256].float()
+        if state["uncond"] is not None:
+            z = z + 2.0 * (z - state["uncond"][a:a + 256].float())
+        z = z.double()
+        logp = torch.log_softmax(z, -1)
+        got[0].append(logp.gather(1, state["tokens"][a:a + 256].long()[:, None])[:, 0])
+        got[1].append(-(logp.exp() * logp).sum(-1))
+        if state["mask"] is not None:
+            z[:, state["mask"]] = -math.inf
+        # Descending, equal ones by index: the index ascending first, then stable.
+        ids = torch.argsort(-z, dim=-1, stable=True)[:, :state["case"]["top"]]
+        got[2].append(ids.to(torch.int32))
+        got[3].append(logp.gather(1, ids))
+    return [torch.cat(g) for g in got]
