@@ -182,7 +182,7 @@ def _tokens(data, dim):
 def _scale(amax):
     """The smallest power of two, 2^-100 or more, that takes amax into +-448."""
     m, e = torch.frexp(amax)
-    e = e - 9 + (m > 0.875).to(e.dtype)
+    e = torch.where(m > 0, e - 9 + (m > 0.875).to(e.dtype), -100)
     return ((e.clamp(min=-100) + 127) << 23).view(torch.float32)
 
 
