@@ -335,6 +335,118 @@ int ovg_op_attention(const void* qkv, void* output, int64_t rows,
                      const int64_t* sequences, int64_t count, void* stream,
                      char* error, size_t error_len);
 
+/* ---- The 8-bit key/value cache ----
+ * Keys and values that a program keeps between calls (prompts, reference
+ * voices, finished chunks), 8 bits each, and the attention that reads them.
+ * No counterpart in the reference, which holds none. The caller owns every
+ * buffer: the pool, the block tables and the workspace. The calls enqueue on
+ * `stream` and return without waiting for it, allocate nothing and can be
+ * captured into a graph; what their device arrays hold (tables, lengths,
+ * begins) is read when they run, so a replayed graph follows arrays that were
+ * updated in place. `stream` has to belong to the current device. Element
+ * types of the tensors: */
+#define OVG_F16 0
+#define OVG_BF16 1
+#define OVG_F32 2
+
+/* A pool of blocks of `block_tokens` tokens (16, 32 or 64) of every kv head.
+ *   data    [blocks][kv_heads][2][block_tokens * head_dim]: e4m3 codes of the
+ *           block's keys (0) and values (1), 16-byte aligned, in groups of 16
+ *           tokens; a group of keys is [dim / 16][token][dim % 16], a group of
+ *           values [dim / 64][token / 4][dim % 16][dim / 16 % 4][token % 4]
+ *   scales  float32 [blocks][kv_heads][2]: x = code * scale, a power of two,
+ *           NaN for a head's block that was given an infinity or a NaN
+ * head_dim is 64 or 128. A block needs no initial contents. */
+typedef struct ovg_kv_cache {
+  void* data;
+  float* scales;
+  int64_t blocks;
+  int64_t block_tokens;
+  int64_t kv_heads;
+  int64_t head_dim;
+} ovg_kv_cache;
+
+/* The sequences of one call. Device int32 arrays:
+ *   tables   [count][table_width]: the pool block of each of a sequence's
+ *            blocks; an entry outside [0, blocks) names none (its tokens are
+ *            not written, read as zeros and not attended)
+ *   lengths  [count]: tokens of the sequence, this call's included
+ *   begins   [count + 1], ascending: rows begins[i] .. begins[i + 1] - 1 of the
+ *            call's tensors are sequence i's last tokens. Rows before
+ *            begins[0] or from begins[count] on belong to nobody and are left
+ *            as they are; so is, of `rows` rows, what begins names past them.
+ * Positions past table_width * block_tokens, or before 0 where a sequence has
+ * more rows than tokens, are treated as those without a block. */
+typedef struct ovg_kv_sequences {
+  const int32_t* tables;
+  const int32_t* lengths;
+  const int32_t* begins;
+  int64_t count;
+  int64_t table_width;
+  int64_t rows;
+} ovg_kv_sequences;
+
+/* Writes k and v ([rows][kv_heads][head_dim] of `type`, rows k_stride and
+ * v_stride elements apart: a fused q|k|v row can be passed as it is) as the
+ * last tokens of their sequences. Per block, head and half the scale is the
+ * smallest power of two, 2^-100 or more, that takes the new tokens into e4m3's
+ * +-448 and, while tokens before them stay in the block, not less than it was;
+ * codes are rounded to nearest even, codes that stay move with the scale, and
+ * the positions behind the sequence's last token are cleared. With an infinity
+ * or a NaN among the new tokens the block's scale is NaN (and stays so while
+ * any of its tokens stays). Writing tokens again at the same lengths replaces
+ * them. No block may take tokens of two sequences in one call. */
+int ovg_op_cache_write(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
+                       const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+                       int type, void* stream, char* error, size_t error_len);
+
+/* The tokens that ovg_op_cache_write put there, code * scale rounded to
+ * `type`, into k and v. */
+int ovg_op_cache_read(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences, void* k,
+                      void* v, int64_t k_stride, int64_t v_stride, int type, void* stream,
+                      char* error, size_t error_len);
+
+/* Attention of q ([rows][heads][head_dim], rows q_stride elements apart, fp16
+ * or bf16) over the sequences' cached tokens, into out (likewise): query head h
+ * reads kv head h / (heads / kv_heads). A query sees every token of its
+ * sequence, or with `causal` those up to its own position (query t of n:
+ * length - n + t). softmax(scale * q . k) v in float32 sums, the probabilities
+ * rounded to `type` for their product with the values; a row that sees nothing
+ * is zero. A query that sees a token of a block whose scale is NaN is NaN.
+ * A value's part is kept to 2^-33 of the loudest value of its head in fp16.
+ * `workspace`: ovg_op_cache_attention_workspace bytes, 16-byte aligned, NULL
+ * where that is 0; it holds nothing between calls, and calls that may overlap
+ * need one each. */
+int64_t ovg_op_cache_attention_workspace(const ovg_kv_cache* cache,
+                                         const ovg_kv_sequences* sequences, int64_t heads);
+int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
+                           const void* q, void* out, int64_t q_stride, int64_t out_stride,
+                           int64_t heads, float scale, int causal, int type, void* workspace,
+                           int64_t workspace_bytes, void* stream, char* error,
+                           size_t error_len);
+
+/* ---- Log probabilities of tokens ----
+ * What ovg_op_score says of its own prediction, for given tokens: per row of
+ * `logits` ([rows][vocab] of `type`, rows `stride` elements apart) the log
+ * probability of tokens[row], the distribution's entropy, and its `top` best
+ * tokens with their log probabilities, descending, equal ones by index. With
+ * `uncond` (NULL without guidance) the logits are z = c + guidance * (c - u),
+ * each step rounded to float32, and -inf where c is. As in ovg_op_score, the
+ * token `mask_id` (-1: none) has its share of the distribution but is not
+ * listed. A token outside the vocabulary has -inf. Where fewer than `top`
+ * tokens can be listed the rest are -1 and -inf. A row without a distribution
+ * (a NaN or +inf among its logits, or only -inf) gets NaN and -1.
+ * logprob (with tokens) and entropy may be NULL, as may top_ids and
+ * top_logprobs [rows][top] where top is 0; top <= 32. `workspace` as above.
+ * Same streams and captures as the cache's calls. */
+int64_t ovg_op_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top);
+int ovg_op_token_logprobs(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
+                          int64_t stride, int64_t uncond_stride, float guidance,
+                          int64_t mask_id, const int32_t* tokens, int64_t top, float* logprob,
+                          float* entropy, int32_t* top_ids, float* top_logprobs, int type,
+                          void* workspace, int64_t workspace_bytes, void* stream, char* error,
+                          size_t error_len);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

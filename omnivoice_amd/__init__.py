@@ -89,6 +89,16 @@ class _EncoderConfig(ctypes.Structure):
                 ("codebook_dim", _i64)]
 
 
+class _KvCache(ctypes.Structure):
+    _fields_ = [("data", _ptr), ("scales", _ptr), ("blocks", _i64),
+                ("block_tokens", _i64), ("kv_heads", _i64), ("head_dim", _i64)]
+
+
+class _KvSequences(ctypes.Structure):
+    _fields_ = [("tables", _ptr), ("lengths", _ptr), ("begins", _ptr),
+                ("count", _i64), ("table_width", _i64), ("rows", _i64)]
+
+
 _CANCEL_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)
 
 EXPORTS = {
@@ -138,6 +148,22 @@ EXPORTS = {
                                       _sz]),
     "ovg_op_attention": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _i64, _ptr, _i64,
                                         _ptr, _err, _sz]),
+    "ovg_op_cache_write": (ctypes.c_int, [ctypes.POINTER(_KvCache),
+                                          ctypes.POINTER(_KvSequences), _ptr, _ptr, _i64,
+                                          _i64, ctypes.c_int, _ptr, _err, _sz]),
+    "ovg_op_cache_read": (ctypes.c_int, [ctypes.POINTER(_KvCache),
+                                         ctypes.POINTER(_KvSequences), _ptr, _ptr, _i64,
+                                         _i64, ctypes.c_int, _ptr, _err, _sz]),
+    "ovg_op_cache_attention_workspace": (_i64, [ctypes.POINTER(_KvCache),
+                                                ctypes.POINTER(_KvSequences), _i64]),
+    "ovg_op_cache_attention": (ctypes.c_int, [ctypes.POINTER(_KvCache),
+                                              ctypes.POINTER(_KvSequences), _ptr, _ptr, _i64,
+                                              _i64, _i64, _f32, ctypes.c_int, ctypes.c_int,
+                                              _ptr, _i64, _ptr, _err, _sz]),
+    "ovg_op_token_logprobs_workspace": (_i64, [_i64, _i64, _i64]),
+    "ovg_op_token_logprobs": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _i64, _i64, _f32, _i64,
+                                             _ptr, _i64, _ptr, _ptr, _ptr, _ptr, ctypes.c_int,
+                                             _ptr, _i64, _ptr, _err, _sz]),
     # the audio decoder (include/omnivoice_codec_mi355x.h)
     "ovc_create": (ctypes.c_int, [ctypes.POINTER(_CodecConfig), ctypes.c_char_p, _u64,
                                   ctypes.POINTER(_ptr), _err, _sz]),
@@ -628,6 +654,267 @@ def op_attention(qkv, out, heads: int, kv_heads: int,
     _check(lib().ovg_op_attention(_dev(qkv), _dev(out), rows, heads, kv_heads,
                                   _p(seq), len(sequences), _stream(stream),
                                   err, len(err)), err)
+
+
+# --------------------------------------------------------------- 8-bit key/value cache
+
+def _type_of(t, name: str, with_f32: bool = True) -> int:
+    """OVG_F16, OVG_BF16 or OVG_F32 of a tensor."""
+    import torch
+    if t.dtype is torch.float16:
+        return 0
+    if t.dtype is torch.bfloat16:
+        return 1
+    if with_f32 and t.dtype is torch.float32:
+        return 2
+    raise GeneratorError(f"{name}: {t.dtype} is not supported")
+
+
+def _expect(t, name: str, dtype, shape: Tuple[int, ...], device) -> None:
+    """A contiguous device tensor of this type and shape on `device`."""
+    if t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous() \
+            or t.device != device:
+        raise GeneratorError(f"{name}: needs a contiguous {dtype} tensor of shape {shape} on "
+                             f"{device}, got {t.dtype} {tuple(t.shape)} on {t.device}"
+                             f"{'' if t.is_contiguous() else ', not contiguous'}")
+
+
+def _row_stride(t, name: str, heads: int, dim: int, device) -> int:
+    """The row stride, in elements, of a [rows][heads][dim] tensor whose rows are
+    contiguous."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.device != device \
+            or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+        raise GeneratorError(f"{name}: needs [rows][{heads}][{dim}] with contiguous rows on "
+                             f"{device}, got {tuple(t.shape)} with strides {t.stride()} on "
+                             f"{t.device}")
+    # A single row has no stride of its own.
+    return t.stride(0) if t.shape[0] > 1 else heads * dim
+
+
+def _launch(device, stream, call) -> None:
+    """call(stream handle) with the tensors' device current; without a stream,
+    on that device's current one."""
+    import torch
+    if device.type != "cuda":
+        raise GeneratorError(f"needs tensors of a GPU, got {device}")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            call(torch.cuda.current_stream(device).cuda_stream if stream is None else stream)
+    else:
+        call(torch.cuda.current_stream().cuda_stream if stream is None else stream)
+
+
+def _workspace(workspace, size: int, device, stream):
+    """(pointer, bytes) of the caller's workspace, or of a new one that stays
+    reserved until the work on `stream` is done. The caller holds what this
+    returns until the launch."""
+    if size == 0 and workspace is None:
+        return None, 0, None
+    if workspace is None:
+        import torch
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        if stream is not None:
+            workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
+                                    else torch.cuda.ExternalStream(stream, device=device))
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise GeneratorError(f"workspace: needs a contiguous tensor on {device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+@dataclass
+class KVCache:
+    """A pool of 8-bit keys and values (ovg_kv_cache): data uint8
+    [blocks][kv_heads][2][block_tokens * head_dim], scales float32
+    [blocks][kv_heads][2], device tensors that the caller owns."""
+    data: "torch.Tensor"  # noqa: F821
+    scales: "torch.Tensor"  # noqa: F821
+    block_tokens: int
+    head_dim: int
+
+    def __post_init__(self):
+        import torch
+        if self.data.dim() != 4:
+            raise GeneratorError("cache data: needs [blocks][kv_heads][2][block_tokens * "
+                                 f"head_dim], got {tuple(self.data.shape)}")
+        blocks, heads = self.data.shape[:2]
+        device = self.data.device
+        _expect(self.data, "cache data", torch.uint8,
+                (blocks, heads, 2, self.block_tokens * self.head_dim), device)
+        _expect(self.scales, "cache scales", torch.float32, (blocks, heads, 2), device)
+        self.kv_heads = heads
+        self.device = device
+        self._c = _KvCache(self.data.data_ptr(), self.scales.data_ptr(), blocks,
+                           self.block_tokens, heads, self.head_dim)
+
+    @classmethod
+    def empty(cls, blocks: int, kv_heads: int = 8, head_dim: int = 128,
+              block_tokens: int = 32, device="cuda") -> "KVCache":
+        import torch
+        return cls(torch.zeros((blocks, kv_heads, 2, block_tokens * head_dim),
+                               dtype=torch.uint8, device=device),
+                   torch.zeros((blocks, kv_heads, 2), dtype=torch.float32, device=device),
+                   block_tokens, head_dim)
+
+
+@dataclass
+class KVSequences:
+    """The sequences of one call (ovg_kv_sequences): tables int32
+    [count][width], lengths int32 [count] (this call's tokens included) and
+    begins int32 [count + 1] (their rows), device tensors that may be updated
+    in place between calls and graph replays."""
+    tables: "torch.Tensor"  # noqa: F821
+    lengths: "torch.Tensor"  # noqa: F821
+    begins: "torch.Tensor"  # noqa: F821
+
+    def __post_init__(self):
+        import torch
+        if self.tables.dim() != 2:
+            raise GeneratorError("tables: needs [count][width], got "
+                                 f"{tuple(self.tables.shape)}")
+        count, width = self.tables.shape
+        device = self.tables.device
+        _expect(self.tables, "tables", torch.int32, (count, width), device)
+        _expect(self.lengths, "lengths", torch.int32, (count,), device)
+        _expect(self.begins, "begins", torch.int32, (count + 1,), device)
+        self.device = device
+
+    def _c(self, rows: int) -> _KvSequences:
+        return _KvSequences(self.tables.data_ptr(), self.lengths.data_ptr(),
+                            self.begins.data_ptr(), self.tables.shape[0],
+                            self.tables.shape[1], rows)
+
+
+def _check_cache(cache: KVCache, sequences: KVSequences) -> None:
+    if sequences.device != cache.device:
+        raise GeneratorError(f"sequences on {sequences.device}, the cache on {cache.device}")
+
+
+def _cache_io(name: str, cache: KVCache, sequences: KVSequences, k, v, stream) -> None:
+    _check_cache(cache, sequences)
+    k_stride = _row_stride(k, "k", cache.kv_heads, cache.head_dim, cache.device)
+    v_stride = _row_stride(v, "v", cache.kv_heads, cache.head_dim, cache.device)
+    if k.shape[0] != v.shape[0] or k.dtype is not v.dtype:
+        raise GeneratorError(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} "
+                             f"{v.dtype}")
+    kind = _type_of(k, "k")
+    seq = sequences._c(k.shape[0])
+    err = _buf()
+    fn = getattr(lib(), name)
+    _launch(cache.device, stream,
+            lambda s: _check(fn(cache._c, seq, _dev(k), _dev(v), k_stride, v_stride, kind, s,
+                                err, len(err)), err))
+
+
+def op_cache_write(cache: KVCache, sequences: KVSequences, k, v, stream=None) -> None:
+    """Quantises k and v [rows][kv_heads][head_dim] (fp16, bf16 or float32
+    device tensors with contiguous rows) into the cache as the last tokens of
+    their sequences. Enqueued on `stream`."""
+    _cache_io("ovg_op_cache_write", cache, sequences, k, v, stream)
+
+
+def op_cache_read(cache: KVCache, sequences: KVSequences, k, v, stream=None) -> None:
+    """The last tokens of the sequences back into k and v
+    [rows][kv_heads][head_dim] (fp16, bf16 or float32). Enqueued on `stream`."""
+    _cache_io("ovg_op_cache_read", cache, sequences, k, v, stream)
+
+
+def op_cache_attention_workspace(cache: KVCache, sequences: KVSequences, rows: int,
+                                 heads: int) -> int:
+    """Bytes of workspace that op_cache_attention needs for `rows` queries."""
+    return int(lib().ovg_op_cache_attention_workspace(cache._c, sequences._c(rows), heads))
+
+
+def op_cache_attention(cache: KVCache, sequences: KVSequences, q, out,
+                       scale: Optional[float] = None, causal: bool = False, workspace=None,
+                       stream=None) -> None:
+    """Attention of q [rows][heads][head_dim] (fp16 or bf16) over the cached
+    tokens of their sequences into out (the same shape and type); scale
+    defaults to head_dim ** -0.5. `workspace`: a device tensor of
+    op_cache_attention_workspace bytes (one is allocated without it). Enqueued
+    on `stream`."""
+    _check_cache(cache, sequences)
+    if q.dim() != 3:
+        raise GeneratorError(f"q: needs [rows][heads][{cache.head_dim}], got {tuple(q.shape)}")
+    rows, heads = q.shape[:2]
+    q_stride = _row_stride(q, "q", heads, cache.head_dim, cache.device)
+    out_stride = _row_stride(out, "out", heads, cache.head_dim, cache.device)
+    if out.shape[0] != rows or out.dtype is not q.dtype:
+        raise GeneratorError(f"q and out differ: {tuple(q.shape)} {q.dtype}, "
+                             f"{tuple(out.shape)} {out.dtype}")
+    kind = _type_of(q, "q", with_f32=False)
+    seq = sequences._c(rows)
+    L = lib()
+    space, size, keep = _workspace(
+        workspace, L.ovg_op_cache_attention_workspace(cache._c, seq, heads), cache.device, stream)
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    err = _buf()
+    _launch(cache.device, stream,
+            lambda s: _check(L.ovg_op_cache_attention(
+                cache._c, seq, _dev(q), _dev(out), q_stride, out_stride, heads, scale,
+                int(causal), kind, space, size, s, err, len(err)), err))
+
+
+# --------------------------------------------------------------- log probabilities
+
+def _logit_stride(t, name: str, rows: int, vocab: int, device, dtype) -> int:
+    if tuple(t.shape) != (rows, vocab) or t.device != device or t.dtype is not dtype \
+            or (vocab > 1 and t.stride(1) != 1):
+        raise GeneratorError(f"{name}: needs [{rows}][{vocab}] {dtype} with contiguous rows on "
+                             f"{device}, got {tuple(t.shape)} {t.dtype} with strides "
+                             f"{t.stride()} on {t.device}")
+    return t.stride(0) if rows > 1 else vocab
+
+
+def op_token_logprobs(logits, tokens, logprob, entropy, top_ids=None, top_logprobs=None,
+                      uncond=None, guidance: float = 0.0, mask_id: Optional[int] = None,
+                      workspace=None, stream=None) -> None:
+    """Per row of logits [rows][vocab] (fp16, bf16 or float32, contiguous
+    rows): the log probability of tokens [rows] (int32) into logprob, the
+    entropy into entropy, and the best top_ids.shape[1] tokens but mask_id with
+    their log probabilities into top_ids (int32) and top_logprobs. With
+    `uncond` the distribution is that of c + guidance * (c - u). tokens and
+    logprob, entropy, and top_ids and top_logprobs may be None. Enqueued on
+    `stream`."""
+    import torch
+    if logits.dim() != 2:
+        raise GeneratorError(f"logits: needs [rows][vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    device = logits.device
+    kind = _type_of(logits, "logits")
+    stride = _logit_stride(logits, "logits", rows, vocab, device, logits.dtype)
+    u_stride = vocab if uncond is None else _logit_stride(uncond, "uncond", rows, vocab, device,
+                                                          logits.dtype)
+    if (tokens is None) != (logprob is None):
+        raise GeneratorError("tokens and logprob go together")
+    if tokens is not None:
+        _expect(tokens, "tokens", torch.int32, (rows,), device)
+        _expect(logprob, "logprob", torch.float32, (rows,), device)
+    if entropy is not None:
+        _expect(entropy, "entropy", torch.float32, (rows,), device)
+    if (top_ids is None) != (top_logprobs is None):
+        raise GeneratorError("top_ids and top_logprobs go together")
+    top = 0
+    if top_ids is not None:
+        if top_ids.dim() != 2:
+            raise GeneratorError(f"top_ids: needs [rows][top], got {tuple(top_ids.shape)}")
+        top = top_ids.shape[1]
+        _expect(top_ids, "top_ids", torch.int32, (rows, top), device)
+        _expect(top_logprobs, "top_logprobs", torch.float32, (rows, top), device)
+    L = lib()
+    space, size, keep = _workspace(
+        workspace, L.ovg_op_token_logprobs_workspace(rows, vocab, top), device, stream)
+
+    def ptr(t):
+        return None if t is None else t.data_ptr()
+
+    err = _buf()
+    _launch(device, stream,
+            lambda s: _check(L.ovg_op_token_logprobs(
+                _dev(logits), ptr(uncond), rows, vocab, stride, u_stride, guidance,
+                -1 if mask_id is None else mask_id, ptr(tokens), top, ptr(logprob),
+                ptr(entropy), ptr(top_ids), ptr(top_logprobs), kind, space, size, s, err,
+                len(err)), err))
 
 
 # --------------------------------------------------------------- audio decoder

@@ -1,0 +1,138 @@
+// The 8-bit key/value cache and the token log probabilities: parameters and
+// launchers of cache_kernels.hip, cache_attention.hip and logprobs.hip.
+#ifndef OMNIVOICE_AMD_CACHE_HPP_
+#define OMNIVOICE_AMD_CACHE_HPP_
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "kernels.hpp"
+
+namespace ovg {
+
+// Element types of the operators' caller tensors (OVG_F16, OVG_BF16, OVG_F32).
+enum class DType : int { kF16 = 0, kBf16 = 1, kF32 = 2 };
+
+// A pool of blocks and the sequences of one call. Device pointers; the
+// values behind them are not known to the host, so every kernel clamps what
+// it reads of them (Span, Page).
+struct CacheView {
+  unsigned char* data;  // [blocks][kv_heads][2][block_tokens * dim], e4m3 codes
+  float* scales;        // [blocks][kv_heads][2]
+  const int* tables;    // [count][table_width]
+  const int* lengths;   // [count]
+  const int* begins;    // [count + 1]
+  int blocks, block_shift, kv_heads, dim;
+  int count, table_width, rows;
+};
+
+// One half (keys 0, values 1) of one head of a block: dim << block_shift codes.
+__device__ __forceinline__ unsigned char* HalfOf(const CacheView& c, int page, int head,
+                                                 int half) {
+  const std::size_t index =
+      (static_cast<std::size_t>(page) * c.kv_heads + head) * 2 + half;
+  return c.data + index * (static_cast<std::size_t>(c.dim) << c.block_shift);
+}
+__device__ __forceinline__ std::size_t ScaleIndex(const CacheView& c, int page, int head,
+                                                  int half) {
+  return (static_cast<std::size_t>(page) * c.kv_heads + head) * 2 + half;
+}
+
+// Sequence i's rows [first, first + count) of the call's tensors and the
+// cache position `start` of its first row (negative where the sequence is
+// shorter than its rows). Rows are clamped into the tensors.
+struct Span {
+  int first, count, start, length;
+};
+__device__ __forceinline__ Span SpanOf(const CacheView& c, int i) {
+  Span s;
+  s.first = min(max(c.begins[i], 0), c.rows);
+  s.count = min(max(c.begins[i + 1], s.first), c.rows) - s.first;
+  s.length = max(c.lengths[i], 0);
+  s.start = s.length - s.count;
+  return s;
+}
+
+// The pool block of a sequence's block `b`, or -1 where the table has none.
+__device__ __forceinline__ int PageOf(const CacheView& c, int sequence, int b) {
+  if (b < 0 || b >= c.table_width)
+    return -1;
+  const int page = c.tables[static_cast<std::size_t>(sequence) * c.table_width + b];
+  return page >= 0 && page < c.blocks ? page : -1;
+}
+
+// Work items of ragged sequences without a list: sequence i owns the items
+// from Base(i) = first_i * scale / tile + slack * i (a whole-number division)
+// up to Base(i + 1), at least rows_i * scale / tile + slack of them. Every lane
+// counts bases of its own, so the search is one memory round trip per 64
+// sequences and not one per halving. Returns the sequence of `item` and takes
+// its base from it; the whole wave calls this.
+__device__ __forceinline__ int SequenceOfItem(const CacheView& c, int scale, int shift, int slack,
+                                              int* item) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int below = 0;
+  for (int i0 = 0; i0 < c.count; i0 += kWave) {
+    const int i = i0 + lane;
+    const int first = min(max(c.begins[min(i, c.count)], 0), c.rows);
+    const bool at = i < c.count && ((first * scale) >> shift) + slack * i <= *item;
+    const unsigned long long ballot = __ballot(at);
+    below += __popcll(ballot);
+    if (ballot != ~0ull)
+      break;
+  }
+  const int sequence = max(below - 1, 0);
+  const int first = min(max(c.begins[sequence], 0), c.rows);
+  *item -= ((first * scale) >> shift) + slack * sequence;
+  return sequence;
+}
+inline int ItemBound(const CacheView& c, int scale, int shift, int slack) {
+  return ((c.rows * scale) >> shift) + slack * c.count;
+}
+
+// ---------------------------------------------------------------- cache
+struct CacheWriteParams {
+  CacheView cache;
+  const void* x[2];  // keys, values [rows][kv_heads][dim], rows `stride` elements apart
+  std::int64_t stride[2];
+};
+void LaunchCacheWrite(const CacheWriteParams& p, DType type, hipStream_t stream);
+
+struct CacheReadParams {
+  CacheView cache;
+  void* x[2];
+  std::int64_t stride[2];
+};
+void LaunchCacheRead(const CacheReadParams& p, DType type, hipStream_t stream);
+
+struct CacheAttentionParams {
+  CacheView cache;
+  const void* q;   // [rows][heads][dim], rows q_stride elements apart
+  void* out;       // [rows][heads][dim], rows out_stride elements apart
+  std::int64_t q_stride, out_stride;
+  int group;       // query heads per kv head
+  bool causal;
+  float scale_log2;  // the softmax's scale * log2(e)
+};
+void LaunchCacheAttention(const CacheAttentionParams& p, DType type, hipStream_t stream);
+
+// ---------------------------------------------------------------- log probabilities
+struct LogprobParams {
+  const void* logits;  // [rows][vocab], rows `stride` elements apart
+  const void* uncond;  // the same, or null
+  std::int64_t stride, uncond_stride;
+  const int* tokens;   // [rows], or null
+  float guidance;
+  int rows, vocab, mask_id, top;
+  float* logprob;        // [rows], or null
+  float* entropy;        // [rows], or null
+  int* top_ids;          // [rows][top]
+  float* top_logprobs;   // [rows][top]
+};
+constexpr int kMostAlternatives = 32;
+void LaunchLogprobs(const LogprobParams& p, DType type, hipStream_t stream);
+
+}  // namespace ovg
+
+#endif  // OMNIVOICE_AMD_CACHE_HPP_

@@ -8,6 +8,7 @@
 #include <string>
 
 #include "../../include/omnivoice_mi355x.h"
+#include "cache.hpp"
 #include "kernels.hpp"
 
 namespace {
@@ -47,6 +48,66 @@ struct Scratch {
       (void)hipFree(data);
   }
 };
+
+// A launch has to go to a device of its own: with another device current the
+// kernel would run there, or fail in ways that depend on peer access.
+void RequireCurrentDevice(hipStream_t stream) {
+  if (stream == nullptr)
+    return;  // the current device's own
+  hipDevice_t of_stream = 0;
+  int current = 0;
+  ovg::Check(hipStreamGetDevice(stream, &of_stream), "hipStreamGetDevice");
+  ovg::Check(hipGetDevice(&current), "hipGetDevice");
+  ovg::Require(of_stream == current, "the stream is not the current device's");
+}
+
+bool Aligned16(const void* p) { return reinterpret_cast<std::uintptr_t>(p) % 16 == 0; }
+
+// The pool and sequences of a call, their sizes checked against what the
+// kernels' 32-bit positions, rows and items hold.
+ovg::CacheView ViewOf(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences) {
+  ovg::Require(cache && sequences, "null pointer");
+  ovg::Require(cache->data && cache->scales, "null pool");
+  ovg::Require(Aligned16(cache->data), "the pool must be 16-byte aligned");
+  ovg::Require(cache->block_tokens == 16 || cache->block_tokens == 32 || cache->block_tokens == 64,
+               "block_tokens must be 16, 32 or 64");
+  ovg::Require(cache->head_dim == 64 || cache->head_dim == 128, "head_dim must be 64 or 128");
+  ovg::Require(cache->kv_heads >= 1 && cache->kv_heads <= 1024, "kv_heads outside [1, 1024]");
+  ovg::Require(cache->blocks >= 1 && FitsInt(cache->blocks), "blocks outside [1, 2^30]");
+  ovg::Require(sequences->count >= 0 && sequences->count <= (1 << 20),
+               "count outside [0, 2^20]");
+  ovg::Require(sequences->rows >= 0 && sequences->rows <= (1 << 24), "rows outside [0, 2^24]");
+  ovg::Require(sequences->table_width >= 1 &&
+                   sequences->table_width <= (int64_t{1} << 30) / cache->block_tokens,
+               "table_width outside [1, 2^30 / block_tokens]");
+  ovg::Require(sequences->count == 0 ||
+                   (sequences->tables && sequences->lengths && sequences->begins),
+               "null pointer");
+  ovg::CacheView c{};
+  c.data = static_cast<unsigned char*>(cache->data);
+  c.scales = cache->scales;
+  c.tables = sequences->tables;
+  c.lengths = sequences->lengths;
+  c.begins = sequences->begins;
+  c.blocks = static_cast<int>(cache->blocks);
+  c.block_shift = cache->block_tokens == 16 ? 4 : cache->block_tokens == 32 ? 5 : 6;
+  c.kv_heads = static_cast<int>(cache->kv_heads);
+  c.dim = static_cast<int>(cache->head_dim);
+  c.count = static_cast<int>(sequences->count);
+  c.table_width = static_cast<int>(sequences->table_width);
+  c.rows = sequences->count == 0 ? 0 : static_cast<int>(sequences->rows);
+  return c;
+}
+
+ovg::DType TypeOf(int type, bool with_f32) {
+  ovg::Require(type == OVG_F16 || type == OVG_BF16 || (with_f32 && type == OVG_F32),
+               with_f32 ? "type must be fp16, bf16 or float32" : "type must be fp16 or bf16");
+  return static_cast<ovg::DType>(type);
+}
+
+void RequireStride(int64_t stride, int64_t width) {
+  ovg::Require(stride >= width && stride <= (int64_t{1} << 40), "row stride below the row's width");
+}
 
 }  // namespace
 
@@ -284,6 +345,144 @@ int ovg_op_attention(const void* qkv, void* output, int64_t rows,
     p.scale_log2 = 1.44269504088896341F / 11.313708498984761F;
     ovg::LaunchAttention(p, s);
     ovg::Check(hipStreamSynchronize(s), "attention");
+  });
+}
+
+int ovg_op_cache_write(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
+                       const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+                       int type, void* stream, char* error, size_t error_len) {
+  return Guard("cache write: ", error, error_len, [&] {
+    ovg::CacheWriteParams p{};
+    p.cache = ViewOf(cache, sequences);
+    const ovg::DType t = TypeOf(type, true);
+    const int64_t width = cache->kv_heads * cache->head_dim;
+    RequireStride(k_stride, width);
+    RequireStride(v_stride, width);
+    if (p.cache.rows == 0)
+      return;
+    ovg::Require(k && v, "null pointer");
+    auto s = static_cast<hipStream_t>(stream);
+    RequireCurrentDevice(s);
+    p.x[0] = k;
+    p.x[1] = v;
+    p.stride[0] = k_stride;
+    p.stride[1] = v_stride;
+    ovg::LaunchCacheWrite(p, t, s);
+  });
+}
+
+int ovg_op_cache_read(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences, void* k,
+                      void* v, int64_t k_stride, int64_t v_stride, int type, void* stream,
+                      char* error, size_t error_len) {
+  return Guard("cache read: ", error, error_len, [&] {
+    ovg::CacheReadParams p{};
+    p.cache = ViewOf(cache, sequences);
+    const ovg::DType t = TypeOf(type, true);
+    const int64_t width = cache->kv_heads * cache->head_dim;
+    RequireStride(k_stride, width);
+    RequireStride(v_stride, width);
+    if (p.cache.rows == 0)
+      return;
+    ovg::Require(k && v, "null pointer");
+    auto s = static_cast<hipStream_t>(stream);
+    RequireCurrentDevice(s);
+    p.x[0] = k;
+    p.x[1] = v;
+    p.stride[0] = k_stride;
+    p.stride[1] = v_stride;
+    ovg::LaunchCacheRead(p, t, s);
+  });
+}
+
+int64_t ovg_op_cache_attention_workspace(const ovg_kv_cache* cache,
+                                         const ovg_kv_sequences* sequences, int64_t heads) {
+  (void)cache;
+  (void)sequences;
+  (void)heads;
+  return 0;
+}
+
+int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
+                           const void* q, void* out, int64_t q_stride, int64_t out_stride,
+                           int64_t heads, float scale, int causal, int type, void* workspace,
+                           int64_t workspace_bytes, void* stream, char* error,
+                           size_t error_len) {
+  return Guard("cache attention: ", error, error_len, [&] {
+    ovg::CacheAttentionParams p{};
+    p.cache = ViewOf(cache, sequences);
+    const ovg::DType t = TypeOf(type, false);
+    ovg::Require(heads >= cache->kv_heads && heads % cache->kv_heads == 0 &&
+                     heads / cache->kv_heads <= 64,
+                 "heads must be 1 to 64 times kv_heads");
+    ovg::Require(scale == scale && scale - scale == 0.0F, "scale must be finite");
+    RequireStride(q_stride, heads * cache->head_dim);
+    RequireStride(out_stride, heads * cache->head_dim);
+    if (p.cache.rows == 0)
+      return;
+    ovg::Require(q && out, "null pointer");
+    auto s = static_cast<hipStream_t>(stream);
+    RequireCurrentDevice(s);
+    (void)workspace;
+    (void)workspace_bytes;
+    p.q = q;
+    p.out = out;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.group = static_cast<int>(heads / cache->kv_heads);
+    p.causal = causal != 0;
+    p.scale_log2 = scale * 1.44269504088896341F;
+    ovg::LaunchCacheAttention(p, t, s);
+  });
+}
+
+int64_t ovg_op_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top) {
+  (void)rows;
+  (void)vocab;
+  (void)top;
+  return 0;
+}
+
+int ovg_op_token_logprobs(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
+                          int64_t stride, int64_t uncond_stride, float guidance,
+                          int64_t mask_id, const int32_t* tokens, int64_t top, float* logprob,
+                          float* entropy, int32_t* top_ids, float* top_logprobs, int type,
+                          void* workspace, int64_t workspace_bytes, void* stream, char* error,
+                          size_t error_len) {
+  return Guard("token logprobs: ", error, error_len, [&] {
+    const ovg::DType t = TypeOf(type, true);
+    ovg::Require(rows >= 0 && FitsInt(rows), "rows outside [0, 2^30]");
+    ovg::Require(vocab >= 1 && FitsInt(vocab), "vocab outside [1, 2^30]");
+    ovg::Require(top >= 0 && top <= ovg::kMostAlternatives, "top outside [0, 32]");
+    ovg::Require(mask_id >= -1 && mask_id < (int64_t{1} << 31), "mask_id must be -1 or a token");
+    ovg::Require(guidance == guidance && guidance - guidance == 0.0F, "guidance must be finite");
+    RequireStride(stride, vocab);
+    if (uncond != nullptr)
+      RequireStride(uncond_stride, vocab);
+    ovg::Require((tokens == nullptr) == (logprob == nullptr), "tokens and logprob go together");
+    if (rows == 0)
+      return;
+    ovg::Require(logits != nullptr, "null pointer");
+    ovg::Require(top == 0 || (top_ids && top_logprobs), "null pointer");
+    auto s = static_cast<hipStream_t>(stream);
+    RequireCurrentDevice(s);
+    (void)workspace;
+    (void)workspace_bytes;
+    ovg::LogprobParams p{};
+    p.logits = logits;
+    p.uncond = uncond;
+    p.stride = stride;
+    p.uncond_stride = uncond_stride;
+    p.tokens = tokens;
+    p.guidance = guidance;
+    p.rows = static_cast<int>(rows);
+    p.vocab = static_cast<int>(vocab);
+    p.mask_id = static_cast<int>(mask_id);
+    p.top = static_cast<int>(top);
+    p.logprob = logprob;
+    p.entropy = entropy;
+    p.top_ids = top_ids;
+    p.top_logprobs = top_logprobs;
+    ovg::LaunchLogprobs(p, t, s);
   });
 }
 
