@@ -414,8 +414,8 @@ int ovg_op_cache_read(const ovg_kv_cache* cache, const ovg_kv_sequences* sequenc
  * rounded to `type` for their product with the values; a row that sees nothing
  * is zero. A query that sees a token of a block whose scale is NaN is NaN.
  * A value's part is kept to 2^-33 of the loudest value of its head in fp16.
- * `workspace`: ovg_op_cache_attention_workspace bytes, 16-byte aligned, NULL
- * where that is 0; it holds nothing between calls, and calls that may overlap
+ * `workspace`: ovg_op_cache_attention_workspace bytes (-1 for arguments that
+ * the call refuses), 16-byte aligned, NULL where that is 0; it holds nothing between calls, and calls that may overlap
  * need one each. */
 int64_t ovg_op_cache_attention_workspace(const ovg_kv_cache* cache,
                                          const ovg_kv_sequences* sequences, int64_t heads);

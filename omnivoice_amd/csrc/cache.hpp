@@ -114,7 +114,31 @@ struct CacheAttentionParams {
   int group;       // query heads per kv head
   bool causal;
   float scale_log2;  // the softmax's scale * log2(e)
+  // The plan's (PlanCacheAttention), and where its splits leave their states:
+  // slot ((item * kv_heads + head) * splits + split) * tile rows + row has its
+  // row's maximum and sum in partial_m and its output, not divided, in partial_o.
+  int tile_shift, splits;
+  float* partial_m;  // [slots][2]
+  float* partial_o;  // [slots][dim]
 };
+// How a call is split: from the shapes that the host knows.
+struct CacheAttentionPlan {
+  int tile_shift = 4;     // log2 of a work-group's rows
+  int splits = 1;         // of each sequence's keys
+  std::size_t slots = 0;  // of the workspace
+};
+constexpr int kMostSplits = 256;
+constexpr int kLeastChunk = 256;    // keys of a split at least
+constexpr int kSplitGroups = 2048;  // work-groups that a split call is to have
+CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group);
+// Keys of each split of a sequence of `length` tokens: a whole number of the
+// four waves' steps.
+__host__ __device__ inline int ChunkOf(int length, int splits) {
+  if (splits == 1)
+    return length;
+  const int even = (length + splits - 1) / splits;
+  return (even > kLeastChunk ? even + 127 : kLeastChunk) & ~127;
+}
 void LaunchCacheAttention(const CacheAttentionParams& p, DType type, hipStream_t stream);
 
 // ---------------------------------------------------------------- log probabilities

@@ -13,7 +13,7 @@
 // values' the float32 sums. The one rounding on the way is that of the
 // probabilities to the queries' type, and the row's sum takes the rounded
 // ones, so that the weights still add up to one.
-#include <type_traits>
+#include <algorithm>
 
 #include "cache.hpp"
 
@@ -40,6 +40,13 @@ struct Types<_Float16> {
   static __device__ __forceinline__ x2 High(unsigned w, float s) {
     return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w), s, true);
   }
+  // To the type, nearest even.
+  static __device__ __forceinline__ x2 Round(float a, float b) {
+    return x2{static_cast<_Float16>(a), static_cast<_Float16>(b)};
+  }
+  static __device__ __forceinline__ float AddPair(x2 pair, float sum) {
+    return __builtin_amdgcn_fdot2(pair, x2{1, 1}, sum, false);
+  }
   static __device__ __forceinline__ floatx4 Mfma16(x8 a, x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -53,6 +60,13 @@ struct Types<__bf16> {
   }
   static __device__ __forceinline__ x2 High(unsigned w, float s) {
     return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), s, true);
+  }
+  // To the type, nearest even.
+  static __device__ __forceinline__ x2 Round(float a, float b) {
+    return x2{static_cast<__bf16>(a), static_cast<__bf16>(b)};
+  }
+  static __device__ __forceinline__ float AddPair(x2 pair, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(pair, x2{static_cast<__bf16>(1.0F), static_cast<__bf16>(1.0F)}, sum, false);
   }
   static __device__ __forceinline__ floatx4 Mfma16(x8 a, x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -68,174 +82,448 @@ __device__ __forceinline__ typename Types<T>::x8 Operand(unsigned lo, unsigned h
   return typename X::x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// max over the lanes l, l ^ 16, l ^ 32, l ^ 48, and their sum: two swaps of
+// rows between registers instead of trips through LDS.
+__device__ __forceinline__ float Partner32(float v, float* other) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  *other = __uint_as_float(r[1]);
+  return __uint_as_float(r[0]);
+}
+__device__ __forceinline__ float Partner16(float v, float* other) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  *other = __uint_as_float(r[1]);
+  return __uint_as_float(r[0]);
+}
+__device__ __forceinline__ float Max32(float v) {
+  float b;
+  const float a = Partner32(v, &b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float Sum32(float v) {
+  float b;
+  const float a = Partner32(v, &b);
+  return a + b;
+}
+__device__ __forceinline__ float Max16(float v) {
+  float b;
+  const float a = Partner16(v, &b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float Sum16(float v) {
+  float b;
+  const float a = Partner16(v, &b);
+  return a + b;
+}
+
+__device__ __forceinline__ float Lane(float v, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+
+// The values' loudness: the scale that the sums are held at, a power of two
+// that only grows. A block's codes are multiplied by its own scale over this one
+// as they are converted, at most 1, so that no fp16 operand overflows however
+// loud a block is; a block quieter than the loudest by 2^15 or more loses the
+// bits under fp16's 2^-24, 2^-33 of that loudest block's largest value.
+constexpr float kQuietest = 7.52316385e-37F;  // 2^-120
+__device__ __forceinline__ float InversePower(float p) {
+  return __uint_as_float((254u << 23) - __float_as_uint(p));
+}
+// 0 for a block without a (numeric) scale.
+__device__ __forceinline__ float Loudness(float scale) { return scale == scale ? scale : 0.0F; }
+
+// How far a row's maximum may rise before its sums are scaled again: their
+// probabilities are then at most 2^8, far inside fp16, and most steps of a long
+// row leave the sums alone.
+constexpr float kSlack = 8.0F;
+
 constexpr int kFewWaves = 4;
-constexpr int kFewRows = 16;
 
-// A work-group takes 16 rows of one sequence and kv head; its waves take the
-// steps of 32 keys in turn, each with a softmax of its own that runs along
-// (maximum m, sum l, output o), and the four are joined in LDS at the end.
-template <typename T, int DIM>
+// A wave's window of the block table: lane i holds the page and scales of the
+// i-th block, so that the steps wait for the table once per 64 blocks and not
+// one after the other.
+struct Window {
+  int page;
+  float k_scale, v_scale;
+  __device__ __forceinline__ void Load(const CacheView& c, int sequence, int head, int first,
+                                       int stop, int lane) {
+    const int block = first + lane;
+    page = (block << c.block_shift) < stop ? PageOf(c, sequence, block) : -1;
+    const std::size_t at = ScaleIndex(c, max(page, 0), head, 0);
+    k_scale = c.scales[at];
+    v_scale = c.scales[at + 1];
+    if (page < 0)
+      k_scale = v_scale = 0.0F;
+  }
+};
+
+// Few rows: a work-group takes 16 NT rows of one sequence and kv head and one
+// split of its keys; each of its four waves takes a quarter of them in steps of
+// 32, with a softmax of its own that runs along (maximum m, sum l, output o), and
+// the four are joined in LDS at the end. The codes go from memory straight into
+// registers, a step ahead, and are converted there: with few rows nothing is
+// gained by sharing them, and what bounds the kernel is the stream of codes.
+template <typename T, int DIM, int NT>
 __global__ __launch_bounds__(kFewWaves* kWave) void FewRowsKernel(CacheAttentionParams p) {
-  typedef typename Types<T>::x8 x8;
-  constexpr int kSteps = DIM / 64;   // 16-byte loads of a key's codes in a lane
+  typedef Types<T> X;
+  typedef typename X::x8 x8;
+  constexpr int kSteps = DIM / 64;  // 16-byte loads of a key's codes in a lane
   constexpr int kTiles = DIM / 16;
+  constexpr int kRows = 16 * NT;
   const CacheView& c = p.cache;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15, quad = lane >> 4;
-  const int head = blockIdx.y;
+  const int head = blockIdx.x;
 
-  int tile = blockIdx.x;
-  const int sequence = SequenceOfItem(c, p.group, 4, 1, &tile);
+  int tile = blockIdx.y;
+  const int sequence =
+      __builtin_amdgcn_readfirstlane(SequenceOfItem(c, p.group, NT == 1 ? 4 : 5, 1, &tile));
+  tile = __builtin_amdgcn_readfirstlane(tile);
   const Span span = SpanOf(c, sequence);
   const int rows = span.count * p.group;
-  if (tile * kFewRows >= rows)
+  if (tile < 0 || tile * kRows >= rows)
     return;
-  const int row = tile * kFewRows + column;
-  const int query = min(row, rows - 1) / p.group;
-  const int of_group = min(row, rows - 1) - query * p.group;
-  const int capacity = c.table_width << c.block_shift;
-  const int length = min(span.length, capacity);
-  // Keys that this row sees, and that any row of the tile sees.
-  const int seen =
-      row >= rows ? 0 : p.causal ? min(span.start + query + 1, length) : length;
-  const int last = min(tile * kFewRows + kFewRows, rows) - 1;
+  const int length = min(span.length, c.table_width << c.block_shift);
+  // Keys that any row of the tile sees, and those of this split.
+  const int last = min(tile * kRows + kRows, rows) - 1;
   const int end = p.causal ? min(span.start + last / p.group + 1, length) : length;
+  const int chunk = ChunkOf(length, p.splits);
+  const int begin = blockIdx.z * chunk;
+  const int stop = min(begin + chunk, end);
 
-  x8 q[kSteps][2];
-  {
+  int query[NT], of_group[NT], seen[NT];
+  x8 q[NT][kSteps][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = tile * kRows + 16 * n + column;
+    query[n] = min(row, rows - 1) / p.group;
+    of_group[n] = min(row, rows - 1) - query[n] * p.group;
+    seen[n] = row >= rows ? 0 : p.causal ? min(span.start + query[n] + 1, length) : length;
     const T* from = static_cast<const T*>(p.q) +
-                    static_cast<std::int64_t>(span.first + query) * p.q_stride +
-                    static_cast<std::int64_t>(head * p.group + of_group) * DIM + 16 * quad;
+                    static_cast<std::int64_t>(span.first + query[n]) * p.q_stride +
+                    static_cast<std::int64_t>(head * p.group + of_group[n]) * DIM + 16 * quad;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      __builtin_memcpy(&q[i][0], from + 64 * i, sizeof(x8));
-      __builtin_memcpy(&q[i][1], from + 64 * i + 8, sizeof(x8));
+      __builtin_memcpy(&q[n][i][0], from + 64 * i, sizeof(x8));
+      __builtin_memcpy(&q[n][i][1], from + 64 * i + 8, sizeof(x8));
     }
   }
 
-  float m = -__builtin_inff(), l = 0.0F;
-  floatx4 o[kTiles] = {};
-  for (int base = wave * 32; base < end; base += kFewWaves * 32) {
-    float s[2][4];
-    u32x4 v[2][kSteps];
-    float level[2];
-    float peak = -__builtin_inff();
+  float m[NT], l[NT];
+  floatx4 o[NT][kTiles];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int key = base + 16 * g;
-      const int page = PageOf(c, sequence, key >> c.block_shift);
-      const int at = max(page, 0);
-      const std::size_t skip = static_cast<std::size_t>(key & ((1 << c.block_shift) - 1)) * DIM;
-      const u32x4* kc = reinterpret_cast<const u32x4*>(HalfOf(c, at, head, 0) + skip);
-      const u32x4* vc = reinterpret_cast<const u32x4*>(HalfOf(c, at, head, 1) + skip);
-      const float k_scale = c.scales[ScaleIndex(c, at, head, 0)];
-      const float v_scale = c.scales[ScaleIndex(c, at, head, 1)];
-      floatx4 acc = {};
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const u32x4 w = kc[i * 64 + lane];
-        v[g][i] = vc[i * 64 + lane];
-        acc = Types<T>::Mfma16(Operand<T>(w[0], w[1], 1.0F), q[i][0], acc);
-        acc = Types<T>::Mfma16(Operand<T>(w[2], w[3], 1.0F), q[i][1], acc);
-      }
-      // A NaN scale, of keys or values, makes the block's scores NaN.
-      const float factor = p.scale_log2 * k_scale + 0.0F * v_scale;
-      level[g] = v_scale == v_scale ? v_scale : 0.0F;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool visible = page >= 0 && key + 4 * quad + r < seen;
-        s[g][r] = visible ? acc[r] * factor : -__builtin_inff();
-        peak = fmaxf(peak, s[g][r]);
-      }
-    }
-    peak = fmaxf(peak, __shfl_xor(peak, 16));
-    peak = fmaxf(peak, __shfl_xor(peak, 32));
-    const float top = fmaxf(m, peak);
-    const float from = top == -__builtin_inff() ? 0.0F : top;
-    const float shrink = __builtin_amdgcn_exp2f(m - from);
-    m = top;
-    l *= shrink;
+  for (int n = 0; n < NT; ++n) {
+    m[n] = -__builtin_inff();
+    l[n] = 0.0F;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
-      o[t] *= shrink;
-    x8 w;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const T rounded = static_cast<T>(__builtin_amdgcn_exp2f(s[g][r] - from));
-        w[4 * g + r] = rounded;
-        l += static_cast<float>(rounded);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      // The values' scales differ by block: each group's product apart.
+      o[n][t] = floatx4{0.0F, 0.0F, 0.0F, 0.0F};
+  }
+  float loud = kQuietest;
+
+  const int quarter = ((stop - begin + kFewWaves * 32 - 1) / (kFewWaves * 32)) * 32;
+  const int wave_begin = begin + wave * quarter;
+  const int wave_stop = min(wave_begin + quarter, stop);
+  const int in_block = (1 << c.block_shift) - 1;
+  const std::size_t half_bytes = static_cast<std::size_t>(DIM) << c.block_shift;
+
+  for (int window = wave_begin; window < wave_stop;) {
+    Window w;
+    const int first_block = window >> c.block_shift;
+    w.Load(c, sequence, head, first_block, wave_stop, lane);
+    const int window_stop = min((first_block + kWave) << c.block_shift, wave_stop);
+
+    struct Codes {
+      u32x4 k[2][kSteps], v[2][kSteps];
+    };
+    const auto load = [&](int key, Codes* d) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        x8 half = {};
+        const int at = min(key, window_stop - 1) + 16 * g;
+        const int block = min((at >> c.block_shift) - first_block, kWave - 1);
+        const int page = max(__builtin_amdgcn_readlane(w.page, block), 0);
+        const unsigned char* from =
+            c.data + (static_cast<std::size_t>(page) * c.kv_heads + head) * 2 * half_bytes +
+            static_cast<std::size_t>(at & in_block & ~15) * DIM;
+        const u32x4* kc = reinterpret_cast<const u32x4*>(from);
+        const u32x4* vc = reinterpret_cast<const u32x4*>(from + half_bytes);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          d->k[g][i] = kc[i * 64 + lane];
+          d->v[g][i] = vc[i * 64 + lane];
+        }
+      }
+    };
+    const auto step = [&](int key, const Codes& d) {
+      float factor[2], level[2];
+      bool there[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int block = ((key + 16 * g) >> c.block_shift) - first_block;
+        const float v_scale = Lane(w.v_scale, block);
+        // A NaN scale, of keys or values, makes the block's scores NaN.
+        factor[g] = p.scale_log2 * Lane(w.k_scale, block) + 0.0F * v_scale;
+        level[g] = Loudness(v_scale);
+        there[g] = __builtin_amdgcn_readlane(w.page, block) >= 0;
+      }
+      const float louder = fmaxf(loud, fmaxf(level[0], level[1]));
+      if (louder > loud) {
+        const float shrink = loud * InversePower(louder);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            o[n][t] *= shrink;
+        loud = louder;
+      }
+      const float unit = InversePower(loud);
+      x8 weights[NT];
+      floatx4 acc[NT][2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          acc[n][g] = floatx4{0.0F, 0.0F, 0.0F, 0.0F};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const x8 a = Operand<T>(d.k[g][i][0], d.k[g][i][1], 1.0F);
+          const x8 b = Operand<T>(d.k[g][i][2], d.k[g][i][3], 1.0F);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            acc[n][g] = X::Mfma16(a, q[n][i][0], acc[n][g]);
+            acc[n][g] = X::Mfma16(b, q[n][i][1], acc[n][g]);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float s[2][4];
+        float peak = -__builtin_inff();
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool visible = there[g] && key + 16 * g + 4 * quad + r < seen[n];
+            s[g][r] = visible ? acc[n][g][r] * factor[g] : -__builtin_inff();
+            peak = fmaxf(peak, s[g][r]);
+          }
+        peak = Max32(Max16(peak));
+        if (__any(peak > m[n] + kSlack)) {
+          const float top = fmaxf(m[n], peak);
+          const float shrink =
+              top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m[n] - top);
+          m[n] = top;
+          l[n] *= shrink;
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            o[n][t] *= shrink;
+        }
+        const float from = m[n] == -__builtin_inff() ? 0.0F : m[n];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; r += 2) {
+            const typename X::x2 pair = X::Round(__builtin_amdgcn_exp2f(s[g][r] - from),
+                                                 __builtin_amdgcn_exp2f(s[g][r + 1] - from));
+            weights[n][4 * g + r] = pair[0];
+            weights[n][4 * g + r + 1] = pair[1];
+            l[n] = X::AddPair(pair, l[n]);
+          }
+      }
+      const float v0 = fmaxf(level[0] * unit, kQuietest), v1 = fmaxf(level[1] * unit, kQuietest);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const unsigned lo = d.v[0][t / 4][t % 4], hi = d.v[1][t / 4][t % 4];
+        const typename X::x2 a = X::Low(lo, v0), b = X::High(lo, v0);
+        const typename X::x2 e = X::Low(hi, v1), f = X::High(hi, v1);
+        const x8 operand{a[0], a[1], b[0], b[1], e[0], e[1], f[0], f[1]};
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          o[n][t] = X::Mfma16(operand, weights[n], o[n][t]);
+      }
+    };
+
+    Codes even, odd;
+    load(window, &even);
+    for (int key = window; key < window_stop; key += 64) {
+      load(key + 32, &odd);
+      step(key, even);
+      if (key + 32 < window_stop) {
+        load(key + 64, &even);
+        step(key + 32, odd);
+      }
+    }
+    window = window_stop;
+  }
+
+  __shared__ float shared_m[kFewWaves][kRows], shared_l[kFewWaves][kRows];
+  __shared__ floatx4 shared_o[kFewWaves][NT * kTiles][64];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    l[n] = Sum32(Sum16(l[n]));
+    if (quad == 0) {
+      shared_m[wave][16 * n + column] = m[n];
+      shared_l[wave][16 * n + column] = l[n];
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+      shared_o[wave][n * kTiles + t][lane] = o[n][t] * loud;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int in_tile = 16 * n + column;
+    const int row = tile * kRows + in_tile;
+    float top = -__builtin_inff(), total = 0.0F;
+    float weight[kFewWaves];
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w)
+      top = fmaxf(top, shared_m[w][in_tile]);
+    const float from = top == -__builtin_inff() ? 0.0F : top;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+      weight[w] = __builtin_amdgcn_exp2f(shared_m[w][in_tile] - from);
+      total += shared_l[w][in_tile] * weight[w];
+    }
+    if (row >= rows)
+      continue;
+    const std::size_t slot =
+        p.splits == 1
+            ? 0
+            : ((static_cast<std::size_t>(blockIdx.y) * c.kv_heads + head) * p.splits +
+               blockIdx.z) * kRows + in_tile;
+    if (p.splits > 1 && wave == 0 && quad == 0) {
+      p.partial_m[2 * slot] = top;
+      p.partial_m[2 * slot + 1] = total;
+    }
+    // Nothing seen: zero.
+    const float scale = total == 0.0F ? 0.0F : 1.0F / total;
+    T* to = static_cast<T*>(p.out) +
+            static_cast<std::int64_t>(span.first + query[n]) * p.out_stride +
+            static_cast<std::int64_t>(head * p.group + of_group[n]) * DIM + 4 * quad;
+    for (int t = wave; t < kTiles; t += kFewWaves) {
+      floatx4 sum = {};
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w)
+        sum += shared_o[w][n * kTiles + t][lane] * weight[w];
+      if (p.splits > 1) {
+        *reinterpret_cast<floatx4*>(p.partial_o + slot * DIM + 16 * t + 4 * quad) = sum;
+      } else {
+        T rounded[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          half[4 * g + r] = w[4 * g + r];
-        const floatx4 zero = {};
-        const floatx4 d = Types<T>::Mfma16(
-            Operand<T>(v[0][t / 4][t % 4], v[1][t / 4][t % 4], 1.0F), half, zero);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          o[t][r] = __builtin_fmaf(d[r], level[g], o[t][r]);
+          rounded[r] = static_cast<T>(sum[r] * scale);
+        __builtin_memcpy(to + 16 * t, rounded, sizeof(rounded));
       }
     }
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
+}
 
-  __shared__ float shared_m[kFewWaves][kFewRows], shared_l[kFewWaves][kFewRows];
-  __shared__ floatx4 shared_o[kFewWaves][kTiles][64];
-  if (quad == 0) {
-    shared_m[wave][column] = m;
-    shared_l[wave][column] = l;
-  }
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t)
-    shared_o[wave][t][lane] = o[t];
-  __syncthreads();
-  float top = -__builtin_inff(), total = 0.0F;
-#pragma unroll
-  for (int w = 0; w < kFewWaves; ++w)
-    top = fmaxf(top, shared_m[w][column]);
-  const float from = top == -__builtin_inff() ? 0.0F : top;
-  float weight[kFewWaves];
-#pragma unroll
-  for (int w = 0; w < kFewWaves; ++w) {
-    weight[w] = __builtin_amdgcn_exp2f(shared_m[w][column] - from);
-    total += shared_l[w][column] * weight[w];
-  }
-  // Nothing seen: zero.
-  const float scale = total == 0.0F ? 0.0F : 1.0F / total;
-  if (row >= rows)
+// Joins the splits of one row: DIM / 4 lanes hold four of its dims each, and the
+// work-group's 256 / (DIM / 4) such groups take its splits in turn.
+template <typename T, int DIM>
+__global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
+  constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
+  const CacheView& c = p.cache;
+  int tile = blockIdx.y;
+  const int sequence = SequenceOfItem(c, p.group, p.tile_shift, 1, &tile);
+  const Span span = SpanOf(c, sequence);
+  const int rows = span.count * p.group;
+  const int in_tile = blockIdx.z;
+  const int row = (tile << p.tile_shift) + in_tile;
+  if (tile < 0 || row >= rows)
     return;
-  T* to = static_cast<T*>(p.out) + static_cast<std::int64_t>(span.first + query) * p.out_stride +
-          static_cast<std::int64_t>(head * p.group + of_group) * DIM + 4 * quad;
-  for (int t = wave; t < kTiles; t += kFewWaves) {
-    floatx4 sum = {};
-#pragma unroll
-    for (int w = 0; w < kFewWaves; ++w)
-      sum += shared_o[w][t][lane] * weight[w];
-    T rounded[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      rounded[r] = static_cast<T>(sum[r] * scale);
-    __builtin_memcpy(to + 16 * t, rounded, sizeof(rounded));
+  const int head = blockIdx.x;
+  const int tid = threadIdx.x, group = tid / kLanes, part = tid % kLanes;
+  const std::size_t first =
+      (((static_cast<std::size_t>(blockIdx.y) * c.kv_heads + head) * p.splits) << p.tile_shift) +
+      in_tile;
+  __shared__ float weights[kMostSplits];
+  __shared__ float wave_top[4];
+  __shared__ float totals[4];
+  __shared__ floatx4 sums[kGroups][kLanes];
+  float m = -__builtin_inff(), l = 0.0F;
+  if (tid < p.splits) {
+    const std::size_t slot = first + (static_cast<std::size_t>(tid) << p.tile_shift);
+    m = p.partial_m[2 * slot];
+    l = p.partial_m[2 * slot + 1];
   }
+  float top = WaveMax(m);
+  if ((tid & 63) == 0)
+    wave_top[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+  const float from = top == -__builtin_inff() ? 0.0F : top;
+  const float weight = __builtin_amdgcn_exp2f(m - from);
+  // A split that saw nothing has left no output: its weight says so.
+  if (tid < kMostSplits)
+    weights[tid] = l == 0.0F ? 0.0F : weight;
+  const float part_total = WaveSum(l * weight);
+  if ((tid & 63) == 0)
+    totals[tid >> 6] = part_total;
+  __syncthreads();
+  const float total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+  floatx4 sum = {};
+  for (int s = group; s < p.splits; s += kGroups) {
+    const float w = weights[s];
+    const std::size_t slot = first + (static_cast<std::size_t>(s) << p.tile_shift);
+    if (w != 0.0F)
+      sum += *reinterpret_cast<const floatx4*>(p.partial_o + slot * DIM + 4 * part) * w;
+  }
+  sums[group][part] = sum;
+  __syncthreads();
+  if (group != 0)
+    return;
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g)
+    sum += sums[g][part];
+  const float scale = total == 0.0F ? 0.0F : 1.0F / total;
+  const int query = row / p.group, of_group = row % p.group;
+  T rounded[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    rounded[r] = static_cast<T>(sum[r] * scale);
+  __builtin_memcpy(static_cast<T*>(p.out) +
+                       static_cast<std::int64_t>(span.first + query) * p.out_stride +
+                       static_cast<std::int64_t>(head * p.group + of_group) * DIM + 4 * part,
+                   rounded, sizeof(rounded));
 }
 
 template <typename T, int DIM>
 void Launch(const CacheAttentionParams& p, hipStream_t stream) {
-  const dim3 grid(ItemBound(p.cache, p.group, 4, 1), p.cache.kv_heads);
-  Dispatch(FewRowsKernel<T, DIM>, grid, dim3(kFewWaves * kWave), 0, stream, true, true, p);
+  const int items = ItemBound(p.cache, p.group, p.tile_shift, 1);
+  const dim3 grid(p.cache.kv_heads, items, p.splits), block(kFewWaves * kWave);
+  const bool last = p.splits == 1;
+  if (p.tile_shift == 4)
+    Dispatch(FewRowsKernel<T, DIM, 1>, grid, block, 0, stream, true, last, p);
+  else
+    Dispatch(FewRowsKernel<T, DIM, 2>, grid, block, 0, stream, true, last, p);
+  if (!last)
+    Dispatch(JoinKernel<T, DIM>, dim3(p.cache.kv_heads, items, 1 << p.tile_shift), dim3(256), 0,
+             stream, false, true, p);
 }
 
 }  // namespace
+
+CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group) {
+  CacheAttentionPlan plan;
+  if (c.rows == 0)
+    return plan;
+  // Rows of a sequence on average: 16 columns of the matrix operand where they
+  // suffice, else 32, which halve what is read of the codes again.
+  plan.tile_shift = static_cast<std::int64_t>(c.rows) * group <= 16ll * c.count ? 4 : 5;
+  const int items = ItemBound(c, group, plan.tile_shift, 1);
+  const std::int64_t groups = static_cast<std::int64_t>(items) * c.kv_heads;
+  const std::int64_t capacity = static_cast<std::int64_t>(c.table_width) << c.block_shift;
+  const std::int64_t wanted = (kSplitGroups + groups - 1) / groups;
+  plan.splits = static_cast<int>(std::max<std::int64_t>(
+      1, std::min({wanted, capacity / kLeastChunk, std::int64_t{kMostSplits}})));
+  if (plan.splits > 1)
+    plan.slots = (static_cast<std::size_t>(groups) * plan.splits) << plan.tile_shift;
+  return plan;
+}
 
 void LaunchCacheAttention(const CacheAttentionParams& p, DType type, hipStream_t stream) {
   if (p.cache.rows == 0)

@@ -105,6 +105,11 @@ ovg::DType TypeOf(int type, bool with_f32) {
   return static_cast<ovg::DType>(type);
 }
 
+// The splits' outputs, then their maxima and sums.
+int64_t AttentionBytes(const ovg::CacheView& c, const ovg::CacheAttentionPlan& plan) {
+  return static_cast<int64_t>(plan.slots) * (c.dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
 void RequireStride(int64_t stride, int64_t width) {
   ovg::Require(stride >= width && stride <= (int64_t{1} << 40), "row stride below the row's width");
 }
@@ -396,10 +401,15 @@ int ovg_op_cache_read(const ovg_kv_cache* cache, const ovg_kv_sequences* sequenc
 
 int64_t ovg_op_cache_attention_workspace(const ovg_kv_cache* cache,
                                          const ovg_kv_sequences* sequences, int64_t heads) {
-  (void)cache;
-  (void)sequences;
-  (void)heads;
-  return 0;
+  try {
+    const ovg::CacheView c = ViewOf(cache, sequences);
+    if (heads < cache->kv_heads || heads / cache->kv_heads > 64)
+      return -1;
+    return AttentionBytes(
+        c, ovg::PlanCacheAttention(c, static_cast<int>(heads / cache->kv_heads)));
+  } catch (const std::exception&) {
+    return -1;  // as the call itself will say
+  }
 }
 
 int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
@@ -422,13 +432,19 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
     ovg::Require(q && out, "null pointer");
     auto s = static_cast<hipStream_t>(stream);
     RequireCurrentDevice(s);
-    (void)workspace;
-    (void)workspace_bytes;
+    p.group = static_cast<int>(heads / cache->kv_heads);
+    const ovg::CacheAttentionPlan plan = ovg::PlanCacheAttention(p.cache, p.group);
+    const int64_t bytes = AttentionBytes(p.cache, plan);
+    ovg::Require(bytes == 0 || (workspace && workspace_bytes >= bytes && Aligned16(workspace)),
+                 "workspace of " + std::to_string(bytes) + " bytes needed, 16-byte aligned");
+    p.tile_shift = plan.tile_shift;
+    p.splits = plan.splits;
+    p.partial_o = static_cast<float*>(workspace);
+    p.partial_m = p.partial_o + plan.slots * p.cache.dim;
     p.q = q;
     p.out = out;
     p.q_stride = q_stride;
     p.out_stride = out_stride;
-    p.group = static_cast<int>(heads / cache->kv_heads);
     p.causal = causal != 0;
     p.scale_log2 = scale * 1.44269504088896341F;
     ovg::LaunchCacheAttention(p, t, s);
