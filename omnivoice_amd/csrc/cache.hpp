@@ -128,6 +128,8 @@ struct CacheAttentionPlan {
   std::size_t slots = 0;  // of the workspace
 };
 constexpr int kMostSplits = 256;
+constexpr int kFewSplits = 8;       // that one group of lanes joins by itself
+constexpr int kManyGroups = 512;    // the same for many rows: two a CU
 constexpr int kLeastChunk = 256;    // keys of a split at least
 constexpr int kSplitGroups = 2048;  // work-groups that a split call is to have
 CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group);

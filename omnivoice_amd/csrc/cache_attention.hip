@@ -50,6 +50,9 @@ struct Types<_Float16> {
   static __device__ __forceinline__ floatx4 Mfma16(x8 a, x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ floatx16 Mfma32(x8 a, x8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
 };
 template <>
 struct Types<__bf16> {
@@ -70,6 +73,9 @@ struct Types<__bf16> {
   }
   static __device__ __forceinline__ floatx4 Mfma16(x8 a, x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ floatx16 Mfma32(x8 a, x8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
 
@@ -135,7 +141,8 @@ __device__ __forceinline__ float Loudness(float scale) { return scale == scale ?
 
 // How far a row's maximum may rise before its sums are scaled again: their
 // probabilities are then at most 2^8, far inside fp16, and most steps of a long
-// row leave the sums alone.
+// row leave the sums alone. Each row goes by its own maximum: what the others
+// hold changes none of its bits.
 constexpr float kSlack = 8.0F;
 
 constexpr int kFewWaves = 4;
@@ -311,7 +318,7 @@ __global__ __launch_bounds__(kFewWaves* kWave) void FewRowsKernel(CacheAttention
           }
         peak = Max32(Max16(peak));
         if (__any(peak > m[n] + kSlack)) {
-          const float top = fmaxf(m[n], peak);
+          const float top = peak > m[n] + kSlack ? peak : m[n];
           const float shrink =
               top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m[n] - top);
           m[n] = top;
@@ -421,6 +428,306 @@ __global__ __launch_bounds__(kFewWaves* kWave) void FewRowsKernel(CacheAttention
   }
 }
 
+constexpr int kManyWaves = 4;
+constexpr int kManyRows = 32 * kManyWaves;
+
+// What a tile's groups of 16 keys need beside their codes.
+template <int GROUPS>
+struct TileScales {
+  typedef float vec __attribute__((ext_vector_type(GROUPS)));
+  vec factor;      // scores to the exponent of two
+  float loud;      // of the values as they are converted: this tile's and all before
+  unsigned there;  // a bit for each group that has a block
+};
+
+// Many rows: a work-group of four waves takes 128 rows of one sequence and kv
+// head, 32 a wave, and goes over the keys in tiles of 64 (128 at 64 dims) that
+// the waves share. The threads fetch a tile's codes while the one before is
+// worked on, convert them once and leave them in LDS in the order of the
+// operands of v_mfma_f32_32x32x16 (64 lanes of 16 bytes in a row, so every
+// write and read is a conflict-free 16 bytes a lane), in one of two buffers of
+// 32 KB: one barrier a tile. The softmax runs in registers, a row in a lane and
+// its partner lane ^ 32.
+template <typename T, int DIM>
+__global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAttentionParams p) {
+  typedef Types<T> X;
+  typedef typename X::x8 x8;
+  constexpr int kKeys = 8192 / DIM;          // of a tile
+  constexpr int kGroups = kKeys / 16, kBlocks = kKeys / 32;
+  constexpr int kK = DIM / 16;               // contraction steps of the scores
+  constexpr int kDims = DIM / 32;            // blocks of 32 dims
+  constexpr int kChunks = DIM;               // 16-byte chunks of a group's keys or values
+  __shared__ x8 key_tiles[2][kKeys * DIM / 8];
+  __shared__ x8 value_tiles[2][kKeys * DIM / 8];
+  const CacheView& c = p.cache;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int column = lane & 31, half = lane >> 5;
+  const int head = blockIdx.x;
+
+  // The last rows of a causal sequence see the most keys: they start first.
+  const int item = gridDim.y - 1 - blockIdx.y;
+  int tile = item;
+  const int sequence = __builtin_amdgcn_readfirstlane(SequenceOfItem(c, p.group, 7, 1, &tile));
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  const Span span = SpanOf(c, sequence);
+  const int rows = span.count * p.group;
+  if (tile < 0 || tile * kManyRows >= rows)
+    return;
+  const int length = min(span.length, c.table_width << c.block_shift);
+  const int last = min(tile * kManyRows + kManyRows, rows) - 1;
+  const int end = p.causal ? min(span.start + last / p.group + 1, length) : length;
+  const int chunk = ChunkOf(length, p.splits);
+  const int begin = blockIdx.z * chunk;
+  const int stop = min(begin + chunk, end);
+
+  const int first_row = tile * kManyRows + 32 * wave;
+  const int row = first_row + column;
+  const int query = min(row, rows - 1) / p.group;
+  const int of_group = min(row, rows - 1) - query * p.group;
+  const int seen = row >= rows ? 0 : p.causal ? min(span.start + query + 1, length) : length;
+  // Keys that every row of the wave sees, and that any does.
+  const int all_see = first_row + 31 >= rows ? 0
+                      : p.causal             ? min(span.start + first_row / p.group + 1, length)
+                                             : length;
+  const int wave_end =
+      first_row >= rows ? 0
+      : p.causal ? min(span.start + min(first_row + 31, rows - 1) / p.group + 1, length)
+                 : length;
+
+  x8 q[kK];
+  {
+    const T* from = static_cast<const T*>(p.q) +
+                    static_cast<std::int64_t>(span.first + query) * p.q_stride +
+                    static_cast<std::int64_t>(head * p.group + of_group) * DIM + 8 * half;
+#pragma unroll
+    for (int i = 0; i < kK; ++i)
+      __builtin_memcpy(&q[i], from + 16 * i, sizeof(x8));
+  }
+
+  float m = -__builtin_inff(), l = 0.0F;
+  floatx16 o[kDims];
+#pragma unroll
+  for (int t = 0; t < kDims; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      o[t][r] = 0.0F;
+  float loud = kQuietest;
+
+  const int in_block = (1 << c.block_shift) - 1;
+  const std::size_t half_bytes = static_cast<std::size_t>(DIM) << c.block_shift;
+  Window window;
+  int window_first = 0, window_stop = begin;  // block, key
+
+  // A thread's chunks of a tile: two of keys (chunk tid + 256 i: group, dims / 16,
+  // token) and a pair of values (group, dims / 64, quad and quad + 2, dim % 16), whose
+  // eight tokens make one lane's operand.
+  const int value_group = tid / (DIM / 2), value_at = tid % (DIM / 2);
+  const int value_chunk = (value_at >> 5) * 64 + (value_at & 31);
+  u32x4 k_codes[2], v_codes[2];
+  float v_level = 0.0F;
+  const auto block_of = [&](int key) {
+    return min((key >> c.block_shift) - window_first, kWave - 1);
+  };
+  const auto fetch = [&](int key) {
+    if (key >= window_stop) {  // never in the middle of a tile: 64 blocks are whole ones
+      window_first = key >> c.block_shift;
+      window.Load(c, sequence, head, window_first, stop, lane);
+      window_stop = (window_first + kWave) << c.block_shift;
+    }
+    const auto base = [&](int group) {
+      const int at = key + 16 * group;
+      const int page = max(__builtin_amdgcn_readlane(window.page, block_of(at)), 0);
+      return c.data + (static_cast<std::size_t>(page) * c.kv_heads + head) * 2 * half_bytes +
+             static_cast<std::size_t>(at & in_block & ~15) * DIM;
+    };
+    if constexpr (DIM == 128) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        k_codes[i] = reinterpret_cast<const u32x4*>(
+            base(2 * i + (wave >> 1)))[(wave & 1) * 64 + lane];
+      const u32x4* from = reinterpret_cast<const u32x4*>(base(wave) + half_bytes);
+      v_codes[0] = from[value_chunk];
+      v_codes[1] = from[value_chunk + 32];
+      v_level = Lane(window.v_scale, block_of(key + 16 * wave));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        k_codes[i] = reinterpret_cast<const u32x4*>(base(4 * i + wave))[lane];
+      const unsigned char* low = base(2 * wave);
+      const unsigned char* high = base(2 * wave + 1);
+      const u32x4* from =
+          reinterpret_cast<const u32x4*>((half == 0 ? low : high) + half_bytes);
+      v_codes[0] = from[value_chunk];
+      v_codes[1] = from[value_chunk + 32];
+      const float even = Lane(window.v_scale, block_of(key + 32 * wave));
+      const float odd = Lane(window.v_scale, block_of(key + 32 * wave + 16));
+      v_level = half == 0 ? even : odd;
+    }
+  };
+  // The tile's scales, while its window is the current one.
+  const auto scales_of = [&](int key, float before) {
+    TileScales<kGroups> s;
+    s.loud = before;
+    s.there = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int block = block_of(key + 16 * g);
+      const float v_scale = Lane(window.v_scale, block);
+      // A NaN scale, of keys or values, makes the block's scores NaN.
+      s.factor[g] = p.scale_log2 * Lane(window.k_scale, block) + 0.0F * v_scale;
+      s.there |= (__builtin_amdgcn_readlane(window.page, block) >= 0 ? 1u : 0u) << g;
+      s.loud = fmaxf(s.loud, Loudness(v_scale));
+    }
+    return s;
+  };
+  const auto convert = [&](const TileScales<kGroups>& s, int buffer) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int index = tid + i * 256;
+      const int group = index / kChunks, at = index % kChunks;
+      x8* to = key_tiles[buffer] + ((group >> 1) * kK + (at >> 4)) * 64 + (group & 1) * 16 +
+               (at & 15);
+      to[0] = Operand<T>(k_codes[i][0], k_codes[i][1], 1.0F);
+      to[32] = Operand<T>(k_codes[i][2], k_codes[i][3], 1.0F);
+    }
+    const float level = fmaxf(Loudness(v_level) * InversePower(s.loud), kQuietest);
+    const int d = value_at & 15, h = (value_at >> 4) & 1, quarter = value_at >> 5;
+    x8* to = value_tiles[buffer] + (value_group * kDims + 2 * quarter) * 64 + 32 * h + d;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      to[(t >> 1) * 64 + (t & 1) * 16] = Operand<T>(v_codes[0][t], v_codes[1][t], level);
+  };
+
+  const auto work = [&](int key, const TileScales<kGroups>& s, int buffer) {
+    if (s.loud > loud) {
+      const float shrink = loud * InversePower(s.loud);
+#pragma unroll
+      for (int t = 0; t < kDims; ++t)
+        o[t] *= shrink;
+      loud = s.loud;
+    }
+    if (key >= wave_end)
+      return;
+    floatx16 acc[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        acc[b][r] = 0.0F;
+#pragma unroll
+      for (int i = 0; i < kK; ++i)
+        acc[b] = X::Mfma32(key_tiles[buffer][(b * kK + i) * 64 + lane], q[i], acc[b]);
+    }
+    float peak = -__builtin_inff();
+    if (s.there == (1u << kGroups) - 1 && key + kKeys <= all_see) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          acc[b][r] *= s.factor[2 * b + r / 8];
+          peak = fmaxf(peak, acc[b][r]);
+        }
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = key + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+          acc[b][r] = (s.there >> (2 * b + r / 8) & 1) != 0 && at < seen ? acc[b][r] * s.factor[2 * b + r / 8]
+                                                          : -__builtin_inff();
+          peak = fmaxf(peak, acc[b][r]);
+        }
+    }
+    peak = Max32(peak);
+    if (__any(peak > m + kSlack)) {
+      const float top = peak > m + kSlack ? peak : m;
+      const float shrink = top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= shrink;
+#pragma unroll
+      for (int t = 0; t < kDims; ++t)
+        o[t] *= shrink;
+    }
+    const float from = m == -__builtin_inff() ? 0.0F : m;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      x8 weights;
+#pragma unroll
+      for (int r = 0; r < 8; r += 2) {
+        const typename X::x2 pair =
+            X::Round(__builtin_amdgcn_exp2f(acc[g / 2][8 * (g & 1) + r] - from),
+                     __builtin_amdgcn_exp2f(acc[g / 2][8 * (g & 1) + r + 1] - from));
+        weights[r] = pair[0];
+        weights[r + 1] = pair[1];
+        l = X::AddPair(pair, l);
+      }
+#pragma unroll
+      for (int t = 0; t < kDims; ++t)
+        o[t] = X::Mfma32(value_tiles[buffer][(g * kDims + t) * 64 + lane], weights, o[t]);
+    }
+  };
+
+  if (begin < stop) {
+    fetch(begin);
+    TileScales<kGroups> now = scales_of(begin, loud), next = now;
+    convert(now, 0);
+    if (begin + kKeys < stop)
+      fetch(begin + kKeys);
+    next = scales_of(begin + kKeys, now.loud);
+    __syncthreads();
+    int buffer = 0;
+    for (int key = begin; key < stop; key += kKeys) {
+      const TileScales<kGroups> coming = next;
+      if (key + kKeys < stop)
+        convert(coming, buffer ^ 1);
+      if (key + 2 * kKeys < stop)
+        fetch(key + 2 * kKeys);
+      next = scales_of(key + 2 * kKeys, coming.loud);
+      work(key, now, buffer);
+      now = coming;
+      buffer ^= 1;
+      __syncthreads();
+    }
+  }
+
+  l = Sum32(l);
+  if (row >= rows)
+    return;
+  if (p.splits > 1) {
+    const std::size_t slot =
+        ((static_cast<std::size_t>(item) * c.kv_heads + head) * p.splits + blockIdx.z) *
+            kManyRows + 32 * wave + column;
+    if (half == 0) {
+      p.partial_m[2 * slot] = m;
+      p.partial_m[2 * slot + 1] = l;
+    }
+#pragma unroll
+    for (int t = 0; t < kDims; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const floatx4 part = {o[t][r] * loud, o[t][r + 1] * loud, o[t][r + 2] * loud,
+                              o[t][r + 3] * loud};
+        *reinterpret_cast<floatx4*>(p.partial_o + slot * DIM + 32 * t + 2 * r + 4 * half) = part;
+      }
+    return;
+  }
+  // Nothing seen: zero.
+  const float scale = l == 0.0F ? 0.0F : loud / l;
+  T* to = static_cast<T*>(p.out) + static_cast<std::int64_t>(span.first + query) * p.out_stride +
+          static_cast<std::int64_t>(head * p.group + of_group) * DIM + 4 * half;
+#pragma unroll
+  for (int t = 0; t < kDims; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      T rounded[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        rounded[e] = static_cast<T>(o[t][r + e] * scale);
+      __builtin_memcpy(to + 32 * t + 2 * r, rounded, sizeof(rounded));
+    }
+}
+
 // Joins the splits of one row: DIM / 4 lanes hold four of its dims each, and the
 // work-group's 256 / (DIM / 4) such groups take its splits in turn.
 template <typename T, int DIM>
@@ -491,6 +798,58 @@ __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
                    rounded, sizeof(rounded));
 }
 
+// Few splits: each group of DIM / 4 lanes joins a row of its own.
+template <typename T, int DIM>
+__global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
+  constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
+  const CacheView& c = p.cache;
+  int tile = blockIdx.y;
+  const int sequence = SequenceOfItem(c, p.group, p.tile_shift, 1, &tile);
+  const Span span = SpanOf(c, sequence);
+  const int rows = span.count * p.group;
+  const int tid = threadIdx.x, part = tid % kLanes;
+  const int in_tile = blockIdx.z * kGroups + tid / kLanes;
+  const int row = (tile << p.tile_shift) + in_tile;
+  if (tile < 0 || row >= rows)
+    return;
+  const int head = blockIdx.x;
+  const std::size_t first =
+      (((static_cast<std::size_t>(blockIdx.y) * c.kv_heads + head) * p.splits) << p.tile_shift) +
+      in_tile;
+  float m[kFewSplits], l[kFewSplits];
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const std::size_t slot =
+        first + (static_cast<std::size_t>(min(s, p.splits - 1)) << p.tile_shift);
+    m[s] = p.partial_m[2 * slot];
+    l[s] = s < p.splits ? p.partial_m[2 * slot + 1] : 0.0F;
+    top = fmaxf(top, m[s]);
+  }
+  const float from = top == -__builtin_inff() ? 0.0F : top;
+  float total = 0.0F;
+  floatx4 sum = {};
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    if (l[s] == 0.0F)  // a split that saw nothing, or none
+      continue;
+    const float w = __builtin_amdgcn_exp2f(m[s] - from);
+    const std::size_t slot = first + (static_cast<std::size_t>(s) << p.tile_shift);
+    total += l[s] * w;
+    sum += *reinterpret_cast<const floatx4*>(p.partial_o + slot * DIM + 4 * part) * w;
+  }
+  const float scale = total == 0.0F ? 0.0F : 1.0F / total;
+  const int query = row / p.group, of_group = row % p.group;
+  T rounded[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    rounded[r] = static_cast<T>(sum[r] * scale);
+  __builtin_memcpy(static_cast<T*>(p.out) +
+                       static_cast<std::int64_t>(span.first + query) * p.out_stride +
+                       static_cast<std::int64_t>(head * p.group + of_group) * DIM + 4 * part,
+                   rounded, sizeof(rounded));
+}
+
 template <typename T, int DIM>
 void Launch(const CacheAttentionParams& p, hipStream_t stream) {
   const int items = ItemBound(p.cache, p.group, p.tile_shift, 1);
@@ -498,9 +857,18 @@ void Launch(const CacheAttentionParams& p, hipStream_t stream) {
   const bool last = p.splits == 1;
   if (p.tile_shift == 4)
     Dispatch(FewRowsKernel<T, DIM, 1>, grid, block, 0, stream, true, last, p);
-  else
+  else if (p.tile_shift == 5)
     Dispatch(FewRowsKernel<T, DIM, 2>, grid, block, 0, stream, true, last, p);
-  if (!last)
+  else
+    Dispatch(ManyRowsKernel<T, DIM>, grid, block, 0, stream, true, last, p);
+  if (last)
+    return;
+  constexpr int kJoined = 256 / (DIM / 4);  // rows of a work-group with few splits
+  if (p.splits <= kFewSplits)
+    Dispatch(JoinFewKernel<T, DIM>,
+             dim3(p.cache.kv_heads, items, ((1 << p.tile_shift) + kJoined - 1) / kJoined),
+             dim3(256), 0, stream, false, true, p);
+  else
     Dispatch(JoinKernel<T, DIM>, dim3(p.cache.kv_heads, items, 1 << p.tile_shift), dim3(256), 0,
              stream, false, true, p);
 }
@@ -513,13 +881,15 @@ CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group) {
     return plan;
   // Rows of a sequence on average: 16 columns of the matrix operand where they
   // suffice, else 32, which halve what is read of the codes again.
-  plan.tile_shift = static_cast<std::int64_t>(c.rows) * group <= 16ll * c.count ? 4 : 5;
+  const std::int64_t all = static_cast<std::int64_t>(c.rows) * group;
+  plan.tile_shift = all <= 16ll * c.count ? 4 : all <= 48ll * c.count ? 5 : 7;
   const int items = ItemBound(c, group, plan.tile_shift, 1);
   const std::int64_t groups = static_cast<std::int64_t>(items) * c.kv_heads;
   const std::int64_t capacity = static_cast<std::int64_t>(c.table_width) << c.block_shift;
-  const std::int64_t wanted = (kSplitGroups + groups - 1) / groups;
+  const std::int64_t aim = plan.tile_shift == 7 ? kManyGroups : kSplitGroups;
+  const std::int64_t least = plan.tile_shift == 7 ? 2 * kLeastChunk : kLeastChunk;
   plan.splits = static_cast<int>(std::max<std::int64_t>(
-      1, std::min({wanted, capacity / kLeastChunk, std::int64_t{kMostSplits}})));
+      1, std::min({(aim + groups - 1) / groups, capacity / least, std::int64_t{kMostSplits}})));
   if (plan.splits > 1)
     plan.slots = (static_cast<std::size_t>(groups) * plan.splits) << plan.tile_shift;
   return plan;
