@@ -691,26 +691,41 @@ def _row_stride(t, name: str, heads: int, dim: int, device) -> int:
     return t.stride(0) if t.shape[0] > 1 else heads * dim
 
 
-def _launch(device, stream, call) -> None:
-    """call(stream handle) with the tensors' device current; without a stream,
-    on that device's current one."""
+def _raw_stream(index: int) -> int:
+    """The handle of a device's current stream."""
+    import torch
+    try:
+        return torch._C._cuda_getCurrentRawStream(index)  # without a Stream object: 2 us less
+    except AttributeError:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def _enqueue(fn, device, stream, *args) -> None:
+    """fn(*args, stream, ...) with the tensors' device current; without a
+    stream, on that device's current one."""
     import torch
     if device.type != "cuda":
         raise GeneratorError(f"needs tensors of a GPU, got {device}")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            call(torch.cuda.current_stream(device).cuda_stream if stream is None else stream)
+    index = device.index
+    if stream is None:
+        stream = _raw_stream(index)
+    err = _buf()
+    if index == torch.cuda.current_device():
+        status = fn(*args, stream, err, 1024)
     else:
-        call(torch.cuda.current_stream().cuda_stream if stream is None else stream)
+        with torch.cuda.device(index):
+            status = fn(*args, stream, err, 1024)
+    if status != OVG_OK:
+        _check(status, err)
 
 
 def _workspace(workspace, size: int, device, stream):
     """(pointer, bytes) of the caller's workspace, or of a new one that stays
     reserved until the work on `stream` is done. The caller holds what this
     returns until the launch."""
-    if size == 0 and workspace is None:
-        return None, 0, None
     if workspace is None:
+        if size <= 0:  # none needed, or arguments that the call will refuse
+            return None, 0, None
         import torch
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         if stream is not None:
@@ -721,30 +736,33 @@ def _workspace(workspace, size: int, device, stream):
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
-@dataclass
 class KVCache:
     """A pool of 8-bit keys and values (ovg_kv_cache): data uint8
     [blocks][kv_heads][2][block_tokens * head_dim], scales float32
     [blocks][kv_heads][2], device tensors that the caller owns."""
-    data: "torch.Tensor"  # noqa: F821
-    scales: "torch.Tensor"  # noqa: F821
-    block_tokens: int
-    head_dim: int
 
-    def __post_init__(self):
+    def __init__(self, data, scales, block_tokens: int, head_dim: int):
         import torch
-        if self.data.dim() != 4:
+        if data.dim() != 4:
             raise GeneratorError("cache data: needs [blocks][kv_heads][2][block_tokens * "
-                                 f"head_dim], got {tuple(self.data.shape)}")
-        blocks, heads = self.data.shape[:2]
-        device = self.data.device
-        _expect(self.data, "cache data", torch.uint8,
-                (blocks, heads, 2, self.block_tokens * self.head_dim), device)
-        _expect(self.scales, "cache scales", torch.float32, (blocks, heads, 2), device)
-        self.kv_heads = heads
-        self.device = device
-        self._c = _KvCache(self.data.data_ptr(), self.scales.data_ptr(), blocks,
-                           self.block_tokens, heads, self.head_dim)
+                                 f"head_dim], got {tuple(data.shape)}")
+        blocks, heads = data.shape[:2]
+        _expect(data, "cache data", torch.uint8, (blocks, heads, 2, block_tokens * head_dim),
+                data.device)
+        _expect(scales, "cache scales", torch.float32, (blocks, heads, 2), data.device)
+        self._data, self._scales = data, scales  # their addresses are taken here, once
+        self.block_tokens, self.head_dim = block_tokens, head_dim
+        self.kv_heads, self.device = heads, data.device
+        self._c = _KvCache(data.data_ptr(), scales.data_ptr(), blocks, block_tokens, heads,
+                           head_dim)
+
+    @property
+    def data(self):
+        return self._data
+
+    @property
+    def scales(self):
+        return self._scales
 
     @classmethod
     def empty(cls, blocks: int, kv_heads: int = 8, head_dim: int = 128,
@@ -756,32 +774,38 @@ class KVCache:
                    block_tokens, head_dim)
 
 
-@dataclass
 class KVSequences:
     """The sequences of one call (ovg_kv_sequences): tables int32
     [count][width], lengths int32 [count] (this call's tokens included) and
     begins int32 [count + 1] (their rows), device tensors that may be updated
     in place between calls and graph replays."""
-    tables: "torch.Tensor"  # noqa: F821
-    lengths: "torch.Tensor"  # noqa: F821
-    begins: "torch.Tensor"  # noqa: F821
 
-    def __post_init__(self):
+    def __init__(self, tables, lengths, begins):
         import torch
-        if self.tables.dim() != 2:
-            raise GeneratorError("tables: needs [count][width], got "
-                                 f"{tuple(self.tables.shape)}")
-        count, width = self.tables.shape
-        device = self.tables.device
-        _expect(self.tables, "tables", torch.int32, (count, width), device)
-        _expect(self.lengths, "lengths", torch.int32, (count,), device)
-        _expect(self.begins, "begins", torch.int32, (count + 1,), device)
-        self.device = device
+        if tables.dim() != 2:
+            raise GeneratorError(f"tables: needs [count][width], got {tuple(tables.shape)}")
+        count, width = tables.shape
+        _expect(tables, "tables", torch.int32, (count, width), tables.device)
+        _expect(lengths, "lengths", torch.int32, (count,), tables.device)
+        _expect(begins, "begins", torch.int32, (count + 1,), tables.device)
+        self._tables, self._lengths, self._begins = tables, lengths, begins
+        self.device = tables.device
+        self._fields = (tables.data_ptr(), lengths.data_ptr(), begins.data_ptr(), count, width)
+
+    @property
+    def tables(self):
+        return self._tables
+
+    @property
+    def lengths(self):
+        return self._lengths
+
+    @property
+    def begins(self):
+        return self._begins
 
     def _c(self, rows: int) -> _KvSequences:
-        return _KvSequences(self.tables.data_ptr(), self.lengths.data_ptr(),
-                            self.begins.data_ptr(), self.tables.shape[0],
-                            self.tables.shape[1], rows)
+        return _KvSequences(*self._fields, rows)
 
 
 def _check_cache(cache: KVCache, sequences: KVSequences) -> None:
@@ -796,13 +820,8 @@ def _cache_io(name: str, cache: KVCache, sequences: KVSequences, k, v, stream) -
     if k.shape[0] != v.shape[0] or k.dtype is not v.dtype:
         raise GeneratorError(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} "
                              f"{v.dtype}")
-    kind = _type_of(k, "k")
-    seq = sequences._c(k.shape[0])
-    err = _buf()
-    fn = getattr(lib(), name)
-    _launch(cache.device, stream,
-            lambda s: _check(fn(cache._c, seq, _dev(k), _dev(v), k_stride, v_stride, kind, s,
-                                err, len(err)), err))
+    _enqueue(getattr(lib(), name), cache.device, stream, cache._c, sequences._c(k.shape[0]),
+             k.data_ptr(), v.data_ptr(), k_stride, v_stride, _type_of(k, "k"))
 
 
 def op_cache_write(cache: KVCache, sequences: KVSequences, k, v, stream=None) -> None:
@@ -848,11 +867,8 @@ def op_cache_attention(cache: KVCache, sequences: KVSequences, q, out,
         workspace, L.ovg_op_cache_attention_workspace(cache._c, seq, heads), cache.device, stream)
     if scale is None:
         scale = cache.head_dim ** -0.5
-    err = _buf()
-    _launch(cache.device, stream,
-            lambda s: _check(L.ovg_op_cache_attention(
-                cache._c, seq, _dev(q), _dev(out), q_stride, out_stride, heads, scale,
-                int(causal), kind, space, size, s, err, len(err)), err))
+    _enqueue(L.ovg_op_cache_attention, cache.device, stream, cache._c, seq, q.data_ptr(),
+             out.data_ptr(), q_stride, out_stride, heads, scale, int(causal), kind, space, size)
 
 
 # --------------------------------------------------------------- log probabilities
@@ -908,13 +924,9 @@ def op_token_logprobs(logits, tokens, logprob, entropy, top_ids=None, top_logpro
     def ptr(t):
         return None if t is None else t.data_ptr()
 
-    err = _buf()
-    _launch(device, stream,
-            lambda s: _check(L.ovg_op_token_logprobs(
-                _dev(logits), ptr(uncond), rows, vocab, stride, u_stride, guidance,
-                -1 if mask_id is None else mask_id, ptr(tokens), top, ptr(logprob),
-                ptr(entropy), ptr(top_ids), ptr(top_logprobs), kind, space, size, s, err,
-                len(err)), err))
+    _enqueue(L.ovg_op_token_logprobs, device, stream, logits.data_ptr(), ptr(uncond), rows, vocab,
+             stride, u_stride, guidance, -1 if mask_id is None else mask_id, ptr(tokens), top,
+             ptr(logprob), ptr(entropy), ptr(top_ids), ptr(top_logprobs), kind, space, size)
 
 
 # --------------------------------------------------------------- audio decoder

@@ -131,7 +131,14 @@ constexpr int kMostSplits = 256;
 constexpr int kFewSplits = 8;       // that one group of lanes joins by itself
 constexpr int kManyGroups = 512;    // the same for many rows: two a CU
 constexpr int kLeastChunk = 256;    // keys of a split at least
-constexpr int kSplitGroups = 2048;  // work-groups that a split call is to have
+// Work-groups that a split call is to have. Alone, a sequence's splits are equal
+// and two a CU keep the memory busy (90001 keys: 41 us with 512, 44 with 1024, whose
+// join takes longer); several are ragged and fill the device better in smaller
+// pieces (48 of up to 8192 keys: 95.6 us with 1024, 99.4 with 512), but for tiles of
+// 32 rows, where a piece's start and end cost as much as 500 keys (20 x 6 tokens of
+// 8 heads: 17.3 us with 512, 19.6 with 1024).
+constexpr int kSplitGroups = 512;
+constexpr int kRaggedSplitGroups = 1024;
 CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group);
 // Keys of each split of a sequence of `length` tokens: a whole number of the
 // four waves' steps.
@@ -155,8 +162,12 @@ struct LogprobParams {
   float* entropy;        // [rows], or null
   int* top_ids;          // [rows][top]
   float* top_logprobs;   // [rows][top]
+  int splits;            // of each row (PlanLogprobs)
+  float* states;         // [rows][splits][4 + 2 top] where there are several
 };
 constexpr int kMostAlternatives = 32;
+constexpr int kLogprobGroups = 512;  // work-groups that a call is to have
+int PlanLogprobs(int rows, int vocab);
 void LaunchLogprobs(const LogprobParams& p, DType type, hipStream_t stream);
 
 }  // namespace ovg

@@ -764,20 +764,29 @@ __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
   top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
   const float from = top == -__builtin_inff() ? 0.0F : top;
   const float weight = __builtin_amdgcn_exp2f(m - from);
-  // A split that saw nothing has left no output: its weight says so.
   if (tid < kMostSplits)
-    weights[tid] = l == 0.0F ? 0.0F : weight;
+    weights[tid] = weight;
   const float part_total = WaveSum(l * weight);
   if ((tid & 63) == 0)
     totals[tid >> 6] = part_total;
   __syncthreads();
   const float total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+  // Eight loads at a time, none under a condition: a split that saw nothing has
+  // left zeros.
+  constexpr int kAhead = 8;
   floatx4 sum = {};
-  for (int s = group; s < p.splits; s += kGroups) {
-    const float w = weights[s];
-    const std::size_t slot = first + (static_cast<std::size_t>(s) << p.tile_shift);
-    if (w != 0.0F)
-      sum += *reinterpret_cast<const floatx4*>(p.partial_o + slot * DIM + 4 * part) * w;
+  for (int s0 = group; s0 < p.splits; s0 += kAhead * kGroups) {
+    floatx4 o[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int s = min(s0 + a * kGroups, p.splits - 1);
+      const std::size_t slot = first + (static_cast<std::size_t>(s) << p.tile_shift);
+      o[a] = *reinterpret_cast<const floatx4*>(p.partial_o + slot * DIM + 4 * part);
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+      if (s0 + a * kGroups < p.splits)
+        sum += o[a] * weights[s0 + a * kGroups];
   }
   sums[group][part] = sum;
   __syncthreads();
@@ -817,6 +826,7 @@ __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
       (((static_cast<std::size_t>(blockIdx.y) * c.kv_heads + head) * p.splits) << p.tile_shift) +
       in_tile;
   float m[kFewSplits], l[kFewSplits];
+  floatx4 o[kFewSplits];
   float top = -__builtin_inff();
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
@@ -824,6 +834,7 @@ __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
         first + (static_cast<std::size_t>(min(s, p.splits - 1)) << p.tile_shift);
     m[s] = p.partial_m[2 * slot];
     l[s] = s < p.splits ? p.partial_m[2 * slot + 1] : 0.0F;
+    o[s] = *reinterpret_cast<const floatx4*>(p.partial_o + slot * DIM + 4 * part);
     top = fmaxf(top, m[s]);
   }
   const float from = top == -__builtin_inff() ? 0.0F : top;
@@ -831,12 +842,10 @@ __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
   floatx4 sum = {};
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
-    if (l[s] == 0.0F)  // a split that saw nothing, or none
-      continue;
     const float w = __builtin_amdgcn_exp2f(m[s] - from);
-    const std::size_t slot = first + (static_cast<std::size_t>(s) << p.tile_shift);
     total += l[s] * w;
-    sum += *reinterpret_cast<const floatx4*>(p.partial_o + slot * DIM + 4 * part) * w;
+    if (s < p.splits)
+      sum += o[s] * w;
   }
   const float scale = total == 0.0F ? 0.0F : 1.0F / total;
   const int query = row / p.group, of_group = row % p.group;
@@ -886,7 +895,9 @@ CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group) {
   const int items = ItemBound(c, group, plan.tile_shift, 1);
   const std::int64_t groups = static_cast<std::int64_t>(items) * c.kv_heads;
   const std::int64_t capacity = static_cast<std::int64_t>(c.table_width) << c.block_shift;
-  const std::int64_t aim = plan.tile_shift == 7 ? kManyGroups : kSplitGroups;
+  const std::int64_t aim = plan.tile_shift == 7                   ? kManyGroups
+                           : plan.tile_shift == 4 && c.count > 1 ? kRaggedSplitGroups
+                                                                 : kSplitGroups;
   const std::int64_t least = plan.tile_shift == 7 ? 2 * kLeastChunk : kLeastChunk;
   plan.splits = static_cast<int>(std::max<std::int64_t>(
       1, std::min({(aim + groups - 1) / groups, capacity / least, std::int64_t{kMostSplits}})));

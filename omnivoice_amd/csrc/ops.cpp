@@ -110,6 +110,11 @@ int64_t AttentionBytes(const ovg::CacheView& c, const ovg::CacheAttentionPlan& p
   return static_cast<int64_t>(plan.slots) * (c.dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
+// The splits' sums and lists.
+int64_t LogprobBytes(int64_t rows, int64_t top, int splits) {
+  return splits == 1 ? 0 : rows * splits * (4 + 2 * top) * static_cast<int64_t>(sizeof(float));
+}
+
 void RequireStride(int64_t stride, int64_t width) {
   ovg::Require(stride >= width && stride <= (int64_t{1} << 40), "row stride below the row's width");
 }
@@ -452,10 +457,10 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
 }
 
 int64_t ovg_op_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top) {
-  (void)rows;
-  (void)vocab;
-  (void)top;
-  return 0;
+  if (!FitsInt(rows) || vocab < 1 || !FitsInt(vocab) || top < 0 || top > ovg::kMostAlternatives)
+    return -1;
+  return LogprobBytes(rows, top,
+                      ovg::PlanLogprobs(static_cast<int>(rows), static_cast<int>(vocab)));
 }
 
 int ovg_op_token_logprobs(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
@@ -481,9 +486,12 @@ int ovg_op_token_logprobs(const void* logits, const void* uncond, int64_t rows, 
     ovg::Require(top == 0 || (top_ids && top_logprobs), "null pointer");
     auto s = static_cast<hipStream_t>(stream);
     RequireCurrentDevice(s);
-    (void)workspace;
-    (void)workspace_bytes;
     ovg::LogprobParams p{};
+    p.splits = ovg::PlanLogprobs(static_cast<int>(rows), static_cast<int>(vocab));
+    const int64_t bytes = LogprobBytes(rows, top, p.splits);
+    ovg::Require(bytes == 0 || (workspace && workspace_bytes >= bytes && Aligned16(workspace)),
+                 "workspace of " + std::to_string(bytes) + " bytes needed, 16-byte aligned");
+    p.states = static_cast<float*>(workspace);
     p.logits = logits;
     p.uncond = uncond;
     p.stride = stride;
