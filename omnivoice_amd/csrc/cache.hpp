@@ -113,7 +113,8 @@ struct CacheAttentionParams {
   std::int64_t q_stride, out_stride;
   int group;       // query heads per kv head
   bool causal;
-  float scale_log2;  // the softmax's scale * log2(e)
+  float scale_log2;  // the softmax's scale * log2(e), without its sign:
+  bool negate;       // the queries take it
   // The plan's (PlanCacheAttention), and where its splits leave their states:
   // slot ((item * kv_heads + head) * splits + split) * tile rows + row has its
   // row's maximum and sum in partial_m and its output, not divided, in partial_o.

@@ -152,16 +152,18 @@ constexpr int kFewWaves = 4;
 // one after the other.
 struct Window {
   int page;
-  float k_scale, v_scale;
-  __device__ __forceinline__ void Load(const CacheView& c, int sequence, int head, int first,
-                                       int stop, int lane) {
+  float factor;  // of the scores, to the exponent of two; NaN where the block is
+  float level;   // the values' loudness
+  __device__ __forceinline__ void Load(const CacheAttentionParams& p, int sequence, int head,
+                                       int first, int stop, int lane) {
+    const CacheView& c = p.cache;
     const int block = first + lane;
     page = (block << c.block_shift) < stop ? PageOf(c, sequence, block) : -1;
     const std::size_t at = ScaleIndex(c, max(page, 0), head, 0);
-    k_scale = c.scales[at];
-    v_scale = c.scales[at + 1];
-    if (page < 0)
-      k_scale = v_scale = 0.0F;
+    const float k_scale = c.scales[at], v_scale = c.scales[at + 1];
+    // A NaN scale, of keys or values, makes the block's scores NaN.
+    factor = page < 0 ? 0.0F : p.scale_log2 * k_scale + 0.0F * v_scale;
+    level = page < 0 ? 0.0F : Loudness(v_scale);
   }
 };
 
@@ -216,6 +218,13 @@ __global__ __launch_bounds__(kFewWaves* kWave) void FewRowsKernel(CacheAttention
       __builtin_memcpy(&q[n][i][0], from + 64 * i, sizeof(x8));
       __builtin_memcpy(&q[n][i][1], from + 64 * i + 8, sizeof(x8));
     }
+    if (p.negate) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        q[n][i][0] = -q[n][i][0];
+        q[n][i][1] = -q[n][i][1];
+      }
+    }
   }
 
   float m[NT], l[NT];
@@ -239,7 +248,7 @@ __global__ __launch_bounds__(kFewWaves* kWave) void FewRowsKernel(CacheAttention
   for (int window = wave_begin; window < wave_stop;) {
     Window w;
     const int first_block = window >> c.block_shift;
-    w.Load(c, sequence, head, first_block, wave_stop, lane);
+    w.Load(p, sequence, head, first_block, wave_stop, lane);
     const int window_stop = min((first_block + kWave) << c.block_shift, wave_stop);
 
     struct Codes {
@@ -269,10 +278,8 @@ __global__ __launch_bounds__(kFewWaves* kWave) void FewRowsKernel(CacheAttention
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const int block = ((key + 16 * g) >> c.block_shift) - first_block;
-        const float v_scale = Lane(w.v_scale, block);
-        // A NaN scale, of keys or values, makes the block's scores NaN.
-        factor[g] = p.scale_log2 * Lane(w.k_scale, block) + 0.0F * v_scale;
-        level[g] = Loudness(v_scale);
+        factor[g] = Lane(w.factor, block);
+        level[g] = Lane(w.level, block);
         there[g] = __builtin_amdgcn_readlane(w.page, block) >= 0;
       }
       const float louder = fmaxf(loud, fmaxf(level[0], level[1]));
@@ -431,24 +438,60 @@ __global__ __launch_bounds__(kFewWaves* kWave) void FewRowsKernel(CacheAttention
 constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;
 
-// What a tile's groups of 16 keys need beside their codes.
-template <int GROUPS>
+// The same for tiles of many rows, whose values are converted for all at once:
+// lane i holds where its block's head begins, the scores' factor, and the
+// values' scale over `loud`, the loudest of this window's blocks and all before.
+struct TileWindow {
+  unsigned offset_low, offset_high;
+  float factor, unit;
+  float loud;                // the same in every lane
+  unsigned long long there;  // a bit for each block that there is
+  __device__ __forceinline__ void Load(const CacheAttentionParams& p, int sequence, int head,
+                                       int first, int stop, int lane) {
+    const CacheView& c = p.cache;
+    const int block = first + lane;
+    const int page = (block << c.block_shift) < stop ? PageOf(c, sequence, block) : -1;
+    there = __ballot(page >= 0);
+    const std::size_t at = ScaleIndex(c, max(page, 0), head, 0);
+    const float k_scale = c.scales[at], v_scale = c.scales[at + 1];
+    const std::size_t offset = at * (static_cast<std::size_t>(c.dim) << c.block_shift);
+    offset_low = static_cast<unsigned>(offset);
+    offset_high = static_cast<unsigned>(offset >> 32);
+    // A NaN scale, of keys or values, makes the block's scores NaN.
+    factor = page < 0 ? 0.0F : p.scale_log2 * k_scale + 0.0F * v_scale;
+    const float level = page < 0 ? 0.0F : Loudness(v_scale);
+    loud = fmaxf(loud, WaveMax(level));
+    unit = fmaxf(level * InversePower(loud), kQuietest);
+  }
+  __device__ __forceinline__ const unsigned char* Base(const unsigned char* data, int i) const {
+    const std::size_t low = __builtin_amdgcn_readlane(offset_low, i);
+    const std::size_t high = __builtin_amdgcn_readlane(offset_high, i);
+    return data + (high << 32 | (low & 0xFFFFFFFFu));
+  }
+};
+
+// What a tile needs beside its codes: a factor for each of its blocks.
+template <int BLOCKS>
 struct TileScales {
-  typedef float vec __attribute__((ext_vector_type(GROUPS)));
-  vec factor;      // scores to the exponent of two
-  float loud;      // of the values as they are converted: this tile's and all before
-  unsigned there;  // a bit for each group that has a block
+  typedef float vec __attribute__((ext_vector_type(BLOCKS)));
+  vec factor;
+  float loud;      // that its values are converted at
+  float unit;      // of the values that this thread converts
+  unsigned there;  // a bit for each block
 };
 
 // Many rows: a work-group of four waves takes 128 rows of one sequence and kv
 // head, 32 a wave, and goes over the keys in tiles of 64 (128 at 64 dims) that
-// the waves share. The threads fetch a tile's codes while the one before is
-// worked on, convert them once and leave them in LDS in the order of the
-// operands of v_mfma_f32_32x32x16 (64 lanes of 16 bytes in a row, so every
-// write and read is a conflict-free 16 bytes a lane), in one of two buffers of
-// 32 KB: one barrier a tile. The softmax runs in registers, a row in a lane and
-// its partner lane ^ 32.
-template <typename T, int DIM>
+// the waves share. The threads fetch a tile's codes ahead, convert them once and
+// leave them in LDS in the order of the operands of v_mfma_f32_32x32x16 (64 lanes
+// of 16 bytes in a row, so every write and read is a conflict-free 16 bytes a
+// lane), in two buffers of 16 KB each for keys and values. The softmax runs in
+// registers, a row in a lane and its partner lane ^ 32. While a tile's
+// probabilities are formed, on the vector unit, the matrix cores form the next
+// tile's scores, which depend on nothing of it; so in iteration i the waves read
+// keys i + 1 and values i and write keys i + 2 and values i + 1, and one barrier
+// an iteration suffices.
+template <typename T, int DIM, int SHIFT>
 __global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAttentionParams p) {
   typedef Types<T> X;
   typedef typename X::x8 x8;
@@ -457,6 +500,10 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAtte
   constexpr int kK = DIM / 16;               // contraction steps of the scores
   constexpr int kDims = DIM / 32;            // blocks of 32 dims
   constexpr int kChunks = DIM;               // 16-byte chunks of a group's keys or values
+  constexpr int kSums = 4;                   // of a row in a lane, to be added at the end
+  constexpr int kPages = kKeys >> SHIFT;     // blocks of the pool in a tile: 1 to 8
+  constexpr std::size_t kHalf = static_cast<std::size_t>(DIM) << SHIFT;  // bytes
+  typedef TileScales<kPages> Scales;
   __shared__ x8 key_tiles[2][kKeys * DIM / 8];
   __shared__ x8 value_tiles[2][kKeys * DIM / 8];
   const CacheView& c = p.cache;
@@ -503,9 +550,15 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAtte
 #pragma unroll
     for (int i = 0; i < kK; ++i)
       __builtin_memcpy(&q[i], from + 16 * i, sizeof(x8));
+    if (p.negate) {
+#pragma unroll
+      for (int i = 0; i < kK; ++i)
+        q[i] = -q[i];
+    }
   }
 
-  float m = -__builtin_inff(), l = 0.0F;
+  float m = -__builtin_inff();
+  float l[kSums] = {};
   floatx16 o[kDims];
 #pragma unroll
   for (int t = 0; t < kDims; ++t)
@@ -514,9 +567,8 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAtte
       o[t][r] = 0.0F;
   float loud = kQuietest;
 
-  const int in_block = (1 << c.block_shift) - 1;
-  const std::size_t half_bytes = static_cast<std::size_t>(DIM) << c.block_shift;
-  Window window;
+  TileWindow window;
+  window.loud = kQuietest;
   int window_first = 0, window_stop = begin;  // block, key
 
   // A thread's chunks of a tile: two of keys (chunk tid + 256 i: group, dims / 16,
@@ -525,63 +577,50 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAtte
   const int value_group = tid / (DIM / 2), value_at = tid % (DIM / 2);
   const int value_chunk = (value_at >> 5) * 64 + (value_at & 31);
   u32x4 k_codes[2], v_codes[2];
-  float v_level = 0.0F;
-  const auto block_of = [&](int key) {
-    return min((key >> c.block_shift) - window_first, kWave - 1);
-  };
-  const auto fetch = [&](int key) {
+  // The tile's scales, the codes of its keys on their way, and where its values are.
+  // A tile begins with a block or with a whole part of one.
+  const auto fetch_keys = [&](int key, const u32x4** values) {
     if (key >= window_stop) {  // never in the middle of a tile: 64 blocks are whole ones
-      window_first = key >> c.block_shift;
-      window.Load(c, sequence, head, window_first, stop, lane);
-      window_stop = (window_first + kWave) << c.block_shift;
+      window_first = key >> SHIFT;
+      window.Load(p, sequence, head, window_first, stop, lane);
+      window_stop = (window_first + kWave) << SHIFT;
     }
+    const int block = (key >> SHIFT) - window_first;
     const auto base = [&](int group) {
-      const int at = key + 16 * group;
-      const int page = max(__builtin_amdgcn_readlane(window.page, block_of(at)), 0);
-      return c.data + (static_cast<std::size_t>(page) * c.kv_heads + head) * 2 * half_bytes +
-             static_cast<std::size_t>(at & in_block & ~15) * DIM;
+      return window.Base(c.data, block + ((16 * group) >> SHIFT)) +
+             (16 * group & ((1 << SHIFT) - 1)) * DIM;
     };
+    Scales s;
+    s.loud = window.loud;
+    s.there = static_cast<unsigned>(window.there >> block) & ((1u << kPages) - 1);
+#pragma unroll
+    for (int g = 0; g < kPages; ++g)
+      s.factor[g] = Lane(window.factor, block + g);
     if constexpr (DIM == 128) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         k_codes[i] = reinterpret_cast<const u32x4*>(
             base(2 * i + (wave >> 1)))[(wave & 1) * 64 + lane];
-      const u32x4* from = reinterpret_cast<const u32x4*>(base(wave) + half_bytes);
-      v_codes[0] = from[value_chunk];
-      v_codes[1] = from[value_chunk + 32];
-      v_level = Lane(window.v_scale, block_of(key + 16 * wave));
+      *values = reinterpret_cast<const u32x4*>(base(wave) + kHalf) + value_chunk;
+      s.unit = Lane(window.unit, block + ((16 * wave) >> SHIFT));
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         k_codes[i] = reinterpret_cast<const u32x4*>(base(4 * i + wave))[lane];
-      const unsigned char* low = base(2 * wave);
-      const unsigned char* high = base(2 * wave + 1);
-      const u32x4* from =
-          reinterpret_cast<const u32x4*>((half == 0 ? low : high) + half_bytes);
-      v_codes[0] = from[value_chunk];
-      v_codes[1] = from[value_chunk + 32];
-      const float even = Lane(window.v_scale, block_of(key + 32 * wave));
-      const float odd = Lane(window.v_scale, block_of(key + 32 * wave + 16));
-      v_level = half == 0 ? even : odd;
-    }
-  };
-  // The tile's scales, while its window is the current one.
-  const auto scales_of = [&](int key, float before) {
-    TileScales<kGroups> s;
-    s.loud = before;
-    s.there = 0;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const int block = block_of(key + 16 * g);
-      const float v_scale = Lane(window.v_scale, block);
-      // A NaN scale, of keys or values, makes the block's scores NaN.
-      s.factor[g] = p.scale_log2 * Lane(window.k_scale, block) + 0.0F * v_scale;
-      s.there |= (__builtin_amdgcn_readlane(window.page, block) >= 0 ? 1u : 0u) << g;
-      s.loud = fmaxf(s.loud, Loudness(v_scale));
+      const unsigned char* even = base(2 * wave);
+      const unsigned char* odd = base(2 * wave + 1);
+      *values = reinterpret_cast<const u32x4*>((half == 0 ? even : odd) + kHalf) + value_chunk;
+      const float even_unit = Lane(window.unit, block + ((32 * wave) >> SHIFT));
+      const float odd_unit = Lane(window.unit, block + ((32 * wave + 16) >> SHIFT));
+      s.unit = half == 0 ? even_unit : odd_unit;
     }
     return s;
   };
-  const auto convert = [&](const TileScales<kGroups>& s, int buffer) {
+  const auto fetch_values = [&](const u32x4* values) {
+    v_codes[0] = values[0];
+    v_codes[1] = values[32];
+  };
+  const auto convert_keys = [&](int buffer) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int index = tid + i * 256;
@@ -591,107 +630,133 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAtte
       to[0] = Operand<T>(k_codes[i][0], k_codes[i][1], 1.0F);
       to[32] = Operand<T>(k_codes[i][2], k_codes[i][3], 1.0F);
     }
-    const float level = fmaxf(Loudness(v_level) * InversePower(s.loud), kQuietest);
+  };
+  const auto convert_values = [&](const Scales& s, int buffer) {
     const int d = value_at & 15, h = (value_at >> 4) & 1, quarter = value_at >> 5;
     x8* to = value_tiles[buffer] + (value_group * kDims + 2 * quarter) * 64 + 32 * h + d;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
-      to[(t >> 1) * 64 + (t & 1) * 16] = Operand<T>(v_codes[0][t], v_codes[1][t], level);
+      to[(t >> 1) * 64 + (t & 1) * 16] = Operand<T>(v_codes[0][t], v_codes[1][t], s.unit);
   };
-
-  const auto work = [&](int key, const TileScales<kGroups>& s, int buffer) {
-    if (s.loud > loud) {
-      const float shrink = loud * InversePower(s.loud);
-#pragma unroll
-      for (int t = 0; t < kDims; ++t)
-        o[t] *= shrink;
-      loud = s.loud;
-    }
-    if (key >= wave_end)
-      return;
-    floatx16 acc[kBlocks];
+  floatx16 scores[kBlocks];
+  const auto score = [&](int buffer, floatx16 (&to)[kBlocks]) {
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
+      floatx16 acc;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        acc[b][r] = 0.0F;
+        acc[r] = 0.0F;
 #pragma unroll
       for (int i = 0; i < kK; ++i)
-        acc[b] = X::Mfma32(key_tiles[buffer][(b * kK + i) * 64 + lane], q[i], acc[b]);
-    }
-    float peak = -__builtin_inff();
-    if (s.there == (1u << kGroups) - 1 && key + kKeys <= all_see) {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          acc[b][r] *= s.factor[2 * b + r / 8];
-          peak = fmaxf(peak, acc[b][r]);
-        }
-    } else {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = key + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-          acc[b][r] = (s.there >> (2 * b + r / 8) & 1) != 0 && at < seen ? acc[b][r] * s.factor[2 * b + r / 8]
-                                                          : -__builtin_inff();
-          peak = fmaxf(peak, acc[b][r]);
-        }
-    }
-    peak = Max32(peak);
-    if (__any(peak > m + kSlack)) {
-      const float top = peak > m + kSlack ? peak : m;
-      const float shrink = top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m - top);
-      m = top;
-      l *= shrink;
-#pragma unroll
-      for (int t = 0; t < kDims; ++t)
-        o[t] *= shrink;
-    }
-    const float from = m == -__builtin_inff() ? 0.0F : m;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      x8 weights;
-#pragma unroll
-      for (int r = 0; r < 8; r += 2) {
-        const typename X::x2 pair =
-            X::Round(__builtin_amdgcn_exp2f(acc[g / 2][8 * (g & 1) + r] - from),
-                     __builtin_amdgcn_exp2f(acc[g / 2][8 * (g & 1) + r + 1] - from));
-        weights[r] = pair[0];
-        weights[r + 1] = pair[1];
-        l = X::AddPair(pair, l);
-      }
-#pragma unroll
-      for (int t = 0; t < kDims; ++t)
-        o[t] = X::Mfma32(value_tiles[buffer][(g * kDims + t) * 64 + lane], weights, o[t]);
+        acc = X::Mfma32(key_tiles[buffer][(b * kK + i) * 64 + lane], q[i], acc);
+      to[b] = acc;
     }
   };
 
   if (begin < stop) {
-    fetch(begin);
-    TileScales<kGroups> now = scales_of(begin, loud), next = now;
-    convert(now, 0);
-    if (begin + kKeys < stop)
-      fetch(begin + kKeys);
-    next = scales_of(begin + kKeys, now.loud);
+    // Tiles now, one and two ahead; past the last one the scales and codes of
+    // whatever block 0 holds, which nothing takes.
+    const u32x4 *values, *values_next, *values_after;
+    Scales now = fetch_keys(begin, &values);
+    fetch_values(values);
+    convert_keys(0);
+    convert_values(now, 0);
+    Scales next = fetch_keys(begin + kKeys, &values_next);
+    fetch_values(values_next);
+    convert_keys(1);
+    Scales after = fetch_keys(begin + 2 * kKeys, &values_after);
     __syncthreads();
-    int buffer = 0;
+    score(0, scores);
+    __syncthreads();
+    int buffer = 0;  // of this tile's keys and values
     for (int key = begin; key < stop; key += kKeys) {
-      const TileScales<kGroups> coming = next;
-      if (key + kKeys < stop)
-        convert(coming, buffer ^ 1);
-      if (key + 2 * kKeys < stop)
-        fetch(key + 2 * kKeys);
-      next = scales_of(key + 2 * kKeys, coming.loud);
-      work(key, now, buffer);
-      now = coming;
+      if (now.loud > loud) {
+        const float shrink = loud * InversePower(now.loud);
+#pragma unroll
+        for (int t = 0; t < kDims; ++t)
+          o[t] *= shrink;
+        loud = now.loud;
+      }
+      if (key < wave_end) {
+        typename Scales::vec factor = now.factor;
+        const auto page_of = [](int group) { return (16 * group) >> SHIFT; };
+        if (now.there != (1u << kPages) - 1 || key + kKeys > all_see) {
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              const int e = 8 * (g & 1) + r;
+              const int at = key + 16 * g + 8 * (r / 4) + 4 * half + r % 4;
+              scores[g / 2][e] = (now.there >> page_of(g) & 1) != 0 && at < seen
+                                     ? scores[g / 2][e] * factor[page_of(g)]
+                                     : -__builtin_inff();
+            }
+#pragma unroll
+          for (int g = 0; g < kPages; ++g)
+            factor[g] = 1.0F;
+        }
+        float peak = -__builtin_inff();
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float most = -__builtin_inff();
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            most = fmaxf(most, scores[g / 2][8 * (g & 1) + r]);
+          peak = fmaxf(peak, most * factor[page_of(g)]);
+        }
+        peak = Max32(peak);
+        if (__any(peak > m + kSlack)) {
+          const float top = peak > m + kSlack ? peak : m;
+          const float shrink = top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m - top);
+          m = top;
+#pragma unroll
+          for (int i = 0; i < kSums; ++i)
+            l[i] *= shrink;
+#pragma unroll
+          for (int t = 0; t < kDims; ++t)
+            o[t] *= shrink;
+        }
+        const float from = m == -__builtin_inff() ? 0.0F : m;
+        floatx16 coming[kBlocks];
+        score(buffer ^ 1, coming);
+        x8 weights[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+          for (int r = 0; r < 8; r += 2) {
+            const int e = 8 * (g & 1) + r;
+            const typename X::x2 pair = X::Round(
+                __builtin_amdgcn_exp2f(__builtin_fmaf(scores[g / 2][e], factor[page_of(g)], -from)),
+                __builtin_amdgcn_exp2f(__builtin_fmaf(scores[g / 2][e + 1], factor[page_of(g)], -from)));
+            weights[g][r] = pair[0];
+            weights[g][r + 1] = pair[1];
+            l[r / 2] = X::AddPair(pair, l[r / 2]);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+          for (int t = 0; t < kDims; ++t)
+            o[t] = X::Mfma32(value_tiles[buffer][(g * kDims + t) * 64 + lane], weights[g], o[t]);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+          scores[b] = coming[b];
+        convert_keys(buffer);
+        convert_values(next, buffer ^ 1);
+      } else {
+        convert_keys(buffer);
+        convert_values(next, buffer ^ 1);
+      }
+      fetch_values(values_after);
+      now = next;
+      next = after;
+      after = fetch_keys(key + 3 * kKeys, &values_after);
       buffer ^= 1;
       __syncthreads();
     }
   }
 
-  l = Sum32(l);
+  const float total = Sum32((l[0] + l[1]) + (l[2] + l[3]));
   if (row >= rows)
     return;
   if (p.splits > 1) {
@@ -700,7 +765,7 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAtte
             kManyRows + 32 * wave + column;
     if (half == 0) {
       p.partial_m[2 * slot] = m;
-      p.partial_m[2 * slot + 1] = l;
+      p.partial_m[2 * slot + 1] = total;
     }
 #pragma unroll
     for (int t = 0; t < kDims; ++t)
@@ -713,7 +778,7 @@ __global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAtte
     return;
   }
   // Nothing seen: zero.
-  const float scale = l == 0.0F ? 0.0F : loud / l;
+  const float scale = total == 0.0F ? 0.0F : loud / total;
   T* to = static_cast<T*>(p.out) + static_cast<std::int64_t>(span.first + query) * p.out_stride +
           static_cast<std::int64_t>(head * p.group + of_group) * DIM + 4 * half;
 #pragma unroll
@@ -868,8 +933,12 @@ void Launch(const CacheAttentionParams& p, hipStream_t stream) {
     Dispatch(FewRowsKernel<T, DIM, 1>, grid, block, 0, stream, true, last, p);
   else if (p.tile_shift == 5)
     Dispatch(FewRowsKernel<T, DIM, 2>, grid, block, 0, stream, true, last, p);
+  else if (p.cache.block_shift == 4)
+    Dispatch(ManyRowsKernel<T, DIM, 4>, grid, block, 0, stream, true, last, p);
+  else if (p.cache.block_shift == 5)
+    Dispatch(ManyRowsKernel<T, DIM, 5>, grid, block, 0, stream, true, last, p);
   else
-    Dispatch(ManyRowsKernel<T, DIM>, grid, block, 0, stream, true, last, p);
+    Dispatch(ManyRowsKernel<T, DIM, 6>, grid, block, 0, stream, true, last, p);
   if (last)
     return;
   constexpr int kJoined = 256 / (DIM / 4);  // rows of a work-group with few splits
@@ -899,8 +968,10 @@ CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group) {
                            : plan.tile_shift == 4 && c.count > 1 ? kRaggedSplitGroups
                                                                  : kSplitGroups;
   const std::int64_t least = plan.tile_shift == 7 ? 2 * kLeastChunk : kLeastChunk;
+  const std::int64_t wanted =
+      plan.tile_shift == 7 ? aim / groups : (aim + groups - 1) / groups;
   plan.splits = static_cast<int>(std::max<std::int64_t>(
-      1, std::min({(aim + groups - 1) / groups, capacity / least, std::int64_t{kMostSplits}})));
+      1, std::min({wanted, capacity / least, std::int64_t{kMostSplits}})));
   if (plan.splits > 1)
     plan.slots = (static_cast<std::size_t>(groups) * plan.splits) << plan.tile_shift;
   return plan;

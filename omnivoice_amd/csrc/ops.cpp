@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <string>
 
@@ -451,7 +452,8 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
     p.q_stride = q_stride;
     p.out_stride = out_stride;
     p.causal = causal != 0;
-    p.scale_log2 = scale * 1.44269504088896341F;
+    p.scale_log2 = std::fabs(scale) * 1.44269504088896341F;
+    p.negate = scale < 0.0F;
     ovg::LaunchCacheAttention(p, t, s);
   });
 }
