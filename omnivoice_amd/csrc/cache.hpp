@@ -40,21 +40,6 @@ __device__ __forceinline__ std::size_t ScaleIndex(const CacheView& c, int page, 
   return (static_cast<std::size_t>(page) * c.kv_heads + head) * 2 + half;
 }
 
-// Sequence i's rows [first, first + count) of the call's tensors and the
-// cache position `start` of its first row (negative where the sequence is
-// shorter than its rows). Rows are clamped into the tensors.
-struct Span {
-  int first, count, start, length;
-};
-__device__ __forceinline__ Span SpanOf(const CacheView& c, int i) {
-  Span s;
-  s.first = min(max(c.begins[i], 0), c.rows);
-  s.count = min(max(c.begins[i + 1], s.first), c.rows) - s.first;
-  s.length = max(c.lengths[i], 0);
-  s.start = s.length - s.count;
-  return s;
-}
-
 // The pool block of a sequence's block `b`, or -1 where the table has none.
 __device__ __forceinline__ int PageOf(const CacheView& c, int sequence, int b) {
   if (b < 0 || b >= c.table_width)
@@ -63,29 +48,48 @@ __device__ __forceinline__ int PageOf(const CacheView& c, int sequence, int b) {
   return page >= 0 && page < c.blocks ? page : -1;
 }
 
+// A sequence's rows [first, first + count) of the call's tensors, clamped into
+// them, and the cache position `start` of its first row (negative where the
+// sequence is shorter than its rows).
+struct Span {
+  int first, count, start, length;
+};
 // Work items of ragged sequences without a list: sequence i owns the items
-// from Base(i) = first_i * scale / tile + slack * i (a whole-number division)
-// up to Base(i + 1), at least rows_i * scale / tile + slack of them. Every lane
-// counts bases of its own, so the search is one memory round trip per 64
-// sequences and not one per halving. Returns the sequence of `item` and takes
-// its base from it; the whole wave calls this.
-__device__ __forceinline__ int SequenceOfItem(const CacheView& c, int scale, int shift, int slack,
-                                              int* item) {
+// from first_i * scale / tile + slack * i (a whole-number division) up to the next
+// one's, at least rows_i * scale / tile + slack of them. Every lane looks at a
+// sequence of its own and holds what belongs to it, so that finding an item and
+// its span is one trip to memory per 64 sequences and none after the other. The
+// whole wave calls this; all it returns is the same in every lane. count 0: the
+// item is nobody's.
+struct Found {
+  int sequence, item;  // item: of the sequence
+  Span span;
+};
+__device__ __forceinline__ Found FindItem(const CacheView& c, int scale, int shift, int slack,
+                                          int item) {
   const int lane = threadIdx.x & (kWave - 1);
-  int below = 0;
+  Found f{0, 0, {0, 0, 0, 0}};
   for (int i0 = 0; i0 < c.count; i0 += kWave) {
-    const int i = i0 + lane;
-    const int first = min(max(c.begins[min(i, c.count)], 0), c.rows);
-    const bool at = i < c.count && ((first * scale) >> shift) + slack * i <= *item;
-    const unsigned long long ballot = __ballot(at);
-    below += __popcll(ballot);
-    if (ballot != ~0ull)
+    const int i = min(i0 + lane, c.count - 1);
+    const int begin = c.begins[i], end = c.begins[i + 1], length = c.lengths[i];
+    const int first = min(max(begin, 0), c.rows);
+    const int rows = min(max(end, first), c.rows) - first;
+    const int base = ((first * scale) >> shift) + slack * i;
+    const unsigned long long at = __ballot(i0 + lane < c.count && base <= item);
+    const int below = __popcll(at);
+    if (below > 0) {
+      const int owner = below - 1;
+      f.sequence = i0 + owner;
+      f.item = item - __builtin_amdgcn_readlane(base, owner);
+      f.span.first = __builtin_amdgcn_readlane(first, owner);
+      f.span.count = __builtin_amdgcn_readlane(rows, owner);
+      f.span.length = max(__builtin_amdgcn_readlane(length, owner), 0);
+      f.span.start = f.span.length - f.span.count;
+    }
+    if (below < kWave)
       break;
   }
-  const int sequence = max(below - 1, 0);
-  const int first = min(max(c.begins[sequence], 0), c.rows);
-  *item -= ((first * scale) >> shift) + slack * sequence;
-  return sequence;
+  return f;
 }
 inline int ItemBound(const CacheView& c, int scale, int shift, int slack) {
   return ((c.rows * scale) >> shift) + slack * c.count;
@@ -112,6 +116,8 @@ struct CacheAttentionParams {
   void* out;       // [rows][heads][dim], rows out_stride elements apart
   std::int64_t q_stride, out_stride;
   int group;       // query heads per kv head
+  int group_inverse;               // 2^16 / group, rounded up
+  unsigned long long group_magic;  // 2^36 / group, rounded up
   bool causal;
   float scale_log2;  // the softmax's scale * log2(e), without its sign:
   bool negate;       // the queries take it
@@ -129,15 +135,16 @@ struct CacheAttentionPlan {
   std::size_t slots = 0;  // of the workspace
 };
 constexpr int kMostSplits = 256;
-constexpr int kFewSplits = 8;       // that one group of lanes joins by itself
-constexpr int kManyGroups = 512;    // the same for many rows: two a CU
-constexpr int kLeastChunk = 256;    // keys of a split at least
+constexpr int kFewSplits = 8;     // that one group of lanes joins by itself
+constexpr int kLeastChunk = 256;  // keys of a split at least
+// The same for tiles of 32 rows, whose splits leave as much as they read: 375
+// queries of two heads over 2000 keys take 16.8 us whole and 20.9 in two, 100 over
+// 16000 take 80 us whole and 30 in four.
+constexpr int kLeastTileChunk = 1024;
 // Work-groups that a split call is to have. Alone, a sequence's splits are equal
 // and two a CU keep the memory busy (90001 keys: 41 us with 512, 44 with 1024, whose
-// join takes longer); several are ragged and fill the device better in smaller
-// pieces (48 of up to 8192 keys: 95.6 us with 1024, 99.4 with 512), but for tiles of
-// 32 rows, where a piece's start and end cost as much as 500 keys (20 x 6 tokens of
-// 8 heads: 17.3 us with 512, 19.6 with 1024).
+// join takes longer); several of few rows are ragged and fill the device better in
+// smaller pieces (48 of up to 8192 keys: 95.6 us with 1024, 99.4 with 512).
 constexpr int kSplitGroups = 512;
 constexpr int kRaggedSplitGroups = 1024;
 CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group);

@@ -6,13 +6,22 @@
 // being query r / group of head r % group: the whole group shares every key
 // and value that is loaded. Scores are formed transposed, S^T = K Q^T, so a
 // lane owns one row's column, and so is the output, O^T = V^T P^T, whose P^T
-// operand is the scores' accumulator itself (v_mfma_f32_16x16x32: lane l
-// holds row l % 16 and, of every 16 keys, keys 4 (l / 16) .. + 3). e4m3 codes
-// are exact in fp16 and bf16, so the products see the queries and codes as
-// they are: the keys' scale joins the softmax's in the float32 scores, the
-// values' the float32 sums. The one rounding on the way is that of the
-// probabilities to the queries' type, and the row's sum takes the rounded
-// ones, so that the weights still add up to one.
+// operand is the scores' accumulator itself. e4m3 codes are exact in fp16 and
+// bf16, so the products see the queries and codes as they are: the keys' scale
+// joins the softmax's in the float32 scores, the values' is a power of two. The
+// one rounding on the way is that of the probabilities to the queries' type, and
+// the row's sum takes the rounded ones, so that the weights still add up to one.
+//
+// A work-group takes 16 or 32 rows of one sequence and kv head and one split of
+// its keys; each of its four waves takes a quarter of those in steps of 32, with a
+// softmax of its own that runs along (maximum m, sum l, output o), and the four are
+// joined in LDS at the end. The pool's order is that of the matrix operands: the
+// codes go from memory straight into registers, a step ahead, and are converted
+// there, with no LDS and no barrier on the way. A version in which 128 rows shared
+// tiles that were converted once and left in LDS was slower at every size (two
+// causal prompts of 2500 tokens 104 us and 81 here, four chunks of 375 frames over
+// 2000 keys 61 and 39): its waves wait for each other at every tile, and a tile of
+// 128 rows leaves CUs idle where there are few.
 #include <algorithm>
 
 #include "cache.hpp"
@@ -123,6 +132,16 @@ __device__ __forceinline__ float Sum16(float v) {
   return a + b;
 }
 
+// Over the lanes of a row: lane, lane ^ 32 and with 16 rows lane ^ 16, ^ 48.
+template <int ROWS>
+__device__ __forceinline__ float RowMax(float v) {
+  return Max32(ROWS == 16 ? Max16(v) : v);
+}
+template <int ROWS>
+__device__ __forceinline__ float RowSum(float v) {
+  return Sum32(ROWS == 16 ? Sum16(v) : v);
+}
+
 __device__ __forceinline__ float Lane(float v, int lane) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
@@ -139,328 +158,62 @@ __device__ __forceinline__ float InversePower(float p) {
 // 0 for a block without a (numeric) scale.
 __device__ __forceinline__ float Loudness(float scale) { return scale == scale ? scale : 0.0F; }
 
+// The query and head of a tile's rows, by products with the host's 2^36 / group
+// (for the tile's first row, below 2^24 group) and 2^16 / group (for the fewer than
+// 128 + 64 rows behind the start of its query), both rounded up and exact there.
+struct RowSplit {
+  int query, left, group, inverse;
+  __device__ __forceinline__ RowSplit(const CacheAttentionParams& p, int first_row) {
+    group = p.group;
+    inverse = p.group_inverse;
+    query = static_cast<int>(static_cast<unsigned long long>(first_row) * p.group_magic >> 36);
+    left = first_row - query * group;
+  }
+  __device__ __forceinline__ int Of(int behind, int* of_group) const {
+    const int more = ((left + behind) * inverse) >> 16;
+    *of_group = left + behind - more * group;
+    return query + more;
+  }
+  __device__ __forceinline__ int At(int row) const {  // the query of a row of the tile
+    return query + (((row - query * group) * inverse) >> 16);
+  }
+};
+
 // How far a row's maximum may rise before its sums are scaled again: their
 // probabilities are then at most 2^8, far inside fp16, and most steps of a long
 // row leave the sums alone. Each row goes by its own maximum: what the others
 // hold changes none of its bits.
 constexpr float kSlack = 8.0F;
 
-constexpr int kFewWaves = 4;
+constexpr int kWaves = 4;
 
-// A wave's window of the block table: lane i holds the page and scales of the
-// i-th block, so that the steps wait for the table once per 64 blocks and not
-// one after the other.
+// A wave's window of the block table: lane i holds, of the i-th block, where the
+// head's part begins, the scores' factor, and the values' scale over `loud`, the
+// loudest of this window's blocks and all before. The steps wait for the table and
+// the scales once per 64 blocks and not one after the other.
 struct Window {
-  int page;
-  float factor;  // of the scores, to the exponent of two; NaN where the block is
-  float level;   // the values' loudness
-  __device__ __forceinline__ void Load(const CacheAttentionParams& p, int sequence, int head,
-                                       int first, int stop, int lane) {
-    const CacheView& c = p.cache;
-    const int block = first + lane;
-    page = (block << c.block_shift) < stop ? PageOf(c, sequence, block) : -1;
-    const std::size_t at = ScaleIndex(c, max(page, 0), head, 0);
-    const float k_scale = c.scales[at], v_scale = c.scales[at + 1];
-    // A NaN scale, of keys or values, makes the block's scores NaN.
-    factor = page < 0 ? 0.0F : p.scale_log2 * k_scale + 0.0F * v_scale;
-    level = page < 0 ? 0.0F : Loudness(v_scale);
-  }
-};
-
-// Few rows: a work-group takes 16 NT rows of one sequence and kv head and one
-// split of its keys; each of its four waves takes a quarter of them in steps of
-// 32, with a softmax of its own that runs along (maximum m, sum l, output o), and
-// the four are joined in LDS at the end. The codes go from memory straight into
-// registers, a step ahead, and are converted there: with few rows nothing is
-// gained by sharing them, and what bounds the kernel is the stream of codes.
-template <typename T, int DIM, int NT>
-__global__ __launch_bounds__(kFewWaves* kWave) void FewRowsKernel(CacheAttentionParams p) {
-  typedef Types<T> X;
-  typedef typename X::x8 x8;
-  constexpr int kSteps = DIM / 64;  // 16-byte loads of a key's codes in a lane
-  constexpr int kTiles = DIM / 16;
-  constexpr int kRows = 16 * NT;
-  const CacheView& c = p.cache;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int column = lane & 15, quad = lane >> 4;
-  const int head = blockIdx.x;
-
-  int tile = blockIdx.y;
-  const int sequence =
-      __builtin_amdgcn_readfirstlane(SequenceOfItem(c, p.group, NT == 1 ? 4 : 5, 1, &tile));
-  tile = __builtin_amdgcn_readfirstlane(tile);
-  const Span span = SpanOf(c, sequence);
-  const int rows = span.count * p.group;
-  if (tile < 0 || tile * kRows >= rows)
-    return;
-  const int length = min(span.length, c.table_width << c.block_shift);
-  // Keys that any row of the tile sees, and those of this split.
-  const int last = min(tile * kRows + kRows, rows) - 1;
-  const int end = p.causal ? min(span.start + last / p.group + 1, length) : length;
-  const int chunk = ChunkOf(length, p.splits);
-  const int begin = blockIdx.z * chunk;
-  const int stop = min(begin + chunk, end);
-
-  int query[NT], of_group[NT], seen[NT];
-  x8 q[NT][kSteps][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int row = tile * kRows + 16 * n + column;
-    query[n] = min(row, rows - 1) / p.group;
-    of_group[n] = min(row, rows - 1) - query[n] * p.group;
-    seen[n] = row >= rows ? 0 : p.causal ? min(span.start + query[n] + 1, length) : length;
-    const T* from = static_cast<const T*>(p.q) +
-                    static_cast<std::int64_t>(span.first + query[n]) * p.q_stride +
-                    static_cast<std::int64_t>(head * p.group + of_group[n]) * DIM + 16 * quad;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      __builtin_memcpy(&q[n][i][0], from + 64 * i, sizeof(x8));
-      __builtin_memcpy(&q[n][i][1], from + 64 * i + 8, sizeof(x8));
-    }
-    if (p.negate) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        q[n][i][0] = -q[n][i][0];
-        q[n][i][1] = -q[n][i][1];
-      }
-    }
-  }
-
-  float m[NT], l[NT];
-  floatx4 o[NT][kTiles];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n] = -__builtin_inff();
-    l[n] = 0.0F;
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-      o[n][t] = floatx4{0.0F, 0.0F, 0.0F, 0.0F};
-  }
-  float loud = kQuietest;
-
-  const int quarter = ((stop - begin + kFewWaves * 32 - 1) / (kFewWaves * 32)) * 32;
-  const int wave_begin = begin + wave * quarter;
-  const int wave_stop = min(wave_begin + quarter, stop);
-  const int in_block = (1 << c.block_shift) - 1;
-  const std::size_t half_bytes = static_cast<std::size_t>(DIM) << c.block_shift;
-
-  for (int window = wave_begin; window < wave_stop;) {
-    Window w;
-    const int first_block = window >> c.block_shift;
-    w.Load(p, sequence, head, first_block, wave_stop, lane);
-    const int window_stop = min((first_block + kWave) << c.block_shift, wave_stop);
-
-    struct Codes {
-      u32x4 k[2][kSteps], v[2][kSteps];
-    };
-    const auto load = [&](int key, Codes* d) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int at = min(key, window_stop - 1) + 16 * g;
-        const int block = min((at >> c.block_shift) - first_block, kWave - 1);
-        const int page = max(__builtin_amdgcn_readlane(w.page, block), 0);
-        const unsigned char* from =
-            c.data + (static_cast<std::size_t>(page) * c.kv_heads + head) * 2 * half_bytes +
-            static_cast<std::size_t>(at & in_block & ~15) * DIM;
-        const u32x4* kc = reinterpret_cast<const u32x4*>(from);
-        const u32x4* vc = reinterpret_cast<const u32x4*>(from + half_bytes);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          d->k[g][i] = kc[i * 64 + lane];
-          d->v[g][i] = vc[i * 64 + lane];
-        }
-      }
-    };
-    const auto step = [&](int key, const Codes& d) {
-      float factor[2], level[2];
-      bool there[2];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int block = ((key + 16 * g) >> c.block_shift) - first_block;
-        factor[g] = Lane(w.factor, block);
-        level[g] = Lane(w.level, block);
-        there[g] = __builtin_amdgcn_readlane(w.page, block) >= 0;
-      }
-      const float louder = fmaxf(loud, fmaxf(level[0], level[1]));
-      if (louder > loud) {
-        const float shrink = loud * InversePower(louder);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-            o[n][t] *= shrink;
-        loud = louder;
-      }
-      const float unit = InversePower(loud);
-      x8 weights[NT];
-      floatx4 acc[NT][2];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          acc[n][g] = floatx4{0.0F, 0.0F, 0.0F, 0.0F};
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const x8 a = Operand<T>(d.k[g][i][0], d.k[g][i][1], 1.0F);
-          const x8 b = Operand<T>(d.k[g][i][2], d.k[g][i][3], 1.0F);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[n][g] = X::Mfma16(a, q[n][i][0], acc[n][g]);
-            acc[n][g] = X::Mfma16(b, q[n][i][1], acc[n][g]);
-          }
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float s[2][4];
-        float peak = -__builtin_inff();
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool visible = there[g] && key + 16 * g + 4 * quad + r < seen[n];
-            s[g][r] = visible ? acc[n][g][r] * factor[g] : -__builtin_inff();
-            peak = fmaxf(peak, s[g][r]);
-          }
-        peak = Max32(Max16(peak));
-        if (__any(peak > m[n] + kSlack)) {
-          const float top = peak > m[n] + kSlack ? peak : m[n];
-          const float shrink =
-              top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m[n] - top);
-          m[n] = top;
-          l[n] *= shrink;
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-            o[n][t] *= shrink;
-        }
-        const float from = m[n] == -__builtin_inff() ? 0.0F : m[n];
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int r = 0; r < 4; r += 2) {
-            const typename X::x2 pair = X::Round(__builtin_amdgcn_exp2f(s[g][r] - from),
-                                                 __builtin_amdgcn_exp2f(s[g][r + 1] - from));
-            weights[n][4 * g + r] = pair[0];
-            weights[n][4 * g + r + 1] = pair[1];
-            l[n] = X::AddPair(pair, l[n]);
-          }
-      }
-      const float v0 = fmaxf(level[0] * unit, kQuietest), v1 = fmaxf(level[1] * unit, kQuietest);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const unsigned lo = d.v[0][t / 4][t % 4], hi = d.v[1][t / 4][t % 4];
-        const typename X::x2 a = X::Low(lo, v0), b = X::High(lo, v0);
-        const typename X::x2 e = X::Low(hi, v1), f = X::High(hi, v1);
-        const x8 operand{a[0], a[1], b[0], b[1], e[0], e[1], f[0], f[1]};
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          o[n][t] = X::Mfma16(operand, weights[n], o[n][t]);
-      }
-    };
-
-    Codes even, odd;
-    load(window, &even);
-    for (int key = window; key < window_stop; key += 64) {
-      load(key + 32, &odd);
-      step(key, even);
-      if (key + 32 < window_stop) {
-        load(key + 64, &even);
-        step(key + 32, odd);
-      }
-    }
-    window = window_stop;
-  }
-
-  __shared__ float shared_m[kFewWaves][kRows], shared_l[kFewWaves][kRows];
-  __shared__ floatx4 shared_o[kFewWaves][NT * kTiles][64];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    l[n] = Sum32(Sum16(l[n]));
-    if (quad == 0) {
-      shared_m[wave][16 * n + column] = m[n];
-      shared_l[wave][16 * n + column] = l[n];
-    }
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-      shared_o[wave][n * kTiles + t][lane] = o[n][t] * loud;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int in_tile = 16 * n + column;
-    const int row = tile * kRows + in_tile;
-    float top = -__builtin_inff(), total = 0.0F;
-    float weight[kFewWaves];
-#pragma unroll
-    for (int w = 0; w < kFewWaves; ++w)
-      top = fmaxf(top, shared_m[w][in_tile]);
-    const float from = top == -__builtin_inff() ? 0.0F : top;
-#pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) {
-      weight[w] = __builtin_amdgcn_exp2f(shared_m[w][in_tile] - from);
-      total += shared_l[w][in_tile] * weight[w];
-    }
-    if (row >= rows)
-      continue;
-    const std::size_t slot =
-        p.splits == 1
-            ? 0
-            : ((static_cast<std::size_t>(blockIdx.y) * c.kv_heads + head) * p.splits +
-               blockIdx.z) * kRows + in_tile;
-    if (p.splits > 1 && wave == 0 && quad == 0) {
-      p.partial_m[2 * slot] = top;
-      p.partial_m[2 * slot + 1] = total;
-    }
-    // Nothing seen: zero.
-    const float scale = total == 0.0F ? 0.0F : 1.0F / total;
-    T* to = static_cast<T*>(p.out) +
-            static_cast<std::int64_t>(span.first + query[n]) * p.out_stride +
-            static_cast<std::int64_t>(head * p.group + of_group[n]) * DIM + 4 * quad;
-    for (int t = wave; t < kTiles; t += kFewWaves) {
-      floatx4 sum = {};
-#pragma unroll
-      for (int w = 0; w < kFewWaves; ++w)
-        sum += shared_o[w][n * kTiles + t][lane] * weight[w];
-      if (p.splits > 1) {
-        *reinterpret_cast<floatx4*>(p.partial_o + slot * DIM + 16 * t + 4 * quad) = sum;
-      } else {
-        T rounded[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          rounded[r] = static_cast<T>(sum[r] * scale);
-        __builtin_memcpy(to + 16 * t, rounded, sizeof(rounded));
-      }
-    }
-  }
-}
-
-constexpr int kManyWaves = 4;
-constexpr int kManyRows = 32 * kManyWaves;
-
-// The same for tiles of many rows, whose values are converted for all at once:
-// lane i holds where its block's head begins, the scores' factor, and the
-// values' scale over `loud`, the loudest of this window's blocks and all before.
-struct TileWindow {
   unsigned offset_low, offset_high;
   float factor, unit;
   float loud;                // the same in every lane
   unsigned long long there;  // a bit for each block that there is
-  __device__ __forceinline__ void Load(const CacheAttentionParams& p, int sequence, int head,
-                                       int first, int stop, int lane) {
-    const CacheView& c = p.cache;
+  __device__ __forceinline__ void LoadPages(const CacheView& c, int sequence, int head, int first,
+                                            int stop, int lane) {
     const int block = first + lane;
     const int page = (block << c.block_shift) < stop ? PageOf(c, sequence, block) : -1;
     there = __ballot(page >= 0);
-    const std::size_t at = ScaleIndex(c, max(page, 0), head, 0);
-    const float k_scale = c.scales[at], v_scale = c.scales[at + 1];
-    const std::size_t offset = at * (static_cast<std::size_t>(c.dim) << c.block_shift);
+    const std::size_t offset =
+        ScaleIndex(c, max(page, 0), head, 0) * (static_cast<std::size_t>(c.dim) << c.block_shift);
     offset_low = static_cast<unsigned>(offset);
     offset_high = static_cast<unsigned>(offset >> 32);
+    scale_at = ScaleIndex(c, max(page, 0), head, 0);
+  }
+  __device__ __forceinline__ void LoadScales(const CacheAttentionParams& p, int lane) {
+    const float k_scale = p.cache.scales[scale_at], v_scale = p.cache.scales[scale_at + 1];
+    const bool here = (there >> lane & 1) != 0;
     // A NaN scale, of keys or values, makes the block's scores NaN.
-    factor = page < 0 ? 0.0F : p.scale_log2 * k_scale + 0.0F * v_scale;
-    const float level = page < 0 ? 0.0F : Loudness(v_scale);
-    loud = fmaxf(loud, WaveMax(level));
+    factor = here ? p.scale_log2 * k_scale + 0.0F * v_scale : 0.0F;
+    const float level = here ? Loudness(v_scale) : 0.0F;
+    loud = fmaxf(loud, WaveMaxFast(level));
     unit = fmaxf(level * InversePower(loud), kQuietest);
   }
   __device__ __forceinline__ const unsigned char* Base(const unsigned char* data, int i) const {
@@ -468,329 +221,335 @@ struct TileWindow {
     const std::size_t high = __builtin_amdgcn_readlane(offset_high, i);
     return data + (high << 32 | (low & 0xFFFFFFFFu));
   }
+
+ private:
+  std::size_t scale_at;
 };
 
-// What a tile needs beside its codes: a factor for each of its blocks.
-template <int BLOCKS>
-struct TileScales {
-  typedef float vec __attribute__((ext_vector_type(BLOCKS)));
-  vec factor;
-  float loud;      // that its values are converted at
-  float unit;      // of the values that this thread converts
-  unsigned there;  // a bit for each block
-};
-
-// Many rows: a work-group of four waves takes 128 rows of one sequence and kv
-// head, 32 a wave, and goes over the keys in tiles of 64 (128 at 64 dims) that
-// the waves share. The threads fetch a tile's codes ahead, convert them once and
-// leave them in LDS in the order of the operands of v_mfma_f32_32x32x16 (64 lanes
-// of 16 bytes in a row, so every write and read is a conflict-free 16 bytes a
-// lane), in two buffers of 16 KB each for keys and values. The softmax runs in
-// registers, a row in a lane and its partner lane ^ 32. While a tile's
-// probabilities are formed, on the vector unit, the matrix cores form the next
-// tile's scores, which depend on nothing of it; so in iteration i the waves read
-// keys i + 1 and values i and write keys i + 2 and values i + 1, and one barrier
-// an iteration suffices.
-template <typename T, int DIM, int SHIFT>
-__global__ __launch_bounds__(kManyWaves* kWave, 2) void ManyRowsKernel(CacheAttentionParams p) {
+// ROWS rows (16 or 32) on v_mfma_f32_16x16x32 or v_mfma_f32_32x32x16: lane l holds
+// row l % ROWS and is part l / ROWS of it. Of every 16 keys a part holds four in a
+// row at 4 part (and with two parts the four at 8 more). A lane's 16 bytes of a key
+// are 16 dims, the next part's the next 16; which dim meets which is the same for the
+// queries. A lane's bytes of the values are four keys of dims 16 apart: with 16 rows
+// the output's tile t is dims 16 t .. + 15; with 32 its two halves of rows stand for
+// dims 64 apart (128 dims) or 32 apart (64).
+// ONE: 32 keys are of one block (blocks of 32 or 64 tokens), else of two of 16.
+template <typename T, int DIM, int ROWS, bool ONE>
+__global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
+    CacheAttentionParams p) {
   typedef Types<T> X;
   typedef typename X::x8 x8;
-  constexpr int kKeys = 8192 / DIM;          // of a tile
-  constexpr int kGroups = kKeys / 16, kBlocks = kKeys / 32;
-  constexpr int kK = DIM / 16;               // contraction steps of the scores
-  constexpr int kDims = DIM / 32;            // blocks of 32 dims
-  constexpr int kChunks = DIM;               // 16-byte chunks of a group's keys or values
-  constexpr int kSums = 4;                   // of a row in a lane, to be added at the end
-  constexpr int kPages = kKeys >> SHIFT;     // blocks of the pool in a tile: 1 to 8
-  constexpr std::size_t kHalf = static_cast<std::size_t>(DIM) << SHIFT;  // bytes
-  typedef TileScales<kPages> Scales;
-  __shared__ x8 key_tiles[2][kKeys * DIM / 8];
-  __shared__ x8 value_tiles[2][kKeys * DIM / 8];
+  constexpr int kParts = kWave / ROWS;
+  constexpr int kSteps = DIM / 16 / kParts;  // 16-byte loads of a key's codes in a lane
+  constexpr int kOfGroup = 16 / kParts;      // a lane's keys of 16
+  constexpr int kTiles = DIM / ROWS;         // of the output
+  constexpr int kFours = ROWS * ROWS / 256;  // a lane's runs of four rows of a tile
+  typedef float acc_t __attribute__((ext_vector_type(4 * kFours)));
+  // A lane's codes of the values of 16 keys: loads, and the bytes of one.
+  constexpr int kValueLoads = ROWS == 16 ? DIM / 64 : 2;
+  constexpr int kValueWords = ROWS == 16 ? 4 : DIM / 32;
+  typedef unsigned value_t __attribute__((ext_vector_type(kValueWords)));
   const CacheView& c = p.cache;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int column = lane & 31, half = lane >> 5;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int column = lane % ROWS, part = lane / ROWS;
   const int head = blockIdx.x;
 
   // The last rows of a causal sequence see the most keys: they start first.
   const int item = gridDim.y - 1 - blockIdx.y;
-  int tile = item;
-  const int sequence = __builtin_amdgcn_readfirstlane(SequenceOfItem(c, p.group, 7, 1, &tile));
-  tile = __builtin_amdgcn_readfirstlane(tile);
-  const Span span = SpanOf(c, sequence);
+  const Found found = FindItem(c, p.group, ROWS == 16 ? 4 : 5, 1, item);
+  const int sequence = found.sequence, tile = found.item;
+  const Span span = found.span;
   const int rows = span.count * p.group;
-  if (tile < 0 || tile * kManyRows >= rows)
+  if (tile < 0 || tile * ROWS >= rows)
     return;
   const int length = min(span.length, c.table_width << c.block_shift);
-  const int last = min(tile * kManyRows + kManyRows, rows) - 1;
-  const int end = p.causal ? min(span.start + last / p.group + 1, length) : length;
+  // Keys that any row of the tile sees, those of this split, and those every row sees.
+  const RowSplit split(p, tile * ROWS);
+  const int last = min(tile * ROWS + ROWS, rows) - 1;
+  const int end = p.causal ? min(span.start + split.At(last) + 1, length) : length;
   const int chunk = ChunkOf(length, p.splits);
   const int begin = blockIdx.z * chunk;
   const int stop = min(begin + chunk, end);
+  const int all_see = p.causal ? min(span.start + split.query + 1, length) : length;
 
-  const int first_row = tile * kManyRows + 32 * wave;
-  const int row = first_row + column;
-  const int query = min(row, rows - 1) / p.group;
-  const int of_group = min(row, rows - 1) - query * p.group;
-  const int seen = row >= rows ? 0 : p.causal ? min(span.start + query + 1, length) : length;
-  // Keys that every row of the wave sees, and that any does.
-  const int all_see = first_row + 31 >= rows ? 0
-                      : p.causal             ? min(span.start + first_row / p.group + 1, length)
-                                             : length;
-  const int wave_end =
-      first_row >= rows ? 0
-      : p.causal ? min(span.start + min(first_row + 31, rows - 1) / p.group + 1, length)
-                 : length;
-
-  x8 q[kK];
+  // Rows past the last one repeat it; nothing of theirs is stored.
+  const int row = tile * ROWS + column;
+  int of_group;
+  const int query = split.Of(min(row, rows - 1) - tile * ROWS, &of_group);
+  const int seen = p.causal ? min(span.start + query + 1, length) : length;
+  x8 q[kSteps][2];
   {
     const T* from = static_cast<const T*>(p.q) +
                     static_cast<std::int64_t>(span.first + query) * p.q_stride +
-                    static_cast<std::int64_t>(head * p.group + of_group) * DIM + 8 * half;
+                    static_cast<std::int64_t>(head * p.group + of_group) * DIM + 16 * part;
 #pragma unroll
-    for (int i = 0; i < kK; ++i)
-      __builtin_memcpy(&q[i], from + 16 * i, sizeof(x8));
+    for (int i = 0; i < kSteps; ++i) {
+      __builtin_memcpy(&q[i][0], from + 16 * kParts * i, sizeof(x8));
+      __builtin_memcpy(&q[i][1], from + 16 * kParts * i + 8, sizeof(x8));
+    }
     if (p.negate) {
 #pragma unroll
-      for (int i = 0; i < kK; ++i)
-        q[i] = -q[i];
+      for (int i = 0; i < kSteps; ++i) {
+        q[i][0] = -q[i][0];
+        q[i][1] = -q[i][1];
+      }
     }
   }
 
-  float m = -__builtin_inff();
-  float l[kSums] = {};
-  floatx16 o[kDims];
+  float m = -__builtin_inff(), l[2] = {0.0F, 0.0F};
+  acc_t o[kTiles];
 #pragma unroll
-  for (int t = 0; t < kDims; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      o[t][r] = 0.0F;
+  for (int t = 0; t < kTiles; ++t)
+    o[t] = acc_t(0.0F);
   float loud = kQuietest;
 
-  TileWindow window;
-  window.loud = kQuietest;
-  int window_first = 0, window_stop = begin;  // block, key
+  const int quarter = ((stop - begin + kWaves * 32 - 1) / (kWaves * 32)) * 32;
+  const int wave_begin = begin + wave * quarter;
+  const int wave_stop = min(wave_begin + quarter, stop);
+  const int in_block = (1 << c.block_shift) - 1;
+  const std::size_t half_bytes = static_cast<std::size_t>(DIM) << c.block_shift;
+  // With 32 rows a lane's key is of the first or the second 16, and its values of
+  // the tiles' first or second 16 rows.
+  const int second = ROWS == 16 ? 0 : (lane >> 4) & 1;
+  const int key_at = part * 256 + (lane & 15) * 16;
+  const int value_at = key_at + second * (DIM == 128 ? 1024 : 8);
 
-  // A thread's chunks of a tile: two of keys (chunk tid + 256 i: group, dims / 16,
-  // token) and a pair of values (group, dims / 64, quad and quad + 2, dim % 16), whose
-  // eight tokens make one lane's operand.
-  const int value_group = tid / (DIM / 2), value_at = tid % (DIM / 2);
-  const int value_chunk = (value_at >> 5) * 64 + (value_at & 31);
-  u32x4 k_codes[2], v_codes[2];
-  // The tile's scales, the codes of its keys on their way, and where its values are.
-  // A tile begins with a block or with a whole part of one.
-  const auto fetch_keys = [&](int key, const u32x4** values) {
-    if (key >= window_stop) {  // never in the middle of a tile: 64 blocks are whole ones
-      window_first = key >> SHIFT;
-      window.Load(p, sequence, head, window_first, stop, lane);
-      window_stop = (window_first + kWave) << SHIFT;
-    }
-    const int block = (key >> SHIFT) - window_first;
-    const auto base = [&](int group) {
-      return window.Base(c.data, block + ((16 * group) >> SHIFT)) +
-             (16 * group & ((1 << SHIFT) - 1)) * DIM;
+  Window w;
+  w.loud = kQuietest;
+  for (int window = wave_begin; window < wave_stop;) {
+    const int first_block = window >> c.block_shift;
+    w.LoadPages(c, sequence, head, first_block, wave_stop, lane);
+    const int window_stop = min((first_block + kWave) << c.block_shift, wave_stop);
+    const int last_step = window + ((window_stop - 1 - window) & ~31);
+
+    struct Codes {
+      u32x4 k[32 / ROWS][kSteps];  // with 16 rows of two groups, else of the lane's own
+      value_t v[2][kValueLoads];
     };
-    Scales s;
-    s.loud = window.loud;
-    s.there = static_cast<unsigned>(window.there >> block) & ((1u << kPages) - 1);
+    const auto load = [&](int key, Codes* d) {
+      const int at = min(key, last_step);
+      const int block = (at >> c.block_shift) - first_block;
+      const unsigned char* group[2];
+      group[0] = w.Base(c.data, block) + (ONE ? at & in_block : 0) * DIM;
+      group[1] = ONE ? group[0] + 16 * DIM : w.Base(c.data, block + 1);
 #pragma unroll
-    for (int g = 0; g < kPages; ++g)
-      s.factor[g] = Lane(window.factor, block + g);
-    if constexpr (DIM == 128) {
+      for (int g = 0; g < 32 / ROWS; ++g) {
+        const unsigned char* from = ROWS == 16 ? group[g] : second == 0 ? group[0] : group[1];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        k_codes[i] = reinterpret_cast<const u32x4*>(
-            base(2 * i + (wave >> 1)))[(wave & 1) * 64 + lane];
-      *values = reinterpret_cast<const u32x4*>(base(wave) + kHalf) + value_chunk;
-      s.unit = Lane(window.unit, block + ((16 * wave) >> SHIFT));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        k_codes[i] = reinterpret_cast<const u32x4*>(base(4 * i + wave))[lane];
-      const unsigned char* even = base(2 * wave);
-      const unsigned char* odd = base(2 * wave + 1);
-      *values = reinterpret_cast<const u32x4*>((half == 0 ? even : odd) + kHalf) + value_chunk;
-      const float even_unit = Lane(window.unit, block + ((32 * wave) >> SHIFT));
-      const float odd_unit = Lane(window.unit, block + ((32 * wave + 16) >> SHIFT));
-      s.unit = half == 0 ? even_unit : odd_unit;
-    }
-    return s;
-  };
-  const auto fetch_values = [&](const u32x4* values) {
-    v_codes[0] = values[0];
-    v_codes[1] = values[32];
-  };
-  const auto convert_keys = [&](int buffer) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int index = tid + i * 256;
-      const int group = index / kChunks, at = index % kChunks;
-      x8* to = key_tiles[buffer] + ((group >> 1) * kK + (at >> 4)) * 64 + (group & 1) * 16 +
-               (at & 15);
-      to[0] = Operand<T>(k_codes[i][0], k_codes[i][1], 1.0F);
-      to[32] = Operand<T>(k_codes[i][2], k_codes[i][3], 1.0F);
-    }
-  };
-  const auto convert_values = [&](const Scales& s, int buffer) {
-    const int d = value_at & 15, h = (value_at >> 4) & 1, quarter = value_at >> 5;
-    x8* to = value_tiles[buffer] + (value_group * kDims + 2 * quarter) * 64 + 32 * h + d;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      to[(t >> 1) * 64 + (t & 1) * 16] = Operand<T>(v_codes[0][t], v_codes[1][t], s.unit);
-  };
-  floatx16 scores[kBlocks];
-  const auto score = [&](int buffer, floatx16 (&to)[kBlocks]) {
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      floatx16 acc;
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        acc[r] = 0.0F;
-#pragma unroll
-      for (int i = 0; i < kK; ++i)
-        acc = X::Mfma32(key_tiles[buffer][(b * kK + i) * 64 + lane], q[i], acc);
-      to[b] = acc;
-    }
-  };
-
-  if (begin < stop) {
-    // Tiles now, one and two ahead; past the last one the scales and codes of
-    // whatever block 0 holds, which nothing takes.
-    const u32x4 *values, *values_next, *values_after;
-    Scales now = fetch_keys(begin, &values);
-    fetch_values(values);
-    convert_keys(0);
-    convert_values(now, 0);
-    Scales next = fetch_keys(begin + kKeys, &values_next);
-    fetch_values(values_next);
-    convert_keys(1);
-    Scales after = fetch_keys(begin + 2 * kKeys, &values_after);
-    __syncthreads();
-    score(0, scores);
-    __syncthreads();
-    int buffer = 0;  // of this tile's keys and values
-    for (int key = begin; key < stop; key += kKeys) {
-      if (now.loud > loud) {
-        const float shrink = loud * InversePower(now.loud);
-#pragma unroll
-        for (int t = 0; t < kDims; ++t)
-          o[t] *= shrink;
-        loud = now.loud;
+        for (int i = 0; i < kSteps; ++i)
+          d->k[g][i] = *reinterpret_cast<const u32x4*>(from + key_at + 256 * kParts * i);
       }
-      if (key < wave_end) {
-        typename Scales::vec factor = now.factor;
-        const auto page_of = [](int group) { return (16 * group) >> SHIFT; };
-        if (now.there != (1u << kPages) - 1 || key + kKeys > all_see) {
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g)
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-              const int e = 8 * (g & 1) + r;
-              const int at = key + 16 * g + 8 * (r / 4) + 4 * half + r % 4;
-              scores[g / 2][e] = (now.there >> page_of(g) & 1) != 0 && at < seen
-                                     ? scores[g / 2][e] * factor[page_of(g)]
-                                     : -__builtin_inff();
-            }
+        for (int i = 0; i < kValueLoads; ++i)
+          d->v[g][i] = *reinterpret_cast<const value_t*>(group[g] + half_bytes + value_at +
+                                                         (ROWS == 16 ? 1024 : 512) * i);
+    };
+    const auto step = [&](int key, const Codes& d) {
+      const int block = (key >> c.block_shift) - first_block;
+      float factor[2], unit[2];
+      bool there[2];
 #pragma unroll
-          for (int g = 0; g < kPages; ++g)
-            factor[g] = 1.0F;
-        }
-        float peak = -__builtin_inff();
+      for (int g = 0; g < 2; ++g) {
+        const int at = ONE ? block : block + g;
+        factor[g] = Lane(w.factor, at);
+        unit[g] = Lane(w.unit, at);
+        there[g] = (w.there >> at & 1) != 0;
+      }
+      float s[2][kOfGroup];
+      if constexpr (ROWS == 16) {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          float most = -__builtin_inff();
+        for (int g = 0; g < 2; ++g) {
+          floatx4 acc = {};
 #pragma unroll
-          for (int r = 0; r < 8; ++r)
-            most = fmaxf(most, scores[g / 2][8 * (g & 1) + r]);
-          peak = fmaxf(peak, most * factor[page_of(g)]);
-        }
-        peak = Max32(peak);
-        if (__any(peak > m + kSlack)) {
-          const float top = peak > m + kSlack ? peak : m;
-          const float shrink = top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m - top);
-          m = top;
-#pragma unroll
-          for (int i = 0; i < kSums; ++i)
-            l[i] *= shrink;
-#pragma unroll
-          for (int t = 0; t < kDims; ++t)
-            o[t] *= shrink;
-        }
-        const float from = m == -__builtin_inff() ? 0.0F : m;
-        floatx16 coming[kBlocks];
-        score(buffer ^ 1, coming);
-        x8 weights[kGroups];
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-#pragma unroll
-          for (int r = 0; r < 8; r += 2) {
-            const int e = 8 * (g & 1) + r;
-            const typename X::x2 pair = X::Round(
-                __builtin_amdgcn_exp2f(__builtin_fmaf(scores[g / 2][e], factor[page_of(g)], -from)),
-                __builtin_amdgcn_exp2f(__builtin_fmaf(scores[g / 2][e + 1], factor[page_of(g)], -from)));
-            weights[g][r] = pair[0];
-            weights[g][r + 1] = pair[1];
-            l[r / 2] = X::AddPair(pair, l[r / 2]);
+          for (int i = 0; i < kSteps; ++i) {
+            acc = X::Mfma16(Operand<T>(d.k[g][i][0], d.k[g][i][1], 1.0F), q[i][0], acc);
+            acc = X::Mfma16(Operand<T>(d.k[g][i][2], d.k[g][i][3], 1.0F), q[i][1], acc);
           }
+#pragma unroll
+          for (int r = 0; r < kOfGroup; ++r)
+            s[g][r] = acc[r];
+        }
+      } else {
+        floatx16 acc = {};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          acc = X::Mfma32(Operand<T>(d.k[0][i][0], d.k[0][i][1], 1.0F), q[i][0], acc);
+          acc = X::Mfma32(Operand<T>(d.k[0][i][2], d.k[0][i][3], 1.0F), q[i][1], acc);
         }
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-          for (int t = 0; t < kDims; ++t)
-            o[t] = X::Mfma32(value_tiles[buffer][(g * kDims + t) * 64 + lane], weights[g], o[t]);
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-          scores[b] = coming[b];
-        convert_keys(buffer);
-        convert_values(next, buffer ^ 1);
-      } else {
-        convert_keys(buffer);
-        convert_values(next, buffer ^ 1);
+        for (int r = 0; r < 16; ++r)
+          s[r / 8][r % 8] = acc[r];
       }
-      fetch_values(values_after);
-      now = next;
-      next = after;
-      after = fetch_keys(key + 3 * kKeys, &values_after);
-      buffer ^= 1;
-      __syncthreads();
+      // Where some row does not see all of the step, what it does not is -inf and the
+      // factors have been taken.
+      if (!(there[0] && there[1]) || key + 32 > all_see) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+#pragma unroll
+          for (int r = 0; r < kOfGroup; ++r) {
+            const int at = key + 16 * g + 4 * (part + kParts * (r / 4)) + r % 4;
+            s[g][r] = there[g] && at < seen ? s[g][r] * factor[g] : -__builtin_inff();
+          }
+          factor[g] = 1.0F;
+        }
+      }
+      float peak = -__builtin_inff();
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        float most = s[g][0];
+#pragma unroll
+        for (int r = 1; r < kOfGroup; ++r)
+          most = fmaxf(most, s[g][r]);
+        peak = fmaxf(peak, factor[g] * most);
+      }
+      peak = RowMax<ROWS>(peak);
+      if (__any(peak > m + kSlack)) {
+        const float top = peak > m + kSlack ? peak : m;
+        const float shrink = top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l[0] *= shrink;
+        l[1] *= shrink;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+          o[t] *= shrink;
+      }
+      const float from = m == -__builtin_inff() ? 0.0F : m;
+      typename X::x2 w2[2][kOfGroup / 2];  // the weights
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int r = 0; r < kOfGroup; r += 2) {
+          w2[g][r / 2] = X::Round(
+              __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][r], factor[g], -from)),
+              __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][r + 1], factor[g], -from)));
+          l[r / 2 % 2] = X::AddPair(w2[g][r / 2], l[r / 2 % 2]);
+        }
+      if constexpr (ROWS == 16) {
+        const x8 weights = {w2[0][0][0], w2[0][0][1], w2[0][1][0], w2[0][1][1],
+                            w2[1][0][0], w2[1][0][1], w2[1][1][0], w2[1][1][1]};
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const unsigned lo = d.v[0][t / 4][t % 4], hi = d.v[1][t / 4][t % 4];
+          const typename X::x2 a = X::Low(lo, unit[0]), b = X::High(lo, unit[0]);
+          const typename X::x2 e = X::Low(hi, unit[1]), f = X::High(hi, unit[1]);
+          const x8 operand{a[0], a[1], b[0], b[1], e[0], e[1], f[0], f[1]};
+          o[t] = X::Mfma16(operand, weights, o[t]);
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const x8 weights = {w2[g][0][0], w2[g][0][1], w2[g][1][0], w2[g][1][1],
+                              w2[g][2][0], w2[g][2][1], w2[g][3][0], w2[g][3][1]};
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            o[t] = X::Mfma32(Operand<T>(d.v[g][0][t], d.v[g][1][t], unit[g]), weights, o[t]);
+        }
+      }
+    };
+
+    // A step's codes are on their way while the one before is worked on. With 16 rows
+    // the loop is kept small and not unrolled: a short call runs it a few times only,
+    // from an instruction cache that has not seen it (430 keys: 7.0 us of the kernel,
+    // 8.2 unrolled four times); with 32 rows two steps save the copies of the codes
+    // (two causal prompts of up to 5000 tokens 238 -> 231 us). The load past the end
+    // fetches the last step again, under no condition, so that the waits stay exact.
+    Codes now;
+    load(window, &now);
+    w.LoadScales(p, lane);  // behind the first codes, which only wait for the pages
+    if (w.loud > loud) {
+      const float shrink = loud * InversePower(w.loud);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        o[t] *= shrink;
+      loud = w.loud;
     }
+    if constexpr (ROWS == 16) {
+#pragma unroll 1
+      for (int key = window; key < window_stop; key += 32) {
+        Codes next;
+        load(key + 32, &next);
+        step(key, now);
+        now = next;
+      }
+    } else {
+#pragma unroll 1
+      for (int key = window; key < window_stop; key += 64) {
+        Codes next;
+        load(key + 32, &next);
+        step(key, now);
+        if (key + 32 >= window_stop)
+          break;
+        load(key + 64, &now);
+        step(key + 32, next);
+      }
+    }
+    window = window_stop;
   }
 
-  const float total = Sum32((l[0] + l[1]) + (l[2] + l[3]));
+  __shared__ float shared_m[kWaves][ROWS], shared_l[kWaves][ROWS];
+  __shared__ floatx4 shared_o[kWaves][kTiles * kFours][64];
+  const float sum = RowSum<ROWS>(l[0] + l[1]);
+  if (part == 0) {
+    shared_m[wave][column] = m;
+    shared_l[wave][column] = sum;
+  }
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int i = 0; i < kFours; ++i)
+      shared_o[wave][t * kFours + i][lane] =
+          floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]} * loud;
+  __syncthreads();
+  float top = -__builtin_inff(), total = 0.0F;
+  float weight[kWaves];
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i)
+    top = fmaxf(top, shared_m[i][column]);
+  const float from = top == -__builtin_inff() ? 0.0F : top;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    weight[i] = __builtin_amdgcn_exp2f(shared_m[i][column] - from);
+    total += shared_l[i][column] * weight[i];
+  }
   if (row >= rows)
     return;
-  if (p.splits > 1) {
-    const std::size_t slot =
-        ((static_cast<std::size_t>(item) * c.kv_heads + head) * p.splits + blockIdx.z) *
-            kManyRows + 32 * wave + column;
-    if (half == 0) {
-      p.partial_m[2 * slot] = m;
-      p.partial_m[2 * slot + 1] = total;
-    }
-#pragma unroll
-    for (int t = 0; t < kDims; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const floatx4 part = {o[t][r] * loud, o[t][r + 1] * loud, o[t][r + 2] * loud,
-                              o[t][r + 3] * loud};
-        *reinterpret_cast<floatx4*>(p.partial_o + slot * DIM + 32 * t + 2 * r + 4 * half) = part;
-      }
-    return;
+  const std::size_t slot =
+      p.splits == 1
+          ? 0
+          : ((static_cast<std::size_t>(item) * c.kv_heads + head) * p.splits + blockIdx.z) * ROWS +
+                column;
+  if (p.splits > 1 && wave == 0 && part == 0) {
+    p.partial_m[2 * slot] = top;
+    p.partial_m[2 * slot + 1] = total;
   }
   // Nothing seen: zero.
-  const float scale = total == 0.0F ? 0.0F : loud / total;
+  const float scale = total == 0.0F ? 0.0F : 1.0F / total;
   T* to = static_cast<T*>(p.out) + static_cast<std::int64_t>(span.first + query) * p.out_stride +
-          static_cast<std::int64_t>(head * p.group + of_group) * DIM + 4 * half;
+          static_cast<std::int64_t>(head * p.group + of_group) * DIM;
 #pragma unroll
-  for (int t = 0; t < kDims; ++t)
+  for (int j = wave; j < kTiles * kFours; j += kWaves) {
+    floatx4 sum = {};
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
+    for (int i = 0; i < kWaves; ++i)
+      sum += shared_o[i][j][lane] * weight[i];
+    // The dims of rows 8 (j % 4) + 4 part .. + 3 of tile j / 4, or 4 part .. + 3 of j.
+    const int t = j / 4, high = j % 4 / 2, d = 8 * (j % 2) + 4 * part;
+    const int dim = ROWS == 16   ? 16 * j + 4 * part
+                    : DIM == 128 ? 64 * high + 16 * t + d
+                                 : 32 * high + 16 * t + d;
+    if (p.splits > 1) {
+      *reinterpret_cast<floatx4*>(p.partial_o + slot * DIM + dim) = sum;
+    } else {
       T rounded[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        rounded[e] = static_cast<T>(o[t][r + e] * scale);
-      __builtin_memcpy(to + 32 * t + 2 * r, rounded, sizeof(rounded));
+      for (int r = 0; r < 4; ++r)
+        rounded[r] = static_cast<T>(sum[r] * scale);
+      __builtin_memcpy(to + dim, rounded, sizeof(rounded));
     }
+  }
 }
 
 // Joins the splits of one row: DIM / 4 lanes hold four of its dims each, and the
@@ -799,9 +558,9 @@ template <typename T, int DIM>
 __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
   constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
   const CacheView& c = p.cache;
-  int tile = blockIdx.y;
-  const int sequence = SequenceOfItem(c, p.group, p.tile_shift, 1, &tile);
-  const Span span = SpanOf(c, sequence);
+  const Found found = FindItem(c, p.group, p.tile_shift, 1, blockIdx.y);
+  const int tile = found.item;
+  const Span span = found.span;
   const int rows = span.count * p.group;
   const int in_tile = blockIdx.z;
   const int row = (tile << p.tile_shift) + in_tile;
@@ -861,7 +620,8 @@ __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
   for (int g = 1; g < kGroups; ++g)
     sum += sums[g][part];
   const float scale = total == 0.0F ? 0.0F : 1.0F / total;
-  const int query = row / p.group, of_group = row % p.group;
+  int of_group;
+  const int query = RowSplit(p, row).Of(0, &of_group);
   T rounded[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -877,9 +637,9 @@ template <typename T, int DIM>
 __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
   constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
   const CacheView& c = p.cache;
-  int tile = blockIdx.y;
-  const int sequence = SequenceOfItem(c, p.group, p.tile_shift, 1, &tile);
-  const Span span = SpanOf(c, sequence);
+  const Found found = FindItem(c, p.group, p.tile_shift, 1, blockIdx.y);
+  const int tile = found.item;
+  const Span span = found.span;
   const int rows = span.count * p.group;
   const int tid = threadIdx.x, part = tid % kLanes;
   const int in_tile = blockIdx.z * kGroups + tid / kLanes;
@@ -913,7 +673,8 @@ __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
       sum += o[s] * w;
   }
   const float scale = total == 0.0F ? 0.0F : 1.0F / total;
-  const int query = row / p.group, of_group = row % p.group;
+  int of_group;
+  const int query = RowSplit(p, row).Of(0, &of_group);
   T rounded[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -927,18 +688,13 @@ __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
 template <typename T, int DIM>
 void Launch(const CacheAttentionParams& p, hipStream_t stream) {
   const int items = ItemBound(p.cache, p.group, p.tile_shift, 1);
-  const dim3 grid(p.cache.kv_heads, items, p.splits), block(kFewWaves * kWave);
-  const bool last = p.splits == 1;
-  if (p.tile_shift == 4)
-    Dispatch(FewRowsKernel<T, DIM, 1>, grid, block, 0, stream, true, last, p);
-  else if (p.tile_shift == 5)
-    Dispatch(FewRowsKernel<T, DIM, 2>, grid, block, 0, stream, true, last, p);
-  else if (p.cache.block_shift == 4)
-    Dispatch(ManyRowsKernel<T, DIM, 4>, grid, block, 0, stream, true, last, p);
-  else if (p.cache.block_shift == 5)
-    Dispatch(ManyRowsKernel<T, DIM, 5>, grid, block, 0, stream, true, last, p);
-  else
-    Dispatch(ManyRowsKernel<T, DIM, 6>, grid, block, 0, stream, true, last, p);
+  const dim3 grid(p.cache.kv_heads, items, p.splits), block(kWaves * kWave);
+  const bool one = p.cache.block_shift > 4, last = p.splits == 1;
+  const auto kernel = p.tile_shift == 4 ? one ? CacheAttentionKernel<T, DIM, 16, true>
+                                              : CacheAttentionKernel<T, DIM, 16, false>
+                      : one             ? CacheAttentionKernel<T, DIM, 32, true>
+                                        : CacheAttentionKernel<T, DIM, 32, false>;
+  Dispatch(kernel, grid, block, 0, stream, true, last, p);
   if (last)
     return;
   constexpr int kJoined = 256 / (DIM / 4);  // rows of a work-group with few splits
@@ -958,20 +714,19 @@ CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group) {
   if (c.rows == 0)
     return plan;
   // Rows of a sequence on average: 16 columns of the matrix operand where they
-  // suffice, else 32, which halve what is read of the codes again.
+  // suffice, else 32.
   const std::int64_t all = static_cast<std::int64_t>(c.rows) * group;
-  plan.tile_shift = all <= 16ll * c.count ? 4 : all <= 48ll * c.count ? 5 : 7;
+  const bool few = all <= 16ll * c.count;
+  plan.tile_shift = few ? 4 : 5;
   const int items = ItemBound(c, group, plan.tile_shift, 1);
   const std::int64_t groups = static_cast<std::int64_t>(items) * c.kv_heads;
   const std::int64_t capacity = static_cast<std::int64_t>(c.table_width) << c.block_shift;
-  const std::int64_t aim = plan.tile_shift == 7                   ? kManyGroups
-                           : plan.tile_shift == 4 && c.count > 1 ? kRaggedSplitGroups
-                                                                 : kSplitGroups;
-  const std::int64_t least = plan.tile_shift == 7 ? 2 * kLeastChunk : kLeastChunk;
   const std::int64_t wanted =
-      plan.tile_shift == 7 ? aim / groups : (aim + groups - 1) / groups;
+      !few ? kSplitGroups / groups
+           : ((c.count > 1 ? kRaggedSplitGroups : kSplitGroups) + groups - 1) / groups;
   plan.splits = static_cast<int>(std::max<std::int64_t>(
-      1, std::min({wanted, capacity / least, std::int64_t{kMostSplits}})));
+      1, std::min({wanted, capacity / (few ? kLeastChunk : kLeastTileChunk),
+                   std::int64_t{kMostSplits}})));
   if (plan.splits > 1)
     plan.slots = (static_cast<std::size_t>(groups) * plan.splits) << plan.tile_shift;
   return plan;

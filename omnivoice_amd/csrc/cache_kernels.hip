@@ -69,14 +69,14 @@ struct Touched {
   int block, page;  // block of the sequence, of the pool
 };
 __device__ __forceinline__ bool Find(const CacheView& c, int item, Touched* t) {
-  const int sequence = SequenceOfItem(c, 1, c.block_shift, 2, &item);
-  t->span = SpanOf(c, sequence);
-  if (t->span.count == 0)
+  const Found f = FindItem(c, 1, c.block_shift, 2, item);
+  t->span = f.span;
+  if (f.span.count == 0 || f.item < 0)
     return false;
-  t->block = (t->span.start >> c.block_shift) + item;
-  if (t->block > (t->span.length - 1) >> c.block_shift)
+  t->block = (f.span.start >> c.block_shift) + f.item;
+  if (t->block > (f.span.length - 1) >> c.block_shift)
     return false;
-  t->page = PageOf(c, sequence, t->block);
+  t->page = PageOf(c, f.sequence, t->block);
   return true;
 }
 

@@ -123,6 +123,27 @@ __device__ __forceinline__ float WaveSumFast(float v) {
   return (r0 + r1) + (r2 + r3);
 }
 
+// Wave maximum the same way.
+template <int CTRL>
+__device__ __forceinline__ float DppMax(float v) {
+  const int bits = __builtin_bit_cast(int, v);
+  const int moved = __builtin_amdgcn_update_dpp(bits, bits, CTRL, 0xF, 0xF, false);
+  return fmaxf(v, __builtin_bit_cast(float, moved));
+}
+
+__device__ __forceinline__ float WaveMaxFast(float v) {
+  v = DppMax<0xB1>(v);
+  v = DppMax<0x4E>(v);
+  v = DppMax<0x141>(v);
+  v = DppMax<0x140>(v);
+  const int bits = __builtin_bit_cast(int, v);
+  const float r0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 0));
+  const float r1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 16));
+  const float r2 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 32));
+  const float r3 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 48));
+  return fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
+}
+
 __device__ __forceinline__ float WaveMax(float v) {
   for (int offset = kWave / 2; offset > 0; offset /= 2)
     v = fmaxf(v, __shfl_xor(v, offset));

@@ -45,23 +45,6 @@ template <int CTRL>
 __device__ __forceinline__ int Dpp(int v) {
   return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false);
 }
-template <int CTRL>
-__device__ __forceinline__ float MaxDpp(float v) {
-  return fmaxf(v, __builtin_bit_cast(float, Dpp<CTRL>(__builtin_bit_cast(int, v))));
-}
-// The wave's maximum without LDS: within rows of 16 lanes, then across them.
-__device__ __forceinline__ float WaveMaxFast(float v) {
-  v = MaxDpp<0xB1>(v);   // quad_perm [1, 0, 3, 2]
-  v = MaxDpp<0x4E>(v);   // quad_perm [2, 3, 0, 1]
-  v = MaxDpp<0x141>(v);  // row_half_mirror
-  v = MaxDpp<0x140>(v);  // row_mirror
-  const int bits = __builtin_bit_cast(int, v);
-  const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 0));
-  const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 16));
-  const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 32));
-  const float d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 48));
-  return fmaxf(fmaxf(a, b), fmaxf(c, d));
-}
 __device__ __forceinline__ float LaneOf(float v, int lane) {
   return __builtin_bit_cast(float,
                             __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));

@@ -439,6 +439,8 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
     auto s = static_cast<hipStream_t>(stream);
     RequireCurrentDevice(s);
     p.group = static_cast<int>(heads / cache->kv_heads);
+    p.group_inverse = ((1 << 16) + p.group - 1) / p.group;
+    p.group_magic = ((1ull << 36) + p.group - 1) / p.group;
     const ovg::CacheAttentionPlan plan = ovg::PlanCacheAttention(p.cache, p.group);
     const int64_t bytes = AttentionBytes(p.cache, plan);
     ovg::Require(bytes == 0 || (workspace && workspace_bytes >= bytes && Aligned16(workspace)),
