@@ -10,9 +10,8 @@
 // second pass; lanes, waves and splits of a row are joined at the end, in a
 // fixed order. The best `top` values are a sorted list in the wave's lanes. A
 // segment of 1024 elements is searched for entrants only where some lane's
-// maximum, which the sums need anyhow, reaches the list's last value; for the
-// first segment of a wave, whose list is empty, the top-th largest of the lanes'
-// maxima stands in (that many elements reach it, so no lower one is listed).
+// maximum, which the sums need anyhow, reaches the list's last value; the first
+// segment of a wave gives its largest elements one after the other.
 //
 // Elements come as aligned 16-byte loads; the up to 14 before a row's first
 // 16-byte border and behind its last are one more segment of single loads. A row
@@ -121,20 +120,93 @@ struct Row {
   }
 };
 
-// Takes z (element e of this lane at index IndexOf(e), -inf for none) into the
-// sums and the list.
-template <int N, typename F>
-__device__ __forceinline__ void Take(const float (&z)[N], F&& index_of, int mask_id, int lane,
-                                     Sums* sums, Alternatives* best) {
-  float peak = z[0];
+// A lane's elements of a segment, -inf for none.
+typedef float segment_t __attribute__((ext_vector_type(kElements)));
+
+// The wave's maximum of whole numbers: within rows of 16 lanes, then across them.
+template <int CTRL>
+__device__ __forceinline__ unsigned DppMaxOf(unsigned v) {
+  return max(v, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xF,
+                                                               0xF, true)));
+}
+__device__ __forceinline__ unsigned WaveMaxOf(unsigned v) {
+  v = DppMaxOf<0xB1>(v);
+  v = DppMaxOf<0x4E>(v);
+  v = DppMaxOf<0x141>(v);
+  v = DppMaxOf<0x140>(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(b[0], b[1]);
+}
+
+// Whole numbers in the order of the floats; 0 is below them all. -0 and +0 are one.
+__device__ __forceinline__ unsigned OrderOf(float v) {
+  const unsigned u = __float_as_uint(v + 0.0F);
+  return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float ValueOf(unsigned order) {
+  return __uint_as_float((order & 0x80000000u) != 0 ? order & 0x7FFFFFFFu : ~order);
+}
+
+// The list of a wave's first segment: `top` times the largest of what is left.
+// A lane's elements are in the order of their indices.
+template <typename F>
+__device__ __forceinline__ void First(const segment_t& z, F&& index_of, int mask_id, int lane,
+                                      Alternatives* best) {
+  unsigned key[kElements];
 #pragma unroll
-  for (int e = 1; e < N; ++e)
-    peak = fmaxf(peak, z[e]);
+  for (int e = 0; e < kElements; ++e)
+    key[e] = z[e] > -Inf() && index_of(e) != mask_id ? OrderOf(z[e]) : 0u;
+  for (int k = 0; k < best->top; ++k) {
+    unsigned most = key[0];
+#pragma unroll
+    for (int e = 1; e < kElements; ++e)
+      most = max(most, key[e]);
+    const unsigned largest = __builtin_amdgcn_readfirstlane(WaveMaxOf(most));
+    if (largest == 0)
+      return;
+    // Where it is first in each lane that has it, and the first of those.
+    int at = kElements;
+#pragma unroll
+    for (int e = kElements - 1; e >= 0; --e)
+      at = key[e] == largest ? e : at;
+    const unsigned long long have = __ballot(at < kElements);
+    int index = index_of(at);
+    int who = __ffsll(have) - 1;
+    if ((have & (have - 1)) != 0) {
+      const unsigned first = ~WaveMaxOf(at < kElements ? ~static_cast<unsigned>(index) : 0u);
+      who = __ffsll(__ballot(at < kElements && static_cast<unsigned>(index) == first)) - 1;
+    }
+    index = __builtin_amdgcn_readlane(index, who);
+    if (lane == k) {
+      best->value = ValueOf(largest);
+      best->index = index;
+    }
+    at = lane == who ? at : kElements;
+#pragma unroll
+    for (int e = 0; e < kElements; ++e)
+      key[e] = at == e ? 0u : key[e];
+  }
+}
+
+// Takes a segment into the sums and the list; index_of(e): its e-th element's.
+// `others`: what the list's last value is known to reach in the end.
+template <typename F>
+__device__ __forceinline__ void Take(const segment_t& z, F&& index_of, float others, int mask_id,
+                                     int lane, Sums* sums, Alternatives* best) {
+  constexpr int kRun = 4;  // elements that are passed over together
+  typedef float peaks_t __attribute__((ext_vector_type(kElements / kRun)));
+  peaks_t peaks;
+#pragma unroll
+  for (int k = 0; k < kElements / kRun; ++k)
+    peaks[k] = fmaxf(fmaxf(z[kRun * k], z[kRun * k + 1]), fmaxf(z[kRun * k + 2], z[kRun * k + 3]));
+  const float peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
   if (peak > sums->m)
     sums->Move(peak);
   const float from = sums->m == -Inf() ? 0.0F : sums->m;
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
+  for (int e = 0; e < kElements; ++e) {
     const float d = (z[e] - from) * kLog2e;
     const float x = __builtin_amdgcn_exp2f(d);
     sums->s += x;
@@ -143,51 +215,75 @@ __device__ __forceinline__ void Take(const float (&z)[N], F&& index_of, int mask
   }
   if (best->top == 0)
     return;
-  float floor = best->Floor();
+  const float floor = fmaxf(best->Floor(), others);
   if (!__any(peak >= floor && peak > -Inf()))
     return;
-  if (floor == -Inf()) {
-    // The list is not full.
-    float mine = -Inf();
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      mine = index_of(e) == mask_id ? mine : fmaxf(mine, z[e]);
-    for (int k = 0; k < best->top; ++k) {
-      floor = WaveMaxFast(mine);
-      if (floor == -Inf())
-        break;
-      if (lane == __ffsll(__ballot(mine == floor)) - 1)
-        mine = -Inf();
-    }
+  if (LaneOf(best->value, 0) == -Inf()) {
+    First(z, index_of, mask_id, lane, best);
+    return;
   }
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
+  // Not unrolled: the registers are indexed.
+#pragma unroll 1
+  for (int e = 0; e < kElements; ++e) {
+    if (e % kRun == 0 && !__any(peaks[e / kRun] >= floor)) {
+      e += kRun - 1;
+      continue;
+    }
+    const float v = z[e];
+    const int i = index_of(e);
+    const bool listed = v >= floor && v > -Inf() && i != mask_id;
+    unsigned long long todo = __ballot(listed);
     // Asked again after each: the list's last value rises, and with equal values
     // one index after another would be turned away.
-    const bool listed = z[e] >= floor && z[e] > -Inf() && index_of(e) != mask_id;
-    unsigned long long todo = __ballot(listed);
-    while ((todo &= __ballot(listed && best->Takes(z[e], index_of(e)))) != 0) {
+    while (todo != 0 && (todo &= __ballot(listed && best->Takes(v, i))) != 0) {
       const int who = __ffsll(todo) - 1;
       todo &= todo - 1;
-      best->Insert(LaneOf(z[e], who), __builtin_amdgcn_readlane(index_of(e), who), lane);
+      best->Insert(LaneOf(v, who), __builtin_amdgcn_readlane(i, who), lane);
     }
   }
 }
 
-// What a row's answers need: its whole sums and list.
+// The same for one element a lane.
+__device__ __forceinline__ void TakeOne(float z, int index, float others, int mask_id, int lane,
+                                        Sums* sums, Alternatives* best) {
+  if (z > sums->m)
+    sums->Move(z);
+  const float d = (z - (sums->m == -Inf() ? 0.0F : sums->m)) * kLog2e;
+  const float x = __builtin_amdgcn_exp2f(d);
+  sums->s += x;
+  sums->t = __builtin_fmaf(x, fmaxf(d, -1000.0F), sums->t);
+  if (best->top == 0)
+    return;
+  const bool listed = z >= others && z > -Inf() && index != mask_id;
+  unsigned long long todo = __ballot(listed);
+  while (todo != 0 && (todo &= __ballot(listed && best->Takes(z, index))) != 0) {
+    const int who = __ffsll(todo) - 1;
+    todo &= todo - 1;
+    best->Insert(LaneOf(z, who), __builtin_amdgcn_readlane(index, who), lane);
+  }
+}
+
+// The given token's (guided) logit. Asked for first, so that its two dependent
+// loads are over when the sums are.
 template <typename T>
-__device__ __forceinline__ void Answer(const LogprobParams& p, std::int64_t row, const Row<T>& from,
+__device__ __forceinline__ float Chosen(const LogprobParams& p, std::int64_t row,
+                                        const Row<T>& from) {
+  if (p.logprob == nullptr)
+    return 0.0F;
+  const int token = p.tokens[row];
+  return token >= 0 && token < p.vocab ? from.At(token) : -Inf();
+}
+
+// A row's answers from its whole sums and list.
+__device__ __forceinline__ void Answer(const LogprobParams& p, std::int64_t row, float chosen,
                                        const Sums& sums, const Alternatives& best, int lane) {
   // No distribution: a NaN or +infinity among the logits, or nothing above -infinity.
   const bool none = !(sums.s > 0.0F && sums.s < Inf());
   const float log_s = logf(sums.s);
   const float nan = __builtin_nanf("");
   if (lane == 0) {
-    if (p.logprob != nullptr) {
-      const int token = p.tokens[row];
-      const float z = token >= 0 && token < p.vocab ? from.At(token) : -Inf();
-      p.logprob[row] = none ? nan : z - sums.m - log_s;
-    }
+    if (p.logprob != nullptr)
+      p.logprob[row] = none ? nan : chosen - sums.m - log_s;
     if (p.entropy != nullptr)
       p.entropy[row] = none ? nan : log_s - sums.t / sums.s * kLn2;
   }
@@ -225,38 +321,88 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
   const int body = alike ? (p.vocab - head) / kVec * kVec : 0;
   const int of_row = WAVES == 1 ? 0 : static_cast<int>(blockIdx.y) * WAVES + wave;
   const int waves = WAVES == 1 ? 1 : p.splits * WAVES;
-  for (int base = of_row * kSegment; base < body; base += waves * kSegment) {
-    float z[kElements];
-    vec c[kVecs], u[kVecs];
+  // What is left, one element a lane in turn: the head and the tail, or all of two
+  // rows that do not lie alike. The first 64 of it are asked for here.
+  const int left = p.vocab - body;
+  const auto left_index = [&](int k) { return k < head ? k : k + body; };
+  const int left_first = of_row * kWave + lane;
+  const float early = left_first < left ? from.At(left_index(left_first)) : -Inf();
+  const bool answers = WAVES == 1 || (wave == 0 && p.splits == 1);
+  const float chosen = answers ? Chosen(p, row, from) : 0.0F;
+
+  // The floors of the row's waves. Each is the last value of a full list of some of
+  // the row's elements, so nothing below the highest can be listed in the end; it is
+  // read without waiting for anyone, an older one only passes over less.
+  __shared__ float floors[kWaves];
+  if constexpr (WAVES > 1) {
+    if (lane == 0)
+      floors[wave] = -Inf();
+    __syncthreads();
+  }
+  const auto known = [&]() {
+    float f = -Inf();
+    if constexpr (WAVES > 1) {
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) {
-      const int at = base + (v * kWave + lane) * kVec;
-      const int safe = head + min(at, body - kVec);
-      c[v] = *reinterpret_cast<const vec*>(from.c + safe);
-      if (GUIDED)
-        u[v] = *reinterpret_cast<const vec*>(from.u + safe);
+      for (int i = 0; i < WAVES; ++i)
+        f = fmaxf(f, __hip_atomic_load(&floors[i], __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_WORKGROUP));
     }
+    return f;
+  };
+
+  vec c[kVecs], u[kVecs];
+  const auto load = [&](int base) {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      const bool there = base + (v * kWave + lane) * kVec < body;
+      const int at = head + min(base + (v * kWave + lane) * kVec, body - kVec);
+      c[v] = *reinterpret_cast<const vec*>(from.c + at);
+      if (GUIDED)
+        u[v] = *reinterpret_cast<const vec*>(from.u + at);
+    }
+  };
+  if (of_row * kSegment < body)
+    load(of_row * kSegment);
+#pragma unroll 1
+  for (int base = of_row * kSegment; base < body; base += waves * kSegment) {
+    segment_t z;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
         const float x = static_cast<float>(c[v][e]);
-        const float guided = GUIDED ? Guide(x, static_cast<float>(u[v][e]), p.guidance) : x;
-        z[v * kVec + e] = there ? guided : -Inf();
+        z[v * kVec + e] = GUIDED ? Guide(x, static_cast<float>(u[v][e]), p.guidance) : x;
       }
+    load(base + waves * kSegment);  // past the end the last ones again
+    if (base + kSegment > body) {
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          z[v * kVec + e] =
+              base + (v * kWave + lane) * kVec < body ? z[v * kVec + e] : -Inf();
     }
+    const float before = best.top > 0 ? best.Floor() : 0.0F;
     Take(z, [&](int e) { return head + base + (e / kVec * kWave + lane) * kVec + e % kVec; },
-         p.mask_id, lane, &sums, &best);
+         known(), p.mask_id, lane, &sums, &best);
+    if constexpr (WAVES > 1) {
+      const float after = best.top > 0 ? best.Floor() : 0.0F;
+      if (after != before && lane == 0)
+        __hip_atomic_store(&floors[wave], after, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
   }
-  // What is left, one element a lane: the head and the tail, or all of two rows
-  // that do not lie alike.
-  const int left = p.vocab - body;
-  for (int base = of_row * kWave; base < left; base += waves * kWave) {
-    const int k = base + lane;
-    const int at = k < head ? k : k + body;
-    const float z[1] = {k < left ? from.At(at) : -Inf()};
-    Take(z, [&](int) { return at; }, p.mask_id, lane, &sums, &best);
+  if (of_row * kWave < left)
+    TakeOne(early, left_index(left_first), known(), p.mask_id, lane, &sums, &best);
+#pragma unroll 1
+  for (int k0 = (of_row + waves) * kWave; k0 < left; k0 += waves * kSegment) {
+    segment_t z;
+#pragma unroll
+    for (int e = 0; e < kElements; ++e) {
+      const int k = k0 + e * waves * kWave + lane;
+      z[e] = k < left ? from.At(left_index(k)) : -Inf();
+    }
+    Take(z, [&](int e) { return left_index(k0 + e * waves * kWave + lane); }, known(), p.mask_id,
+         lane, &sums, &best);
   }
 
   sums.JoinWave();
@@ -302,7 +448,7 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
       return;
     }
   }
-  Answer(p, row, from, sums, best, lane);
+  Answer(p, row, chosen, sums, best, lane);
 }
 
 // One wave per row: lane i takes split i's sums.
@@ -311,6 +457,12 @@ __global__ __launch_bounds__(kWave) void JoinLogprobsKernel(LogprobParams p) {
   const int lane = threadIdx.x;
   const std::int64_t row = blockIdx.x;
   const float* states = p.states + row * p.splits * (4 + 2 * p.top);
+  Row<T> from;
+  from.c = static_cast<const T*>(p.logits) + row * p.stride;
+  from.u = p.uncond == nullptr ? nullptr
+                               : static_cast<const T*>(p.uncond) + row * p.uncond_stride;
+  from.g = p.guidance;
+  const float chosen = Chosen(p, row, from);
   Sums sums{-Inf(), 0.0F, 0.0F};
   Alternatives best{-Inf(), -1, p.top};
   if (lane < p.splits) {
@@ -330,12 +482,7 @@ __global__ __launch_bounds__(kWave) void JoinLogprobsKernel(LogprobParams p) {
     index = next_index;
   }
   sums.JoinWave();
-  Row<T> from;
-  from.c = static_cast<const T*>(p.logits) + row * p.stride;
-  from.u = p.uncond == nullptr ? nullptr
-                               : static_cast<const T*>(p.uncond) + row * p.uncond_stride;
-  from.g = p.guidance;
-  Answer(p, row, from, sums, best, lane);
+  Answer(p, row, chosen, sums, best, lane);
 }
 
 constexpr int kOneWave = 2048;  // elements of a row that one wave takes
