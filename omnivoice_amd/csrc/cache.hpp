@@ -175,6 +175,7 @@ struct LogprobParams {
 };
 constexpr int kMostAlternatives = 32;
 constexpr int kLogprobGroups = 512;  // work-groups that a call is to have
+constexpr int kMostLogprobSplits = 16;
 int PlanLogprobs(int rows, int vocab);
 void LaunchLogprobs(const LogprobParams& p, DType type, hipStream_t stream);
 

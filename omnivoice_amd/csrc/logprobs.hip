@@ -8,16 +8,23 @@
 // A lane keeps the maximum m of what it has seen, s = sum exp(z - m) and
 // t = sum exp(z - m) log2 exp(z - m), so that H = log s - ln 2 t / s needs no
 // second pass; lanes, waves and splits of a row are joined at the end, in a
-// fixed order. The best `top` values are a sorted list in the wave's lanes. A
-// segment of 1024 elements is searched for entrants only where some lane's
-// maximum, which the sums need anyhow, reaches the list's last value; the first
-// segment of a wave gives its largest elements one after the other.
+// fixed order.
 //
-// Elements come as aligned 16-byte loads; the up to 14 before a row's first
-// 16-byte border and behind its last are one more segment of single loads. A row
-// belongs to one wave up to 2048 elements (four rows to a work-group), else to
-// the four waves of a work-group, and where there are too few rows for the
-// device to several of those, whose states a second kernel joins.
+// For the alternatives a lane keeps the three loudest of its runs of 16 elements,
+// by their largest element, which costs 13 operations a run. The row's `top` best
+// elements lie in its `top` loudest runs (equal ones by place: whatever lies in
+// another run has the loudest elements of those before it), so at the end a wave
+// picks that many runs, fetches them again and ranks the few elements that reach
+// the last one's loudest. Where a lane would have to give a fourth run, or more than
+// 64 elements are equal to the last, the wave searches all its elements once more,
+// with a sorted list in its lanes.
+//
+// Elements come as 16-byte loads, 16 elements in a row to a lane, a segment of 1024
+// to a wave; the up to 14 before a row's first 16-byte border and behind its last are
+// one more load each of single elements. A row belongs to one wave up to 2048
+// elements (four rows to a work-group), else to the four waves of a work-group, and
+// where there are too few rows for the device to several of those, whose states a
+// second kernel joins.
 #include <algorithm>
 
 #include "cache.hpp"
@@ -35,11 +42,6 @@ constexpr float kLn2 = 0.693147180559945309F;
 
 __device__ __forceinline__ float Inf() { return __builtin_inff(); }
 
-// (value, index) pairs in descending order, equal values by index.
-__device__ __forceinline__ bool Before(float a, int i, float b, int j) {
-  return a > b || (a == b && i < j);
-}
-
 template <int CTRL>
 __device__ __forceinline__ int Dpp(int v) {
   return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false);
@@ -49,36 +51,66 @@ __device__ __forceinline__ float LaneOf(float v, int lane) {
                             __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-// The `top` best so far: lane j holds the j-th, (-inf, -1) where there is none.
+// Whole numbers in the order of the floats; 0 is below them all. -0 and +0 are one.
+__device__ __forceinline__ unsigned OrderOf(float v) {
+  const unsigned u = __float_as_uint(v + 0.0F);
+  return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float ValueOf(unsigned order) {
+  if (order == 0)
+    return -Inf();
+  return __uint_as_float((order & 0x80000000u) != 0 ? order & 0x7FFFFFFFu : ~order);
+}
+
+// The wave's maximum of whole numbers: within rows of 16 lanes, then across them.
+template <int CTRL>
+__device__ __forceinline__ unsigned DppMaxOf(unsigned v) {
+  return max(v, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xF,
+                                                               0xF, true)));
+}
+__device__ __forceinline__ unsigned WaveMaxOf(unsigned v) {
+  v = DppMaxOf<0xB1>(v);
+  v = DppMaxOf<0x4E>(v);
+  v = DppMaxOf<0x141>(v);
+  v = DppMaxOf<0x140>(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(max(b[0], b[1]));
+}
+
+// The `top` best so far: lane j holds the j-th's order and index, (0, -1) where
+// there is none, and what lies behind the last is below it. The last one is kept
+// apart, the same in every lane.
 struct Alternatives {
-  float value;
+  unsigned order;
   int index;
   int top;
-  __device__ __forceinline__ float Floor() const { return LaneOf(value, top - 1); }
-  __device__ __forceinline__ int FloorIndex() const {
-    return __builtin_amdgcn_readlane(index, top - 1);
+  unsigned floor;
+  int floor_index;
+  __device__ __forceinline__ explicit Alternatives(int top_)
+      : order(0), index(-1), top(top_), floor(0), floor_index(-1) {}
+  __device__ __forceinline__ bool Takes(unsigned o, int i) const {
+    return o > floor || (o == floor && o != 0 && i < floor_index);
   }
-  // Whether (v, i) belongs into the list.
-  __device__ __forceinline__ bool Takes(float v, int i) const {
-    return Before(v, i, Floor(), FloorIndex());
-  }
-  // (v, i), the same in every lane, that belongs into it.
-  __device__ __forceinline__ void Insert(float v, int i, int lane) {
-    const int at = __popcll(__ballot(lane < top && Before(value, index, v, i)));
-    const float up = __builtin_bit_cast(float, Dpp<0x138>(__builtin_bit_cast(int, value)));
+  // What it takes, the same in every lane.
+  __device__ __forceinline__ void Insert(unsigned o, int i, int lane) {
+    const int at = __popcll(__ballot(order > o || (order == o && index < i)));
+    const unsigned up = static_cast<unsigned>(Dpp<0x138>(static_cast<int>(order)));
     const int up_index = Dpp<0x138>(index);  // wave_shr: 1
-    value = lane == at ? v : lane > at ? up : value;
+    order = lane == at ? o : lane > at ? up : order;
     index = lane == at ? i : lane > at ? up_index : index;
+    floor = __builtin_amdgcn_readlane(order, top - 1);
+    floor_index = __builtin_amdgcn_readlane(index, top - 1);
   }
-  // Another sorted list: nothing behind the first that does not belong does.
-  template <typename V, typename I>
-  __device__ __forceinline__ void Merge(V&& value_of, I&& index_of, int lane) {
+  // Another sorted list, lane k holding its k-th.
+  __device__ __forceinline__ void Merge(unsigned o, int i, int lane) {
     for (int k = 0; k < top; ++k) {
-      const float v = value_of(k);
-      const int i = index_of(k);
-      if (!Takes(v, i))
-        break;
-      Insert(v, i, lane);
+      const unsigned one = __builtin_amdgcn_readlane(o, k);
+      const int at = __builtin_amdgcn_readlane(i, k);
+      if (!Takes(one, at))
+        return;  // nor does it take any behind
+      Insert(one, at, lane);
     }
   }
 };
@@ -123,145 +155,228 @@ struct Row {
 // A lane's elements of a segment, -inf for none.
 typedef float segment_t __attribute__((ext_vector_type(kElements)));
 
-// The wave's maximum of whole numbers: within rows of 16 lanes, then across them.
-template <int CTRL>
-__device__ __forceinline__ unsigned DppMaxOf(unsigned v) {
-  return max(v, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xF,
-                                                               0xF, true)));
-}
-__device__ __forceinline__ unsigned WaveMaxOf(unsigned v) {
-  v = DppMaxOf<0xB1>(v);
-  v = DppMaxOf<0x4E>(v);
-  v = DppMaxOf<0x141>(v);
-  v = DppMaxOf<0x140>(v);
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = max(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return max(b[0], b[1]);
-}
-
-// Whole numbers in the order of the floats; 0 is below them all. -0 and +0 are one.
-__device__ __forceinline__ unsigned OrderOf(float v) {
-  const unsigned u = __float_as_uint(v + 0.0F);
-  return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float ValueOf(unsigned order) {
-  return __uint_as_float((order & 0x80000000u) != 0 ? order & 0x7FFFFFFFu : ~order);
-}
-
-// The list of a wave's first segment: `top` times the largest of what is left.
-// A lane's elements are in the order of their indices.
-template <typename F>
-__device__ __forceinline__ void First(const segment_t& z, F&& index_of, int mask_id, int lane,
-                                      Alternatives* best) {
-  unsigned key[kElements];
+// Takes the first `count` (a constant) of a segment's elements into the list;
+// index_of(e) is the e-th's, -1 for one that is not to be listed. peak: the lane's
+// largest. others: an order that the list's last is known to reach in the end.
+template <int COUNT, typename F>
+__device__ __forceinline__ void Search(const segment_t& z, float peak, F&& index_of,
+                                       unsigned others, int lane, Alternatives* best) {
+  constexpr float kLowest = -3.402823466e38F;
+  unsigned floor = max(best->floor, others);
+  if (!__any(peak >= fmaxf(ValueOf(floor), kLowest)))
+    return;
+  if (floor == 0 && COUNT > 1) {
+    // The list is not full: the top-th largest of the lanes' own largest stands in.
+    // That many elements reach it, so nothing below it is listed.
+    unsigned mine = 0;
 #pragma unroll
-  for (int e = 0; e < kElements; ++e)
-    key[e] = z[e] > -Inf() && index_of(e) != mask_id ? OrderOf(z[e]) : 0u;
-  for (int k = 0; k < best->top; ++k) {
-    unsigned most = key[0];
-#pragma unroll
-    for (int e = 1; e < kElements; ++e)
-      most = max(most, key[e]);
-    const unsigned largest = __builtin_amdgcn_readfirstlane(WaveMaxOf(most));
-    if (largest == 0)
-      return;
-    // Where it is first in each lane that has it, and the first of those.
-    int at = kElements;
-#pragma unroll
-    for (int e = kElements - 1; e >= 0; --e)
-      at = key[e] == largest ? e : at;
-    const unsigned long long have = __ballot(at < kElements);
-    int index = index_of(at);
-    int who = __ffsll(have) - 1;
-    if ((have & (have - 1)) != 0) {
-      const unsigned first = ~WaveMaxOf(at < kElements ? ~static_cast<unsigned>(index) : 0u);
-      who = __ffsll(__ballot(at < kElements && static_cast<unsigned>(index) == first)) - 1;
+    for (int e = 0; e < COUNT; ++e)
+      mine = z[e] >= kLowest && index_of(e) >= 0 ? max(mine, OrderOf(z[e])) : mine;
+    for (int k = 0; k < best->top; ++k) {
+      floor = WaveMaxOf(mine);
+      if (floor == 0)
+        break;
+      const unsigned long long have = __ballot(mine == floor);
+      mine = lane == __ffsll(have) - 1 ? 0u : mine;
     }
-    index = __builtin_amdgcn_readlane(index, who);
-    if (lane == k) {
-      best->value = ValueOf(largest);
-      best->index = index;
-    }
-    at = lane == who ? at : kElements;
+  }
+  // A bit for each element that may be listed. Taken one after the other, the list's
+  // last value rises; when it turns one away the bits are drawn anew by value and
+  // index, so that equal values do not queue.
+  const float least = fmaxf(ValueOf(floor), kLowest);
+  unsigned bits = 0;
 #pragma unroll
-    for (int e = 0; e < kElements; ++e)
-      key[e] = at == e ? 0u : key[e];
+  for (int e = 0; e < COUNT; ++e)
+    bits |= z[e] >= least && index_of(e) >= 0 ? 1u << e : 0u;
+  for (unsigned long long lanes = __ballot(bits != 0); lanes != 0;) {
+    const int who = __ffsll(lanes) - 1;
+    const int e = __ffs(__builtin_amdgcn_readlane(bits, who)) - 1;
+    const unsigned order = OrderOf(LaneOf(z[e], who));
+    const int index = __builtin_amdgcn_readlane(index_of(e), who);
+    if (best->Takes(order, index)) {
+      best->Insert(order, index, lane);
+      if (lane == who)
+        bits &= bits - 1;
+    } else {
+      const float last = ValueOf(best->floor);
+#pragma unroll
+      for (int e2 = 0; e2 < COUNT; ++e2)
+        if (!(z[e2] > last || (z[e2] == last && index_of(e2) < best->floor_index)))
+          bits &= ~(1u << e2);
+    }
+    lanes = __ballot(bits != 0);
   }
 }
 
-// Takes a segment into the sums and the list; index_of(e): its e-th element's.
-// `others`: what the list's last value is known to reach in the end.
-template <typename F>
-__device__ __forceinline__ void Take(const segment_t& z, F&& index_of, float others, int mask_id,
-                                     int lane, Sums* sums, Alternatives* best) {
-  constexpr int kRun = 4;  // elements that are passed over together
-  typedef float peaks_t __attribute__((ext_vector_type(kElements / kRun)));
-  peaks_t peaks;
-#pragma unroll
-  for (int k = 0; k < kElements / kRun; ++k)
-    peaks[k] = fmaxf(fmaxf(z[kRun * k], z[kRun * k + 1]), fmaxf(z[kRun * k + 2], z[kRun * k + 3]));
-  const float peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
+// Takes a segment, of which the lane's largest element is `peak`, into the sums.
+template <int COUNT>
+__device__ __forceinline__ void Add(const segment_t& z, float peak, Sums* sums) {
   if (peak > sums->m)
     sums->Move(peak);
   const float from = sums->m == -Inf() ? 0.0F : sums->m;
 #pragma unroll
-  for (int e = 0; e < kElements; ++e) {
+  for (int e = 0; e < COUNT; ++e) {
     const float d = (z[e] - from) * kLog2e;
     const float x = __builtin_amdgcn_exp2f(d);
     sums->s += x;
     // 0 * -inf stays 0; a NaN is x's already.
     sums->t = __builtin_fmaf(x, fmaxf(d, -1000.0F), sums->t);
   }
-  if (best->top == 0)
-    return;
-  const float floor = fmaxf(best->Floor(), others);
-  if (!__any(peak >= floor && peak > -Inf()))
-    return;
-  if (LaneOf(best->value, 0) == -Inf()) {
-    First(z, index_of, mask_id, lane, best);
-    return;
-  }
-  // Not unrolled: the registers are indexed.
-#pragma unroll 1
-  for (int e = 0; e < kElements; ++e) {
-    if (e % kRun == 0 && !__any(peaks[e / kRun] >= floor)) {
-      e += kRun - 1;
-      continue;
-    }
-    const float v = z[e];
-    const int i = index_of(e);
-    const bool listed = v >= floor && v > -Inf() && i != mask_id;
-    unsigned long long todo = __ballot(listed);
-    // Asked again after each: the list's last value rises, and with equal values
-    // one index after another would be turned away.
-    while (todo != 0 && (todo &= __ballot(listed && best->Takes(v, i))) != 0) {
-      const int who = __ffsll(todo) - 1;
-      todo &= todo - 1;
-      best->Insert(LaneOf(v, who), __builtin_amdgcn_readlane(i, who), lane);
-    }
-  }
 }
 
-// The same for one element a lane.
-__device__ __forceinline__ void TakeOne(float z, int index, float others, int mask_id, int lane,
-                                        Sums* sums, Alternatives* best) {
-  if (z > sums->m)
-    sums->Move(z);
-  const float d = (z - (sums->m == -Inf() ? 0.0F : sums->m)) * kLog2e;
-  const float x = __builtin_amdgcn_exp2f(d);
-  sums->s += x;
-  sums->t = __builtin_fmaf(x, fmaxf(d, -1000.0F), sums->t);
-  if (best->top == 0)
-    return;
-  const bool listed = z >= others && z > -Inf() && index != mask_id;
-  unsigned long long todo = __ballot(listed);
-  while (todo != 0 && (todo &= __ballot(listed && best->Takes(z, index))) != 0) {
-    const int who = __ffsll(todo) - 1;
-    todo &= todo - 1;
-    best->Insert(LaneOf(z, who), __builtin_amdgcn_readlane(index, who), lane);
-  }
+__device__ __forceinline__ float Peak(const segment_t& z) {
+  float peak = z[0];
+#pragma unroll
+  for (int e = 1; e < kElements; ++e)
+    peak = fmaxf(peak, z[e]);
+  return peak;
 }
+
+struct Entry {
+  unsigned order;
+  int index;
+};
+
+// The list of what is in a wave's COUNT elements a lane (index_of(e): -1 for one
+// that is not to be listed): those that reach `known` are gathered in `slots` (64,
+// the wave's own) and each finds its place by counting the ones before it. known: an
+// order that `top` elements at least reach, or 0. False where over 64 reach it.
+template <int COUNT, typename Z, typename F>
+__device__ __forceinline__ bool Rank(const Z& z, F&& index_of, unsigned known, int lane,
+                                     Entry* slots, Alternatives* best) {
+  constexpr float kLowest = -3.402823466e38F;
+  const float least = fmaxf(ValueOf(known), kLowest);
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < COUNT; ++e) {
+    const int index = index_of(e);
+    const bool in = z[e] >= least && index >= 0;
+    const unsigned long long all = __ballot(in);
+    if (all == 0)
+      continue;
+    const int at = count + __builtin_amdgcn_mbcnt_hi(
+                               static_cast<unsigned>(all >> 32),
+                               __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(all), 0));
+    if (in && at < kWave)
+      slots[at] = {OrderOf(z[e]), index};
+    count += __popcll(all);
+  }
+  if (count > kWave)
+    return false;
+  __builtin_amdgcn_wave_barrier();
+  const Entry own = lane < count ? slots[lane] : Entry{0, -1};
+  int before = 0;
+  for (int j = 0; j < count; ++j) {
+    const unsigned order = __builtin_amdgcn_readlane(own.order, j);
+    const int index = __builtin_amdgcn_readlane(own.index, j);
+    before += order > own.order || (order == own.order && index < own.index) ? 1 : 0;
+  }
+  __builtin_amdgcn_wave_barrier();
+  if (lane < count)
+    slots[before] = own;
+  __builtin_amdgcn_wave_barrier();
+  const Entry mine = lane < min(count, best->top) ? slots[lane] : Entry{0, -1};
+  best->order = mine.order;
+  best->index = mine.index;
+  best->floor = __builtin_amdgcn_readlane(best->order, max(best->top, 1) - 1);
+  best->floor_index = __builtin_amdgcn_readlane(best->index, max(best->top, 1) - 1);
+  return true;
+}
+
+// A lane's three loudest runs, in order, equal ones by place.
+struct Runs {
+  float peak[3];
+  int segment[3];
+  __device__ __forceinline__ Runs()
+      : peak{-Inf(), -Inf(), -Inf()}, segment{-1, -1, -1} {}
+  __device__ __forceinline__ void Add(float p, int s) {
+    const bool a = p > peak[0], b = p > peak[1], c = p > peak[2];
+    peak[2] = b ? peak[1] : c ? p : peak[2];
+    segment[2] = b ? segment[1] : c ? s : segment[2];
+    peak[1] = a ? peak[0] : b ? p : peak[1];
+    segment[1] = a ? segment[0] : b ? s : segment[1];
+    peak[0] = a ? p : peak[0];
+    segment[0] = a ? s : segment[0];
+  }
+  // The largest three of what the wave's lanes hold, into this lane if `here`.
+  __device__ __forceinline__ void Largest(Runs from, bool here) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      int segment_of;
+      const unsigned largest = from.Pop(&segment_of, nullptr);
+      if (here) {
+        peak[k] = ValueOf(largest);
+        segment[k] = segment_of;
+      }
+    }
+  }
+  // Takes the loudest run out of the wave's: its order (0: none), segment and lane.
+  __device__ __forceinline__ unsigned Pop(int* of_segment, int* of_lane) {
+    const unsigned order = peak[0] > -Inf() ? OrderOf(peak[0]) : 0u;
+    const unsigned largest = WaveMaxOf(order);
+    *of_segment = -1;
+    if (largest == 0)
+      return 0;
+    unsigned long long have = __ballot(order == largest);
+    if ((have & (have - 1)) != 0) {
+      const unsigned first =
+          ~WaveMaxOf(order == largest ? ~static_cast<unsigned>(segment[0]) : 0u);
+      have = __ballot(order == largest && static_cast<unsigned>(segment[0]) == first);
+    }
+    const int who = __ffsll(have) - 1;
+    *of_segment = __builtin_amdgcn_readlane(segment[0], who);
+    if (of_lane != nullptr)
+      *of_lane = who;
+    if (static_cast<int>(threadIdx.x & (kWave - 1)) == who) {
+      peak[0] = peak[1];
+      segment[0] = segment[1];
+      peak[1] = peak[2];
+      segment[1] = segment[2];
+      peak[2] = -Inf();
+    }
+    return largest;
+  }
+  // The wave's `top` loudest runs: lane k gets the k-th's segment (-1: none) and lane.
+  // The wave took the segments first, first + stride, ..., `seen` of them; a lane
+  // that has given all three it kept gets the next three by peak_of(segment, lane),
+  // which each lane calls for other segments. Returns the last one's order, 1 where
+  // there are fewer than top.
+  template <typename F>
+  __device__ __forceinline__ unsigned Pick(int top, int first, int stride, int seen, F&& peak_of,
+                                           int lane, int* segment_of, int* lane_of) {
+    *segment_of = -1;
+    *lane_of = 0;
+    int given = 0;
+    unsigned last = 1;
+    for (int k = 0; k < top; ++k) {
+      int s, who = 0;
+      const unsigned largest = Pop(&s, &who);
+      if (largest == 0)
+        return 1;
+      last = largest;
+      if (lane == k) {
+        *segment_of = s;
+        *lane_of = who;
+      }
+      given += lane == who ? 1 : 0;
+      if (__builtin_amdgcn_readlane(given, who) == 3 && seen > 3 && k + 1 < top) {
+        Runs others;
+        for (int i0 = 0; i0 < seen; i0 += kWave) {
+          const int at = first + min(i0 + lane, seen - 1) * stride;
+          float p = peak_of(at, who);
+          for (int j = 0; j <= k; ++j)
+            if (__builtin_amdgcn_readlane(*lane_of, j) == who &&
+                __builtin_amdgcn_readlane(*segment_of, j) == at)
+              p = -Inf();
+          others.Add(i0 + lane < seen ? p : -Inf(), at);
+        }
+        Largest(others, lane == who);
+        given = lane == who ? 0 : given;
+      }
+    }
+    return last;
+  }
+};
 
 // The given token's (guided) logit. Asked for first, so that its two dependent
 // loads are over when the sums are.
@@ -289,7 +404,7 @@ __device__ __forceinline__ void Answer(const LogprobParams& p, std::int64_t row,
   }
   if (lane < p.top) {
     p.top_ids[row * p.top + lane] = none ? -1 : best.index;
-    p.top_logprobs[row * p.top + lane] = none ? nan : best.value - sums.m - log_s;
+    p.top_logprobs[row * p.top + lane] = none ? nan : ValueOf(best.order) - sums.m - log_s;
   }
 }
 
@@ -310,7 +425,7 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
   from.u = GUIDED ? static_cast<const T*>(p.uncond) + row * p.uncond_stride : nullptr;
   from.g = p.guidance;
   Sums sums{-Inf(), 0.0F, 0.0F};
-  Alternatives best{-Inf(), -1, p.top};
+  Alternatives best(p.top);
 
   // [head, head + body) in 16-byte loads, a whole number of them; both tensors' rows
   // have to lie alike.
@@ -330,40 +445,19 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
   const bool answers = WAVES == 1 || (wave == 0 && p.splits == 1);
   const float chosen = answers ? Chosen(p, row, from) : 0.0F;
 
-  // The floors of the row's waves. Each is the last value of a full list of some of
-  // the row's elements, so nothing below the highest can be listed in the end; it is
-  // read without waiting for anyone, an older one only passes over less.
-  __shared__ float floors[kWaves];
-  if constexpr (WAVES > 1) {
-    if (lane == 0)
-      floors[wave] = -Inf();
-    __syncthreads();
-  }
-  const auto known = [&]() {
-    float f = -Inf();
-    if constexpr (WAVES > 1) {
-#pragma unroll
-      for (int i = 0; i < WAVES; ++i)
-        f = fmaxf(f, __hip_atomic_load(&floors[i], __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_WORKGROUP));
-    }
-    return f;
-  };
-
+  const auto but_mask = [&](int i) { return i == p.mask_id ? -1 : i; };
   vec c[kVecs], u[kVecs];
   const auto load = [&](int base) {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      const int at = head + min(base + (v * kWave + lane) * kVec, body - kVec);
+      const int at = head + min(base + lane * kElements + v * kVec, body - kVec);
       c[v] = *reinterpret_cast<const vec*>(from.c + at);
       if (GUIDED)
         u[v] = *reinterpret_cast<const vec*>(from.u + at);
     }
   };
-  if (of_row * kSegment < body)
-    load(of_row * kSegment);
-#pragma unroll 1
-  for (int base = of_row * kSegment; base < body; base += waves * kSegment) {
+  // What was loaded, as elements base + 16 lane .. + 15 of the body.
+  const auto elements = [&](int base, int of_lane) {
     segment_t z;
 #pragma unroll
     for (int v = 0; v < kVecs; ++v)
@@ -372,50 +466,119 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
         const float x = static_cast<float>(c[v][e]);
         z[v * kVec + e] = GUIDED ? Guide(x, static_cast<float>(u[v][e]), p.guidance) : x;
       }
-    load(base + waves * kSegment);  // past the end the last ones again
-    if (base + kSegment > body) {
+    if (__any(base + kSegment > body)) {
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          z[v * kVec + e] =
-              base + (v * kWave + lane) * kVec < body ? z[v * kVec + e] : -Inf();
+      for (int e = 0; e < kElements; ++e)
+        z[e] = base + of_lane * kElements + e / kVec * kVec < body ? z[e] : -Inf();
     }
-    const float before = best.top > 0 ? best.Floor() : 0.0F;
-    Take(z, [&](int e) { return head + base + (e / kVec * kWave + lane) * kVec + e % kVec; },
-         known(), p.mask_id, lane, &sums, &best);
-    if constexpr (WAVES > 1) {
-      const float after = best.top > 0 ? best.Floor() : 0.0F;
-      if (after != before && lane == 0)
-        __hip_atomic_store(&floors[wave], after, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_WORKGROUP);
+    return z;
+  };
+  Runs runs;
+  int seen = 0;
+  if (of_row * kSegment < body)
+    load(of_row * kSegment);
+#pragma unroll 1
+  for (int base = of_row * kSegment; base < body; base += waves * kSegment) {
+    const segment_t z = elements(base, lane);
+    load(base + waves * kSegment);  // past the end the last ones again
+    const float peak = Peak(z);
+    Add<kElements>(z, peak, &sums);
+    if (p.top > 0) {
+      float listed = peak;
+      const int hidden = p.mask_id - head - base;  // of the segment
+      if (hidden >= 0 && hidden < kSegment) {
+        segment_t others = z;
+#pragma unroll
+        for (int e = 0; e < kElements; ++e)
+          others[e] = hidden == lane * kElements + e ? -Inf() : z[e];
+        listed = Peak(others);
+      }
+      runs.Add(listed, base / kSegment);
+      ++seen;
     }
   }
-  if (of_row * kWave < left)
-    TakeOne(early, left_index(left_first), known(), p.mask_id, lane, &sums, &best);
-#pragma unroll 1
-  for (int k0 = (of_row + waves) * kWave; k0 < left; k0 += waves * kSegment) {
+  // What is left, one element a lane.
+  if (of_row * kWave < left) {
     segment_t z;
+    z[0] = early;
+    Add<1>(z, early, &sums);
+  }
+  const bool unlike = left > waves * kWave;  // rows that do not lie alike
+#pragma unroll 1
+  for (int k = left_first + waves * kWave; unlike && k - lane < left; k += waves * kWave) {
+    segment_t z;
+    z[0] = k < left ? from.At(left_index(k)) : -Inf();
+    Add<1>(z, z[0], &sums);
+  }
+
+  __shared__ Entry slots[kWaves][kWave];
+  if (p.top > 0) {
+    // Run `segment` of lane `of_lane`, into c and u.
+    const auto load_run = [&](int segment, int of_lane) {
 #pragma unroll
-    for (int e = 0; e < kElements; ++e) {
-      const int k = k0 + e * waves * kWave + lane;
-      z[e] = k < left ? from.At(left_index(k)) : -Inf();
+      for (int v = 0; v < kVecs; ++v) {
+        const int at = min(segment * kSegment + of_lane * kElements + v * kVec, body - kVec);
+        c[v] = *reinterpret_cast<const vec*>(from.c + head + at);
+        if (GUIDED)
+          u[v] = *reinterpret_cast<const vec*>(from.u + head + at);
+      }
+    };
+    const auto peak_of = [&](int segment, int of_lane) {
+      load_run(segment, of_lane);
+      segment_t z = elements(segment * kSegment, of_lane);
+      const int hidden = p.mask_id - head - segment * kSegment - of_lane * kElements;
+#pragma unroll
+      for (int e = 0; e < kElements; ++e)
+        z[e] = hidden == e ? -Inf() : z[e];
+      return Peak(z);
+    };
+    int of_segment, of_lane;
+    const unsigned known =
+        runs.Pick(p.top, of_row, waves, seen, peak_of, lane, &of_segment, &of_lane);
+    bool whole = !unlike;
+    if (whole) {
+      // The runs again, and the element that was left.
+      const int at = of_segment * kSegment + of_lane * kElements;  // of the body
+      if (of_segment >= 0)
+        load_run(of_segment, of_lane);
+      const segment_t run = elements(of_segment * kSegment, of_lane);
+      float z[kElements + 1];
+#pragma unroll
+      for (int e = 0; e < kElements; ++e)
+        z[e] = of_segment >= 0 ? run[e] : -Inf();
+      z[kElements] = early;
+      whole = Rank<kElements + 1>(
+          z,
+          [&](int e) { return but_mask(e < kElements ? head + at + e : left_index(left_first)); },
+          known, lane, slots[wave], &best);
     }
-    Take(z, [&](int e) { return left_index(k0 + e * waves * kWave + lane); }, known(), p.mask_id,
-         lane, &sums, &best);
+    if (!whole) {
+      // All the wave's elements once more: the body, then what is left.
+#pragma unroll 1
+      for (int base = of_row * kSegment; base < body; base += waves * kSegment) {
+        load(base);
+        const segment_t z = elements(base, lane);
+        Search<kElements>(
+            z, Peak(z), [&](int e) { return but_mask(head + base + lane * kElements + e); }, 0,
+            lane, &best);
+      }
+#pragma unroll 1
+      for (int k = left_first; k - lane < left; k += waves * kWave) {
+        segment_t z;
+        z[0] = k < left ? from.At(left_index(k)) : -Inf();
+        Search<1>(z, z[0], [&](int) { return but_mask(left_index(k)); }, 0, lane, &best);
+      }
+    }
   }
 
   sums.JoinWave();
   if constexpr (WAVES > 1) {
     __shared__ Sums shared[WAVES];
-    __shared__ float shared_value[WAVES][kMostAlternatives];
-    __shared__ int shared_index[WAVES][kMostAlternatives];
+    __shared__ Entry lists[WAVES][kMostAlternatives];
     if (lane == 0)
       shared[wave] = sums;
-    if (lane < p.top) {
-      shared_value[wave][lane] = best.value;
-      shared_index[wave][lane] = best.index;
-    }
+    if (lane < p.top)
+      lists[wave][lane] = {best.order, best.index};
     __syncthreads();
     if (wave != 0)
       return;
@@ -430,9 +593,30 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
       part.Move(top == -Inf() ? part.m : top);
       sums.s += part.s;
       sums.t += part.t;
-      if (p.top > 0)
-        best.Merge([&](int k) { return shared_value[w][k]; },
-                   [&](int k) { return shared_index[w][k]; }, lane);
+    }
+    if (p.top > 0) {
+      // Up to 128 entries, two a lane, of which those matter that reach the highest of
+      // the lists' last ones.
+      constexpr int kEach = WAVES * kMostAlternatives / kWave;
+      float z[kEach];
+      int index[kEach];
+      unsigned known = 1;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+        known = max(known, lists[w][p.top - 1].order);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int w = (e * kWave + lane) / kMostAlternatives, k = lane % kMostAlternatives;
+        const Entry entry = lists[w][k];
+        z[e] = k < p.top ? ValueOf(entry.order) : -Inf();
+        index[e] = entry.index;
+      }
+      if (!Rank<kEach>(z, [&](int e) { return index[e]; }, known, lane, slots[0], &best)) {
+        for (int w = 1; w < WAVES; ++w) {
+          const Entry entry = lists[w][lane % kMostAlternatives];
+          best.Merge(entry.order, entry.index, lane);
+        }
+      }
     }
     if (p.splits > 1) {
       float* state = p.states + (row * p.splits + blockIdx.y) * (4 + 2 * p.top);
@@ -442,7 +626,7 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
         state[2] = sums.t;
       }
       if (lane < p.top) {
-        state[4 + lane] = best.value;
+        state[4 + lane] = ValueOf(best.order);
         state[4 + p.top + lane] = __int_as_float(best.index);
       }
       return;
@@ -451,12 +635,14 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
   Answer(p, row, chosen, sums, best, lane);
 }
 
-// One wave per row: lane i takes split i's sums.
+// One wave per row: lane i takes split i's sums, and the splits' lists, element k of
+// split s being the (s top + k)-th, are searched as a row's elements are.
 template <typename T>
 __global__ __launch_bounds__(kWave) void JoinLogprobsKernel(LogprobParams p) {
   const int lane = threadIdx.x;
   const std::int64_t row = blockIdx.x;
-  const float* states = p.states + row * p.splits * (4 + 2 * p.top);
+  const int state_size = 4 + 2 * p.top;
+  const float* states = p.states + row * p.splits * state_size;
   Row<T> from;
   from.c = static_cast<const T*>(p.logits) + row * p.stride;
   from.u = p.uncond == nullptr ? nullptr
@@ -464,22 +650,37 @@ __global__ __launch_bounds__(kWave) void JoinLogprobsKernel(LogprobParams p) {
   from.g = p.guidance;
   const float chosen = Chosen(p, row, from);
   Sums sums{-Inf(), 0.0F, 0.0F};
-  Alternatives best{-Inf(), -1, p.top};
+  Alternatives best(p.top);
   if (lane < p.splits) {
-    const float* state = states + lane * (4 + 2 * p.top);
+    const float* state = states + lane * state_size;
     sums = {state[0], state[1], state[2]};
   }
-  // Lane k of the s-th list; the next one is on its way while this one is offered.
-  float value = lane < p.top ? states[4 + lane] : -Inf();
-  int index = lane < p.top ? __float_as_int(states[4 + p.top + lane]) : -1;
-  for (int s = 0; s < p.splits && p.top > 0; ++s) {
-    const float* next = states + min(s + 1, p.splits - 1) * (4 + 2 * p.top);
-    const float next_value = lane < p.top ? next[4 + lane] : -Inf();
-    const int next_index = lane < p.top ? __float_as_int(next[4 + p.top + lane]) : -1;
-    best.Merge([&](int k) { return LaneOf(value, k); },
-               [&](int k) { return __builtin_amdgcn_readlane(index, k); }, lane);
-    value = next_value;
-    index = next_index;
+  // Element k of split s is the (32 s + k)-th, of up to 512: 8 a lane.
+  if (p.top > 0) {
+    constexpr int kEach = kMostLogprobSplits * kMostAlternatives / kWave;
+    __shared__ Entry slots[kWave];
+    float z[kEach];
+    int index[kEach];
+    unsigned floor = 1;
+    if (lane < p.splits)
+      floor = max(floor, OrderOf(states[lane * state_size + 4 + p.top - 1]));
+    const unsigned known = WaveMaxOf(floor);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int split = e * (kWave / kMostAlternatives) + lane / kMostAlternatives;
+      const int k = lane % kMostAlternatives;
+      const bool there = split < p.splits && k < p.top;
+      const float* state = states + min(split, p.splits - 1) * state_size + 4 + min(k, p.top - 1);
+      z[e] = state[0];
+      index[e] = there ? __float_as_int(state[p.top]) : -1;
+    }
+    if (!Rank<kEach>(z, [&](int e) { return index[e]; }, known, lane, slots, &best)) {
+      segment_t all;
+#pragma unroll
+      for (int e = 0; e < kElements; ++e)
+        all[e] = e < kEach ? z[e % kEach] : -Inf();
+      Search<kElements>(all, Peak(all), [&](int e) { return index[e % kEach]; }, 0, lane, &best);
+    }
   }
   sums.JoinWave();
   Answer(p, row, chosen, sums, best, lane);
@@ -508,7 +709,7 @@ int PlanLogprobs(int rows, int vocab) {
     return 1;
   const int wanted = (kLogprobGroups + rows - 1) / rows;
   const int most = (vocab + kWaves * kSegment - 1) / (kWaves * kSegment);
-  return std::max(1, std::min({wanted, most, kWave}));
+  return std::max(1, std::min({wanted, most, kMostLogprobSplits}));
 }
 
 void LaunchLogprobs(const LogprobParams& p, DType type, hipStream_t stream) {
