@@ -661,34 +661,36 @@ def op_attention(qkv, out, heads: int, kv_heads: int,
 def _type_of(t, name: str, with_f32: bool = True) -> int:
     """OVG_F16, OVG_BF16 or OVG_F32 of a tensor."""
     import torch
-    if t.dtype is torch.float16:
+    dtype = t.dtype
+    if dtype is torch.float16:
         return 0
-    if t.dtype is torch.bfloat16:
+    if dtype is torch.bfloat16:
         return 1
-    if with_f32 and t.dtype is torch.float32:
+    if with_f32 and dtype is torch.float32:
         return 2
-    raise GeneratorError(f"{name}: {t.dtype} is not supported")
+    raise GeneratorError(f"{name}: {dtype} is not supported")
 
 
 def _expect(t, name: str, dtype, shape: Tuple[int, ...], device) -> None:
     """A contiguous device tensor of this type and shape on `device`."""
-    if t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous() \
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() \
             or t.device != device:
         raise GeneratorError(f"{name}: needs a contiguous {dtype} tensor of shape {shape} on "
                              f"{device}, got {t.dtype} {tuple(t.shape)} on {t.device}"
                              f"{'' if t.is_contiguous() else ', not contiguous'}")
 
 
-def _row_stride(t, name: str, heads: int, dim: int, device) -> int:
+def _row_stride(t, name: str, rows: int, heads: int, dim: int, device) -> int:
     """The row stride, in elements, of a [rows][heads][dim] tensor whose rows are
     contiguous."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.device != device \
-            or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
-        raise GeneratorError(f"{name}: needs [rows][{heads}][{dim}] with contiguous rows on "
-                             f"{device}, got {tuple(t.shape)} with strides {t.stride()} on "
+    strides = t.stride()
+    if t.shape != (rows, heads, dim) or t.device != device \
+            or strides[2] != 1 or (heads > 1 and strides[1] != dim):
+        raise GeneratorError(f"{name}: needs [{rows}][{heads}][{dim}] with contiguous rows on "
+                             f"{device}, got {tuple(t.shape)} with strides {strides} on "
                              f"{t.device}")
     # A single row has no stride of its own.
-    return t.stride(0) if t.shape[0] > 1 else heads * dim
+    return strides[0] if rows > 1 else heads * dim
 
 
 def _raw_stream(index: int) -> int:
@@ -813,28 +815,29 @@ def _check_cache(cache: KVCache, sequences: KVSequences) -> None:
         raise GeneratorError(f"sequences on {sequences.device}, the cache on {cache.device}")
 
 
-def _cache_io(name: str, cache: KVCache, sequences: KVSequences, k, v, stream) -> None:
+def _cache_io(fn, cache: KVCache, sequences: KVSequences, k, v, stream) -> None:
     _check_cache(cache, sequences)
-    k_stride = _row_stride(k, "k", cache.kv_heads, cache.head_dim, cache.device)
-    v_stride = _row_stride(v, "v", cache.kv_heads, cache.head_dim, cache.device)
-    if k.shape[0] != v.shape[0] or k.dtype is not v.dtype:
-        raise GeneratorError(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} "
-                             f"{v.dtype}")
-    _enqueue(getattr(lib(), name), cache.device, stream, cache._c, sequences._c(k.shape[0]),
-             k.data_ptr(), v.data_ptr(), k_stride, v_stride, _type_of(k, "k"))
+    device, heads, dim = cache.device, cache.kv_heads, cache.head_dim
+    rows = k.shape[0] if k.dim() else 0
+    k_stride = _row_stride(k, "k", rows, heads, dim, device)
+    v_stride = _row_stride(v, "v", rows, heads, dim, device)
+    if k.dtype is not v.dtype:
+        raise GeneratorError(f"k and v differ: {k.dtype}, {v.dtype}")
+    _enqueue(fn, device, stream, cache._c, sequences._c(rows), k.data_ptr(), v.data_ptr(),
+             k_stride, v_stride, _type_of(k, "k"))
 
 
 def op_cache_write(cache: KVCache, sequences: KVSequences, k, v, stream=None) -> None:
     """Quantises k and v [rows][kv_heads][head_dim] (fp16, bf16 or float32
     device tensors with contiguous rows) into the cache as the last tokens of
     their sequences. Enqueued on `stream`."""
-    _cache_io("ovg_op_cache_write", cache, sequences, k, v, stream)
+    _cache_io(lib().ovg_op_cache_write, cache, sequences, k, v, stream)
 
 
 def op_cache_read(cache: KVCache, sequences: KVSequences, k, v, stream=None) -> None:
     """The last tokens of the sequences back into k and v
     [rows][kv_heads][head_dim] (fp16, bf16 or float32). Enqueued on `stream`."""
-    _cache_io("ovg_op_cache_read", cache, sequences, k, v, stream)
+    _cache_io(lib().ovg_op_cache_read, cache, sequences, k, v, stream)
 
 
 def op_cache_attention_workspace(cache: KVCache, sequences: KVSequences, rows: int,
@@ -854,32 +857,33 @@ def op_cache_attention(cache: KVCache, sequences: KVSequences, q, out,
     _check_cache(cache, sequences)
     if q.dim() != 3:
         raise GeneratorError(f"q: needs [rows][heads][{cache.head_dim}], got {tuple(q.shape)}")
-    rows, heads = q.shape[:2]
-    q_stride = _row_stride(q, "q", heads, cache.head_dim, cache.device)
-    out_stride = _row_stride(out, "out", heads, cache.head_dim, cache.device)
-    if out.shape[0] != rows or out.dtype is not q.dtype:
-        raise GeneratorError(f"q and out differ: {tuple(q.shape)} {q.dtype}, "
-                             f"{tuple(out.shape)} {out.dtype}")
+    device, dim = cache.device, cache.head_dim
+    rows, heads, _ = q.shape
+    q_stride = _row_stride(q, "q", rows, heads, dim, device)
+    out_stride = _row_stride(out, "out", rows, heads, dim, device)
+    if out.dtype is not q.dtype:
+        raise GeneratorError(f"q and out differ: {q.dtype}, {out.dtype}")
     kind = _type_of(q, "q", with_f32=False)
     seq = sequences._c(rows)
     L = lib()
     space, size, keep = _workspace(
-        workspace, L.ovg_op_cache_attention_workspace(cache._c, seq, heads), cache.device, stream)
+        workspace, L.ovg_op_cache_attention_workspace(cache._c, seq, heads), device, stream)
     if scale is None:
-        scale = cache.head_dim ** -0.5
-    _enqueue(L.ovg_op_cache_attention, cache.device, stream, cache._c, seq, q.data_ptr(),
+        scale = dim ** -0.5
+    _enqueue(L.ovg_op_cache_attention, device, stream, cache._c, seq, q.data_ptr(),
              out.data_ptr(), q_stride, out_stride, heads, scale, int(causal), kind, space, size)
 
 
 # --------------------------------------------------------------- log probabilities
 
 def _logit_stride(t, name: str, rows: int, vocab: int, device, dtype) -> int:
-    if tuple(t.shape) != (rows, vocab) or t.device != device or t.dtype is not dtype \
-            or (vocab > 1 and t.stride(1) != 1):
+    strides = t.stride()
+    if t.shape != (rows, vocab) or t.device != device or t.dtype is not dtype \
+            or (vocab > 1 and strides[1] != 1):
         raise GeneratorError(f"{name}: needs [{rows}][{vocab}] {dtype} with contiguous rows on "
                              f"{device}, got {tuple(t.shape)} {t.dtype} with strides "
-                             f"{t.stride()} on {t.device}")
-    return t.stride(0) if rows > 1 else vocab
+                             f"{strides} on {t.device}")
+    return strides[0] if rows > 1 else vocab
 
 
 def op_token_logprobs(logits, tokens, logprob, entropy, top_ids=None, top_logprobs=None,

@@ -135,18 +135,24 @@ struct CacheAttentionPlan {
   std::size_t slots = 0;  // of the workspace
 };
 constexpr int kMostSplits = 256;
-constexpr int kFewSplits = 8;     // that one group of lanes joins by itself
-constexpr int kLeastChunk = 256;  // keys of a split at least
-// The same for tiles of 32 rows, whose splits leave as much as they read: 375
-// queries of two heads over 2000 keys take 16.8 us whole and 20.9 in two, 100 over
-// 16000 take 80 us whole and 30 in four.
-constexpr int kLeastTileChunk = 1024;
-// Work-groups that a split call is to have. Alone, a sequence's splits are equal
-// and two a CU keep the memory busy (90001 keys: 41 us with 512, 44 with 1024, whose
-// join takes longer); several of few rows are ragged and fill the device better in
-// smaller pieces (48 of up to 8192 keys: 95.6 us with 1024, 99.4 with 512).
+constexpr int kFewSplits = 8;  // that one group of lanes joins by itself
+// Sequences of few rows (16-row tiles) that leave CUs idle are split until every CU
+// has a work-group, into 256 keys at least and only from 1024 tokens on: the second
+// launch costs what 500 keys do (8 heads, us of the GPU: 500 keys 6.3 whole and 7.4
+// in two, 1000 keys 8.2 and 7.1 in eight, 4000 keys 19.7 and 8.6 in sixteen, 90001
+// keys 34 in 16 to 64; 16 sequences of 1000 keys 9.6 whole, 11.6 in two).
+constexpr int kFullGroups = 256;
+constexpr int kLeastSplit = 1024;
+constexpr int kLeastChunk = 256;
+// Many of them are ragged and fill the device better in smaller pieces, of 1024 keys
+// at least: 48 of up to 8192 keys take 102 us whole, 95.5 in four, 32 of 4000 keys
+// 48.4 and 46.3.
+constexpr int kRaggedGroups = 2048;
+// Tiles of 32 rows leave as much as they read when they are split: 375 queries of two
+// heads over 2000 keys take 16.8 us whole and 20.9 in two, 100 over 16000 take 80 us
+// whole and 30 in four.
 constexpr int kSplitGroups = 512;
-constexpr int kRaggedSplitGroups = 1024;
+constexpr int kLeastTileChunk = 1024;
 CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group);
 // Keys of each split of a sequence of `length` tokens: a whole number of the
 // four waves' steps.

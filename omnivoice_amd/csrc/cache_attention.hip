@@ -721,12 +721,15 @@ CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group) {
   const int items = ItemBound(c, group, plan.tile_shift, 1);
   const std::int64_t groups = static_cast<std::int64_t>(items) * c.kv_heads;
   const std::int64_t capacity = static_cast<std::int64_t>(c.table_width) << c.block_shift;
-  const std::int64_t wanted =
-      !few ? kSplitGroups / groups
-           : ((c.count > 1 ? kRaggedSplitGroups : kSplitGroups) + groups - 1) / groups;
+  std::int64_t wanted = kSplitGroups / groups, least = kLeastTileChunk;
+  if (few && groups < kFullGroups) {
+    wanted = capacity < kLeastSplit ? 1 : kFullGroups / groups;
+    least = kLeastChunk;
+  } else if (few) {
+    wanted = kRaggedGroups / groups;
+  }
   plan.splits = static_cast<int>(std::max<std::int64_t>(
-      1, std::min({wanted, capacity / (few ? kLeastChunk : kLeastTileChunk),
-                   std::int64_t{kMostSplits}})));
+      1, std::min({wanted, capacity / least, std::int64_t{kMostSplits}})));
   if (plan.splits > 1)
     plan.slots = (static_cast<std::size_t>(groups) * plan.splits) << plan.tile_shift;
   return plan;
