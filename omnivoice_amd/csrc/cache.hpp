@@ -125,6 +125,7 @@ struct CacheAttentionParams {
   // slot ((item * kv_heads + head) * splits + split) * tile rows + row has its
   // row's maximum and sum in partial_m and its output, not divided, in partial_o.
   int tile_shift, splits;
+  int items, first_item;  // tiles in all, and the first of a launch
   float* partial_m;  // [slots][2]
   float* partial_o;  // [slots][dim]
 };

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
   const int head = blockIdx.x;
 
   // The last rows of a causal sequence see the most keys: they start first.
-  const int item = gridDim.y - 1 - blockIdx.y;
+  const int item = p.items - 1 - p.first_item - static_cast<int>(blockIdx.y);
   const Found found = FindItem(c, p.group, ROWS == 16 ? 4 : 5, 1, item);
   const int sequence = found.sequence, tile = found.item;
   const Span span = found.span;
@@ -558,7 +558,8 @@ template <typename T, int DIM>
 __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
   constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
   const CacheView& c = p.cache;
-  const Found found = FindItem(c, p.group, p.tile_shift, 1, blockIdx.y);
+  const int item = p.first_item + static_cast<int>(blockIdx.y);
+  const Found found = FindItem(c, p.group, p.tile_shift, 1, item);
   const int tile = found.item;
   const Span span = found.span;
   const int rows = span.count * p.group;
@@ -569,7 +570,7 @@ __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
   const int head = blockIdx.x;
   const int tid = threadIdx.x, group = tid / kLanes, part = tid % kLanes;
   const std::size_t first =
-      (((static_cast<std::size_t>(blockIdx.y) * c.kv_heads + head) * p.splits) << p.tile_shift) +
+      (((static_cast<std::size_t>(item) * c.kv_heads + head) * p.splits) << p.tile_shift) +
       in_tile;
   __shared__ float weights[kMostSplits];
   __shared__ float wave_top[4];
@@ -637,7 +638,8 @@ template <typename T, int DIM>
 __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
   constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
   const CacheView& c = p.cache;
-  const Found found = FindItem(c, p.group, p.tile_shift, 1, blockIdx.y);
+  const int item = p.first_item + static_cast<int>(blockIdx.y);
+  const Found found = FindItem(c, p.group, p.tile_shift, 1, item);
   const int tile = found.item;
   const Span span = found.span;
   const int rows = span.count * p.group;
@@ -648,7 +650,7 @@ __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
     return;
   const int head = blockIdx.x;
   const std::size_t first =
-      (((static_cast<std::size_t>(blockIdx.y) * c.kv_heads + head) * p.splits) << p.tile_shift) +
+      (((static_cast<std::size_t>(item) * c.kv_heads + head) * p.splits) << p.tile_shift) +
       in_tile;
   float m[kFewSplits], l[kFewSplits];
   floatx4 o[kFewSplits];
@@ -685,26 +687,39 @@ __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
                    rounded, sizeof(rounded));
 }
 
+constexpr int kMostItems = 65535;  // of a grid's second dimension
+
 template <typename T, int DIM>
 void Launch(const CacheAttentionParams& p, hipStream_t stream) {
-  const int items = ItemBound(p.cache, p.group, p.tile_shift, 1);
-  const dim3 grid(p.cache.kv_heads, items, p.splits), block(kWaves * kWave);
   const bool one = p.cache.block_shift > 4, last = p.splits == 1;
   const auto kernel = p.tile_shift == 4 ? one ? CacheAttentionKernel<T, DIM, 16, true>
                                               : CacheAttentionKernel<T, DIM, 16, false>
                       : one             ? CacheAttentionKernel<T, DIM, 32, true>
                                         : CacheAttentionKernel<T, DIM, 32, false>;
-  Dispatch(kernel, grid, block, 0, stream, true, last, p);
-  if (last)
-    return;
   constexpr int kJoined = 256 / (DIM / 4);  // rows of a work-group with few splits
-  if (p.splits <= kFewSplits)
-    Dispatch(JoinFewKernel<T, DIM>,
-             dim3(p.cache.kv_heads, items, ((1 << p.tile_shift) + kJoined - 1) / kJoined),
-             dim3(256), 0, stream, false, true, p);
-  else
-    Dispatch(JoinKernel<T, DIM>, dim3(p.cache.kv_heads, items, 1 << p.tile_shift), dim3(256), 0,
-             stream, false, true, p);
+  const int in_tile = 1 << p.tile_shift;
+  CacheAttentionParams part = p;
+  part.items = ItemBound(p.cache, p.group, p.tile_shift, 1);
+  // A launch holds 65535 items; the heads come first, so that with 8 of them the
+  // tiles of a head share their XCD's L2.
+  for (part.first_item = 0; part.first_item < part.items; part.first_item += kMostItems) {
+    const int items = std::min(part.items - part.first_item, kMostItems);
+    const bool first = part.first_item == 0, end = part.first_item + items == part.items;
+    Dispatch(kernel, dim3(p.cache.kv_heads, items, p.splits), dim3(kWaves * kWave), 0, stream,
+             first, end && last, part);
+    if (last)
+      continue;
+    // The items that this launch took, counted from the last one.
+    CacheAttentionParams join = part;
+    join.first_item = part.items - part.first_item - items;
+    if (p.splits <= kFewSplits)
+      Dispatch(JoinFewKernel<T, DIM>,
+               dim3(p.cache.kv_heads, items, (in_tile + kJoined - 1) / kJoined), dim3(256), 0,
+               stream, false, end, join);
+    else
+      Dispatch(JoinKernel<T, DIM>, dim3(p.cache.kv_heads, items, in_tile), dim3(256), 0, stream,
+               false, end, join);
+  }
 }
 
 }  // namespace

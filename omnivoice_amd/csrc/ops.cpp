@@ -461,7 +461,7 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
 }
 
 int64_t ovg_op_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top) {
-  if (!FitsInt(rows) || vocab < 1 || !FitsInt(vocab) || top < 0 || top > ovg::kMostAlternatives)
+  if (rows < 0 || rows > (1 << 23) || vocab < 1 || !FitsInt(vocab) || top < 0 || top > ovg::kMostAlternatives)
     return -1;
   return LogprobBytes(rows, top,
                       ovg::PlanLogprobs(static_cast<int>(rows), static_cast<int>(vocab)));
@@ -475,7 +475,8 @@ int ovg_op_token_logprobs(const void* logits, const void* uncond, int64_t rows, 
                           size_t error_len) {
   return Guard("token logprobs: ", error, error_len, [&] {
     const ovg::DType t = TypeOf(type, true);
-    ovg::Require(rows >= 0 && FitsInt(rows), "rows outside [0, 2^30]");
+    // A work-group of 256 a row, in a grid that counts 2^32 threads.
+    ovg::Require(rows >= 0 && rows <= (1 << 23), "rows outside [0, 2^23]");
     ovg::Require(vocab >= 1 && FitsInt(vocab), "vocab outside [1, 2^30]");
     ovg::Require(top >= 0 && top <= ovg::kMostAlternatives, "top outside [0, 32]");
     ovg::Require(mask_id >= -1 && mask_id < (int64_t{1} << 31), "mask_id must be -1 or a token");

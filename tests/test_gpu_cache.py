@@ -440,6 +440,54 @@ def test_attention_of_many_sequences(new, lengths):
     attention_case(3, new, lengths, 2, 2, 64, 16, "f16", True)
 
 
+def test_more_sequences_than_a_launch_holds():
+    """70000 sequences of one token each over eight shared blocks, and some of
+    none: against the same rows in calls of their own."""
+    rng = np.random.default_rng(20)
+    count, dim, block, heads = 70000, 64, 16, 1
+    table = rng.integers(0, 8, (count, 1))
+    lengths = rng.integers(1, 17, count)
+    new = np.where(rng.random(count) < 0.01, 0, 1)
+    begins = np.concatenate([[0], np.cumsum(new)])
+    cache = filled(rng, 8, heads, dim, block)
+    q = tensor(rng.standard_normal((begins[-1], 1, dim)), "f16")
+    out = torch.full_like(q, 9.0)
+    ov.op_cache_attention(cache, sequences(table, lengths, begins), q, out, causal=True)
+    again = torch.full_like(q, 9.0)
+    for a in range(0, count, 25000):
+        rows = slice(begins[a], begins[min(a + 25000, count)])
+        ov.op_cache_attention(
+            cache, sequences(table[a:a + 25000], lengths[a:a + 25000],
+                             begins[a:a + 25001] - begins[a]), q[rows], again[rows], causal=True)
+    assert torch.equal(out, again) and (out != 9).any(-1).all()
+    pick = rng.permutation(np.flatnonzero(new))[:300]
+    check_attention(cache, (table[pick], lengths[pick], np.arange(301)), q[begins[pick]],
+                    out[begins[pick]], 1, "f16", dim ** -0.5, True)
+    k = tensor(rng.standard_normal((begins[-1], 1, dim)), "f16")
+    v = torch.empty_like(k)
+    ov.op_cache_read(cache, sequences(table, lengths, begins), k, v)
+    plain = Plain(cache)
+    at = np.stack([plain.read(table[i], lengths[i] - 1, lengths[i])[1][0] for i in pick])
+    np.testing.assert_array_equal(np64(v[begins[pick]]), at)
+
+
+def test_long_tables_of_small_blocks():
+    """20000 tokens in blocks of 16: each wave goes through several windows of the
+    table, some of whose blocks are missing or NaN behind the rows' sight."""
+    rng = np.random.default_rng(21)
+    for new, dtype in ((1, "f16"), (30, "bf16")):
+        table, blocks = tables_of(rng, [20000], 16)
+        table[0, rng.permutation(1250)[:200]] = -1
+        cache = filled(rng, blocks, 1, 64, 16)
+        cache.scales[:, :, 1] *= torch.from_numpy(
+            np.ldexp(1.0, rng.integers(0, 8, (blocks, 1))).astype(np.float32)).cuda()
+        q = tensor(rng.standard_normal((new, 2, 64)), dtype)
+        out = torch.empty_like(q)
+        seq_np = (table, np.array([20000]), np.array([0, new]))
+        ov.op_cache_attention(cache, sequences(*seq_np), q, out, causal=True)
+        check_attention(cache, seq_np, q, out, 2, dtype, 0.125, True)
+
+
 @pytest.mark.parametrize("new", [2, 60, 200])
 def test_attention_rows_that_see_nothing(new):
     """More rows than tokens (causal: the first ones come before position 0),

@@ -45,7 +45,7 @@ def plain(z, tokens, top, mask):
         log_s = np.log(e.sum())
         logprob[r] = d[tokens[r]] - log_s if 0 <= tokens[r] < vocab else -np.inf
         entropy[r] = log_s - (e[e > 0] * d[e > 0]).sum() / e.sum()
-        order = np.argsort(-z[r], kind="stable")
+        order = np.argsort(-z[r], kind="stable")[:top + 1]
         order = [i for i in order if i != mask and z[r, i] > -np.inf][:top]
         ids[r, :len(order)] = order
         best[r, :len(order)] = d[order] - log_s
@@ -144,6 +144,29 @@ def test_ties_go_to_the_lowest_index(dtype, vocab):
     c = torch.from_numpy(x).to(TYPES[dtype]).cuda()
     for mask in (None, 0, int(np.argmax(x[2])), vocab - 1):
         check(c, None, rng.integers(0, vocab, rows), 32, 0.0, mask)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("step", [16, 1024, 4096, 8192, 1040])
+@pytest.mark.parametrize("mask", [None, 80])
+def test_best_tokens_in_a_row_of_steps(dtype, step, mask):
+    """The best tokens every so many places apart, rising and falling, among
+    smaller ones: all in one lane's runs, in one run, in one wave's, and equal."""
+    rng = np.random.default_rng(step)
+    vocab = 150000
+    x = rng.random((3, vocab)).astype(np.float32)
+    at = 80 + np.arange(36) * step
+    at = at[at < vocab]
+    x[0, at] = 5 + np.arange(len(at)) / 4
+    x[1, at] = 50 - np.arange(len(at)) / 4
+    x[2, at] = 7.0
+    c = torch.from_numpy(x).to(TYPES[dtype]).cuda()
+    got = check(c, None, [80, 81, 149999], 32, 0.0, mask)
+    # The same rows many times: whole in a work-group each instead of split.
+    many = call(c.repeat(200, 1), None, [80, 81, 149999] * 200, 7, 0.0, mask)
+    np.testing.assert_array_equal(many[2].cpu().numpy(), np.tile(got[2][:, :7], (200, 1)))
+    np.testing.assert_allclose(many[3].cpu().numpy(), np.tile(got[3][:, :7], (200, 1)),
+                               atol=2 * (vocab / 64 + 40) * 2.0 ** -24)
 
 
 @pytest.mark.parametrize("vocab", [70, 1025, 40000])
