@@ -376,7 +376,8 @@ typedef struct ovg_kv_cache {
  *            begins[0] or from begins[count] on belong to nobody and are left
  *            as they are; so is, of `rows` rows, what begins names past them.
  * Positions past table_width * block_tokens, or before 0 where a sequence has
- * more rows than tokens, are treated as those without a block. */
+ * more rows than tokens, are treated as those without a block. Up to 2^24 rows,
+ * 2^20 sequences, 2^30 positions and 1024 kv heads. */
 typedef struct ovg_kv_sequences {
   const int32_t* tables;
   const int32_t* lengths;
@@ -413,10 +414,12 @@ int ovg_op_cache_read(const ovg_kv_cache* cache, const ovg_kv_sequences* sequenc
  * length - n + t). softmax(scale * q . k) v in float32 sums, the probabilities
  * rounded to `type` for their product with the values; a row that sees nothing
  * is zero. A query that sees a token of a block whose scale is NaN is NaN.
- * A value's part is kept to 2^-33 of the loudest value of its head in fp16.
- * `workspace`: ovg_op_cache_attention_workspace bytes (-1 for arguments that
- * the call refuses), 16-byte aligned, NULL where that is 0; it holds nothing between calls, and calls that may overlap
- * need one each. */
+ * In fp16 a value counts to 2^-33 of the most that its head's largest value
+ * scale holds. `out` may be `q` itself. `workspace`:
+ * ovg_op_cache_attention_workspace bytes (-1 for arguments that the call
+ * refuses), 16-byte aligned, NULL where that is 0; it holds nothing between
+ * calls, and calls that may overlap need one each. heads is 1 to 64 times
+ * kv_heads; scale may be negative. */
 int64_t ovg_op_cache_attention_workspace(const ovg_kv_cache* cache,
                                          const ovg_kv_sequences* sequences, int64_t heads);
 int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
@@ -437,7 +440,8 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
  * tokens can be listed the rest are -1 and -inf. A row without a distribution
  * (a NaN or +inf among its logits, or only -inf) gets NaN and -1.
  * logprob (with tokens) and entropy may be NULL, as may top_ids and
- * top_logprobs [rows][top] where top is 0; top <= 32. `workspace` as above.
+ * top_logprobs [rows][top] where top is 0; top <= 32, rows <= 2^23.
+ * `workspace` as above.
  * Same streams and captures as the cache's calls. */
 int64_t ovg_op_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top);
 int ovg_op_token_logprobs(const void* logits, const void* uncond, int64_t rows, int64_t vocab,

@@ -57,10 +57,10 @@ struct Span {
 // Work items of ragged sequences without a list: sequence i owns the items
 // from first_i * scale / tile + slack * i (a whole-number division) up to the next
 // one's, at least rows_i * scale / tile + slack of them. Every lane looks at a
-// sequence of its own and holds what belongs to it, so that finding an item and
-// its span is one trip to memory per 64 sequences and none after the other. The
-// whole wave calls this; all it returns is the same in every lane. count 0: the
-// item is nobody's.
+// sequence of its own and holds what belongs to it, so that finding an item and its
+// span is one trip to memory for up to 64 sequences; where there are more, a trip
+// before it leaves a 64th of them. The whole wave calls this; all it returns is the
+// same in every lane. count 0: the item is nobody's.
 struct Found {
   int sequence, item;  // item: of the sequence
   Span span;
@@ -69,25 +69,32 @@ __device__ __forceinline__ Found FindItem(const CacheView& c, int scale, int shi
                                           int item) {
   const int lane = threadIdx.x & (kWave - 1);
   Found f{0, 0, {0, 0, 0, 0}};
-  for (int i0 = 0; i0 < c.count; i0 += kWave) {
-    const int i = min(i0 + lane, c.count - 1);
-    const int begin = c.begins[i], end = c.begins[i + 1], length = c.lengths[i];
-    const int first = min(max(begin, 0), c.rows);
-    const int rows = min(max(end, first), c.rows) - first;
+  int low = 0, count = c.count;  // the owner is one of these
+  while (count > kWave) {
+    const int stride = (count + kWave - 1) / kWave;
+    const int i = min(low + lane * stride, c.count - 1);
+    const int first = min(max(c.begins[i], 0), c.rows);
     const int base = ((first * scale) >> shift) + slack * i;
-    const unsigned long long at = __ballot(i0 + lane < c.count && base <= item);
-    const int below = __popcll(at);
-    if (below > 0) {
-      const int owner = below - 1;
-      f.sequence = i0 + owner;
-      f.item = item - __builtin_amdgcn_readlane(base, owner);
-      f.span.first = __builtin_amdgcn_readlane(first, owner);
-      f.span.count = __builtin_amdgcn_readlane(rows, owner);
-      f.span.length = max(__builtin_amdgcn_readlane(length, owner), 0);
-      f.span.start = f.span.length - f.span.count;
-    }
-    if (below < kWave)
-      break;
+    const int below = __popcll(__ballot(lane * stride < count && base <= item));
+    if (below == 0)
+      return f;
+    low += (below - 1) * stride;
+    count = min(stride, count - (below - 1) * stride);
+  }
+  const int i = min(low + lane, c.count - 1);
+  const int begin = c.begins[i], end = c.begins[i + 1], length = c.lengths[i];
+  const int first = min(max(begin, 0), c.rows);
+  const int rows = min(max(end, first), c.rows) - first;
+  const int base = ((first * scale) >> shift) + slack * i;
+  const int below = __popcll(__ballot(lane < count && base <= item));
+  if (below > 0) {
+    const int owner = below - 1;
+    f.sequence = low + owner;
+    f.item = item - __builtin_amdgcn_readlane(base, owner);
+    f.span.first = __builtin_amdgcn_readlane(first, owner);
+    f.span.count = __builtin_amdgcn_readlane(rows, owner);
+    f.span.length = max(__builtin_amdgcn_readlane(length, owner), 0);
+    f.span.start = f.span.length - f.span.count;
   }
   return f;
 }

@@ -15,9 +15,10 @@
 // elements lie in its `top` loudest runs (equal ones by place: whatever lies in
 // another run has the loudest elements of those before it), so at the end a wave
 // picks that many runs, fetches them again and ranks the few elements that reach
-// the last one's loudest. Where a lane would have to give a fourth run, or more than
-// 64 elements are equal to the last, the wave searches all its elements once more,
-// with a sorted list in its lanes.
+// the last one's loudest. A lane that has given its three gets the next three from
+// its segments, which the wave asks for again. Where more than 64 elements reach the
+// last one's loudest, or the rows of the two tensors do not lie alike, the wave
+// searches all its elements once more, with a sorted list in its lanes.
 //
 // Elements come as 16-byte loads, 16 elements in a row to a lane, a segment of 1024
 // to a wave; the up to 14 before a row's first 16-byte border and behind its last are
@@ -155,14 +156,13 @@ struct Row {
 // A lane's elements of a segment, -inf for none.
 typedef float segment_t __attribute__((ext_vector_type(kElements)));
 
-// Takes the first `count` (a constant) of a segment's elements into the list;
-// index_of(e) is the e-th's, -1 for one that is not to be listed. peak: the lane's
-// largest. others: an order that the list's last is known to reach in the end.
+// Takes the first COUNT of a segment's elements into the list; index_of(e) is the
+// e-th's, -1 for one that is not to be listed. peak: the lane's largest.
 template <int COUNT, typename F>
 __device__ __forceinline__ void Search(const segment_t& z, float peak, F&& index_of,
-                                       unsigned others, int lane, Alternatives* best) {
+                                       int lane, Alternatives* best) {
   constexpr float kLowest = -3.402823466e38F;
-  unsigned floor = max(best->floor, others);
+  unsigned floor = best->floor;
   if (!__any(peak >= fmaxf(ValueOf(floor), kLowest)))
     return;
   if (floor == 0 && COUNT > 1) {
@@ -237,6 +237,13 @@ struct Entry {
   int index;
 };
 
+// Between a wave's own writes to LDS and its reads of what other lanes wrote: LDS
+// takes a wave's accesses in order, so only the compiler has to keep theirs.
+__device__ __forceinline__ void WaveFence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // The list of what is in a wave's COUNT elements a lane (index_of(e): -1 for one
 // that is not to be listed): those that reach `known` are gathered in `slots` (64,
 // the wave's own) and each finds its place by counting the ones before it. known: an
@@ -263,7 +270,7 @@ __device__ __forceinline__ bool Rank(const Z& z, F&& index_of, unsigned known, i
   }
   if (count > kWave)
     return false;
-  __builtin_amdgcn_wave_barrier();
+  WaveFence();
   const Entry own = lane < count ? slots[lane] : Entry{0, -1};
   int before = 0;
   for (int j = 0; j < count; ++j) {
@@ -271,10 +278,10 @@ __device__ __forceinline__ bool Rank(const Z& z, F&& index_of, unsigned known, i
     const int index = __builtin_amdgcn_readlane(own.index, j);
     before += order > own.order || (order == own.order && index < own.index) ? 1 : 0;
   }
-  __builtin_amdgcn_wave_barrier();
+  WaveFence();
   if (lane < count)
     slots[before] = own;
-  __builtin_amdgcn_wave_barrier();
+  WaveFence();
   const Entry mine = lane < min(count, best->top) ? slots[lane] : Entry{0, -1};
   best->order = mine.order;
   best->index = mine.index;
@@ -559,14 +566,14 @@ __global__ __launch_bounds__(kWaves* kWave) void LogprobKernel(LogprobParams p) 
         load(base);
         const segment_t z = elements(base, lane);
         Search<kElements>(
-            z, Peak(z), [&](int e) { return but_mask(head + base + lane * kElements + e); }, 0,
-            lane, &best);
+            z, Peak(z), [&](int e) { return but_mask(head + base + lane * kElements + e); }, lane,
+            &best);
       }
 #pragma unroll 1
       for (int k = left_first; k - lane < left; k += waves * kWave) {
         segment_t z;
         z[0] = k < left ? from.At(left_index(k)) : -Inf();
-        Search<1>(z, z[0], [&](int) { return but_mask(left_index(k)); }, 0, lane, &best);
+        Search<1>(z, z[0], [&](int) { return but_mask(left_index(k)); }, lane, &best);
       }
     }
   }
@@ -679,7 +686,7 @@ __global__ __launch_bounds__(kWave) void JoinLogprobsKernel(LogprobParams p) {
 #pragma unroll
       for (int e = 0; e < kElements; ++e)
         all[e] = e < kEach ? z[e % kEach] : -Inf();
-      Search<kElements>(all, Peak(all), [&](int e) { return index[e % kEach]; }, 0, lane, &best);
+      Search<kElements>(all, Peak(all), [&](int e) { return index[e % kEach]; }, lane, &best);
     }
   }
   sums.JoinWave();

@@ -430,7 +430,8 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
     ovg::Require(heads >= cache->kv_heads && heads % cache->kv_heads == 0 &&
                      heads / cache->kv_heads <= 64,
                  "heads must be 1 to 64 times kv_heads");
-    ovg::Require(scale == scale && scale - scale == 0.0F, "scale must be finite");
+    const float scale_log2 = std::fabs(scale) * 1.44269504088896341F;
+    ovg::Require(scale_log2 - scale_log2 == 0.0F, "scale must be finite, also times log2(e)");
     RequireStride(q_stride, heads * cache->head_dim);
     RequireStride(out_stride, heads * cache->head_dim);
     if (p.cache.rows == 0)
@@ -454,14 +455,15 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
     p.q_stride = q_stride;
     p.out_stride = out_stride;
     p.causal = causal != 0;
-    p.scale_log2 = std::fabs(scale) * 1.44269504088896341F;
+    p.scale_log2 = scale_log2;
     p.negate = scale < 0.0F;
     ovg::LaunchCacheAttention(p, t, s);
   });
 }
 
 int64_t ovg_op_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top) {
-  if (rows < 0 || rows > (1 << 23) || vocab < 1 || !FitsInt(vocab) || top < 0 || top > ovg::kMostAlternatives)
+  if (rows < 0 || rows > (1 << 23) || vocab < 1 || !FitsInt(vocab) || top < 0 ||
+      top > ovg::kMostAlternatives)
     return -1;
   return LogprobBytes(rows, top,
                       ovg::PlanLogprobs(static_cast<int>(rows), static_cast<int>(vocab)));

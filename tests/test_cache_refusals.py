@@ -79,6 +79,7 @@ def test_attention_refuses():
     assert "stride" in call(cache(), sequences(), os=100)
     assert "scale" in call(cache(), sequences(), scale=float("inf"))
     assert "scale" in call(cache(), sequences(), scale=float("nan"))
+    assert "scale" in call(cache(), sequences(), scale=-3e38)  # its log2(e)-fold is not
     assert "type" in call(cache(), sequences(), kind=2)
 
 
