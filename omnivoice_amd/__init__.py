@@ -722,17 +722,20 @@ def _enqueue(fn, device, stream, *args) -> None:
 
 
 def _workspace(workspace, size: int, device, stream):
-    """(pointer, bytes) of the caller's workspace, or of a new one that stays
-    reserved until the work on `stream` is done. The caller holds what this
-    returns until the launch."""
+    """(pointer, bytes) of the caller's workspace, or of a new one: `stream`'s
+    own memory (without one the current stream's), which only work behind this
+    call's takes again. The caller holds what this returns until the launch."""
     if workspace is None:
         if size <= 0:  # none needed, or arguments that the call will refuse
             return None, 0, None
         import torch
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        if stream is not None:
-            workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
-                                    else torch.cuda.ExternalStream(stream, device=device))
+        if stream is None:
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        else:
+            if not isinstance(stream, torch.cuda.Stream):
+                stream = torch.cuda.ExternalStream(stream, device=device)
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(size, dtype=torch.uint8, device=device)
     elif workspace.device != device or not workspace.is_contiguous():
         raise GeneratorError(f"workspace: needs a contiguous tensor on {device}")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace

@@ -647,6 +647,22 @@ def test_attention_strided_queries_and_output():
             assert (left == 9).all()
 
 
+@pytest.mark.parametrize("new,lengths", [([1, 1, 1], [70, 900, 33]), ([1], [9000]),
+                                         ([40, 3, 129], [100, 3, 640]), ([200], [6000])])
+def test_attention_in_place(new, lengths):
+    """Into the queries' own rows: whole, and in splits that are joined."""
+    rng = np.random.default_rng(24)
+    dim, block, heads, group = 128, 32, 2, 3
+    table, blocks = tables_of(rng, lengths, block)
+    cache = filled(rng, blocks, heads, dim, block)
+    seq = sequences(table, lengths, np.concatenate([[0], np.cumsum(new)]))
+    q = tensor(rng.standard_normal((sum(new), heads * group, dim)), "f16")
+    out = torch.empty_like(q)
+    ov.op_cache_attention(cache, seq, q, out, causal=True)
+    ov.op_cache_attention(cache, seq, q, q, causal=True)
+    assert torch.equal(out, q)
+
+
 def test_attention_single_tokens_do_not_depend_on_their_batch():
     """A sequence's rows are the same bits alone and among others."""
     rng = np.random.default_rng(15)
@@ -769,6 +785,19 @@ def test_calls_on_a_stream_of_their_own():
     plain = Plain(cache)
     assert (plain.scales > 0)[table[0]].all()
     check_attention(cache, seq_np, q, out, 2, "f16", dim ** -0.5, False)
+
+
+def test_a_new_workspace_is_its_streams_own():
+    """Memory that the current stream still uses must not serve another one."""
+    side = torch.cuda.Stream()
+    device = torch.device("cuda", torch.cuda.current_device())
+    for stream, handle in ((side, side.cuda_stream), (side.cuda_stream, side.cuda_stream),
+                           (None, 0)):
+        at, size, keep = ov._workspace(None, 5 << 20, device, stream)
+        assert size == 5 << 20
+        owner = [s["stream"] for s in torch.cuda.memory_snapshot()
+                 if s["address"] <= at < s["address"] + s["total_size"]]
+        assert owner == [handle]
 
 
 def test_a_workspace_of_the_callers():
