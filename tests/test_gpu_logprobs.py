@@ -131,6 +131,24 @@ def test_first_alternative_is_what_score_predicts():
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("vocab", [20, 65, 98, 130, 500, 1024, 1040, 2500])
+def test_long_lists_of_small_vocabularies(dtype, vocab):
+    """More tokens listed than there are runs of 16, magnitudes far apart, both
+    signs, and levels that more than 64 tokens share."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((7, vocab)).astype(np.float32)
+    x[1] = 10.0 ** rng.uniform(-4, 3, vocab) * rng.choice([-1.0, 1.0], vocab)
+    x[2] = -10.0 ** rng.uniform(-4, 3, vocab)
+    x[3] = np.round(x[3])                            # a few levels
+    x[4] = np.where(rng.random(vocab) < 0.7, 1.0, x[4])  # most of them one
+    x[5] = np.where(rng.random(vocab) < 0.7, -np.inf, x[5])
+    x[6] = np.where(np.arange(vocab) % 3 == 1, 0.0, -0.0)  # one value
+    c = torch.from_numpy(x).to(TYPES[dtype]).cuda()
+    for top, mask in ((1, None), (7, vocab // 2), (20, 0), (32, vocab - 1)):
+        check(c, None, rng.integers(0, vocab, 7), top, 0.0, mask)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("vocab", [100, 1025, 5000, 70000])
 def test_ties_go_to_the_lowest_index(dtype, vocab):
     rng = np.random.default_rng(4)
