@@ -131,7 +131,7 @@ struct CacheAttentionParams {
   // The plan's (PlanCacheAttention), and where its splits leave their states:
   // slot ((item * kv_heads + head) * splits + split) * tile rows + row has its
   // row's maximum and sum in partial_m and its output, not divided, in partial_o.
-  int tile_shift, splits;
+  int tile_shift, splits, own_shift;
   int items, first_item;  // tiles in all, and the first of a launch
   float* partial_m;  // [slots][2]
   float* partial_o;  // [slots][dim]
@@ -140,6 +140,7 @@ struct CacheAttentionParams {
 struct CacheAttentionPlan {
   int tile_shift = 4;     // log2 of a work-group's rows
   int splits = 1;         // of each sequence's keys
+  int own_shift = 0;      // log2 of a work-group's tiles
   std::size_t slots = 0;  // of the workspace
 };
 constexpr int kMostSplits = 256;
@@ -161,6 +162,15 @@ constexpr int kRaggedGroups = 2048;
 // whole and 30 in four.
 constexpr int kSplitGroups = 512;
 constexpr int kLeastTileChunk = 1024;
+// A wave takes a whole tile of 32 rows instead of a quarter of its keys where that
+// still fills the device, two work-groups a CU (128 dims) or four (64), and the keys
+// are few, so that the waves' join is much of the work: 32 sequences of 120 queries of
+// two heads over 256 keys 21.6 us and 32.1 in quarters, over 1024 47.6 and 56.0 (16 of
+// them, half of the device, 44.3 and 31.3; with 64 dims 39.1 and 31.3, 64 of them 51.8
+// and 56.8). With 128 dims it also pays over any keys from two fills on: two causal
+// prompts of 5000 tokens 234.5 and 239.9, 64 sequences of 120 over 2048 170 and 188.
+constexpr int kOwnTiles = 2048;  // of 128 dims that fill the device
+constexpr int kOwnKeys = 1024;
 CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group);
 // Keys of each split of a sequence of `length` tokens: a whole number of the
 // four waves' steps.

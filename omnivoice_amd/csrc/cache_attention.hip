@@ -15,7 +15,8 @@
 // A work-group takes 16 or 32 rows of one sequence and kv head and one split of
 // its keys; each of its four waves takes a quarter of those in steps of 32, with a
 // softmax of its own that runs along (maximum m, sum l, output o), and the four are
-// joined in LDS at the end. The pool's order is that of the matrix operands: the
+// joined in LDS at the end. Where there are rows enough, each wave takes 32 of them
+// and all their keys instead, and nothing is joined. The pool's order is that of the matrix operands: the
 // codes go from memory straight into registers, a step ahead, and are converted
 // there, with no LDS and no barrier on the way. A version in which 128 rows shared
 // tiles that were converted once and left in LDS was slower at every size (two
@@ -25,8 +26,8 @@
 //
 // Bound: memory where rows are few, 48 sequences of up to 8192 tokens (474 MB) in
 // 95.6 us, 5.0 TB/s. With many the issue of matrix and vector instructions: two causal
-// prompts of up to 5000 tokens (198 GFLOP) in 232 us, 854 TFLOP/s, the matrix cores
-// 42 % and the vector unit 36 % of the time; of the largest library product 1174. A
+// prompts of up to 5000 tokens (198 GFLOP) in 228 us, 868 TFLOP/s, the matrix cores
+// busy 46 % and vector instructions 38 % of the time; of the largest library product 1174. A
 // third work-group to a CU, its queries in LDS, did not raise that. A short call is a
 // chain of trips to memory: one token over 430 takes the kernel 6.5 us.
 #include <algorithm>
@@ -233,6 +234,16 @@ struct Window {
   std::size_t scale_at;
 };
 
+// The first of the four dims of a lane's j-th run of output: of rows 8 (j % 4) + 4 part
+// .. + 3 of tile j / 4, or 4 part .. + 3 of tile j.
+template <int DIM, int ROWS>
+__device__ __forceinline__ int DimOf(int j, int part) {
+  const int t = j / 4, high = j % 4 / 2, d = 8 * (j % 2) + 4 * part;
+  return ROWS == 16   ? 16 * j + 4 * part
+         : DIM == 128 ? 64 * high + 16 * t + d
+                      : 32 * high + 16 * t + d;
+}
+
 // ROWS rows (16 or 32) on v_mfma_f32_16x16x32 or v_mfma_f32_32x32x16: lane l holds
 // row l % ROWS and is part l / ROWS of it. Of every 16 keys a part holds four in a
 // row at 4 part (and with two parts the four at 8 more). A lane's 16 bytes of a key
@@ -241,7 +252,10 @@ struct Window {
 // the output's tile t is dims 16 t .. + 15; with 32 its two halves of rows stand for
 // dims 64 apart (128 dims) or 32 apart (64).
 // ONE: 32 keys are of one block (blocks of 32 or 64 tokens), else of two of 16.
-template <typename T, int DIM, int ROWS, bool ONE>
+// OWN: a wave takes a tile of its own with all its keys, the work-group's four one
+// after the other, instead of a quarter of one tile's keys: nothing is joined, and
+// the four read the same codes at about the same time, three of them out of the L1.
+template <typename T, int DIM, int ROWS, bool ONE, bool OWN>
 __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
     CacheAttentionParams p) {
   typedef Types<T> X;
@@ -264,8 +278,9 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
 
   // The last rows of a causal sequence see the most keys: they start first.
   const int item = p.items - 1 - p.first_item - static_cast<int>(blockIdx.y);
-  const Found found = FindItem(c, p.group, ROWS == 16 ? 4 : 5, 1, item);
-  const int sequence = found.sequence, tile = found.item;
+  const Found found = FindItem(c, p.group, ROWS == 16 ? 4 : OWN ? 7 : 5, 1, item);
+  const int sequence = found.sequence;
+  const int tile = OWN ? found.item * kWaves + wave : found.item;
   const Span span = found.span;
   const int rows = span.count * p.group;
   if (tile < 0 || tile * ROWS >= rows)
@@ -312,8 +327,8 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
   float loud = kQuietest;
 
   const int quarter = ((stop - begin + kWaves * 32 - 1) / (kWaves * 32)) * 32;
-  const int wave_begin = begin + wave * quarter;
-  const int wave_stop = min(wave_begin + quarter, stop);
+  const int wave_begin = OWN ? begin : begin + wave * quarter;
+  const int wave_stop = OWN ? stop : min(wave_begin + quarter, stop);
   const int in_block = (1 << c.block_shift) - 1;
   const std::size_t half_bytes = static_cast<std::size_t>(DIM) << c.block_shift;
   // With 32 rows a lane's key is of the first or the second 16, and its values of
@@ -496,6 +511,25 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
     window = window_stop;
   }
 
+  if constexpr (OWN) {
+    const float sum = RowSum<ROWS>(l[0] + l[1]);
+    if (row >= rows)
+      return;
+    const float scale = sum == 0.0F ? 0.0F : 1.0F / sum;
+    T* to = static_cast<T*>(p.out) + static_cast<std::int64_t>(span.first + query) * p.out_stride +
+            static_cast<std::int64_t>(head * p.group + of_group) * DIM;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < kFours; ++i) {
+        T rounded[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          rounded[r] = static_cast<T>(o[t][4 * i + r] * loud * scale);
+        __builtin_memcpy(to + DimOf<DIM, ROWS>(t * kFours + i, part), rounded, sizeof(rounded));
+      }
+    return;
+  }
   __shared__ float shared_m[kWaves][ROWS], shared_l[kWaves][ROWS];
   __shared__ floatx4 shared_o[kWaves][kTiles * kFours][64];
   const float sum = RowSum<ROWS>(l[0] + l[1]);
@@ -542,11 +576,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
 #pragma unroll
     for (int i = 0; i < kWaves; ++i)
       sum += shared_o[i][j][lane] * weight[i];
-    // The dims of rows 8 (j % 4) + 4 part .. + 3 of tile j / 4, or 4 part .. + 3 of j.
-    const int t = j / 4, high = j % 4 / 2, d = 8 * (j % 2) + 4 * part;
-    const int dim = ROWS == 16   ? 16 * j + 4 * part
-                    : DIM == 128 ? 64 * high + 16 * t + d
-                                 : 32 * high + 16 * t + d;
+    const int dim = DimOf<DIM, ROWS>(j, part);
     if (p.splits > 1) {
       *reinterpret_cast<floatx4*>(p.partial_o + slot * DIM + dim) = sum;
     } else {
@@ -699,14 +729,17 @@ constexpr int kMostItems = 65535;  // of a grid's second dimension
 template <typename T, int DIM>
 void Launch(const CacheAttentionParams& p, hipStream_t stream) {
   const bool one = p.cache.block_shift > 4, last = p.splits == 1;
-  const auto kernel = p.tile_shift == 4 ? one ? CacheAttentionKernel<T, DIM, 16, true>
-                                              : CacheAttentionKernel<T, DIM, 16, false>
-                      : one             ? CacheAttentionKernel<T, DIM, 32, true>
-                                        : CacheAttentionKernel<T, DIM, 32, false>;
+  const auto kernel = p.tile_shift == 4 ? one ? CacheAttentionKernel<T, DIM, 16, true, false>
+                                              : CacheAttentionKernel<T, DIM, 16, false, false>
+                      : p.own_shift > 0
+                          ? one ? CacheAttentionKernel<T, DIM, 32, true, true>
+                                : CacheAttentionKernel<T, DIM, 32, false, true>
+                      : one ? CacheAttentionKernel<T, DIM, 32, true, false>
+                            : CacheAttentionKernel<T, DIM, 32, false, false>;
   constexpr int kJoined = 256 / (DIM / 4);  // rows of a work-group with few splits
   const int in_tile = 1 << p.tile_shift;
   CacheAttentionParams part = p;
-  part.items = ItemBound(p.cache, p.group, p.tile_shift, 1);
+  part.items = ItemBound(p.cache, p.group, p.tile_shift + p.own_shift, 1);
   // A launch holds 65535 items; the heads come first, so that with 8 of them the
   // tiles of a head share their XCD's L2.
   for (part.first_item = 0; part.first_item < part.items; part.first_item += kMostItems) {
@@ -752,6 +785,10 @@ CacheAttentionPlan PlanCacheAttention(const CacheView& c, int group) {
   }
   plan.splits = static_cast<int>(std::max<std::int64_t>(
       1, std::min({wanted, capacity / least, std::int64_t{kMostSplits}})));
+  const std::int64_t fill = kOwnTiles * 128 / c.dim;
+  if (plan.splits == 1 && !few &&
+      (capacity <= kOwnKeys ? groups >= fill : c.dim == 128 && groups >= 2 * fill))
+    plan.own_shift = 2;
   if (plan.splits > 1)
     plan.slots = (static_cast<std::size_t>(groups) * plan.splits) << plan.tile_shift;
   return plan;

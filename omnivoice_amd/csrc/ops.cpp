@@ -448,6 +448,7 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
                  "workspace of " + std::to_string(bytes) + " bytes needed, 16-byte aligned");
     p.tile_shift = plan.tile_shift;
     p.splits = plan.splits;
+    p.own_shift = plan.own_shift;
     p.partial_o = static_cast<float*>(workspace);
     p.partial_m = p.partial_o + plan.slots * p.cache.dim;
     p.q = q;

@@ -440,6 +440,33 @@ def test_attention_of_many_sequences(new, lengths):
     attention_case(3, new, lengths, 2, 2, 64, 16, "f16", True)
 
 
+@pytest.mark.parametrize("new,lengths,heads,group,dim,block,dtype,causal", [
+    ([250, 1, 0, 131, 64], [400, 300, 9, 131, 70], 16, 9, 128, 32, "f16", True),
+    ([250, 33, 131], [300, 1000, 131], 16, 12, 128, 16, "bf16", False),
+    ([300, 2, 130], [310, 40, 200], 32, 10, 64, 64, "bf16", True),
+    ([300, 2, 130], [310, 40, 200], 32, 10, 64, 16, "f16", False),
+    ([520, 40], [1700, 1100], 16, 15, 128, 64, "f16", True),
+])
+def test_attention_of_rows_that_fill_the_device(new, lengths, heads, group, dim, block, dtype,
+                                                causal):
+    """A tile to a wave: tiles that end inside a work-group, sequences without rows.
+    Two kv heads are compared."""
+    rng = np.random.default_rng(25)
+    table, blocks = tables_of(rng, lengths, block)
+    cache = filled(rng, blocks, heads, dim, block)
+    begins = np.concatenate([[0], np.cumsum(new)])
+    q = tensor(rng.standard_normal((begins[-1], heads * group, dim)), dtype)
+    out = torch.full_like(q, 9.0)
+    ov.op_cache_attention(cache, sequences(table, lengths, begins), q, out, causal=causal)
+    assert torch.isfinite(out).all() and (out != 9).any(-1).all()
+    for head in (1, heads - 1):
+        one = ov.KVCache(cache.data[:, head:head + 1].contiguous(),
+                         cache.scales[:, head:head + 1].contiguous(), block, dim)
+        rows = slice(head * group, (head + 1) * group)
+        check_attention(one, (table, np.array(lengths), begins), q[:, rows], out[:, rows], group,
+                        dtype, dim ** -0.5, causal)
+
+
 def test_more_sequences_than_a_launch_holds():
     """70000 sequences of one token each over eight shared blocks, and some of
     none: against the same rows in calls of their own."""
