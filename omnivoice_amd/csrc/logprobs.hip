@@ -125,9 +125,11 @@ struct Alternatives {
 
 struct Sums {
   float m, s, t;
-  // The same sums relative to another maximum.
+  // The same sums relative to another maximum. The difference from a mask of the type's
+  // lowest value, or its product with s, would be -infinity, which f, 0 from -150 down,
+  // makes a NaN.
   __device__ __forceinline__ void Move(float to) {
-    const float d = m == -Inf() ? 0.0F : (m - to) * kLog2e;
+    const float d = m == -Inf() ? 0.0F : fmaxf((m - to) * kLog2e, -1000.0F);
     const float f = __builtin_amdgcn_exp2f(d);
     t = (t + s * d) * f;
     s = s * f;

@@ -295,3 +295,55 @@ def test_tensors_are_checked():
         with pytest.raises(ov.GeneratorError):
             ov.op_token_logprobs(**args)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("vocab", [40, 100, 1025, 2500, 40000, 151936])
+def test_masks_of_the_types_lowest_value(dtype, vocab):
+    """Masked ranges hold the type's lowest value, not -infinity: a lane's run, the
+    elements before the first 16-byte border and behind the last, whole waves and
+    whole splits; and the same from a logit next to the largest one. Few rows are
+    split over work-groups, many are not."""
+    rng = np.random.default_rng(vocab)
+    low, high = (float(f(torch.finfo(TYPES[dtype]))) for f in
+                 (lambda t: t.min, lambda t: t.max))
+    x = rng.standard_normal((9, vocab)).astype(np.float32)
+    x[0, 16:40] = low
+    x[1, :17] = x[1, -17:] = low
+    x[2, 5:] = low
+    x[3, :vocab - 5] = low
+    x[4, :vocab // 2] = low
+    x[5, vocab // 2:] = low
+    x[6, np.arange(vocab) // 1024 % 3 != 1] = low
+    x[6, -1] = 0.0
+    x[7, :vocab // 2] = low
+    x[7, vocab // 2:] = high
+    x[8, :vocab - 1] = low
+    tokens = np.array([50 % vocab, 20, 2, vocab - 2, vocab - 1, 0, vocab - 1, vocab - 1, 0])
+    flat = torch.empty((900, vocab + 3), dtype=TYPES[dtype], device="cuda")
+    c = flat[:, 1:vocab + 1]
+    c.copy_(torch.from_numpy(x).cuda().repeat(100, 1))
+    got = check(c[:9], None, tokens, 5, 0.0, None)
+    assert np.isfinite(got[1]).all()
+    check(c[:9], None, tokens, 5, 0.0, vocab // 3)
+    many = call(c, None, np.tile(tokens, 100), 5, 0.0, None)
+    want = plain(c[:9].double().cpu().numpy(), tokens, 5, None)[1]
+    # check()'s tolerance of the entropy.
+    tol = (vocab / 64 + 32 + 4 * want) * 2.0 ** -24 * (1 + want) + 4 * 2.0 ** -24 * want
+    err = np.abs(many[1].double().cpu().numpy().reshape(100, 9) - want)
+    assert (err <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [100, 1025, 40000])
+def test_guided_masks_far_below(dtype, vocab):
+    """Masked logits whose guided ones are near float32's lowest, and masked in both."""
+    rng = np.random.default_rng(vocab)
+    c, u = rng.standard_normal((2, 4, vocab)).astype(np.float32)
+    c[0, 16:60] = -1e38
+    c[1, :vocab // 2] = -1e38
+    c[2, 30:] = u[2, 30:] = float(torch.finfo(TYPES[dtype]).min)
+    c[3, :vocab - 3] = -3e37
+    c, u = (torch.from_numpy(x).to(TYPES[dtype]).cuda() for x in (c, u))
+    got = check(c, u, [1, vocab - 1, 2, vocab - 2], 3, 2.0, None)
+    assert np.isfinite(got[1]).all()
