@@ -198,7 +198,10 @@ constexpr int kWaves = 4;
 // A wave's window of the block table: lane i holds, of the i-th block, where the
 // head's part begins, the scores' factor, and the values' scale over `loud`, the
 // loudest of this window's blocks and all before. The steps wait for the table and
-// the scales once per 64 blocks and not one after the other.
+// the scales once per 64 blocks and not one after the other. Where a block is not there
+// (no name in the table, or behind the keys) a step reads the window's first one that
+// is: its rows have no weight, but only a block that was written holds nothing but
+// numbers, and 0 times a NaN code would be NaN.
 struct Window {
   unsigned offset_low, offset_high;
   float factor, unit;
@@ -209,11 +212,13 @@ struct Window {
     const int block = first + lane;
     const int page = (block << c.block_shift) < stop ? PageOf(c, sequence, block) : -1;
     there = __ballot(page >= 0);
-    const std::size_t offset =
-        ScaleIndex(c, max(page, 0), head, 0) * (static_cast<std::size_t>(c.dim) << c.block_shift);
+    if (there == 0)
+      return;  // nothing to read
+    const int some = __builtin_amdgcn_readlane(page, __ffsll(there) - 1);
+    scale_at = ScaleIndex(c, page >= 0 ? page : some, head, 0);
+    const std::size_t offset = scale_at * (static_cast<std::size_t>(c.dim) << c.block_shift);
     offset_low = static_cast<unsigned>(offset);
     offset_high = static_cast<unsigned>(offset >> 32);
-    scale_at = ScaleIndex(c, max(page, 0), head, 0);
   }
   __device__ __forceinline__ void LoadScales(const CacheAttentionParams& p, int lane) {
     const float k_scale = p.cache.scales[scale_at], v_scale = p.cache.scales[scale_at + 1];
@@ -343,6 +348,10 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
     const int first_block = window >> c.block_shift;
     w.LoadPages(c, sequence, head, first_block, wave_stop, lane);
     const int window_stop = min((first_block + kWave) << c.block_shift, wave_stop);
+    if (w.there == 0) {
+      window = window_stop;
+      continue;
+    }
     const int last_step = window + ((window_stop - 1 - window) & ~31);
 
     struct Codes {

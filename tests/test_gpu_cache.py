@@ -866,3 +866,104 @@ def test_tensors_are_checked():
     none = sequences(np.zeros((0, 1)), [], [0])
     ov.op_cache_read(cache, none, x, x)
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ blocks that are not there
+
+def gaps_of(table, lengths, block, blocks):
+    """The same sequences over a pool whose first block is nobody's, with a part of
+    each one's blocks missing (names outside the pool); and the blocks left unnamed."""
+    table = np.where(table >= 0, table + 1, table)
+    for i, length in enumerate(lengths):
+        n = -(-length // block)
+        table[i, n // 6:n // 2] = no_names(n // 2 - n // 6)
+    return table, np.setdiff1d(np.arange(blocks + 1), table)
+
+
+def no_names(n):
+    return np.resize(np.array([-1, 2 ** 31 - 1, -2 ** 31], dtype=np.int64), n).astype(np.int32)
+
+
+def spoil(cache, blocks):
+    """What memory that nobody wrote may hold: codes and scales that are no numbers."""
+    at = torch.from_numpy(np.asarray(blocks)).cuda()
+    cache.data[at] = 255
+    cache.scales[at] = float("nan")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("block", [16, 32, 64])
+@pytest.mark.parametrize("new,lengths", [
+    ([1, 1, 1, 1], [1, 17, 45, 200]),    # tiles of 16 rows
+    ([1], [9001]),                       # split, some splits without any block
+    ([2, 1, 2, 1], [2000, 90, 1500, 16]),
+    ([40, 1, 33], [40, 17, 300]),        # tiles of 32 rows
+    ([60], [5001]),                      # and split
+])
+def test_attention_beside_blocks_without_contents(dtype, dim, block, new, lengths):
+    """Blocks that no sequence names hold codes and scales that are no numbers, the
+    pool's first among them, and some of each sequence's blocks are missing: nothing
+    of either reaches a row."""
+    rng = np.random.default_rng(block + dim)
+    table, blocks = tables_of(rng, lengths, block)
+    table, rest = gaps_of(table, lengths, block, blocks)
+    cache = filled(rng, blocks + 1, 2, dim, block)
+    spoil(cache, rest)
+    begins = np.concatenate([[0], np.cumsum(new)])
+    q = tensor(rng.standard_normal((begins[-1], 4, dim)), dtype)
+    for causal in (False, True):
+        out = torch.full_like(q, 9.0)
+        ov.op_cache_attention(cache, sequences(table, lengths, begins), q, out, causal=causal)
+        check_attention(cache, (table, np.array(lengths), begins), q, out, 2, dtype, dim ** -0.5,
+                        causal)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("block", [16, 32, 64])
+def test_attention_of_many_rows_beside_blocks_without_contents(dtype, block):
+    """The same where a wave takes a tile with all its keys: rows that fill the
+    device (at least 2048 tiles of 128 dims over the kv heads, 1024 positions at
+    most). Two kv heads are compared."""
+    rng = np.random.default_rng(block)
+    new, lengths, heads, group, dim = [250, 1, 131, 3], [300, 17, 131, 20], 16, 12, 128
+    table, blocks = tables_of(rng, lengths, block)
+    table, rest = gaps_of(table, lengths, block, blocks)
+    cache = filled(rng, blocks + 1, heads, dim, block)
+    spoil(cache, rest)
+    begins = np.concatenate([[0], np.cumsum(new)])
+    q = tensor(rng.standard_normal((begins[-1], heads * group, dim)), dtype)
+    out = torch.full_like(q, 9.0)
+    ov.op_cache_attention(cache, sequences(table, lengths, begins), q, out, causal=True)
+    assert torch.isfinite(out).all() and (out != 9).any(-1).all()
+    for head in (0, heads - 1):
+        one = ov.KVCache(cache.data[:, head:head + 1].contiguous(),
+                         cache.scales[:, head:head + 1].contiguous(), block, dim)
+        rows = slice(head * group, (head + 1) * group)
+        check_attention(one, (table, np.array(lengths), begins), q[:, rows], out[:, rows], group,
+                        dtype, dim ** -0.5, True)
+
+
+@pytest.mark.parametrize("block", [16, 32, 64])
+def test_a_pool_without_initial_contents(block):
+    """Written, attended and read back in a pool of which every byte was 255."""
+    rng = np.random.default_rng(31)
+    lengths = np.array([1, 16, 17, 33, 64, 65, 130])
+    table, blocks = tables_of(rng, lengths, block)
+    table = np.where(table >= 0, table + 1, table)
+    cache = ov.KVCache.empty(blocks + 1, 2, 64, block)
+    spoil(cache, np.arange(blocks + 1))
+    begins = np.concatenate([[0], np.cumsum(lengths)])
+    k, v = (tensor(rng.standard_normal((begins[-1], 2, 64)), "f16") for _ in range(2))
+    q = tensor(rng.standard_normal((begins[-1], 4, 64)), "f16")
+    seq = sequences(table, lengths, begins)
+    ov.op_cache_write(cache, seq, k, v)
+    out, one = torch.full_like(q, 9.0), torch.full_like(q[:len(lengths)], 9.0)
+    ov.op_cache_attention(cache, seq, q, out, causal=True)
+    check_attention(cache, (table, lengths, begins), q, out, 2, "f16", 0.125, True)
+    last = np.arange(len(lengths) + 1)
+    ov.op_cache_attention(cache, sequences(table, lengths, last), q[begins[1:] - 1], one)
+    check_attention(cache, (table, lengths, last), q[begins[1:] - 1], one, 2, "f16", 0.125, False)
+    back = [torch.empty_like(k) for _ in range(2)]
+    ov.op_cache_read(cache, seq, *back)
+    assert torch.isfinite(back[0]).all() and torch.isfinite(back[1]).all()
