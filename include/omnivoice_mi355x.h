@@ -374,7 +374,10 @@ typedef struct ovg_kv_cache {
  *   begins   [count + 1], ascending: rows begins[i] .. begins[i + 1] - 1 of the
  *            call's tensors are sequence i's last tokens. Rows before
  *            begins[0] or from begins[count] on belong to nobody and are left
- *            as they are; so is, of `rows` rows, what begins names past them.
+ *            as they are. What begins names outside the `rows` rows is left
+ *            out, and its tokens are not written; the rows that there are keep
+ *            their places (row r of sequence i is its token
+ *            lengths[i] - (begins[i + 1] - r)).
  * Positions past table_width * block_tokens, or before 0 where a sequence has
  * more rows than tokens, are treated as those without a block. Up to 2^24 rows,
  * 2^20 sequences, 2^30 positions and 1024 kv heads. */
@@ -393,10 +396,10 @@ typedef struct ovg_kv_sequences {
  * smallest power of two, 2^-100 or more, that takes the new tokens into e4m3's
  * +-448 and, while tokens before them stay in the block, not less than it was;
  * codes are rounded to nearest even, codes that stay move with the scale, and
- * the positions behind the sequence's last token are cleared. With an infinity
- * or a NaN among the new tokens the block's scale is NaN (and stays so while
- * any of its tokens stays). Writing tokens again at the same lengths replaces
- * them. No block may take tokens of two sequences in one call. */
+ * the block's positions behind the call's last token are cleared. With an
+ * infinity or a NaN among the new tokens the block's scale is NaN (and stays so
+ * while any of its tokens stays). Writing tokens again at the same lengths
+ * replaces them. No block may take tokens of two sequences in one call. */
 int ovg_op_cache_write(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
                        const void* k, const void* v, int64_t k_stride, int64_t v_stride,
                        int type, void* stream, char* error, size_t error_len);

@@ -49,8 +49,9 @@ __device__ __forceinline__ int PageOf(const CacheView& c, int sequence, int b) {
 }
 
 // A sequence's rows [first, first + count) of the call's tensors, clamped into
-// them, and the cache position `start` of its first row (negative where the
-// sequence is shorter than its rows).
+// them, and the cache position `start` of the first of these (-count where all of
+// them come before position 0, else negative where the sequence is shorter than its
+// rows). The rows' last position is length - 1 unless rows were cut off behind.
 struct Span {
   int first, count, start, length;
 };
@@ -85,6 +86,8 @@ __device__ __forceinline__ Found FindItem(const CacheView& c, int scale, int shi
   const int begin = c.begins[i], end = c.begins[i + 1], length = c.lengths[i];
   const int first = min(max(begin, 0), c.rows);
   const int rows = min(max(end, first), c.rows) - first;
+  // Row r is token length - (end - r), also where there are fewer rows than begins says.
+  const int start = max(max(length, 0) - max(end, first) + first, -rows);
   const int base = ((first * scale) >> shift) + slack * i;
   const int below = __popcll(__ballot(lane < count && base <= item));
   if (below > 0) {
@@ -94,7 +97,7 @@ __device__ __forceinline__ Found FindItem(const CacheView& c, int scale, int shi
     f.span.first = __builtin_amdgcn_readlane(first, owner);
     f.span.count = __builtin_amdgcn_readlane(rows, owner);
     f.span.length = max(__builtin_amdgcn_readlane(length, owner), 0);
-    f.span.start = f.span.length - f.span.count;
+    f.span.start = __builtin_amdgcn_readlane(start, owner);
   }
   return f;
 }

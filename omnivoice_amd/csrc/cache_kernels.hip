@@ -71,6 +71,7 @@ __device__ __forceinline__ int ValueByte(int token, int dim, int width) {
 // The block of the pool that work-group `item` handles, or false.
 struct Touched {
   Span span;
+  int end;          // position behind the rows' last
   int block, page;  // block of the sequence, of the pool
 };
 __device__ __forceinline__ bool Find(const CacheView& c, int item, Touched* t) {
@@ -78,8 +79,9 @@ __device__ __forceinline__ bool Find(const CacheView& c, int item, Touched* t) {
   t->span = f.span;
   if (f.span.count == 0 || f.item < 0)
     return false;
+  t->end = f.span.start + f.span.count;
   t->block = (f.span.start >> c.block_shift) + f.item;
-  if (t->block > (f.span.length - 1) >> c.block_shift)
+  if (t->block > (t->end - 1) >> c.block_shift)
     return false;
   t->page = PageOf(c, f.sequence, t->block);
   return true;
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(kThreads) void CacheWriteKernel(CacheWriteParams p)
   const int head = blockIdx.y, half = blockIdx.z, tid = threadIdx.x;
   const int first = t.block << SHIFT;
   const int kept = max(t.span.start - first, 0);                // tokens that stay
-  const int live = min(t.span.length - first, kBlock);          // and the block's last
+  const int live = min(t.end - first, kBlock);                  // and the block's last
   unsigned char* const codes = HalfOf(c, t.page, head, half);
   const std::size_t scale_at = ScaleIndex(c, t.page, head, half);
   const T* const x = static_cast<const T*>(p.x[half]) + static_cast<std::int64_t>(head) * DIM;

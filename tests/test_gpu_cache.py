@@ -967,3 +967,56 @@ def test_a_pool_without_initial_contents(block):
     back = [torch.empty_like(k) for _ in range(2)]
     ov.op_cache_read(cache, seq, *back)
     assert torch.isfinite(back[0]).all() and torch.isfinite(back[1]).all()
+
+
+# ------------------------------------------------------------------ borders outside the rows
+
+@pytest.mark.parametrize("begins,lengths,rows", [
+    ([0, 12], [20], 10), ([0, 30], [40], 17), ([2, 30, 41], [50, 60], 35),
+    ([-5, 9, 30], [40, 21], 20), ([-9, 40], [45], 20), ([0, 25], [20], 12),
+    ([0, 3, 2 ** 31 - 1], [30, 2 ** 31 - 1], 9), ([0, 2 ** 31 - 1], [40], 9)])
+@pytest.mark.parametrize("block", [16, 32])
+def test_rows_keep_their_places_where_begins_names_more(begins, lengths, rows, block):
+    """Row r of a sequence whose rows end at `end` is its token length - (end - r),
+    whichever of its rows there are: written there, read from there, and seeing as
+    far. Tokens whose rows are not there are not written."""
+    rng = np.random.default_rng(rows)
+    heads, dim = 2, 64
+    table, blocks = tables_of(rng, [64] * len(lengths), block)
+    cache = filled(rng, blocks, heads, dim, block)
+    plain = Plain(cache)
+    k, v = (tensor(rng.standard_normal((rows, heads, dim)), "f16") for _ in range(2))
+    q = tensor(rng.standard_normal((rows, 2 * heads, dim)), "f16")
+    seq = sequences(table, lengths, begins)
+    ov.op_cache_write(cache, seq, k, v)
+    spans = []  # rows, and the place behind the last one's
+    for i, length in enumerate(lengths):
+        first, last = max(begins[i], 0), min(begins[i + 1], rows)
+        spans.append((slice(first, max(first, last)), length - begins[i + 1] + last))
+        sl, end = spans[-1]
+        if sl.stop > sl.start and end > 0:
+            plain.write(table[i], end, np64(k)[sl][-end:], np64(v)[sl][-end:])
+    same(cache, plain)
+    back = [torch.full((rows, heads, dim), 9.0, dtype=torch.float32, device="cuda")
+            for _ in range(2)]
+    ov.op_cache_read(cache, seq, *back)
+    for half in (0, 1):
+        want = np.full((rows, heads, dim), 9.0)
+        for i, (sl, end) in enumerate(spans):
+            want[sl] = plain.read(table[i], end - (sl.stop - sl.start), end)[half]
+        np.testing.assert_array_equal(np64(back[half]), want)
+    for causal in (False, True):
+        out = torch.full_like(q, 9.0)
+        ov.op_cache_attention(cache, seq, q, out, causal=causal)
+        got = np64(out)
+        for i, (sl, end) in enumerate(spans):
+            n = sl.stop - sl.start
+            if n == 0:
+                continue
+            # A causal call's rows see as far as those of a sequence that ends there.
+            sees = min(end if causal else lengths[i], 64)
+            if sees <= 0:
+                assert (got[sl] == 0).all()
+                continue
+            check_attention(cache, (table[i:i + 1], np.array([sees]), np.array([0, n])), q[sl],
+                            out[sl], 2, "f16", dim ** -0.5, causal)
