@@ -133,7 +133,8 @@ struct CacheAttentionParams {
   bool negate;       // the queries take it
   // The plan's (PlanCacheAttention), and where its splits leave their states:
   // slot ((item * kv_heads + head) * splits + split) * tile rows + row has its
-  // row's maximum and sum in partial_m and its output, not divided, in partial_o.
+  // row's maximum and sum in partial_m and its output over a power of two (PowerAbove)
+  // in partial_o.
   int tile_shift, splits, own_shift;
   int items, first_item;  // tiles in all, and the first of a launch
   float* partial_m;  // [slots][2]

@@ -163,6 +163,12 @@ constexpr float kQuietest = 7.52316385e-37F;  // 2^-120
 __device__ __forceinline__ float InversePower(float p) {
   return __uint_as_float((254u << 23) - __float_as_uint(p));
 }
+// The power of two above a row's sum of weights (0, or from 1 to 2^38). Outputs are
+// taken over that much before they meet their loudness: averages of the type's largest
+// values are finite where their sums are not, and powers of two round nothing.
+__device__ __forceinline__ float PowerAbove(float sum) {
+  return __uint_as_float((__float_as_uint(fmaxf(sum, 1.0F)) & 0x7F800000u) + (1u << 23));
+}
 // 0 for a block without a (numeric) scale.
 __device__ __forceinline__ float Loudness(float scale) { return scale == scale ? scale : 0.0F; }
 
@@ -524,7 +530,9 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
     const float sum = RowSum<ROWS>(l[0] + l[1]);
     if (row >= rows)
       return;
-    const float scale = sum == 0.0F ? 0.0F : 1.0F / sum;
+    const float above = PowerAbove(sum);
+    const float held = loud * InversePower(above);
+    const float scale = sum == 0.0F ? 0.0F : above / sum;
     T* to = static_cast<T*>(p.out) + static_cast<std::int64_t>(span.first + query) * p.out_stride +
             static_cast<std::int64_t>(head * p.group + of_group) * DIM;
 #pragma unroll
@@ -534,7 +542,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
         T rounded[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          rounded[r] = static_cast<T>(o[t][4 * i + r] * loud * scale);
+          rounded[r] = static_cast<T>(o[t][4 * i + r] * held * scale);
         __builtin_memcpy(to + DimOf<DIM, ROWS>(t * kFours + i, part), rounded, sizeof(rounded));
       }
     return;
@@ -546,12 +554,13 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
     shared_m[wave][column] = m;
     shared_l[wave][column] = sum;
   }
+  const float held = loud * InversePower(PowerAbove(sum));
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
     for (int i = 0; i < kFours; ++i)
       shared_o[wave][t * kFours + i][lane] =
-          floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]} * loud;
+          floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]} * held;
   __syncthreads();
   float top = -__builtin_inff(), total = 0.0F;
   float weight[kWaves];
@@ -566,6 +575,10 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
   }
   if (row >= rows)
     return;
+  const float above = PowerAbove(total);
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i)
+    weight[i] *= PowerAbove(shared_l[i][column]) * InversePower(above);
   const std::size_t slot =
       p.splits == 1
           ? 0
@@ -576,7 +589,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
     p.partial_m[2 * slot + 1] = total;
   }
   // Nothing seen: zero.
-  const float scale = total == 0.0F ? 0.0F : 1.0F / total;
+  const float scale = total == 0.0F ? 0.0F : above / total;
   T* to = static_cast<T*>(p.out) + static_cast<std::int64_t>(span.first + query) * p.out_stride +
           static_cast<std::int64_t>(head * p.group + of_group) * DIM;
 #pragma unroll
@@ -598,6 +611,8 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
   }
 }
 
+// A split has left its row's maximum and sum of weights, and its output over the power
+// of two above that sum.
 // Joins the splits of one row: DIM / 4 lanes hold four of its dims each, and the
 // work-group's 256 / (DIM / 4) such groups take its splits in turn.
 template <typename T, int DIM>
@@ -636,12 +651,13 @@ __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
   const float from = top == -__builtin_inff() ? 0.0F : top;
   const float weight = __builtin_amdgcn_exp2f(m - from);
   if (tid < kMostSplits)
-    weights[tid] = weight;
+    weights[tid] = weight * PowerAbove(l);
   const float part_total = WaveSum(l * weight);
   if ((tid & 63) == 0)
     totals[tid >> 6] = part_total;
   __syncthreads();
   const float total = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+  const float above = PowerAbove(total), held = InversePower(above);
   // Eight loads at a time, none under a condition: a split that saw nothing has
   // left zeros.
   constexpr int kAhead = 8;
@@ -657,7 +673,7 @@ __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
       if (s0 + a * kGroups < p.splits)
-        sum += o[a] * weights[s0 + a * kGroups];
+        sum += o[a] * (weights[s0 + a * kGroups] * held);
   }
   sums[group][part] = sum;
   __syncthreads();
@@ -666,7 +682,7 @@ __global__ __launch_bounds__(256) void JoinKernel(CacheAttentionParams p) {
 #pragma unroll
   for (int g = 1; g < kGroups; ++g)
     sum += sums[g][part];
-  const float scale = total == 0.0F ? 0.0F : 1.0F / total;
+  const float scale = total == 0.0F ? 0.0F : above / total;
   int of_group;
   const int query = RowSplit(p, row).Of(0, &of_group);
   T rounded[4];
@@ -712,15 +728,18 @@ __global__ __launch_bounds__(256) void JoinFewKernel(CacheAttentionParams p) {
   }
   const float from = top == -__builtin_inff() ? 0.0F : top;
   float total = 0.0F;
-  floatx4 sum = {};
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
-    const float w = __builtin_amdgcn_exp2f(m[s] - from);
-    total += l[s] * w;
-    if (s < p.splits)
-      sum += o[s] * w;
+    m[s] = __builtin_amdgcn_exp2f(m[s] - from);
+    total += l[s] * m[s];
   }
-  const float scale = total == 0.0F ? 0.0F : 1.0F / total;
+  const float above = PowerAbove(total), held = InversePower(above);
+  floatx4 sum = {};
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s)
+    if (s < p.splits)
+      sum += o[s] * (m[s] * (PowerAbove(l[s]) * held));
+  const float scale = total == 0.0F ? 0.0F : above / total;
   int of_group;
   const int query = RowSplit(p, row).Of(0, &of_group);
   T rounded[4];

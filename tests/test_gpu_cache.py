@@ -1020,3 +1020,34 @@ def test_rows_keep_their_places_where_begins_names_more(begins, lengths, rows, b
                 continue
             check_attention(cache, (table[i:i + 1], np.array([sees]), np.array([0, n])), q[sl],
                             out[sl], 2, "f16", dim ** -0.5, causal)
+
+
+# ------------------------------------------------------------------ the type's largest values
+
+@pytest.mark.parametrize("new,total,heads,group", [
+    (1, 900, 1, 2),     # one work-group a head
+    (1, 2000, 2, 2),    # few splits, joined by groups of lanes
+    (1, 9000, 1, 2),    # many
+    (50, 700, 1, 2), (60, 5000, 1, 2), (260, 300, 16, 16)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_of_values_near_the_types_largest(new, total, heads, group, sign):
+    """Averages of many values of bfloat16's upper end are finite, though their sums
+    are not: 1e38 to 3e38, equal scores and random ones."""
+    rng = np.random.default_rng(total)
+    dim, block = 128, 32
+    table, blocks = tables_of(rng, [total], block)
+    cache = ov.KVCache.empty(blocks, heads, dim, block)
+    k = rng.standard_normal((total, heads, dim)) * (np.arange(heads)[:, None] > 0)
+    v = sign * rng.uniform(1e38, 3e38, (total, heads, dim))
+    ov.op_cache_write(cache, sequences(table, [total], [0, total]), tensor(k, "bf16"),
+                      tensor(v, "bf16"))
+    q = tensor(rng.standard_normal((new, heads * group, dim)), "bf16")
+    out = torch.empty_like(q)
+    seq_np = (table, np.array([total]), np.array([0, new]))
+    ov.op_cache_attention(cache, sequences(*seq_np), q, out, causal=True)
+    assert torch.isfinite(out).all()
+    for head in sorted({0, heads - 1}):
+        one = ov.KVCache(cache.data[:, head:head + 1].contiguous(),
+                         cache.scales[:, head:head + 1].contiguous(), block, dim)
+        rows = slice(head * group, (head + 1) * group)
+        check_attention(one, seq_np, q[:, rows], out[:, rows], group, "bf16", dim ** -0.5, True)
