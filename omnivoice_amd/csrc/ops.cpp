@@ -106,6 +106,14 @@ ovg::DType TypeOf(int type, bool with_f32) {
   return static_cast<ovg::DType>(type);
 }
 
+// Query heads of a kv head, for the attention and for its workspace's size.
+int GroupOf(const ovg_kv_cache* cache, int64_t heads) {
+  ovg::Require(heads >= cache->kv_heads && heads % cache->kv_heads == 0 &&
+                   heads / cache->kv_heads <= 64,
+               "heads must be 1 to 64 times kv_heads");
+  return static_cast<int>(heads / cache->kv_heads);
+}
+
 // The splits' outputs, then their maxima and sums.
 int64_t AttentionBytes(const ovg::CacheView& c, const ovg::CacheAttentionPlan& plan) {
   return static_cast<int64_t>(plan.slots) * (c.dim + 2) * static_cast<int64_t>(sizeof(float));
@@ -409,10 +417,7 @@ int64_t ovg_op_cache_attention_workspace(const ovg_kv_cache* cache,
                                          const ovg_kv_sequences* sequences, int64_t heads) {
   try {
     const ovg::CacheView c = ViewOf(cache, sequences);
-    if (heads < cache->kv_heads || heads / cache->kv_heads > 64)
-      return -1;
-    return AttentionBytes(
-        c, ovg::PlanCacheAttention(c, static_cast<int>(heads / cache->kv_heads)));
+    return AttentionBytes(c, ovg::PlanCacheAttention(c, GroupOf(cache, heads)));
   } catch (const std::exception&) {
     return -1;  // as the call itself will say
   }
@@ -427,9 +432,7 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
     ovg::CacheAttentionParams p{};
     p.cache = ViewOf(cache, sequences);
     const ovg::DType t = TypeOf(type, false);
-    ovg::Require(heads >= cache->kv_heads && heads % cache->kv_heads == 0 &&
-                     heads / cache->kv_heads <= 64,
-                 "heads must be 1 to 64 times kv_heads");
+    p.group = GroupOf(cache, heads);
     const float scale_log2 = std::fabs(scale) * 1.44269504088896341F;
     ovg::Require(scale_log2 - scale_log2 == 0.0F, "scale must be finite, also times log2(e)");
     RequireStride(q_stride, heads * cache->head_dim);
@@ -439,7 +442,6 @@ int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* se
     ovg::Require(q && out, "null pointer");
     auto s = static_cast<hipStream_t>(stream);
     RequireCurrentDevice(s);
-    p.group = static_cast<int>(heads / cache->kv_heads);
     p.group_inverse = ((1 << 16) + p.group - 1) / p.group;
     p.group_magic = ((1ull << 36) + p.group - 1) / p.group;
     const ovg::CacheAttentionPlan plan = ovg::PlanCacheAttention(p.cache, p.group);

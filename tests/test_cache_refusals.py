@@ -119,3 +119,27 @@ def test_nothing_to_do_is_no_error():
                                     256) == ov.OVG_OK
     assert L.ovg_op_token_logprobs(None, None, 0, 10, 10, 10, 0.0, -1, None, 0, None, None, None,
                                    None, 2, None, 0, None, err, 256) == ov.OVG_OK
+
+
+def test_workspace_queries_refuse_what_their_calls_refuse():
+    L = ov.lib()
+
+    def attention(c, s, heads=16):
+        return L.ovg_op_cache_attention_workspace(c, s, heads)
+    long = sequences(count=1, rows=1, table_width=300)
+    assert attention(cache(), long) > 0
+    assert attention(cache(), sequences(rows=0)) == 0
+    for over, _ in BAD_POOLS:
+        assert attention(cache(**over), long) == -1
+    for over, _ in BAD_SEQUENCES:
+        assert attention(cache(), sequences(**over)) == -1
+    assert attention(None, long) == -1
+    assert attention(cache(), None) == -1
+    for heads in (-16, 0, 4, 12, 8 * 64 + 1, 8 * 65, 2 ** 40):
+        assert attention(cache(), long, heads) == -1, heads
+    logprobs = L.ovg_op_token_logprobs_workspace
+    assert logprobs(1, 151936, 4) > 0
+    assert logprobs(0, 151936, 4) == 0
+    for args in ((-1, 100, 4), (2 ** 23 + 1, 100, 4), (1, 0, 4), (1, 2 ** 31, 4), (1, 100, -1),
+                 (1, 100, 33)):
+        assert logprobs(*args) == -1, args
