@@ -726,7 +726,7 @@ def _workspace(workspace, size: int, device, stream):
     own memory (without one the current stream's), which only work behind this
     call's takes again. The caller holds what this returns until the launch."""
     if workspace is None:
-        if size <= 0:  # none needed, or arguments that the call will refuse
+        if size <= 0 or device.type != "cuda":  # none needed, or what the call will refuse
             return None, 0, None
         import torch
         if stream is None:

@@ -143,3 +143,22 @@ def test_workspace_queries_refuse_what_their_calls_refuse():
     for args in ((-1, 100, 4), (2 ** 23 + 1, 100, 4), (1, 0, 4), (1, 2 ** 31, 4), (1, 100, -1),
                  (1, 100, 33)):
         assert logprobs(*args) == -1, args
+
+
+@pytest.mark.parametrize("stream", [None, 0, HERE])
+def test_host_tensors_are_refused(stream):
+    torch = pytest.importorskip("torch")
+    pool = ov.KVCache.empty(4, 1, 128, 32, device="cpu")
+    seq = ov.KVSequences(torch.zeros((1, 300), dtype=torch.int32),
+                         torch.tensor([9000], dtype=torch.int32),
+                         torch.tensor([0, 1], dtype=torch.int32))
+    q, k = torch.zeros((1, 2, 128)).half(), torch.zeros((1, 1, 128)).half()
+    assert ov.op_cache_attention_workspace(pool, seq, 1, 2) > 0  # the call would take one
+    logits, ids = torch.zeros((1, 151936)), torch.zeros((1, 4), dtype=torch.int32)
+    for call in (lambda: ov.op_cache_write(pool, seq, k, k, stream=stream),
+                 lambda: ov.op_cache_read(pool, seq, k, k, stream=stream),
+                 lambda: ov.op_cache_attention(pool, seq, q, q, stream=stream),
+                 lambda: ov.op_token_logprobs(logits, None, None, None, ids, torch.zeros((1, 4)),
+                                              stream=stream)):
+        with pytest.raises(ov.GeneratorError, match="needs tensors of a GPU, got cpu"):
+            call()
