@@ -1051,3 +1051,77 @@ def test_attention_of_values_near_the_types_largest(new, total, heads, group, si
                          cache.scales[:, head:head + 1].contiguous(), block, dim)
         rows = slice(head * group, (head + 1) * group)
         check_attention(one, seq_np, q[:, rows], out[:, rows], group, "bf16", dim ** -0.5, True)
+
+
+# ------------------------------------------------------------------ batches and tables
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lengths,heads,group", [
+    ([1, 2, 2, 1], [37, 5000, 700, 16], 2, 2), ([1] * 40, [100 + 7 * i for i in range(40)], 8, 2),
+    ([40, 3, 129, 1], [100, 3, 640, 900], 2, 3), ([250, 131, 1, 3], [300, 131, 90, 64], 16, 12)])
+def test_a_sequence_has_the_same_bits_beside_any_others(dtype, new, lengths, heads, group):
+    """The others' queries, keys and values changed, infinities among them, and all of
+    them in another order: the calls are planned alike, so the bits stay."""
+    rng = np.random.default_rng(26)
+    dim, block = 128, 32
+    table, blocks = tables_of(rng, lengths, block)
+    cache = filled(rng, blocks, heads, dim, block)
+    begins = np.concatenate([[0], np.cumsum(new)])
+    q = tensor(rng.standard_normal((begins[-1], heads * group, dim)), dtype)
+    out = torch.full_like(q, 9.0)
+    ov.op_cache_attention(cache, sequences(table, lengths, begins), q, out, causal=True)
+    order = rng.permutation(len(new))
+    moved = np.concatenate([np.arange(begins[i], begins[i + 1]) for i in order])
+    again = torch.full_like(q, 9.0)
+    ov.op_cache_attention(
+        cache, sequences(table[order], np.array(lengths)[order],
+                         np.concatenate([[0], np.cumsum(np.array(new)[order])])),
+        q[torch.from_numpy(moved).cuda()].contiguous(), again, causal=True)
+    assert torch.equal(again, out[torch.from_numpy(moved).cuda()])
+    for keep in sorted({0, len(new) // 2, len(new) - 1}):
+        other = filled(rng, blocks, heads, dim, block, loud=2.0 ** 20)
+        mine = torch.from_numpy(table[keep][table[keep] >= 0].astype(np.int64)).cuda()
+        other.data[mine], other.scales[mine] = cache.data[mine], cache.scales[mine]
+        rows = slice(begins[keep], begins[keep + 1])
+        x = torch.full_like(q, float("inf"))
+        x[rows] = q[rows]
+        ov.op_cache_attention(other, sequences(table, lengths, begins), x, again, causal=True)
+        assert torch.equal(again[rows], out[rows])
+
+
+@pytest.mark.parametrize("new,dtype", [(1, "f16"), (30, "bf16"), (200, "f16")])
+@pytest.mark.parametrize("block", [16, 64])
+def test_no_numbers_behind_the_rows_sight(new, dtype, block):
+    """A long causal sequence whose table goes on behind it, with blocks whose scales
+    and codes are no numbers, others missing: the rows are those without them."""
+    rng = np.random.default_rng(27)
+    total, dim = 20000, 64
+    table, blocks = tables_of(rng, [total + 50 * block], block)
+    table[0, rng.permutation(total // block)[:100]] = -1
+    cache = filled(rng, blocks, 1, dim, block)
+    seen = table[0, :-(-total // block)]
+    spoil(cache, np.setdiff1d(np.arange(blocks), seen))
+    q = tensor(rng.standard_normal((new, 2, dim)), dtype)
+    out = torch.full_like(q, 9.0)
+    seq_np = (table, np.array([total]), np.array([0, new]))
+    ov.op_cache_attention(cache, sequences(*seq_np), q, out, causal=True)
+    check_attention(cache, seq_np, q, out, 2, dtype, dim ** -0.5, True)
+    # Inside the sequence, behind all rows but the last ones.
+    if new > block:
+        last = (total - 1) // block
+        kept = torch.from_numpy(np.arange(new) < last * block - (total - new)).cuda()
+        cache.scales[int(table[0, last])] = float("nan")
+        again = torch.full_like(q, 9.0)
+        ov.op_cache_attention(cache, sequences(*seq_np), q, again, causal=True)
+        assert torch.equal(again[kept], out[kept]) and torch.isnan(again[~kept]).all()
+
+
+@pytest.mark.parametrize("new,lengths,width,group,dtype", [
+    ([1], [430], 4096, 2, "f16"), ([1, 1, 3], [1, 17, 2000], 4096, 2, "bf16"),
+    ([40], [100], 2048, 2, "f16"), ([600, 1, 1, 5], [700, 20000, 90, 4000], None, 2, "f16"),
+    ([2048, 1], [2048, 9001], None, 1, "bf16")])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_of_wide_tables_and_mixed_calls(new, lengths, width, group, dtype, causal):
+    """Tables far wider than their sequences, whose splits are mostly empty, and
+    prompts beside single tokens over long sequences."""
+    attention_case(28, new, lengths, 1, group, 64, 32, dtype, causal, width=width)
