@@ -415,10 +415,15 @@ int ovg_op_cache_read(const ovg_kv_cache* cache, const ovg_kv_sequences* sequenc
  * reads kv head h / (heads / kv_heads). A query sees every token of its
  * sequence, or with `causal` those up to its own position (query t of n:
  * length - n + t). softmax(scale * q . k) v in float32 sums, the probabilities
- * rounded to `type` for their product with the values; a row that sees nothing
- * is zero. A query that sees a token of a block whose scale is NaN is NaN.
- * In fp16 a value counts to 2^-33 of the most that its head's largest value
- * scale holds. `out` may be `q` itself. `workspace`:
+ * rounded to `type` for their product with the values (in fp16 one under 2^-25
+ * of its row's largest may count as none). A row that sees nothing, or no score
+ * above -infinity, is zero; one that sees a token of a block whose scale is NaN,
+ * or a score of NaN or +infinity, is NaN. A value counts to 2^-33 (bf16: 2^-120)
+ * of the most that the largest value scale of its sequence and head holds, be
+ * that in the row's sight or not. How the work is split goes by the mean of the
+ * sequences' rows and by table_width: one token over a long sequence is slow in
+ * a call with long prompts, and faster in one of its own. `out` may be `q`
+ * itself. `workspace`:
  * ovg_op_cache_attention_workspace bytes (-1 for arguments that the call
  * refuses), 16-byte aligned, NULL where that is 0; it holds nothing between
  * calls, and calls that may overlap need one each. heads is 1 to 64 times

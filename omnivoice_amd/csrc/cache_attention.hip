@@ -25,11 +25,12 @@
 // 128 rows leaves CUs idle where there are few.
 //
 // Bound: memory where rows are few, 48 sequences of up to 8192 tokens (474 MB) in
-// 95.6 us, 5.0 TB/s. With many the issue of matrix and vector instructions: two causal
-// prompts of up to 5000 tokens (198 GFLOP) in 228 us, 868 TFLOP/s, the matrix cores
-// busy 46 % and vector instructions 38 % of the time; of the largest library product 1174. A
-// third work-group to a CU, its queries in LDS, did not raise that. A short call is a
-// chain of trips to memory: one token over 430 takes the kernel 6.5 us.
+// 95.8 us, 4.9 TB/s. With many the issue of matrix and vector instructions: two causal
+// prompts of up to 5000 tokens (198 GFLOP) in 231 us on one card and 241 on another, 860
+// and 825 TFLOP/s, the matrix cores busy 46 % and vector instructions 38 % of the time;
+// of the largest library product 1174. A third work-group to a CU, its queries in LDS,
+// did not raise that. A short call is a chain of trips to memory: one token over 430
+// takes the kernel 7 us.
 #include <algorithm>
 
 #include "cache.hpp"
@@ -196,7 +197,9 @@ struct RowSplit {
 // How far a row's maximum may rise before its sums are scaled again: their
 // probabilities are then at most 2^8, far inside fp16, and most steps of a long
 // row leave the sums alone. Each row goes by its own maximum: what the others
-// hold changes none of its bits.
+// hold changes none of its bits. (The values' loudness is that of all the sequence's
+// blocks so far, also of those that a row does not see; a power of two, it rounds
+// only what lies 2^-33 under it in fp16.)
 constexpr float kSlack = 8.0F;
 
 constexpr int kWaves = 4;
