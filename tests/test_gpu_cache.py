@@ -1125,3 +1125,74 @@ def test_attention_of_wide_tables_and_mixed_calls(new, lengths, width, group, dt
     """Tables far wider than their sequences, whose splits are mostly empty, and
     prompts beside single tokens over long sequences."""
     attention_case(28, new, lengths, 1, group, 64, 32, dtype, causal, width=width)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("total", [300, 3000])
+def test_attention_of_infinite_scores(new, total):
+    """Scores that overflow: -infinity has no weight, a row of nothing else is zero,
+    +infinity makes its row NaN."""
+    rng = np.random.default_rng(29)
+    dim, block = 64, 32
+    table, blocks = tables_of(rng, [total], block)
+    cache = ov.KVCache.empty(blocks, 1, dim, block)
+    k = np.zeros((total, 1, dim), np.float32)
+    k[::2, 0, 0] = 100.0   # the first query head's scores there are -infinity
+    k[:, 0, 1] = 100.0     # and all of the second's, and the third's +infinity
+    v = rng.standard_normal((total, 1, dim))
+    ov.op_cache_write(cache, sequences(table, [total], [0, total]), tensor(k, "bf16"),
+                      tensor(v, "bf16"))
+    q = torch.zeros((new, 4, dim), dtype=torch.bfloat16, device="cuda")
+    q[:, 0, 0] = -3e38
+    q[:, 1, 1] = -3e38
+    q[:, 2, 1] = 3e38
+    out = torch.full_like(q, 9.0)
+    ov.op_cache_attention(cache, sequences(table, [total], [0, new]), q, out, scale=8.0)
+    got = np64(out)
+    held = Plain(cache).read(table[0], 0, total)[1][:, 0]
+    # Equal weights of one, float32 sums: half a step of the output and 2^-18 of the mass.
+    for head, x in ((0, held[1::2]), (3, held)):
+        tol = 2.0 ** -8 * np.abs(x.mean(0)) + 2.0 ** -18 * np.abs(x).mean(0)
+        assert (np.abs(got[:, head] - x.mean(0)) <= tol).all()
+    assert (got[:, 1] == 0).all() and np.isnan(got[:, 2]).all()
+
+
+@pytest.mark.parametrize("block,dim", [(16, 64), (32, 128)])
+def test_offsets_past_32_bits(block, dim):
+    """Blocks more than 2^32 bytes into the pool, and rows more than 2^32 elements
+    apart: the same as in a small pool and from packed rows."""
+    rng = np.random.default_rng(30)
+    heads, n = 8, 500
+    per = heads * 2 * block * dim
+    blocks = (5 << 30) // per
+    ids = blocks - 1 - rng.permutation(3000)[:-(-n // block)]
+    pool = torch.empty((blocks, heads, 2, block * dim), dtype=torch.uint8, device="cuda")
+    big = ov.KVCache(pool, torch.empty((blocks, heads, 2), device="cuda"), block, dim)
+    small = ov.KVCache.empty(len(ids), heads, dim, block)
+    assert int(ids.min()) * per > 2 ** 32
+    k, v = (tensor(rng.standard_normal((n, heads, dim)), "f16") for _ in range(2))
+    q = tensor(rng.standard_normal((3, 2 * heads, dim)), "f16")
+    flat = torch.empty((2 << 31) + (1 << 20), dtype=torch.float16, device="cuda")
+    wide = {h: flat[at:].as_strided((3, h, dim), (1 << 31, dim, 1))
+            for at, h in ((0, heads), (1 << 16, 2 * heads))}
+    wide[heads].copy_(k[-3:])
+    wide[2 * heads].copy_(q)
+    got = []
+    for cache, table in ((small, np.arange(len(ids))), (big, ids)):
+        seq, last = sequences([table], [n], [0, n]), sequences([table], [n], [0, 3])
+        ov.op_cache_write(cache, seq, k, v)
+        if cache is big:
+            ov.op_cache_write(cache, last, wide[heads], v[-3:])
+        at = torch.from_numpy(np.asarray(table)).cuda()
+        back = [torch.empty_like(k) for _ in range(2)]
+        ov.op_cache_read(cache, seq, *back)
+        x = q if cache is small else wide[2 * heads]
+        out = torch.empty_like(q)
+        ov.op_cache_attention(cache, last, x, out, causal=True)
+        if cache is big:
+            ov.op_cache_read(cache, last, wide[heads], torch.empty_like(k[:3]))
+            assert torch.equal(wide[heads], back[0][-3:])
+            ov.op_cache_attention(cache, last, x, wide[2 * heads], causal=True)
+            assert torch.equal(wide[2 * heads], out)
+        got.append([cache.data[at], cache.scales[at], *back, out])
+    assert all(torch.equal(a, b) for a, b in zip(*got))

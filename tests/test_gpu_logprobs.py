@@ -347,3 +347,15 @@ def test_guided_masks_far_below(dtype, vocab):
     c, u = (torch.from_numpy(x).to(TYPES[dtype]).cuda() for x in (c, u))
     got = check(c, u, [1, vocab - 1, 2, vocab - 2], 3, 2.0, None)
     assert np.isfinite(got[1]).all()
+
+
+def test_rows_past_32_bits():
+    """Rows more than 2^31 elements apart, conditional and unconditional."""
+    rng = np.random.default_rng(9)
+    vocab = 1025
+    flat = torch.empty((2 << 31) + (1 << 16), dtype=torch.float16, device="cuda")
+    c, u = (flat[at:].as_strided((3, vocab), (1 << 31, 1)) for at in (0, 1 << 12))
+    for x in (c, u):
+        x.copy_(torch.from_numpy(rng.standard_normal((3, vocab)).astype(np.float32)))
+    check(c, None, [5, 0, 1024], 6, 0.0, None)
+    check(c, u, [5, 0, 1024], 6, 2.0, 1024)
