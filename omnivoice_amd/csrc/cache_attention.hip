@@ -202,6 +202,12 @@ struct RowSplit {
 // only what lies 2^-33 under it in fp16.)
 constexpr float kSlack = 8.0F;
 
+// A weight's exponent is one fused step from the score's product, score * factor - maximum,
+// whose maximum was rounded: by 2^-8 at most below 2^16 in size, which every weight of the
+// row shares, but by more than the weights' range from 2^28 on. Rows whose maximum is
+// larger than this round their products first, as the maximum is.
+constexpr float kLarge = 65536.0F;
+
 constexpr int kWaves = 4;
 
 // A wave's window of the block table: lane i holds, of the i-th block, where the
@@ -339,6 +345,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
   for (int t = 0; t < kTiles; ++t)
     o[t] = acc_t(0.0F);
   float loud = kQuietest;
+  bool large = false;  // some row's maximum is
 
   const int quarter = ((stop - begin + kWaves * 32 - 1) / (kWaves * 32)) * 32;
   const int wave_begin = OWN ? begin : begin + wave * quarter;
@@ -450,6 +457,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
         const float top = peak > m + kSlack ? peak : m;
         const float shrink = top == -__builtin_inff() ? 1.0F : __builtin_amdgcn_exp2f(m - top);
         m = top;
+        large = __any(fabsf(m) > kLarge && m > -__builtin_inff());
         l[0] *= shrink;
         l[1] *= shrink;
 #pragma unroll
@@ -457,14 +465,25 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void CacheAttentionKernel(
           o[t] *= shrink;
       }
       const float from = m == -__builtin_inff() ? 0.0F : m;
+      if (__builtin_expect(large, 0)) {
+        // Row by row, and the exponents at once: no row's bits depend on another's size.
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int r = 0; r < kOfGroup; ++r)
+            s[g][r] = fabsf(from) > kLarge ? s[g][r] * factor[g] - from
+                                           : __builtin_fmaf(s[g][r], factor[g], -from);
+        factor[0] = factor[1] = 1.0F;
+      }
+      const float less = large ? 0.0F : from;
       typename X::x2 w2[2][kOfGroup / 2];  // the weights
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int r = 0; r < kOfGroup; r += 2) {
           w2[g][r / 2] = X::Round(
-              __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][r], factor[g], -from)),
-              __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][r + 1], factor[g], -from)));
+              __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][r], factor[g], -less)),
+              __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][r + 1], factor[g], -less)));
           l[r / 2 % 2] = X::AddPair(w2[g][r / 2], l[r / 2 % 2]);
         }
       if constexpr (ROWS == 16) {

@@ -1196,3 +1196,59 @@ def test_offsets_past_32_bits(block, dim):
             assert torch.equal(wide[2 * heads], out)
         got.append([cache.data[at], cache.scales[at], *back, out])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("new,total,heads,group", [
+    (1, 300, 1, 2), (1, 9000, 1, 2), (50, 700, 1, 2), (60, 5000, 1, 2), (260, 300, 16, 16)])
+@pytest.mark.parametrize("dtype,loud", [("f16", 3e4), ("bf16", 3e4), ("bf16", 1e15)])
+@pytest.mark.parametrize("offset", [0.0, 1.0])
+def test_attention_of_large_scores(new, total, heads, group, dtype, loud, offset):
+    """Finite scores of 1e8 and more, positive or (with an offset) all negative, under
+    scales that are no power of two: the keys of the largest share all of the weight,
+    the next code's scores being a sixteenth of it away, a thousand and more."""
+    rng = np.random.default_rng(33)
+    dim, block = 128, 32
+    table, blocks = tables_of(rng, [total], block)
+    cache = ov.KVCache.empty(blocks, heads, dim, block)
+    k = np.zeros((total, heads, dim), np.float32)
+    k[..., 0] = loud * (rng.uniform(0.2, 1.0, (total, heads)) - 1.3 * offset)
+    v = rng.standard_normal((total, heads, dim))
+    ov.op_cache_write(cache, sequences(table, [total], [0, total]), tensor(k, dtype),
+                      tensor(v, dtype))
+    q = torch.zeros((new, heads * group, dim), dtype=TYPES[dtype], device="cuda")
+    q[..., 0] = loud
+    q[:, 1::2, 0] *= 0.37
+    keys, values = Plain(cache).read(table[0], 0, total)
+    for scale in (0.1, 0.113, 0.7):
+        out = torch.full_like(q, 9.0)
+        ov.op_cache_attention(cache, sequences(table, [total], [0, new]), q, out, scale=scale)
+        got = np64(out)
+        for head in sorted({0, heads - 1}):
+            best = keys[:, head, 0] == keys[:, head, 0].max()
+            x = values[best, head]
+            # The weights are equal and rounded alike, the sums float32: half a step.
+            tol = HALF_STEP[dtype] * np.abs(x.mean(0)) + 2.0 ** -18 * np.abs(x).mean(0) + 2.0 ** -25
+            err = np.abs(got[:, head * group:(head + 1) * group] - x.mean(0))
+            assert (err <= tol).all(), (scale, head, float(np.nanmax(err / tol)))
+
+
+@pytest.mark.parametrize("new", [8, 40, 200])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_large_scores_stay_in_their_rows(new, dtype):
+    """One row with scores of 1e4 and more, one with scores of infinity: the others'
+    bits are those without them."""
+    rng = np.random.default_rng(34)
+    table, blocks = tables_of(rng, [700], 32)
+    cache = filled(rng, blocks, 2, 128, 32)
+    q = tensor(rng.standard_normal((new, 4, 128)), dtype)
+    seq = sequences(table, [700], [0, new])
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    ov.op_cache_attention(cache, seq, q, clean, causal=True)
+    bad = q.clone()
+    bad[new // 2, 1] *= 1e4
+    bad[new // 2, 2, 5] = float("inf")
+    ov.op_cache_attention(cache, seq, bad, out, causal=True, scale=128 ** -0.5)
+    want = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+    want[new // 2, 1:3] = False
+    assert torch.equal(out[want], clean[want])
+    assert torch.isfinite(out[new // 2, 1]).all()
