@@ -25,9 +25,9 @@
 // 128 rows leaves CUs idle where there are few.
 //
 // Bound: memory where rows are few, 48 sequences of up to 8192 tokens (474 MB) in
-// 95.8 us, 4.9 TB/s. With many the issue of matrix and vector instructions: two causal
-// prompts of up to 5000 tokens (198 GFLOP) in 231 us on one card and 241 on another, 860
-// and 825 TFLOP/s, the matrix cores busy 46 % and vector instructions 38 % of the time;
+// 96.0 us, 4.9 TB/s. With many the issue of matrix and vector instructions: two causal
+// prompts of up to 5000 tokens (198 GFLOP) in 230 us on one card and 240 on another, 860
+// and 828 TFLOP/s, the matrix cores busy 46 % and vector instructions 38 % of the time;
 // of the largest library product 1174. A third work-group to a CU, its queries in LDS,
 // did not raise that. A short call is a chain of trips to memory: one token over 430
 // takes the kernel 7 us.

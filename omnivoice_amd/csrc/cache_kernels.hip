@@ -19,7 +19,7 @@
 // order and the pool's in LDS.
 //
 // Bound: memory. 16 prompts of up to 2048 tokens (8 heads of 128, fp16, 163 MB both
-// ways) are written in 35.5 us, 4.6 TB/s (29 when the same prompts are written again and
+// ways) are written in 35.5 to 36 us, 4.6 TB/s (29 when the same prompts are written again and
 // come out of the Infinity Cache), 32 sequences of up to 4096 (612 MB) read in 133 us,
 // 4.6 TB/s, where a copy of 1 GiB reaches 5.05. One token each of 64 sequences is the
 // chain of the sequence, the table, the old scale and the old codes, 6 us.
