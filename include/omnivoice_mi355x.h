@@ -398,8 +398,10 @@ typedef struct ovg_kv_sequences {
  * codes are rounded to nearest even, codes that stay move with the scale, and
  * the block's positions behind the call's last token are cleared. With an
  * infinity or a NaN among the new tokens the block's scale is NaN (and stays so
- * while any of its tokens stays). Writing tokens again at the same lengths
- * replaces them. No block may take tokens of two sequences in one call. */
+ * while any of its tokens stays); magnitudes from 3.3e38 on (float32 and bf16)
+ * have codes that stand for 2^128 and read back as infinities. Writing tokens
+ * again at the same lengths replaces them. No block may take tokens of two
+ * sequences in one call. */
 int ovg_op_cache_write(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
                        const void* k, const void* v, int64_t k_stride, int64_t v_stride,
                        int type, void* stream, char* error, size_t error_len);
@@ -427,7 +429,8 @@ int ovg_op_cache_read(const ovg_kv_cache* cache, const ovg_kv_sequences* sequenc
  * ovg_op_cache_attention_workspace bytes (-1 for arguments that the call
  * refuses), 16-byte aligned, NULL where that is 0; it holds nothing between
  * calls, and calls that may overlap need one each. heads is 1 to 64 times
- * kv_heads; scale may be negative. */
+ * kv_heads; scale may be negative, and log2(e) |scale| times the scale of keys
+ * that a row sees has to be finite, else the row is not defined. */
 int64_t ovg_op_cache_attention_workspace(const ovg_kv_cache* cache,
                                          const ovg_kv_sequences* sequences, int64_t heads);
 int ovg_op_cache_attention(const ovg_kv_cache* cache, const ovg_kv_sequences* sequences,
