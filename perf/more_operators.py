@@ -243,7 +243,7 @@ def _run_own(state):
                           scales=state["scales"])
         return [state[n] for n in ("total", "out", "scales")]
     if kind == "quantize":
-        ov.op_quantize(state["x"], state["codes"], state["scales"], gate=state["gate"])
+        ov.op_quantize8(state["x"], state["codes"], state["scales"], gate=state["gate"])
         return [state["codes"], state["scales"]]
     if kind == "linear":
         ov.op_linear8(state["x"], state["x_scales"], state["w"], state["w_scales"], state["y"])
