@@ -462,6 +462,117 @@ int ovg_op_token_logprobs(const void* logits, const void* uncond, int64_t rows, 
                           void* workspace, int64_t workspace_bytes, void* stream, char* error,
                           size_t error_len);
 
+/* ---- A token's step ----
+ * What a program that decodes over the cache runs around its calls: the norm that
+ * adds the residual, rows in 8 bits and their product with 8-bit weights, rotary
+ * positions before ovg_op_cache_write, and the draw of a token from the logits that
+ * ovg_op_token_logprobs rates. No counterpart in the reference, whose layers are
+ * fused into its one forward pass. Same streams and captures as the cache's calls:
+ * they enqueue on `stream`, which has to belong to the current device, wait for
+ * nothing and allocate nothing. Rows are `..._stride` elements apart, elements of a
+ * row next to each other; an output may be the input that it is said to replace,
+ * and no tensors may overlap in another way.
+ *
+ * 8-bit rows are e4m3 codes (OVG_E4M3) and one float32 scale a row: the smallest
+ * power of two, 2^-100 or more, that takes the row's largest magnitude into +-448,
+ * value = code * scale. A row that has an infinity or a NaN gets the scale NaN and
+ * codes of 0; magnitudes from 3.3e38 on have codes that stand for 2^128. */
+#define OVG_E4M3 3
+
+/* total = x + residual (in float32, rounded to the residual's type), out =
+ * weight * total * rsqrt(mean(total^2) + epsilon) per row, in out_type; e4m3 with
+ * scales [rows]. residual and total are NULL without a residual (out is x's norm),
+ * residual_type is x's or float32. total may be residual, or x where the types are
+ * the same; out may be x or residual where its type is the same and it is not total.
+ * x_type and out_type fp16, bf16 or float32, weight float32 [width]; width <= 65536,
+ * rows <= 2^22, epsilon > 0. */
+int ovg_op_add_rmsnorm(const void* x, int64_t x_stride, int x_type, const void* residual,
+                       int64_t residual_stride, void* total, int64_t total_stride,
+                       int residual_type, const float* weight, void* out, int64_t out_stride,
+                       int out_type, float* scales, int64_t rows, int64_t width, float epsilon,
+                       void* stream, char* error, size_t error_len);
+
+/* x, or x * silu(gate) with a gate of x's type, in 8 bits: weights that are prepared
+ * once, activations before a product. width <= 65536, rows <= 2^22. */
+int ovg_op_quantize8(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                    int type, void* codes, int64_t codes_stride, float* scales, int64_t rows,
+                    int64_t width, void* stream, char* error, size_t error_len);
+
+/* y[rows][out] = x[rows][in] w[out][in]^T of 8-bit rows in float32 sums, each times its
+ * row's and its column's scale (in this order; any scales), rounded to `type`. `in` is a
+ * multiple of 16 up to 65536; x and w are 16-byte aligned, x_stride a multiple of 16;
+ * rows and out up to 2^22. The order of a sum goes by the call's shape. */
+int ovg_op_linear8(const void* x, int64_t x_stride, const float* x_scales, const void* w,
+                   const float* w_scales, void* y, int64_t y_stride, int type, int64_t rows,
+                   int64_t in, int64_t out, void* stream, char* error, size_t error_len);
+
+/* Frequencies of rotary positions on the host: frequencies[rotary / 2] =
+ * theta^(-2 i / rotary), for contexts `factor` times as long as the trained one
+ *   OVG_ROTARY_LINEAR  all divided by factor
+ *   OVG_ROTARY_BASE    of theta * factor^(rotary / (rotary - 2)): the last one divided
+ *                      by factor, the first one kept
+ *   OVG_ROTARY_PARTS   those that turn less than once over original_positions divided by
+ *                      factor, those that turn over 32 times kept, a ramp over the pairs
+ *                      between; magnitude 0.1 ln(factor) + 1
+ * with the magnitude (1 but for parts) that ovg_op_rotary takes. theta > 1, factor >= 1.
+ * Returns OVG_ERROR for what it does not cover. */
+#define OVG_ROTARY_PLAIN 0
+#define OVG_ROTARY_LINEAR 1
+#define OVG_ROTARY_BASE 2
+#define OVG_ROTARY_PARTS 3
+int ovg_rotary_frequencies(int64_t rotary, double theta, int scaling, double factor,
+                           double original_positions, float* frequencies, float* magnitude);
+
+/* Turns the pairs of every head's first `rotary` dims by their row's position:
+ * (a, b) -> (a cos t - b sin t, b cos t + a sin t) * magnitude, t = position *
+ * frequencies[i], pair i being dims i and i + rotary / 2, or 2 i and 2 i + 1 where
+ * `interleaved`; the dims behind stay. q [rows][heads][head_dim] into q_out, k
+ * [rows][kv_heads][head_dim] into k_out (kv_heads 0: none), each `type` and possibly the
+ * same tensor; q|k of a fused q|k|v row can be one q of all their heads where they have
+ * one norm. q_norm and k_norm (float32 [head_dim], or NULL) norm each head first, as
+ * ovg_op_add_rmsnorm does. The positions are `positions` [rows] (negative ones turn back),
+ * or with `sequences` those of the rows' tokens, as ovg_op_cache_write places them
+ * (tables are not read; rows of nobody are left as they were). Angles are formed in 64
+ * bits: right to 2^-22 for positions up to 2^30 of frequencies up to 1. head_dim up to 512, rows
+ * up to 2^24. */
+int ovg_op_rotary(const void* q, void* q_out, int64_t q_stride, int64_t q_out_stride,
+                  int64_t heads, const void* k, void* k_out, int64_t k_stride,
+                  int64_t k_out_stride, int64_t kv_heads, int type, int64_t rows,
+                  int64_t head_dim, int64_t rotary, const float* frequencies, float magnitude,
+                  int interleaved, const int32_t* positions, const ovg_kv_sequences* sequences,
+                  const float* q_norm, const float* k_norm, float epsilon, void* stream,
+                  char* error, size_t error_len);
+
+/* The draw's settings: the numbers hold for every row, or device arrays [rows] hold one
+ * for each (NULL: the number). */
+typedef struct ovg_sampling {
+  float temperature; /* 0 or less: the best token */
+  int32_t top_k;     /* the first k tokens; 0 or less: all */
+  float top_p;       /* the shortest prefix with this share of their weight; 1: all */
+  float min_p;       /* what weighs at least this share of the best; 0: all */
+  const float* temperatures;
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+} ovg_sampling;
+
+/* Draws tokens[row] from logits ([rows][vocab] of `type`, rows `stride` elements apart)
+ * by random[row] in [0, 1). With `uncond` the logits are z = c + guidance * (c - u) as in
+ * ovg_op_token_logprobs; the token `mask_id` (-1: none) and those of -infinity are never
+ * drawn. Tokens are ordered by z, equal ones by index, and weigh
+ * w = exp((z - max z) / temperature); top_k keeps the first of them, top_p a prefix of
+ * what top_k keeps, min_p what weighs enough, and the best always stays. The token is the
+ * first, by index, at which the kept weights pass random * their sum. Weights count in
+ * units of 2^-shift (shift: 51, or 62 less the vocabulary's bits where that is less), so
+ * that a token under half a unit is never drawn; sums are exact, and the result does not
+ * depend on the order of the work. A row with a NaN or +infinity among its logits,
+ * without a token to draw, or with a NaN among its numbers has the token -1; random numbers
+ * outside [0, 1) count as the nearest inside. rows up to 2^22. */
+int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
+                  int64_t stride, int64_t uncond_stride, float guidance, int64_t mask_id,
+                  const ovg_sampling* sampling, const float* random, int32_t* tokens, int type,
+                  void* stream, char* error, size_t error_len);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -99,6 +99,12 @@ class _KvSequences(ctypes.Structure):
                 ("count", _i64), ("table_width", _i64), ("rows", _i64)]
 
 
+class _Sampling(ctypes.Structure):
+    _fields_ = [("temperature", _f32), ("top_k", ctypes.c_int32), ("top_p", _f32),
+                ("min_p", _f32), ("temperatures", _ptr), ("top_ks", _ptr), ("top_ps", _ptr),
+                ("min_ps", _ptr)]
+
+
 _CANCEL_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)
 
 EXPORTS = {
@@ -164,6 +170,23 @@ EXPORTS = {
     "ovg_op_token_logprobs": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _i64, _i64, _f32, _i64,
                                              _ptr, _i64, _ptr, _ptr, _ptr, _ptr, ctypes.c_int,
                                              _ptr, _i64, _ptr, _err, _sz]),
+    "ovg_op_add_rmsnorm": (ctypes.c_int, [_ptr, _i64, ctypes.c_int, _ptr, _i64, _ptr, _i64,
+                                          ctypes.c_int, _ptr, _ptr, _i64, ctypes.c_int, _ptr,
+                                          _i64, _i64, _f32, _ptr, _err, _sz]),
+    "ovg_op_quantize8": (ctypes.c_int, [_ptr, _i64, _ptr, _i64, ctypes.c_int, _ptr, _i64, _ptr,
+                                       _i64, _i64, _ptr, _err, _sz]),
+    "ovg_op_linear8": (ctypes.c_int, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i64, ctypes.c_int,
+                                      _i64, _i64, _i64, _ptr, _err, _sz]),
+    "ovg_rotary_frequencies": (ctypes.c_int, [_i64, ctypes.c_double, ctypes.c_int,
+                                              ctypes.c_double, ctypes.c_double, _ptr,
+                                              ctypes.POINTER(_f32)]),
+    "ovg_op_rotary": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64,
+                                     ctypes.c_int, _i64, _i64, _i64, _ptr, _f32, ctypes.c_int,
+                                     _ptr, ctypes.POINTER(_KvSequences), _ptr, _ptr, _f32, _ptr,
+                                     _err, _sz]),
+    "ovg_op_sample": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _i64, _i64, _f32, _i64,
+                                     ctypes.POINTER(_Sampling), _ptr, _ptr, ctypes.c_int, _ptr,
+                                     _err, _sz]),
     # the audio decoder (include/omnivoice_codec_mi355x.h)
     "ovc_create": (ctypes.c_int, [ctypes.POINTER(_CodecConfig), ctypes.c_char_p, _u64,
                                   ctypes.POINTER(_ptr), _err, _sz]),
@@ -934,6 +957,228 @@ def op_token_logprobs(logits, tokens, logprob, entropy, top_ids=None, top_logpro
     _enqueue(L.ovg_op_token_logprobs, device, stream, logits.data_ptr(), ptr(uncond), rows, vocab,
              stride, u_stride, guidance, -1 if mask_id is None else mask_id, ptr(tokens), top,
              ptr(logprob), ptr(entropy), ptr(top_ids), ptr(top_logprobs), kind, space, size)
+
+
+# --------------------------------------------------------------- a token's step
+
+def _matrix_stride(t, name: str, rows: int, width: int, device) -> int:
+    """The row stride, in elements, of a [rows][width] tensor whose rows are
+    contiguous."""
+    strides = t.stride()
+    if t.shape != (rows, width) or t.device != device or (width > 1 and strides[1] != 1):
+        raise GeneratorError(f"{name}: needs [{rows}][{width}] with contiguous rows on {device}, "
+                             f"got {tuple(t.shape)} with strides {strides} on {t.device}")
+    return strides[0] if rows > 1 else width  # a single row has no stride of its own
+
+
+def _is_e4m3(t) -> bool:
+    import torch
+    return t.dtype is torch.float8_e4m3fn or t.dtype is torch.uint8
+
+
+def op_add_rmsnorm(x, weight, out, eps: float = 1e-6, residual=None, total=None, scales=None,
+                   stream=None) -> None:
+    """The RMS norm of x [rows][width] (fp16, bf16 or float32), or of total = x +
+    residual (of x's type or float32; total defaults to the residual itself), times
+    weight (float32 [width]) into out [rows][width]: fp16, bf16, float32, or e4m3 codes
+    (float8_e4m3fn or uint8) with scales (float32 [rows]). Enqueued on `stream`."""
+    import torch
+    if x.dim() != 2:
+        raise GeneratorError(f"x: needs [rows][width], got {tuple(x.shape)}")
+    rows, width = x.shape
+    device = x.device
+    kind = _type_of(x, "x")
+    stride = _matrix_stride(x, "x", rows, width, device)
+    out_stride = _matrix_stride(out, "out", rows, width, device)
+    _expect(weight, "weight", torch.float32, (width,), device)
+    r_ptr = t_ptr = s_ptr = None
+    r_stride = t_stride = width
+    r_kind = 0
+    if residual is not None:
+        if total is None:
+            total = residual
+        if total.dtype is not residual.dtype:
+            raise GeneratorError(f"residual and total differ: {residual.dtype}, {total.dtype}")
+        r_kind = _type_of(residual, "residual")
+        r_stride = _matrix_stride(residual, "residual", rows, width, device)
+        t_stride = _matrix_stride(total, "total", rows, width, device)
+        r_ptr, t_ptr = residual.data_ptr(), total.data_ptr()
+    elif total is not None:
+        raise GeneratorError("total goes with a residual")
+    if scales is not None:
+        if not _is_e4m3(out):
+            raise GeneratorError(f"scales go with an out of 8 bits, got {out.dtype}")
+        _expect(scales, "scales", torch.float32, (rows,), device)
+        s_ptr, o_kind = scales.data_ptr(), 3
+    else:
+        o_kind = _type_of(out, "out without scales")
+    _enqueue(lib().ovg_op_add_rmsnorm, device, stream, x.data_ptr(), stride, kind, r_ptr,
+             r_stride, t_ptr, t_stride, r_kind, weight.data_ptr(), out.data_ptr(), out_stride,
+             o_kind, s_ptr, rows, width, eps)
+
+
+def op_quantize8(x, codes, scales, gate=None, stream=None) -> None:
+    """Rows of x [rows][width] (fp16, bf16 or float32), or of x * silu(gate), as e4m3
+    codes [rows][width] (float8_e4m3fn or uint8) and power-of-two scales (float32
+    [rows]). Enqueued on `stream`."""
+    import torch
+    if x.dim() != 2:
+        raise GeneratorError(f"x: needs [rows][width], got {tuple(x.shape)}")
+    rows, width = x.shape
+    device = x.device
+    kind = _type_of(x, "x")
+    stride = _matrix_stride(x, "x", rows, width, device)
+    codes_stride = _matrix_stride(codes, "codes", rows, width, device)
+    if not _is_e4m3(codes):
+        raise GeneratorError(f"codes: {codes.dtype} is not supported")
+    _expect(scales, "scales", torch.float32, (rows,), device)
+    g_ptr, g_stride = None, width
+    if gate is not None:
+        if gate.dtype is not x.dtype:
+            raise GeneratorError(f"x and gate differ: {x.dtype}, {gate.dtype}")
+        g_stride = _matrix_stride(gate, "gate", rows, width, device)
+        g_ptr = gate.data_ptr()
+    _enqueue(lib().ovg_op_quantize8, device, stream, x.data_ptr(), stride, g_ptr, g_stride, kind,
+             codes.data_ptr(), codes_stride, scales.data_ptr(), rows, width)
+
+
+def op_linear8(x, x_scales, w, w_scales, y, stream=None) -> None:
+    """y [rows][out] (fp16, bf16 or float32) = x [rows][in] w [out][in]^T of e4m3 codes
+    (float8_e4m3fn or uint8) with the rows' scales (float32 [rows], [out]), as
+    op_quantize8 gives them. `in` is a multiple of 16. Enqueued on `stream`."""
+    import torch
+    if x.dim() != 2 or w.dim() != 2:
+        raise GeneratorError(f"x, w: need [rows][in] and [out][in], got {tuple(x.shape)} and "
+                             f"{tuple(w.shape)}")
+    rows, width = x.shape
+    out = w.shape[0]
+    device = x.device
+    if not _is_e4m3(x) or not _is_e4m3(w):
+        raise GeneratorError(f"x, w: {x.dtype}, {w.dtype} are not supported")
+    stride = _matrix_stride(x, "x", rows, width, device)
+    _expect(w, "w", w.dtype, (out, width), device)
+    _expect(x_scales, "x_scales", torch.float32, (rows,), device)
+    _expect(w_scales, "w_scales", torch.float32, (out,), device)
+    y_stride = _matrix_stride(y, "y", rows, out, device)
+    _enqueue(lib().ovg_op_linear8, device, stream, x.data_ptr(), stride, x_scales.data_ptr(),
+             w.data_ptr(), w_scales.data_ptr(), y.data_ptr(), y_stride, _type_of(y, "y"), rows,
+             width, out)
+
+
+ROTARY_SCALINGS = {None: 0, "linear": 1, "base": 2, "parts": 3}
+
+
+def rotary_frequencies(rotary: int, theta: float = 1e6, scaling: Optional[str] = None,
+                       factor: float = 1.0, original_positions: float = 0.0
+                       ) -> Tuple[np.ndarray, float]:
+    """(float32 [rotary / 2], magnitude) for op_rotary: theta^(-2 i / rotary), for
+    contexts `factor` times as long as the trained one by "linear", "base" or "parts"
+    (ovg_rotary_frequencies), the last of which needs the trained length."""
+    if scaling not in ROTARY_SCALINGS:
+        raise GeneratorError(f"scaling: {scaling!r} is none of {list(ROTARY_SCALINGS)}")
+    out = np.zeros(max(rotary // 2, 1), dtype=np.float32)
+    magnitude = _f32()
+    if lib().ovg_rotary_frequencies(rotary, theta, ROTARY_SCALINGS[scaling], factor,
+                                    original_positions, _p(out),
+                                    ctypes.byref(magnitude)) != OVG_OK:
+        raise GeneratorError("bad rotary arguments")
+    return out, magnitude.value
+
+
+def op_rotary(q, q_out, k, k_out, frequencies, positions=None,
+              sequences: Optional[KVSequences] = None, interleaved: bool = False,
+              magnitude: float = 1.0, q_norm=None, k_norm=None, eps: float = 1e-6,
+              stream=None) -> None:
+    """Turns the first 2 * len(frequencies) dims of every head of q [rows][heads][dim]
+    into q_out, and of k [rows][kv_heads][dim] into k_out (None: no keys), by their rows'
+    positions (int32 [rows]), or those of the sequences' tokens as op_cache_write places
+    them. Outputs may be the inputs. q_norm, k_norm (float32 [dim]) norm the heads first.
+    fp16, bf16 or float32 with contiguous rows, frequencies float32 on the device.
+    Enqueued on `stream`."""
+    import torch
+    if q.dim() != 3:
+        raise GeneratorError(f"q: needs [rows][heads][dim], got {tuple(q.shape)}")
+    rows, heads, dim = q.shape
+    device = q.device
+    kind = _type_of(q, "q")
+    strides = [_row_stride(q, "q", rows, heads, dim, device),
+               _row_stride(q_out, "q_out", rows, heads, dim, device)]
+    if (k is None) != (k_out is None):
+        raise GeneratorError("k and k_out go together")
+    kv_heads, k_ptr, k_out_ptr = 0, None, None
+    k_strides = [0, 0]
+    if k is not None:
+        if k.dim() != 3:
+            raise GeneratorError(f"k: needs [rows][kv_heads][dim], got {tuple(k.shape)}")
+        kv_heads = k.shape[1]
+        k_strides = [_row_stride(k, "k", rows, kv_heads, dim, device),
+                     _row_stride(k_out, "k_out", rows, kv_heads, dim, device)]
+        k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
+    for t, name in ((q_out, "q_out"), (k, "k"), (k_out, "k_out")):
+        if t is not None and t.dtype is not q.dtype:
+            raise GeneratorError(f"q and {name} differ: {q.dtype}, {t.dtype}")
+    if frequencies.dim() != 1:
+        raise GeneratorError(f"frequencies: needs [pairs], got {tuple(frequencies.shape)}")
+    pairs = frequencies.shape[0]
+    _expect(frequencies, "frequencies", torch.float32, (pairs,), device)
+    norms = []
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if t is not None:
+            _expect(t, name, torch.float32, (dim,), device)
+        norms.append(None if t is None else t.data_ptr())
+    if (positions is None) == (sequences is None):
+        raise GeneratorError("either positions or sequences")
+    seq = p_ptr = None
+    if sequences is not None:
+        if sequences.device != device:
+            raise GeneratorError(f"sequences on {sequences.device}, q on {device}")
+        seq = sequences._c(rows)
+    else:
+        _expect(positions, "positions", torch.int32, (rows,), device)
+        p_ptr = positions.data_ptr()
+    _enqueue(lib().ovg_op_rotary, device, stream, q.data_ptr(), q_out.data_ptr(), *strides, heads,
+             k_ptr, k_out_ptr, *k_strides, kv_heads, kind, rows, dim, 2 * pairs,
+             frequencies.data_ptr(), magnitude, int(interleaved), p_ptr, seq, *norms, eps)
+
+
+def op_sample(logits, random, tokens, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, uncond=None,
+              guidance: float = 0.0, mask_id: Optional[int] = None, stream=None) -> None:
+    """Draws tokens [rows] (int32) from logits [rows][vocab] (fp16, bf16 or float32,
+    contiguous rows) by the numbers random [rows] (float32 in [0, 1)), at a temperature (0:
+    the best) among the top_k best, of these the shortest prefix that holds top_p of their
+    weight, and what weighs min_p of the best or more. Each setting is a number or a device
+    tensor [rows] (float32, top_k int32). With `uncond` the logits are
+    c + guidance * (c - u); mask_id is never drawn. Enqueued on `stream`."""
+    import torch
+    if logits.dim() != 2:
+        raise GeneratorError(f"logits: needs [rows][vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    device = logits.device
+    kind = _type_of(logits, "logits")
+    stride = _logit_stride(logits, "logits", rows, vocab, device, logits.dtype)
+    u_ptr, u_stride = None, vocab
+    if uncond is not None:
+        u_stride = _logit_stride(uncond, "uncond", rows, vocab, device, logits.dtype)
+        u_ptr = uncond.data_ptr()
+    _expect(random, "random", torch.float32, (rows,), device)
+    _expect(tokens, "tokens", torch.int32, (rows,), device)
+    numbers, arrays = [], []
+    for value, name, dtype, off in ((temperature, "temperature", torch.float32, 1.0),
+                                    (top_k, "top_k", torch.int32, 0),
+                                    (top_p, "top_p", torch.float32, 1.0),
+                                    (min_p, "min_p", torch.float32, 0.0)):
+        if isinstance(value, torch.Tensor):
+            _expect(value, name, dtype, (rows,), device)
+            numbers.append(off)
+            arrays.append(value.data_ptr())
+        else:
+            numbers.append(value)
+            arrays.append(None)
+    if not -2 ** 31 <= numbers[1] < 2 ** 31:
+        raise GeneratorError(f"top_k: {numbers[1]} is no 32-bit number")
+    _enqueue(lib().ovg_op_sample, device, stream, logits.data_ptr(), u_ptr, rows, vocab, stride,
+             u_stride, guidance, -1 if mask_id is None else mask_id,
+             _Sampling(*numbers, *arrays), random.data_ptr(), tokens.data_ptr(), kind)
 
 
 # --------------------------------------------------------------- audio decoder

@@ -12,8 +12,9 @@
 
 namespace ovg {
 
-// Element types of the operators' caller tensors (OVG_F16, OVG_BF16, OVG_F32).
-enum class DType : int { kF16 = 0, kBf16 = 1, kF32 = 2 };
+// Element types of the operators' caller tensors (OVG_F16, OVG_BF16, OVG_F32,
+// OVG_E4M3).
+enum class DType : int { kF16 = 0, kBf16 = 1, kF32 = 2, kE4m3 = 3 };
 
 // A pool of blocks and the sequences of one call. Device pointers; the
 // values behind them are not known to the host, so every kernel clamps what

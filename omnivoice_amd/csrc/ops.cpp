@@ -5,35 +5,13 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstring>
 #include <string>
 
-#include "../../include/omnivoice_mi355x.h"
-#include "cache.hpp"
-#include "kernels.hpp"
+#include "ops.hpp"
 
 namespace {
 
-void SetError(char* error, std::size_t len, const std::string& message) {
-  if (error == nullptr || len == 0)
-    return;
-  const std::size_t n = std::min(len - 1, message.size());
-  std::memcpy(error, message.data(), n);
-  error[n] = '\0';
-}
-
-template <typename F>
-int Guard(const char* prefix, char* error, std::size_t len, F&& body) {
-  try {
-    body();
-    return OVG_OK;
-  } catch (const std::exception& failure) {
-    SetError(error, len, std::string(prefix) + failure.what());
-    return OVG_ERROR;
-  }
-}
-
-bool FitsInt(int64_t v) { return v >= 0 && v <= (int64_t{1} << 30); }
+using namespace ovg::ops;
 
 // A device allocation that lives for one operator call.
 template <typename T>
@@ -49,20 +27,6 @@ struct Scratch {
       (void)hipFree(data);
   }
 };
-
-// A launch has to go to a device of its own: with another device current the
-// kernel would run there, or fail in ways that depend on peer access.
-void RequireCurrentDevice(hipStream_t stream) {
-  if (stream == nullptr)
-    return;  // the current device's own
-  hipDevice_t of_stream = 0;
-  int current = 0;
-  ovg::Check(hipStreamGetDevice(stream, &of_stream), "hipStreamGetDevice");
-  ovg::Check(hipGetDevice(&current), "hipGetDevice");
-  ovg::Require(of_stream == current, "the stream is not the current device's");
-}
-
-bool Aligned16(const void* p) { return reinterpret_cast<std::uintptr_t>(p) % 16 == 0; }
 
 // The pool and sequences of a call, their sizes checked against what the
 // kernels' 32-bit positions, rows and items hold.
@@ -100,12 +64,6 @@ ovg::CacheView ViewOf(const ovg_kv_cache* cache, const ovg_kv_sequences* sequenc
   return c;
 }
 
-ovg::DType TypeOf(int type, bool with_f32) {
-  ovg::Require(type == OVG_F16 || type == OVG_BF16 || (with_f32 && type == OVG_F32),
-               with_f32 ? "type must be fp16, bf16 or float32" : "type must be fp16 or bf16");
-  return static_cast<ovg::DType>(type);
-}
-
 // Query heads of a kv head, for the attention and for its workspace's size.
 int GroupOf(const ovg_kv_cache* cache, int64_t heads) {
   ovg::Require(heads >= cache->kv_heads && heads % cache->kv_heads == 0 &&
@@ -122,10 +80,6 @@ int64_t AttentionBytes(const ovg::CacheView& c, const ovg::CacheAttentionPlan& p
 // The splits' sums and lists.
 int64_t LogprobBytes(int64_t rows, int64_t top, int splits) {
   return splits == 1 ? 0 : rows * splits * (4 + 2 * top) * static_cast<int64_t>(sizeof(float));
-}
-
-void RequireStride(int64_t stride, int64_t width) {
-  ovg::Require(stride >= width && stride <= (int64_t{1} << 40), "row stride below the row's width");
 }
 
 }  // namespace
