@@ -562,16 +562,17 @@ typedef struct ovg_sampling {
  * drawn. Tokens are ordered by z, equal ones by index, and weigh
  * w = exp((z - max z) / temperature); top_k keeps the first of them, top_p a prefix of
  * what top_k keeps, min_p what weighs enough, and the best always stays. The token is the
- * first, by index, at which the kept weights pass random * their sum. Weights count in
- * units of 2^-shift (shift: 51, or 62 less the vocabulary's bits where that is less), so
- * that a token under half a unit is never drawn; sums are exact, and the result does not
- * depend on the order of the work. A row with a NaN or +infinity among its logits,
+ * first, by index, at which the kept weights pass random * their sum; one that weighs less
+ * than 2^-50 of the best counts as none. Weights and sums are right to 2^-40 of the sum and
+ * do not depend on the order of the work. A row with a NaN or +infinity among its logits,
  * without a token to draw, or with a NaN among its numbers has the token -1; random numbers
- * outside [0, 1) count as the nearest inside. rows up to 2^22. */
+ * outside [0, 1) count as the nearest inside. rows up to 2^22. `workspace` as above. */
+int64_t ovg_op_sample_workspace(int64_t rows, int64_t vocab);
 int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
                   int64_t stride, int64_t uncond_stride, float guidance, int64_t mask_id,
                   const ovg_sampling* sampling, const float* random, int32_t* tokens, int type,
-                  void* stream, char* error, size_t error_len);
+                  void* workspace, int64_t workspace_bytes, void* stream, char* error,
+                  size_t error_len);
 
 #ifdef __cplusplus
 }  /* extern "C" */

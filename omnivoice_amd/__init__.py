@@ -184,9 +184,10 @@ EXPORTS = {
                                      ctypes.c_int, _i64, _i64, _i64, _ptr, _f32, ctypes.c_int,
                                      _ptr, ctypes.POINTER(_KvSequences), _ptr, _ptr, _f32, _ptr,
                                      _err, _sz]),
+    "ovg_op_sample_workspace": (_i64, [_i64, _i64]),
     "ovg_op_sample": (ctypes.c_int, [_ptr, _ptr, _i64, _i64, _i64, _i64, _f32, _i64,
                                      ctypes.POINTER(_Sampling), _ptr, _ptr, ctypes.c_int, _ptr,
-                                     _err, _sz]),
+                                     _i64, _ptr, _err, _sz]),
     # the audio decoder (include/omnivoice_codec_mi355x.h)
     "ovc_create": (ctypes.c_int, [ctypes.POINTER(_CodecConfig), ctypes.c_char_p, _u64,
                                   ctypes.POINTER(_ptr), _err, _sz]),
@@ -1141,14 +1142,21 @@ def op_rotary(q, q_out, k, k_out, frequencies, positions=None,
              frequencies.data_ptr(), magnitude, int(interleaved), p_ptr, seq, *norms, eps)
 
 
+def op_sample_workspace(rows: int, vocab: int) -> int:
+    """Bytes of workspace that op_sample needs."""
+    return int(lib().ovg_op_sample_workspace(rows, vocab))
+
+
 def op_sample(logits, random, tokens, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, uncond=None,
-              guidance: float = 0.0, mask_id: Optional[int] = None, stream=None) -> None:
+              guidance: float = 0.0, mask_id: Optional[int] = None, workspace=None,
+              stream=None) -> None:
     """Draws tokens [rows] (int32) from logits [rows][vocab] (fp16, bf16 or float32,
     contiguous rows) by the numbers random [rows] (float32 in [0, 1)), at a temperature (0:
     the best) among the top_k best, of these the shortest prefix that holds top_p of their
     weight, and what weighs min_p of the best or more. Each setting is a number or a device
     tensor [rows] (float32, top_k int32). With `uncond` the logits are
-    c + guidance * (c - u); mask_id is never drawn. Enqueued on `stream`."""
+    c + guidance * (c - u); mask_id is never drawn. `workspace`: a device tensor of
+    op_sample_workspace bytes (one is allocated without it). Enqueued on `stream`."""
     import torch
     if logits.dim() != 2:
         raise GeneratorError(f"logits: needs [rows][vocab], got {tuple(logits.shape)}")
@@ -1176,9 +1184,12 @@ def op_sample(logits, random, tokens, temperature=1.0, top_k=0, top_p=1.0, min_p
             arrays.append(None)
     if not -2 ** 31 <= numbers[1] < 2 ** 31:
         raise GeneratorError(f"top_k: {numbers[1]} is no 32-bit number")
-    _enqueue(lib().ovg_op_sample, device, stream, logits.data_ptr(), u_ptr, rows, vocab, stride,
+    L = lib()
+    space, size, keep = _workspace(workspace, L.ovg_op_sample_workspace(rows, vocab), device,
+                                   stream)
+    _enqueue(L.ovg_op_sample, device, stream, logits.data_ptr(), u_ptr, rows, vocab, stride,
              u_stride, guidance, -1 if mask_id is None else mask_id,
-             _Sampling(*numbers, *arrays), random.data_ptr(), tokens.data_ptr(), kind)
+             _Sampling(*numbers, *arrays), random.data_ptr(), tokens.data_ptr(), kind, space, size)
 
 
 # --------------------------------------------------------------- audio decoder

@@ -79,7 +79,9 @@ struct SampleParams {
   const int* top_ks;
   const float* top_ps;
   const float* min_ps;
+  unsigned* work;  // SampleWorkBytes
 };
+std::int64_t SampleWorkBytes(std::int64_t rows, std::int64_t vocab);
 void LaunchSample(const SampleParams& p, DType type, hipStream_t stream);
 
 // ---------------------------------------------------------------- device helpers

@@ -242,10 +242,17 @@ int ovg_op_rotary(const void* q, void* q_out, int64_t q_stride, int64_t q_out_st
   });
 }
 
+int64_t ovg_op_sample_workspace(int64_t rows, int64_t vocab) {
+  if (rows < 0 || rows > ovg::kMostRows || vocab < 1 || !FitsInt(vocab))
+    return -1;
+  return ovg::SampleWorkBytes(rows, vocab);
+}
+
 int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
                   int64_t stride, int64_t uncond_stride, float guidance, int64_t mask_id,
                   const ovg_sampling* sampling, const float* random, int32_t* tokens, int type,
-                  void* stream, char* error, size_t error_len) {
+                  void* workspace, int64_t workspace_bytes, void* stream, char* error,
+                  size_t error_len) {
   return Guard("sample: ", error, error_len, [&] {
     const ovg::DType t = TypeOf(type, true);
     ovg::Require(rows >= 0 && rows <= ovg::kMostRows, "rows outside [0, 2^22]");
@@ -267,7 +274,11 @@ int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t 
     ovg::Require(logits && random && tokens, "null pointer");
     auto s = static_cast<hipStream_t>(stream);
     RequireCurrentDevice(s);
+    const int64_t bytes = ovg::SampleWorkBytes(rows, vocab);
+    ovg::Require(bytes == 0 || (workspace && workspace_bytes >= bytes && Aligned16(workspace)),
+                 "workspace of " + std::to_string(bytes) + " bytes needed, 16-byte aligned");
     ovg::SampleParams p{};
+    p.work = static_cast<unsigned*>(workspace);
     p.logits = logits;
     p.uncond = uncond;
     p.stride = stride;

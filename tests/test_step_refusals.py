@@ -146,13 +146,13 @@ def test_rotary_refuses():
 
 
 def sample(call=refused, z=HERE, u=None, rows=4, vocab=100, stride=100, us=100, g=0.0, mask=-1,
-           setting=None, r=HERE, t=HERE, kind=2, **numbers):
+           setting=None, r=HERE, t=HERE, kind=2, space=None, size=0, **numbers):
     if setting is None:
         n = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
         n.update(numbers)
         setting = ov._Sampling(**n)
     return call("ovg_op_sample", z, u, rows, vocab, stride, us, g, mask, setting or None, r, t,
-                kind, None)
+                kind, space, size, None)
 
 
 def test_sample_refuses():
@@ -173,6 +173,10 @@ def test_sample_refuses():
     for name in ("temperature", "top_p", "min_p"):
         assert name in sample(**{name: NAN})
     assert sample(answer, rows=0, z=None, r=None, t=None)[0] == ov.OVG_OK
+    need = ov.op_sample_workspace(4, 9000)
+    assert need > 0 and ov.op_sample_workspace(4, 2048) == 0
+    for args in ((-1, 100), (2 ** 22 + 1, 100), (4, 0), (4, 2 ** 31)):
+        assert ov.op_sample_workspace(*args) == -1
 
 
 @pytest.mark.parametrize("stream", [None, 0, HERE])
