@@ -16,10 +16,11 @@
 // chunk's weight beside its own largest. The second has a work-group for every row.
 // Without filters it finds the chunk by the chunks' weights and reads only that one. The
 // k best lie in the k quarters with the largest keys, so with filters it reads those (64
-// for top_p alone) and selects among the few elements that reach the last one's. Where
-// that is not enough (a large k, a share that needs more) it reads the row again: three
-// passes over 11, 11 and 10 bits of the keys with sums in LDS, and one for the chunks'
-// kept weights.
+// for top_p alone) and ranks the few elements that reach the last one's. Where that is
+// not enough (a large k, a share that needs more) it reads the row again: sums of 2048
+// steps of the logit, passes over what the step that was found holds, and one for the
+// chunks' kept weights. With few rows these take launches of their own, in which all CUs
+// share the rows, and which end at once where no row needs them.
 //
 // A draw lands where sums of up to 2^17 weights say, so weights have 2^-42 and better:
 // 2^x in 64 bits from a table of 256 powers and three terms. Sums that several lanes
@@ -43,9 +44,10 @@ constexpr int kRowThreads = 512;            // of a row's work-group in the seco
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kMostQuarters = 2048;         // that are ranked
 constexpr int kMostOpened = 256;            // quarters that are read for a list
-constexpr int kList = 512;                  // elements of it
+constexpr int kShortList = 512;             // of which every element is ranked
+constexpr int kList = 2048;                 // elements of a list
 constexpr int kShareOpened = 64;            // opened for a share alone
-constexpr double kLeast = -50.0;            // log2 of the smallest weight that counts
+constexpr int kOctaves = 50;                // weights below 2^-50 do not count
 constexpr int kTable = 256;
 
 // ---------------------------------------------------------------- lanes
@@ -98,14 +100,30 @@ __device__ __forceinline__ unsigned WaveMaxKey(unsigned v) {
 __device__ __forceinline__ unsigned WaveMinKey(unsigned v) {
   return WaveJoin(v, [](unsigned a, unsigned b) { return min(a, b); });
 }
-// The lanes' sums up to and with themselves.
+// The lanes' sums up to and with themselves: within rows of 16 lanes, then the rows'
+// last lanes to the rows behind.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned Shifted(unsigned v) {
+  return static_cast<unsigned>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 Shifted(u64 v) {
+  return static_cast<u64>(Shifted<CTRL, ROWS>(static_cast<unsigned>(v >> 32))) << 32 |
+         Shifted<CTRL, ROWS>(static_cast<unsigned>(v));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double Shifted(double v) {
+  return __builtin_bit_cast(double, Shifted<CTRL, ROWS>(__builtin_bit_cast(u64, v)));
+}
 template <typename V>
 __device__ __forceinline__ V WaveScan(V v) {
-  const int lane = threadIdx.x % kWave;
-  for (int offset = 1; offset < kWave; offset *= 2) {
-    const V before = __shfl_up(v, offset);
-    v = lane >= offset ? v + before : v;
-  }
+  v += Shifted<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += Shifted<0x112, 0xF>(v);
+  v += Shifted<0x114, 0xF>(v);
+  v += Shifted<0x118, 0xF>(v);
+  v += Shifted<0x142, 0xA>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+  v += Shifted<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
   return v;
 }
 
@@ -114,25 +132,26 @@ __device__ __forceinline__ V WaveScan(V v) {
 constexpr unsigned kKeyOfInf = 0xFF800000u;  // and NaN from here on
 constexpr unsigned kKeyOfMinusInf = 0x007FFFFFu;
 __device__ __forceinline__ unsigned KeyOf(float z) {
-  if (z != z)
-    return ~0u;
   const unsigned bits = __float_as_uint(z + 0.0F);  // one zero
-  const unsigned key = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-  return key <= kKeyOfMinusInf ? 0 : key;
+  unsigned key = bits ^ (static_cast<unsigned>(static_cast<int>(bits) >> 31) | 0x80000000u);
+  key = key > kKeyOfMinusInf ? key : 0;
+  return z == z ? key : ~0u;
 }
 __device__ __forceinline__ float LogitOf(unsigned key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// The lane's run of keys at d .. d + 7: 0 before `d` where the row's end moved the run
-// forward (RunStart), and for the masked token.
-__device__ __forceinline__ int RunStart(int d, int vocab) {
+// A lane's run of eight logits of quarter q. The row's last run is moved to its end, so
+// that no load is conditional: RunStart is its first element. What the run before has,
+// what is behind the row and the masked token are -infinity.
+__device__ __forceinline__ int RunStart(int q, int vocab) {
+  const int d = (q * kWave + static_cast<int>(threadIdx.x % kWave)) * kRun;
   return vocab >= kRun ? min(d, vocab - kRun) : 0;
 }
 template <typename T>
-__device__ __forceinline__ void LoadRun(const T* row, int d, int vocab, float (&v)[kRun]) {
+__device__ __forceinline__ void LoadRun(const T* row, int start, int vocab, float (&v)[kRun]) {
   if (vocab >= kRun) {
-    LoadFloats<kRun>(row + RunStart(d, vocab), v);
+    LoadFloats<kRun>(row + start, v);
   } else {
 #pragma unroll
     for (int i = 0; i < kRun; ++i)
@@ -140,55 +159,81 @@ __device__ __forceinline__ void LoadRun(const T* row, int d, int vocab, float (&
   }
 }
 template <typename T>
-__device__ __forceinline__ void LoadKeys(const SampleParams& p, std::int64_t row, int d,
-                                         unsigned (&key)[kRun]) {
-  float c[kRun], u[kRun];
-  LoadRun(static_cast<const T*>(p.logits) + row * p.stride, d, p.vocab, c);
+__device__ __forceinline__ void LoadLogits(const SampleParams& p, std::int64_t row, int q,
+                                           float (&z)[kRun]) {
+  const int start = RunStart(q, p.vocab);
+  LoadRun(static_cast<const T*>(p.logits) + row * p.stride, start, p.vocab, z);
   if (p.uncond != nullptr) {
-    LoadRun(static_cast<const T*>(p.uncond) + row * p.uncond_stride, d, p.vocab, u);
+    float u[kRun];
+    LoadRun(static_cast<const T*>(p.uncond) + row * p.uncond_stride, start, p.vocab, u);
 #pragma unroll
-    for (int i = 0; i < kRun; ++i)
-      c[i] = c[i] == -__builtin_inff() ? c[i] : c[i] + p.guidance * (c[i] - u[i]);
+    for (int i = 0; i < kRun; ++i) {
+      const float guided = z[i] + p.guidance * (z[i] - u[i]);
+      z[i] = z[i] == -__builtin_inff() ? z[i] : guided;
+    }
   }
-  const int start = RunStart(d, p.vocab);
+  const int first = q * kQuarter;
+  if (first + kQuarter > p.vocab || (p.mask_id >= first && p.mask_id < first + kQuarter)) {
+    const int d = first + static_cast<int>(threadIdx.x % kWave) * kRun;
 #pragma unroll
-  for (int i = 0; i < kRun; ++i) {
-    const int e = start + i;
-    key[i] = e >= d && e < p.vocab && e != p.mask_id ? KeyOf(c[i]) : 0;
+    for (int i = 0; i < kRun; ++i) {
+      const int e = start + i;
+      const bool in = (e >= d) & (e < p.vocab) & (e != p.mask_id);
+      z[i] = in ? z[i] : -__builtin_inff();
+    }
   }
+}
+template <typename T>
+__device__ __forceinline__ void LoadKeys(const SampleParams& p, std::int64_t row, int q,
+                                         unsigned (&key)[kRun]) {
+  float z[kRun];
+  LoadLogits<T>(p, row, q, z);
+#pragma unroll
+  for (int i = 0; i < kRun; ++i)
+    key[i] = KeyOf(z[i]);
 }
 
 // ---------------------------------------------------------------- weights
-// powers[j] = 2^(j / 256), by the series of e^x.
-__device__ __forceinline__ void FillTable(double* powers) {
-  for (int j = threadIdx.x; j < kTable; j += blockDim.x) {
+// 2^(j / 256), by the series of e^x.
+struct Powers {
+  double v[kTable];
+};
+constexpr Powers PowersOfTwo() {
+  Powers t{};
+  for (int j = 0; j < kTable; ++j) {
     const double x = j * (0.69314718055994530942 / kTable);
     double e = 1.0;
     for (int n = 18; n > 0; --n)
       e = 1.0 + e * x / n;
-    powers[j] = e;
+    t.v[j] = e;
   }
+  return t;
+}
+__device__ const Powers kPowers = PowersOfTwo();
+__device__ __forceinline__ void FillTable(double* powers) {
+  for (int j = threadIdx.x; j < kTable; j += blockDim.x)
+    powers[j] = kPowers.v[j];
 }
 
 struct Weigher {
   const double* powers;  // in LDS
   double top, per;       // the largest logit; 256 log2(e) / T
-  // 2^((z - top) per / 256): the table's power times three terms of the rest, which is
-  // under ln 2 / 512, so that 1.4e-13 is left out.
-  __device__ __forceinline__ double operator()(unsigned key) const {
-    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: whole numbers behind it
+  // 2^((z - top) per / 256): the table's power times three terms of the rest,
+  // which is under ln 2 / 512, so that 1.4e-13 is left out.
+  __device__ __forceinline__ double Raw(float z) const {
     constexpr double kA = 0.69314718055994530942 / kTable;
-    const double t = (static_cast<double>(LogitOf(key)) - top) * per;
-    const double y = t + kMagic;
-    const int k = static_cast<int>(__builtin_bit_cast(u64, y));
-    const double r = t - (y - kMagic);
+    const double t = fmax((static_cast<double>(z) - top) * per, -1e9);  // also of -infinity
+    const double whole = __builtin_rint(t);
+    const double r = t - whole;
+    const int k = static_cast<int>(whole);
     double e = __fma_rn(r, kA * kA * kA / 6, kA * kA / 2);
     e = __fma_rn(r, e, kA);
     e = __fma_rn(r, e, 1.0);
-    e *= powers[k & (kTable - 1)];
-    u64 bits = __builtin_bit_cast(u64, e);
-    bits += static_cast<u64>(static_cast<unsigned>(k >> 8) << 20) << 32;
-    return key != 0 && t >= kLeast * kTable ? __builtin_bit_cast(double, bits) : 0.0;
+    return ldexp(e * powers[k & (kTable - 1)], k >> 8);
+  }
+  __device__ __forceinline__ double operator()(unsigned key) const {
+    const double w = Raw(LogitOf(key));
+    return (key != 0) & (w >= 0x1p-50) ? w : 0.0;
   }
 };
 // In whole units of 2^-shift, shift <= 51: the last bits of a sum with 2^(52 - shift).
@@ -347,15 +392,56 @@ struct Held {
   }
 };
 
+// Of R elements a lane in the row's order, lane by lane: whether the kept weights pass
+// `left` here, and then which element of which lane. `need` and `left` go on to what
+// follows.
+template <int R>
+__device__ __forceinline__ bool DrawOf(const unsigned (&key)[R], const u64 (&weight)[R],
+                                       unsigned t, u64* need, u64* left, int* lane, int* place) {
+  unsigned equal = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    equal += key[i] == t;
+  // Most runs have no equal: their scan is left out.
+  const bool equals = __ballot(equal != 0) != 0;
+  const unsigned equal_to = equals ? WaveScan(equal) : 0;
+  u64 seen = equal_to - equal, mine = 0;
+  u64 to_place[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    mine += key[i] > t || (key[i] == t && seen++ < *need) ? weight[i] : 0;
+    to_place[i] = mine;
+  }
+  const u64 to = WaveScan(mine);
+  const u64 hit = __ballot(to > *left);
+  if (hit == 0) {
+    *left -= Lane64(to, kWave - 1);
+    *need -= min(*need, static_cast<u64>(__builtin_amdgcn_readlane(equal_to, kWave - 1)));
+    return false;
+  }
+  *lane = __builtin_ctzll(hit);
+  int at = R - 1;
+#pragma unroll
+  for (int i = R - 2; i >= 0; --i)
+    at = to - mine + to_place[i] > *left ? i : at;
+  *place = __builtin_amdgcn_readlane(at, *lane);
+  return true;
+}
+
 // ---------------------------------------------------------------- small rows
-// A wave a row of up to 512 Q tokens.
+// A wave a row of up to 512 Q tokens. With a top_k of 64 or less, the lanes' largest keys
+// give a floor that the k best reach, and the few elements that do go through LDS, in the
+// row's order, to two a lane.
+constexpr int kFew = 2 * kWave;
+
 template <typename T, int Q>
 __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shift) {
   constexpr int N = Q * kRun;
   __shared__ double powers[kTable];
+  __shared__ u64 few[kWaves][kFew];  // key, index
   FillTable(powers);
-  const int lane = threadIdx.x % kWave;
-  const int row = blockIdx.x * kWaves + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int row = blockIdx.x * kWaves + wave;
   Held<N> held;
   held.used = N;
   Settings s{};
@@ -364,7 +450,7 @@ __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shif
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       unsigned key[kRun];
-      LoadKeys<T>(p, row, (q * kWave + lane) * kRun, key);
+      LoadKeys<T>(p, row, q, key);
 #pragma unroll
       for (int i = 0; i < kRun; ++i)
         held.key[q * kRun + i] = key[i];
@@ -373,11 +459,11 @@ __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shif
   __syncthreads();
   if (row >= p.rows)
     return;
-  unsigned best = 0;
+  unsigned most = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    best = max(best, held.key[i]);
-  best = WaveMaxKey(best);
+    most = max(most, held.key[i]);
+  const unsigned best = WaveMaxKey(most);
   if (best == 0 || best >= kKeyOfInf || s.lost) {
     if (lane == 0)
       p.tokens[row] = -1;
@@ -385,6 +471,57 @@ __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shif
   }
   const Weigher w = WeigherOf(powers, best, s.greedy ? 1.0F : s.temperature);
   Kept kept{best, 1, 1};
+  u64 left, need;
+  int of, place;
+  if (!s.greedy && s.top_k > 0 && s.top_k <= kWave) {
+    const unsigned floor = Held<1>::Search(1, best, [&](unsigned t) {
+      return __popcll(__ballot(most >= t)) >= s.top_k;
+    });
+    unsigned from[Q];  // where the lane's elements go
+    int listed = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      unsigned n = 0;
+#pragma unroll
+      for (int i = 0; i < kRun; ++i)
+        n += held.key[q * kRun + i] >= floor;
+      const unsigned to = WaveScan(n);
+      from[q] = listed + to - n;
+      listed += __builtin_amdgcn_readlane(to, kWave - 1);
+    }
+    if (listed <= kFew) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int start = RunStart(q, p.vocab);
+#pragma unroll
+        for (int i = 0; i < kRun; ++i)
+          if (held.key[q * kRun + i] >= floor)
+            few[wave][from[q]++] = static_cast<u64>(held.key[q * kRun + i]) << 32 |
+                                   static_cast<unsigned>(start + i);
+      }
+      // The wave's own part of LDS: its writes are done before its reads.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      Held<2> best_few;
+      best_few.used = 2;
+      int index[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u64 e = 2 * lane + i < listed ? few[wave][2 * lane + i] : 0;
+        best_few.key[i] = static_cast<unsigned>(e >> 32);
+        index[i] = static_cast<int>(e);
+        best_few.weight[i] = UnitsOf(w(best_few.key[i]), shift);
+      }
+      best_few.Select(s, w, best, shift, nullptr, &kept);
+      left = TargetOf(s.u, kept.weight);
+      need = kept.need;
+      if (DrawOf(best_few.key, best_few.weight, kept.t, &need, &left, &of, &place)) {
+        const int token = place == 0 ? index[0] : index[1];
+        if (lane == of)
+          p.tokens[row] = token;
+      }
+      return;
+    }
+  }
   if (s.greedy) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -395,42 +532,22 @@ __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shif
       held.weight[i] = UnitsOf(w(held.key[i]), shift);
     held.Select(s, w, best, shift, nullptr, &kept);
   }
-  // In the order of the row: quarters, lanes, elements.
-  u64 left = TargetOf(s.greedy ? 0.0F : s.u, kept.weight);
-  u64 need = kept.need;
+  left = TargetOf(s.greedy ? 0.0F : s.u, kept.weight);
+  need = kept.need;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
-    const auto run = [&](auto&& f) {
+    unsigned key[kRun];
+    u64 weight[kRun];
 #pragma unroll
-      for (int i = 0; i < kRun; ++i)
-        f(i, held.key[q * kRun + i], held.weight[q * kRun + i]);
-    };
-    u64 equal = 0;
-    run([&](int, unsigned key, u64) { equal += key == kept.t; });
-    const u64 equal_to = WaveScan(static_cast<unsigned>(equal));
-    u64 before = equal_to - equal, mine = 0, seen = before;
-    run([&](int, unsigned key, u64 weight) {
-      mine += key > kept.t || (key == kept.t && seen++ < need) ? weight : 0;
-    });
-    const u64 to = WaveScan(mine);
-    const u64 hit = __ballot(to > left);
-    if (hit != 0) {
-      if (lane == __builtin_ctzll(hit)) {
-        u64 at = to - mine;
-        int token = -1;
-        const int start = RunStart((q * kWave + lane) * kRun, p.vocab);
-        run([&](int i, unsigned key, u64 weight) {
-          at += key > kept.t || (key == kept.t && before++ < need) ? weight : 0;
-          if (token < 0 && at > left)
-            token = start + i;
-        });
-        p.tokens[row] = token;
-      }
+    for (int i = 0; i < kRun; ++i) {
+      key[i] = held.key[q * kRun + i];
+      weight[i] = held.weight[q * kRun + i];
+    }
+    if (DrawOf(key, weight, kept.t, &need, &left, &of, &place)) {
+      if (lane == of)
+        p.tokens[row] = RunStart(q, p.vocab) + place;
       return;
     }
-    left -= Lane64(to, kWave - 1);
-    const u64 equals = __builtin_amdgcn_readlane(static_cast<int>(equal_to), kWave - 1);
-    need -= min(need, equals);
   }
 }
 
@@ -442,9 +559,23 @@ struct Work {
   unsigned* equal;
   unsigned* most;
 };
+// What a row goes on with in the launches of its own passes, and their sums.
+struct RowState {
+  enum : unsigned { kDone, kSearch, kPick };
+  unsigned status, t;
+  u64 need;
+  unsigned counts[kList];
+  u64 weights[kList];
+};
+constexpr int kSplitRows = 256;
+__host__ __device__ constexpr std::int64_t WorkWords(std::int64_t chunks) {
+  return (chunks * (2 + 1 + kQuarters) + 3) / 4 * 4;
+}
+__device__ __forceinline__ RowState* StateOf(const SampleParams& p, int row, int chunks) {
+  return reinterpret_cast<RowState*>(p.work + WorkWords(chunks) * p.rows) + row;
+}
 __device__ __forceinline__ Work WorkOf(const SampleParams& p, int row, int chunks) {
-  const std::size_t each = static_cast<std::size_t>(chunks) * (2 + 1 + kQuarters);
-  double* const base = reinterpret_cast<double*>(p.work + (each + (each & 1)) * row);
+  double* const base = reinterpret_cast<double*>(p.work + WorkWords(chunks) * row);
   unsigned* const equal = reinterpret_cast<unsigned*>(base + chunks);
   return {base, equal, equal + chunks};
 }
@@ -454,68 +585,77 @@ __device__ __forceinline__ Work WorkOf(const SampleParams& p, int row, int chunk
 template <typename T>
 __global__ __launch_bounds__(kThreads) void ChunkKernel(SampleParams p, int chunks, int groups) {
   __shared__ double powers[kTable];
+  __builtin_assume(p.vocab > kChunk);
   FillTable(powers);
   const int lane = threadIdx.x % kWave;
   const int row = blockIdx.x / groups;
   const int chunk = (blockIdx.x - row * groups) * kWaves + threadIdx.x / kWave;
-  unsigned key[kQuarters][kRun];
+  float z[kQuarters][kRun];
   Settings s{};
   if (chunk < chunks) {
     s = SettingsOf(p, row);
 #pragma unroll
     for (int q = 0; q < kQuarters; ++q)
-      LoadKeys<T>(p, row, chunk * kChunk + (q * kWave + lane) * kRun, key[q]);
+      LoadLogits<T>(p, row, chunk * kQuarters + q, z[q]);
   }
   __syncthreads();
   if (chunk >= chunks)
     return;
   const Work work = WorkOf(p, row, chunks);
-  unsigned best = 0;
+  float best = -__builtin_inff();
+  bool lost = false;
 #pragma unroll
   for (int q = 0; q < kQuarters; ++q) {
-    unsigned most = 0;
+    float most = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < kRun; ++i)
-      most = max(most, key[q][i]);
-    most = WaveMaxKey(most);
+    for (int i = 0; i < kRun; ++i) {
+      most = fmaxf(most, z[q][i]);
+      lost |= __builtin_amdgcn_classf(z[q][i], 0x203);  // a NaN or +infinity
+    }
+    most = WaveMaxFast(most);
+    best = fmaxf(best, most);
     if (lane == 0)
-      work.most[chunk * kQuarters + q] = most;
-    best = max(best, most);
+      work.most[chunk * kQuarters + q] = KeyOf(most);
   }
-  if (!s.Whole() || best >= kKeyOfInf)
+  if (__ballot(lost) != 0) {
+    if (lane == 0)
+      work.most[chunk * kQuarters] = ~0u;
     return;
-  double sum = 0.0;
-  if (best != 0) {
-    const Weigher w = WeigherOf(powers, best, s.temperature);
+  }
+  if (!s.Whole())
+    return;
+  double sum[2] = {0.0, 0.0};
+  if (best != -__builtin_inff()) {
+    const Weigher w{powers, best, kTable * 1.4426950408889634074 / s.temperature};
 #pragma unroll
     for (int q = 0; q < kQuarters; ++q)
 #pragma unroll
       for (int i = 0; i < kRun; ++i)
-        sum += w(key[q][i]);
+        sum[i & 1] += w.Raw(z[q][i]);
   }
-  sum = WaveSum64(sum);
+  const double all = WaveSum64(sum[0] + sum[1]);
   if (lane == 0)
-    work.weight[chunk] = sum;
+    work.weight[chunk] = all;
 }
 
 struct RowShared {
   double powers[kTable];
-  u64 weights[2048];      // of a pass's bins
-  unsigned counts[2048];
+  u64 weights[kList];  // of a pass's bins; as 64-bit numbers, the chunks'
+  unsigned counts[kList];
   unsigned most[kMostQuarters];
-  u64 list[kList];        // index, key
+  u64 list[kList];     // key, index
+  u64 before[kShortList];
+  int rank[kShortList];
   u64 slots[kRowWaves];
-  double sums[kRowWaves];
-  unsigned listed;
-  Kept kept;
-  int mode;
-  unsigned t;
+  unsigned listed, t;
+  int bin;
   u64 above_weight, above_count;
 };
 
 template <typename V, typename F>
-__device__ __forceinline__ V RowJoin(V v, V* slots, F&& join) {
+__device__ __forceinline__ V RowJoin(V v, u64* scratch, F&& join) {
   // v is the same in every lane of a wave
+  V* const slots = reinterpret_cast<V*>(scratch);
   __syncthreads();
   if (threadIdx.x % kWave == 0)
     slots[threadIdx.x / kWave] = v;
@@ -526,281 +666,584 @@ __device__ __forceinline__ V RowJoin(V v, V* slots, F&& join) {
   return v;
 }
 
-// Calls f(key, index) for every element of the row, a wave a quarter.
+// What a search goes over: the row, or the list of all its keys from some key on.
+struct Source {
+  bool list;
+  int count;
+};
+
+// Calls f(key, index) for the elements, a wave a chunk of the row.
 template <typename T, typename F>
-__device__ __forceinline__ void EachKey(const SampleParams& p, int row, int quarters, F&& f) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  for (int q = wave; q < quarters; q += kRowWaves) {
-    const int d = (q * kWave + lane) * kRun;
-    unsigned key[kRun];
-    LoadKeys<T>(p, row, d, key);
-    const int start = RunStart(d, p.vocab);
+__device__ __forceinline__ void EachKey(const SampleParams& p, int row, int chunks,
+                                        const RowShared& sh, const Source& from, F&& f) {
+  if (from.list) {
+    for (int i = threadIdx.x; i < from.count; i += kRowThreads)
+      f(static_cast<unsigned>(sh.list[i] >> 32), static_cast<int>(sh.list[i]));
+    return;
+  }
+  for (int c = threadIdx.x / kWave; c < chunks; c += kRowWaves) {
+    float z[kQuarters][kRun];
 #pragma unroll
-    for (int i = 0; i < kRun; ++i)
-      f(key[i], start + i);
+    for (int q = 0; q < kQuarters; ++q)
+      LoadLogits<T>(p, row, c * kQuarters + q, z[q]);
+#pragma unroll
+    for (int q = 0; q < kQuarters; ++q) {
+      const int start = RunStart(c * kQuarters + q, p.vocab);
+#pragma unroll
+      for (int i = 0; i < kRun; ++i)
+        f(KeyOf(z[q][i]), start + i);
+    }
   }
 }
 
-// The threshold at which the keys' count (or their weight) reaches `want`, by three
-// passes over the row: sums of 2048 bins of the keys that share the bits found so far.
-// Below `floor` nothing counts. The whole work-group calls this.
-template <typename T, bool WEIGHT>
-__device__ __forceinline__ void RowSearch(const SampleParams& p, int row, int quarters,
-                                          RowShared& sh, const Weigher& w, int shift,
-                                          unsigned floor, u64 want) {
-  const int tid = threadIdx.x;
-  unsigned prefix = 0;
-  u64 above_weight = 0, above_count = 0;
-  for (int level = 0; level < 3; ++level) {
-    const int low = level == 0 ? 21 : level == 1 ? 10 : 0;
-    const int bins = level == 2 ? 1024 : 2048;
-    const int high = low + (level == 2 ? 10 : 11);  // bits of the prefix begin here
-    for (int i = tid; i < 2048; i += kRowThreads) {
-      sh.weights[i] = 0;
-      sh.counts[i] = 0;
-    }
-    __syncthreads();
-    EachKey<T>(p, row, quarters, [&](unsigned key, int) {
-      if (key >= floor && (level == 0 || key >> high == prefix >> high)) {
-        const int bin = (key >> low) & (bins - 1);
-        atomicAdd(&sh.counts[bin], 1u);
-        if constexpr (WEIGHT)
-          atomicAdd(&sh.weights[bin], UnitsOf(w(key), shift));
+// The list of the row's keys from `floor` to `high`; false where it does not hold them.
+// Quarters without any are not read. The whole work-group calls this.
+template <typename T>
+__device__ __forceinline__ bool Gather(const SampleParams& p, int row, int quarters,
+                                       RowShared& sh, const unsigned* most, unsigned floor,
+                                       unsigned high) {
+  __syncthreads();
+  if (threadIdx.x == 0)
+    sh.listed = 0;
+  __syncthreads();
+  const auto take = [&](int q, const float (&z)[kRun]) {
+    const int start = RunStart(q, p.vocab);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const unsigned key = KeyOf(z[i]);
+      if (key >= floor && key <= high) {
+        const unsigned at = atomicAdd(&sh.listed, 1u);
+        if (at < kList)
+          sh.list[at] = static_cast<u64>(key) << 32 | static_cast<unsigned>(start + i);
       }
-    });
+    }
+  };
+  // Two quarters' loads at once.
+  int held = -1;
+  for (int q = threadIdx.x / kWave; q < quarters; q += kRowWaves) {
+    if (most[q] < floor)
+      continue;
+    if (held < 0) {
+      held = q;
+      continue;
+    }
+    float z[2][kRun];
+    LoadLogits<T>(p, row, held, z[0]);
+    LoadLogits<T>(p, row, q, z[1]);
+    take(held, z[0]);
+    take(q, z[1]);
+    held = -1;
+  }
+  if (held >= 0) {
+    float z[kRun];
+    LoadLogits<T>(p, row, held, z);
+    take(held, z);
+  }
+  __syncthreads();
+  return sh.listed <= kList;
+}
+
+// 2048 equal steps of the logit from the best down to the smallest weight that counts.
+struct Steps {
+  float top, scale;
+  __device__ __forceinline__ int operator()(unsigned key) const {
+    const float at = fminf(top - LogitOf(key), 3e38F) * scale;
+    return at < static_cast<float>(kList) ? static_cast<int>(at) : kList;
+  }
+  // The smallest key of a step up to `last`; 64 keys at once.
+  __device__ __forceinline__ unsigned Least(unsigned best, int last) const {
+    unsigned low = kKeyOfMinusInf, high = best;
+    while (high - low > 1) {
+      const unsigned step = (high - low + kWave - 1) / kWave;
+      const unsigned key = min(low + step * (threadIdx.x % kWave + 1), high);
+      const int at = __builtin_ctzll(__ballot(key == high || (*this)(key) <= last));
+      high = min(low + step * (at + 1), high);
+      low += step * at;
+    }
+    return high;
+  }
+};
+__device__ __forceinline__ Steps StepsOf(const Weigher& w) {
+  return {static_cast<float>(w.top),
+          fminf(static_cast<float>(w.per * (static_cast<double>(kList) / (kOctaves * kTable))),
+                1e30F)};
+}
+
+// The key at which the count of keys (or their weight) reaches `want`, from the top: sums
+// of the logit's steps (from `state`, or a pass over the elements), then of equal ranges
+// of the keys in the step that was found, until that is one key. Where the first sums
+// leave few elements the passes go over a list, of all from that step up if it holds
+// them. Below `floor` nothing counts. The whole work-group calls this; the result is in
+// sh.t, sh.above_count and sh.above_weight.
+template <typename T, bool WEIGHT>
+__device__ __forceinline__ void RowSearch(const SampleParams& p, int row, int chunks,
+                                          int quarters, const unsigned* most, RowShared& sh,
+                                          Source* from, const RowState* state, const Weigher& w,
+                                          int shift, unsigned best, unsigned floor, u64 want) {
+  constexpr int kBins = kList;
+  const int tid = threadIdx.x, lane = tid % kWave;
+  u64 above_weight = 0, above_count = 0;
+  // The bin in which the sums of the bins (0 is the top one) reach.
+  const auto find = [&] {
     __syncthreads();
-    // The first wave sums from the top, 32 bins a lane (16 in the last pass).
     if (tid < kWave) {
-      const int each = bins / kWave, top = bins - 1 - tid * each;
+      constexpr int kEach = kBins / kWave;
       u64 weight = 0, count = 0;
-      for (int i = 0; i < each; ++i) {
-        weight += sh.weights[top - i];
-        count += sh.counts[top - i];
+      for (int i = 0; i < kEach; ++i) {
+        weight += sh.weights[lane * kEach + i];
+        count += sh.counts[lane * kEach + i];
       }
       const u64 weight_to = WaveScan(weight), count_to = WaveScan(count);
-      const u64 at = WEIGHT ? above_weight + weight_to : above_count + count_to;
-      const u64 hit = __ballot(at >= want);
-      // Fixed-point shares round up to what there is, so some lane is hit; the last one
-      // takes what rounding leaves.
-      const int owner = hit != 0 ? __builtin_ctzll(hit) : kWave - 1;
-      if (tid == owner) {
+      const u64 hit =
+          __ballot((WEIGHT ? above_weight + weight_to : above_count + count_to) >= want);
+      // The last bin takes what fewer keys or the sums' rounding leave.
+      if (lane == (hit != 0 ? __builtin_ctzll(hit) : kWave - 1)) {
         u64 aw = above_weight + weight_to - weight, ac = above_count + count_to - count;
-        int bin = top;
-        for (int i = 0; i < each - 1; ++i, --bin) {
-          const u64 next = WEIGHT ? aw + sh.weights[bin] : ac + sh.counts[bin];
-          if (next >= want)
+        int bin = lane * kEach;
+        for (int i = 0; i < kEach - 1; ++i, ++bin) {
+          if ((WEIGHT ? aw + sh.weights[bin] : ac + sh.counts[bin]) >= want)
             break;
           aw += sh.weights[bin];
           ac += sh.counts[bin];
         }
-        sh.t = prefix | static_cast<unsigned>(bin) << low;
+        sh.bin = bin;
         sh.above_weight = aw;
         sh.above_count = ac;
       }
     }
     __syncthreads();
-    prefix = sh.t;
     above_weight = sh.above_weight;
     above_count = sh.above_count;
+    return sh.bin;
+  };
+  const auto pass = [&](const Source& source, auto&& bin_of) {
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kRowThreads) {
+      sh.weights[i] = 0;
+      sh.counts[i] = 0;
+    }
+    __syncthreads();
+    EachKey<T>(p, row, chunks, sh, source, [&](unsigned key, int) {
+      const int bin = bin_of(key);
+      if (key >= floor && bin < kBins) {
+        atomicAdd(&sh.counts[bin], 1u);
+        if constexpr (WEIGHT)
+          atomicAdd(&sh.weights[bin], UnitsOf(w(key), shift));
+      }
+    });
+    return find();
+  };
+  const Steps steps = StepsOf(w);
+  int first;
+  if (state != nullptr && !from->list) {
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kRowThreads) {
+      sh.weights[i] = state->weights[i];
+      sh.counts[i] = state->counts[i];
+    }
+    first = find();
+  } else {
+    first = pass(*from, steps);
+  }
+  const unsigned held = sh.counts[first];
+  unsigned low = max(steps.Least(best, first), floor);
+  unsigned high = first == 0 ? best : steps.Least(best, first - 1) - 1;
+  Source source = *from;
+  if (!from->list && held <= kList && low < high) {
+    const bool all = above_count + held <= kList;
+    source.list = Gather<T>(p, row, quarters, sh, most, low, all ? best : high);
+    source.count = static_cast<int>(sh.listed);
+    if (all)
+      *from = source;
+  }
+  while (low < high) {
+    const int bits = 32 - __builtin_clz(high - low);
+    const int down = bits > 11 ? bits - 11 : 0;
+    const int bin = pass(source, [&](unsigned key) {
+      return key >= low && key <= high ? static_cast<int>((high - key) >> down) : kBins;
+    });
+    high -= min(static_cast<unsigned>(bin) << down, high - low);
+    low = max(low, down == 0 ? high : high - min(high, (1u << down) - 1));
+  }
+  __syncthreads();
+  if (tid == 0)
+    sh.t = high;
+  __syncthreads();
+}
+
+// The draw from a short list, whose elements are ranked by the waves, an element at a
+// time against all; false where the list does not hold the share. The whole work-group
+// calls this.
+__device__ __forceinline__ bool DrawFromList(const SampleParams& p, int row, RowShared& sh,
+                                             int listed, const Settings& s, const Weigher& w,
+                                             int shift, double all) {
+  constexpr int N = kShortList / kWave;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const bool share = s.top_p < 1.0F;
+  u64 whole = static_cast<u64>(ldexp(all, shift));
+  if (s.top_k > 0)  // few elements take finer units, where they are all that counts
+    shift = 51;
+  const int used = (listed + kWave - 1) / kWave;
+  unsigned key[N], index[N];
+  u64 weight[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = i * kWave + lane;
+    const u64 e = at < listed ? sh.list[at] : 0;
+    key[i] = static_cast<unsigned>(e >> 32);
+    index[i] = static_cast<unsigned>(e);
+    weight[i] = UnitsOf(w(key[i]), shift);
+  }
+  const auto sum = [&](auto&& value) {
+    u64 n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i >= used)
+        break;
+      n += value(i);
+    }
+    return WaveSum64(n);
+  };
+  if (share && s.top_k == 0 && sum([&](int i) { return weight[i]; }) < ShareOf(s.top_p, whole))
+    return false;
+  for (int e = wave; e < listed; e += kRowWaves) {
+    const u64 mine = sh.list[e];
+    const unsigned k = static_cast<unsigned>(mine >> 32), at = static_cast<unsigned>(mine);
+    int rank = 0;
+    u64 before = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i >= used)
+        break;
+      const bool ahead = key[i] > k || (key[i] == k && index[i] < at);
+      rank += __popcll(__ballot(ahead));
+      before += ahead ? weight[i] : 0;
+    }
+    if (share)
+      before = WaveSum64(before);
+    if (lane == 0) {
+      sh.rank[e] = rank;
+      sh.before[e] = before;
+    }
+  }
+  __syncthreads();
+  const int most = s.top_k > 0 ? s.top_k : listed;
+  if (s.top_k > 0)
+    whole = sum([&](int i) {
+      const int at = i * kWave + lane;
+      return at < listed && sh.rank[at] < most ? weight[i] : 0;
+    });
+  const u64 want = share ? ShareOf(s.top_p, whole) : kAll;
+  const double least = fmin(static_cast<double>(s.min_p), 1.0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = i * kWave + lane;
+    const int rank = at < listed ? sh.rank[at] : kList;
+    const bool in = rank < most && sh.before[min(at, kShortList - 1)] < want && w(key[i]) >= least;
+    weight[i] = in || rank == 0 ? weight[i] : 0;
+  }
+  const u64 target = TargetOf(s.u, sum([&](int i) { return weight[i]; }));
+  for (int e = wave; e < listed; e += kRowWaves) {
+    const unsigned at = static_cast<unsigned>(sh.list[e]);
+    const u64 to = sum([&](int i) { return index[i] <= at ? weight[i] : 0; });
+    const u64 to_before = sum([&](int i) { return index[i] < at ? weight[i] : 0; });
+    if (to > target && to_before <= target && lane == 0)
+      p.tokens[row] = static_cast<int>(at);
+  }
+  return true;
+}
+
+// The chunk's kept weight: above the threshold, and how many equal it. A wave's.
+template <typename T>
+__device__ __forceinline__ void KeptOfChunk(const SampleParams& p, int row, int c, unsigned t,
+                                            const Weigher& w, double* weight, unsigned* equals) {
+  double sum = 0.0;
+  unsigned equal = 0;
+  float z[kQuarters][kRun];
+#pragma unroll
+  for (int q = 0; q < kQuarters; ++q)
+    LoadLogits<T>(p, row, c * kQuarters + q, z[q]);
+#pragma unroll
+  for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const unsigned key = KeyOf(z[q][i]);
+      if (key > t)
+        sum += w(key);
+      equal += key == t;
+    }
+  sum = WaveSum64(sum);
+  const u64 n = WaveSum64(static_cast<u64>(equal));
+  if (threadIdx.x % kWave == 0) {
+    *weight = sum;
+    *equals = static_cast<unsigned>(n);
   }
 }
 
+// The draw by the chunks' kept weights: one wave finds the chunk, 64 at a time, then the
+// place in it. Without a threshold (t is 0) `all` is what is kept.
 template <typename T>
+__device__ __forceinline__ void Pick(const SampleParams& p, int row, int chunks,
+                                     const double* weights, const unsigned* equals,
+                                     const Settings& s, const Weigher& w, unsigned t, u64 need0,
+                                     double all) {
+  const int lane = threadIdx.x % kWave;
+  const bool chunked = t == 0;
+  const double each = chunked ? 0.0 : w(t);
+  // The kept weight of the lane's chunk and the equals before it, of 64 chunks with `need`
+  // equals left.
+  const auto chunk_weight = [&](int c, u64 need, u64* equal_to, u64* equal_before) {
+    const unsigned equal = c < chunks && !chunked ? equals[c] : 0;
+    *equal_to = chunked ? 0 : WaveScan(static_cast<u64>(equal));
+    *equal_before = *equal_to - equal;
+    const u64 in = need > *equal_before ? min(need - *equal_before, static_cast<u64>(equal)) : 0;
+    return (c < chunks ? weights[c] : 0.0) + static_cast<double>(in) * each;
+  };
+  const auto last_lane = [](double v) {
+    return __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, v), kWave - 1));
+  };
+  u64 need = need0, equal_to, equal_before;
+  double total = all;
+  if (!chunked) {
+    total = 0.0;
+    for (int c0 = 0; c0 < chunks; c0 += kWave) {
+      total += WaveSum64(chunk_weight(c0 + lane, need, &equal_to, &equal_before));
+      need -= min(need, Lane64(equal_to, kWave - 1));
+    }
+  }
+  double left = static_cast<double>(fminf(fmaxf(s.u, 0.0F), 1.0F)) * total;
+  if (!(left < total))
+    left = total * (1.0 - 0x1p-53);
+  need = need0;
+  bool done = false;
+  double before = 0.0;
+  int last = 0;  // the chunk; the last one that keeps any where rounding leaves none
+  double last_before = 0.0;
+  u64 last_need = 0;
+  for (int c0 = 0; c0 < chunks && !done; c0 += kWave) {
+    const double mine = chunk_weight(c0 + lane, need, &equal_to, &equal_before);
+    const double to = before + WaveScan(mine);
+    const u64 hit = __ballot(mine > 0.0 && to > left);
+    const u64 any = __ballot(mine > 0.0);
+    if (any != 0) {
+      const int l = hit != 0 ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
+      last = c0 + l;
+      last_before = __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, to - mine), l));
+      last_need = need - min(need, Lane64(equal_before, l));
+    }
+    done = hit != 0;
+    before = last_lane(to);
+    need -= min(need, Lane64(equal_to, kWave - 1));
+  }
+  left -= last_before;
+  need = last_need;
+  unsigned key[kQuarters][kRun];
+#pragma unroll
+  for (int q = 0; q < kQuarters; ++q)
+    LoadKeys<T>(p, row, last * kQuarters + q, key[q]);
+  int token = -1, most_of = -1;  // the last kept one, where rounding leaves none
+#pragma unroll
+  for (int q = 0; q < kQuarters; ++q) {
+    if (token >= 0)
+      break;
+    unsigned equal = 0;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i)
+      equal += !chunked && key[q][i] == t;
+    const unsigned equals_to = __ballot(equal != 0) != 0 ? WaveScan(equal) : 0;
+    u64 seen = equals_to - equal;
+    double to_place[kRun], mine = 0.0;
+    int end = -1;  // the lane's last kept one
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const bool in = chunked || key[q][i] > t || (key[q][i] == t && seen++ < need);
+      const double weight = in ? w(key[q][i]) : 0.0;
+      end = weight > 0.0 ? i : end;
+      mine += weight;
+      to_place[i] = mine;
+    }
+    const double to = WaveScan(mine);
+    const u64 hit = __ballot(mine > 0.0 && to > left);
+    const u64 any = __ballot(mine > 0.0);
+    int place = end;
+#pragma unroll
+    for (int i = kRun - 1; i >= 0; --i) {
+      const double before_it = i > 0 ? to_place[i - 1] : 0.0;
+      place = to_place[i] > before_it && (to - mine) + to_place[i] > left ? i : place;
+    }
+    place += RunStart(last * kQuarters + q, p.vocab);
+    if (any != 0) {
+      most_of = __builtin_amdgcn_readlane(place, hit != 0 ? __builtin_ctzll(hit)
+                                                          : 63 - __builtin_clzll(any));
+      token = hit != 0 ? most_of : -1;
+    }
+    left -= last_lane(to);
+    need -= min(need, static_cast<u64>(__builtin_amdgcn_readlane(equals_to, kWave - 1)));
+  }
+  if (lane == 0)
+    p.tokens[row] = token >= 0 ? token : most_of;
+}
+
+// kWhole: a row from the chunks' numbers to its token. Else the row's passes are launches
+// of their own: kFirst does what needs none, kSearch finds the threshold from their sums,
+// kPick draws from the chunks' kept weights.
+enum class Phase { kWhole, kFirst, kSearch, kPick };
+
+template <typename T, Phase PHASE>
 __global__ __launch_bounds__(kRowThreads) void RowKernel(SampleParams p, int chunks, int quarters,
-                                                         int row_shift) {
+                                                         int shift) {
   __shared__ RowShared sh;
+  __builtin_assume(p.vocab > kChunk);
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int row = blockIdx.x;
+  RowState* const state = PHASE == Phase::kWhole ? nullptr : StateOf(p, row, chunks);
+  if (PHASE == Phase::kSearch && state->status != RowState::kSearch)
+    return;
+  if (PHASE == Phase::kPick && state->status != RowState::kPick)
+    return;
   const Settings s = SettingsOf(p, row);
   const Work work = WorkOf(p, row, chunks);
   FillTable(sh.powers);
-  if (tid == 0)
-    sh.listed = 0;
+  // The chunks' and quarters' numbers, in LDS where they fit.
+  double* const weights =
+      chunks <= kList ? reinterpret_cast<double*>(sh.weights) : work.weight;
+  unsigned* const equals = chunks <= kList ? sh.counts : work.equal;
+  const bool ranked = quarters <= kMostQuarters;
+  const unsigned* const most = ranked ? sh.most : work.most;
+  if (PHASE == Phase::kFirst && tid == 0)
+    state->status = RowState::kDone;
 
   unsigned best = 0;
   for (int i = tid; i < quarters; i += kRowThreads) {
-    const unsigned most = work.most[i];
-    if (i < kMostQuarters)
-      sh.most[i] = most;
-    best = max(best, most);
+    const unsigned m = work.most[i];
+    if (ranked)
+      sh.most[i] = m;
+    best = max(best, m);
   }
-  best = static_cast<unsigned>(RowJoin(static_cast<u64>(WaveMaxKey(best)), sh.slots,
-                                       [](u64 a, u64 b) { return a > b ? a : b; }));
+  best = RowJoin(WaveMaxKey(best), sh.slots, [](unsigned a, unsigned b) { return max(a, b); });
   if (best == 0 || best >= kKeyOfInf || s.lost) {
     if (tid == 0)
       p.tokens[row] = -1;
     return;
   }
   if (s.greedy) {
-    u64 first = ~u64{0};
-    for (int i = tid; i < quarters && first == ~u64{0}; i += kRowThreads)
-      if (work.most[i] == best)
+    unsigned first = ~0u;
+    for (int i = tid; i < quarters && first == ~0u; i += kRowThreads)
+      if (most[i] == best)
         first = i;
-    first = WaveMinKey(static_cast<unsigned>(min(first, u64{0xFFFFFFFFu})));
-    first = RowJoin(first, sh.slots, [](u64 a, u64 b) { return min(a, b); });
+    first = RowJoin(WaveMinKey(first), sh.slots,
+                    [](unsigned a, unsigned b) { return min(a, b); });
     if (wave == 0) {
-      const int d = (static_cast<int>(first) * kWave + lane) * kRun;
       unsigned key[kRun];
-      LoadKeys<T>(p, row, d, key);
-      int token = 0x7FFFFFFF;
+      LoadKeys<T>(p, row, static_cast<int>(first), key);
+      unsigned token = ~0u;
 #pragma unroll
       for (int i = kRun - 1; i >= 0; --i)
-        token = key[i] == best ? RunStart(d, p.vocab) + i : token;
-      token = static_cast<int>(WaveMinKey(static_cast<unsigned>(token)));
+        token = key[i] == best ? RunStart(static_cast<int>(first), p.vocab) + i : token;
+      token = WaveMinKey(token);
       if (lane == 0)
-        p.tokens[row] = token;
+        p.tokens[row] = static_cast<int>(token);
     }
     return;
   }
 
   const Weigher w = WeigherOf(sh.powers, best, s.temperature);
+  if constexpr (PHASE == Phase::kPick) {
+    if (wave == 0)
+      Pick<T>(p, row, chunks, work.weight, work.equal, s, w, state->t, state->need, 0.0);
+    return;
+  }
   const bool share = s.top_p < 1.0F;
   // The whole row's weight, where the first launch left the chunks'.
   double all = 0.0;
   if (s.top_k == 0) {
     for (int i = tid; i < chunks; i += kRowThreads) {
-      const unsigned* most = work.most + i * kQuarters;
       unsigned top = 0;
-      for (int q = 0; q < kQuarters; ++q)
-        top = max(top, i * kQuarters + q < quarters ? most[q] : 0);
+      for (int q = i * kQuarters; q < min((i + 1) * kQuarters, quarters); ++q)
+        top = max(top, most[q]);
       const double sum = work.weight[i] * w(top);
-      work.weight[i] = sum;
+      weights[i] = sum;
       all += sum;
     }
-    all = RowJoin(WaveSum64(all), sh.sums, [](double a, double b) { return a + b; });
+    all = RowJoin(WaveSum64(all), sh.slots, [](double a, double b) { return a + b; });
+  }
+  if (s.top_k == 0 && !share && !(s.min_p > 0.0F)) {
+    __threadfence_block();
+    __syncthreads();
+    if (wave == 0)
+      Pick<T>(p, row, chunks, weights, equals, s, w, 0, 0, all);
+    return;
   }
 
   Kept kept{1, kAll, 0};
-  bool chunked = s.top_k == 0 && !share && !(s.min_p > 0.0F);  // the chunks' weights are it
-  const bool ranked = quarters <= kMostQuarters;
+  Source from{false, 0};
+  bool known = s.top_k == 0 && !share;  // min_p says the threshold itself
+  if (known)
+    kept.t = KeyOfShare(w, best, s.min_p);
   const int opened = s.top_k > 0 ? s.top_k : kShareOpened;
-  if (!chunked && ranked && (s.top_k > 0 || share) && opened <= kMostOpened &&
-      opened <= quarters) {
-    // The list: what reaches the last of the loudest quarters.
-    unsigned floor = 0;
-    {
-      int n = 0;
-      unsigned low = 1, high = best;
-      while (low < high) {  // every wave by itself
-        const unsigned mid = low + (high - low + 1) / 2;
-        n = 0;
-        for (int i = 0; i < quarters; i += kWave)
-          n += __popcll(__ballot(i + lane < quarters && sh.most[i + lane] >= mid));
-        if (n >= opened)
-          low = mid;
-        else
-          high = mid - 1;
-      }
-      floor = low;
-    }
-    for (int q = wave; q < quarters; q += kRowWaves) {
-      if (sh.most[q] < floor)
-        continue;
-      const int d = (q * kWave + lane) * kRun;
-      unsigned key[kRun];
-      LoadKeys<T>(p, row, d, key);
+  if (PHASE != Phase::kSearch && ranked && (known || (opened <= kMostOpened && opened <= quarters))) {
+    unsigned floor = kept.t;
+    if (!known) {
+      // What reaches the last of the loudest quarters.
+      Held<8> loud;  // of up to 262144 tokens; every wave by itself
+      loud.used = min((quarters + kWave - 1) / kWave, 8);
 #pragma unroll
-      for (int i = 0; i < kRun; ++i)
-        if (key[i] >= floor) {
-          const unsigned at = atomicAdd(&sh.listed, 1u);
-          if (at < kList)
-            sh.list[at] = static_cast<u64>(key[i]) << 32 |
-                          static_cast<unsigned>(RunStart(d, p.vocab) + i);
-        }
+      for (int i = 0; i < 8; ++i)
+        loud.key[i] = i * kWave + lane < quarters ? sh.most[i * kWave + lane] : 0;
+      floor = Held<8>::Search(1, best, [&](unsigned t) {
+        int n = loud.Count(t);
+        for (int i = 8 * kWave; i < quarters; i += kWave)
+          n += __popcll(__ballot(i + lane < quarters && sh.most[i + lane] >= t));
+        return n >= opened;
+      });
     }
-    __syncthreads();
+    const bool fits = Gather<T>(p, row, quarters, sh, most, floor, best);
     const int listed = static_cast<int>(sh.listed);
-    if (listed <= kList) {
-      if (wave == 0) {
-        constexpr int N = kList / kWave;
-        // Few elements are finer units, where the list is all that counts.
-        const int shift = s.top_k > 0 ? 51 : row_shift;
-        Held<N> held;
-        unsigned index[N];
-        held.used = (listed + kWave - 1) / kWave;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int at = i * kWave + lane;
-          const u64 e = at < listed ? sh.list[at] : 0;
-          held.key[i] = static_cast<unsigned>(e >> 32);
-          index[i] = static_cast<unsigned>(e);
-          held.weight[i] = UnitsOf(w(held.key[i]), shift);
-        }
-        const u64 whole = static_cast<u64>(ldexp(all, shift));
-        Kept k;
-        const bool done = held.Select(s, w, best, shift, s.top_k > 0 ? nullptr : &whole, &k);
-        if (lane == 0) {
-          sh.mode = done;
-          sh.kept = k;
-        }
-        if (done) {
-          // The equals that are kept are those up to some index, and so is the draw.
-          const auto up_to = [&](auto&& value) {
-            unsigned low = 0, high = p.vocab - 1;  // the first index that reaches
-            while (low < high) {
-              const unsigned mid = (low + high) / 2;
-              if (value(mid))
-                high = mid;
-              else
-                low = mid + 1;
-            }
-            return low;
-          };
-          unsigned last = p.vocab;
-          if (k.need != kAll)
-            last = up_to([&](unsigned m) {
-              u64 n = 0;
-#pragma unroll
-              for (int i = 0; i < N; ++i)
-                n += __popcll(__ballot(held.key[i] == k.t && index[i] <= m));
-              return n >= k.need;
-            });
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (!(held.key[i] > k.t || (held.key[i] == k.t && index[i] <= last)))
-              held.weight[i] = 0;
-          const u64 target = TargetOf(s.u, k.weight);
-          const unsigned token = up_to([&](unsigned m) {
-            u64 n = 0;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-              n += index[i] <= m ? held.weight[i] : 0;
-            return WaveSum64(n) > target;
-          });
-          if (lane == 0)
-            p.tokens[row] = static_cast<int>(token);
-        }
-      }
-      __syncthreads();
-      if (sh.mode)
-        return;
+    if (listed <= kShortList && DrawFromList(p, row, sh, listed, s, w, shift, all))
+      return;
+    if (fits && (known || s.top_k > 0))
+      from = Source{true, listed};
+  }
+  if (PHASE == Phase::kFirst && !from.list) {
+    // The row's passes are the next launches.
+    for (int i = tid; i < kList; i += kRowThreads) {
+      state->counts[i] = 0;
+      state->weights[i] = 0;
     }
+    if (tid == 0) {
+      state->status = known ? RowState::kPick : RowState::kSearch;
+      state->t = kept.t;
+      state->need = kept.need;
+    }
+    return;
   }
 
-  const int shift = row_shift;
-  if (!chunked) {
-    // The thresholds from passes over the row.
+  if (!known) {
+    const RowState* const sums = PHASE == Phase::kSearch ? state : nullptr;
     u64 whole = s.top_k == 0 ? static_cast<u64>(ldexp(all, shift)) : 0;
     if (s.top_k > 0) {
-      RowSearch<T, false>(p, row, quarters, sh, w, shift, 1, s.top_k);
-      if (sh.t != 0) {
-        kept.t = sh.t;
-        kept.need = s.top_k - sh.above_count;
+      RowSearch<T, false>(p, row, chunks, quarters, most, sh, &from, sums, w, shift, best, 1,
+                          s.top_k);
+      kept.t = sh.t;
+      kept.need = s.top_k - sh.above_count;  // of those that there are
+      if (share) {
+        // The weight of what top_k keeps.
+        u64 sum = 0, equal = 0;
+        EachKey<T>(p, row, chunks, sh, from, [&](unsigned key, int) {
+          if (key > kept.t)
+            sum += UnitsOf(w(key), shift);
+          equal += key == kept.t;
+        });
+        const auto add = [](u64 a, u64 b) { return a + b; };
+        whole = RowJoin(WaveSum64(sum), sh.slots, add);
+        kept.need = min(kept.need, RowJoin(WaveSum64(equal), sh.slots, add));
+        whole += kept.need * UnitsOf(w(kept.t), shift);
       }
     }
     if (share) {
-      if (s.top_k > 0) {
-        // The weight of what top_k keeps.
-        u64 sum = 0;
-        EachKey<T>(p, row, quarters, [&](unsigned key, int) {
-          sum += key > kept.t ? UnitsOf(w(key), shift) : 0;
-        });
-        whole = RowJoin(WaveSum64(sum), sh.slots, [](u64 a, u64 b) { return a + b; }) +
-                kept.need * UnitsOf(w(kept.t), shift);
-      }
       const u64 want = ShareOf(s.top_p, whole);
-      __syncthreads();
-      RowSearch<T, true>(p, row, quarters, sh, w, shift, kept.t, want);
+      RowSearch<T, true>(p, row, chunks, quarters, most, sh, &from, sums, w, shift, best, kept.t,
+                         want);
       const u64 each = UnitsOf(w(sh.t), shift);
       const u64 need = each > 0 && want > sh.above_weight
                            ? (want - sh.above_weight + each - 1) / each
@@ -815,125 +1258,128 @@ __global__ __launch_bounds__(kRowThreads) void RowKernel(SampleParams p, int chu
         kept.need = kAll;
       }
     }
-    // The chunks' kept weights: above the threshold, and how many equal it.
-    __syncthreads();
-    for (int c = wave; c < chunks; c += kRowWaves) {
-      double sum = 0.0;
-      unsigned equal = 0;
-      for (int q = 0; q < kQuarters; ++q) {
-        if (work.most[c * kQuarters + q] < kept.t)
-          continue;
-        unsigned key[kRun];
-        LoadKeys<T>(p, row, c * kChunk + (q * kWave + lane) * kRun, key);
-#pragma unroll
-        for (int i = 0; i < kRun; ++i) {
-          if (key[i] > kept.t)
-            sum += w(key[i]);
-          equal += key[i] == kept.t;
-        }
-      }
-      sum = WaveSum64(sum);
-      const u64 equals = WaveSum64(static_cast<u64>(equal));
-      if (lane == 0) {
-        work.weight[c] = sum;
-        work.equal[c] = static_cast<unsigned>(equals);
-      }
-    }
   }
+  // The chunks' kept weights.
+  __syncthreads();
+  if (from.list && chunks <= kList) {
+    for (int i = tid; i < chunks; i += kRowThreads) {
+      sh.weights[i] = 0;
+      equals[i] = 0;
+    }
+    __syncthreads();
+    EachKey<T>(p, row, chunks, sh, from, [&](unsigned key, int index) {
+      if (key > kept.t)
+        atomicAdd(&sh.weights[index / kChunk], UnitsOf(w(key), shift));
+      else if (key == kept.t)
+        atomicAdd(&equals[index / kChunk], 1u);
+    });
+    __syncthreads();
+    for (int i = tid; i < chunks; i += kRowThreads)
+      weights[i] = ldexp(static_cast<double>(sh.weights[i]), -shift);
+  } else if (PHASE == Phase::kSearch) {
+    if (tid == 0) {
+      state->status = RowState::kPick;
+      state->t = kept.t;
+      state->need = kept.need;
+    }
+    return;
+  } else {
+    for (int c = wave; c < chunks; c += kRowWaves)
+      KeptOfChunk<T>(p, row, c, kept.t, w, weights + c, equals + c);
+  }
+  if (PHASE == Phase::kSearch && tid == 0)
+    state->status = RowState::kDone;
   __threadfence_block();
   __syncthreads();
-  if (wave != 0)
+  if (wave == 0)
+    Pick<T>(p, row, chunks, weights, equals, s, w, kept.t, kept.need, 0.0);
+}
+
+// The best key of a row, by one wave.
+__device__ __forceinline__ unsigned BestOf(const Work& work, int quarters) {
+  unsigned best = 0;
+  for (int i = threadIdx.x % kWave; i < quarters; i += kWave)
+    best = max(best, work.most[i]);
+  return WaveMaxKey(best);
+}
+
+// The sums of the logit's steps of the rows that search a threshold.
+constexpr int kStepChunks = 8;  // of a work-group
+template <typename T>
+__global__ __launch_bounds__(kThreads) void StepKernel(SampleParams p, int chunks, int quarters,
+                                                       int shift, int groups) {
+  __shared__ double powers[kTable];
+  __shared__ unsigned counts[kList];
+  __shared__ u64 weights[kList];
+  __builtin_assume(p.vocab > kChunk);
+  const int row = blockIdx.x / groups;
+  RowState* const state = StateOf(p, row, chunks);
+  if (state->status != RowState::kSearch)
     return;
-  // The first wave finds the chunk, 64 at a time, then the place in it.
-  const double each = chunked ? 0.0 : w(kept.t);
-  u64 need = chunked ? 0 : kept.need;
-  const auto chunk_weight = [&](int c, u64* equal_before) {
-    // Of chunk c (lanes' own, neighbouring ones), with the equals kept before it.
-    const bool there = c < chunks;
-    const unsigned equal = there && !chunked ? work.equal[c] : 0;
-    const u64 to = WaveScan(static_cast<u64>(equal));
-    *equal_before = to;
-    const u64 before = to - equal;
-    const u64 kept_equal = need > before ? min(need - before, static_cast<u64>(equal)) : 0;
-    return (there ? work.weight[c] : 0.0) + static_cast<double>(kept_equal) * each;
-  };
-  double total = 0.0;
-  for (int c0 = 0; c0 < chunks; c0 += kWave) {
-    u64 equal_to;
-    total += WaveSum64(chunk_weight(c0 + lane, &equal_to));
-    need -= min(need, Lane64(equal_to, kWave - 1));
+  const Settings s = SettingsOf(p, row);
+  const unsigned best = BestOf(WorkOf(p, row, chunks), quarters);
+  FillTable(powers);
+  for (int i = threadIdx.x; i < kList; i += kThreads) {
+    counts[i] = 0;
+    weights[i] = 0;
   }
-  const double u = fminf(fmaxf(s.u, 0.0F), 1.0F);
-  double left = u * total;
-  if (!(left < total))
-    left = total * (1.0 - 0x1p-53);
-  need = chunked ? 0 : kept.need;
-  bool done = false;
-  double before = 0.0;
-  int last = 0;  // the chunk; the last one that keeps any where rounding leaves none
-  double last_before = 0.0;
-  u64 last_need = 0;
-  for (int c0 = 0; c0 < chunks && !done; c0 += kWave) {
-    u64 equal_to;
-    const double mine = chunk_weight(c0 + lane, &equal_to);
-    const double to = before + WaveScan(mine);
-    const u64 hit = __ballot(mine > 0.0 && to > left);
-    const u64 any = __ballot(mine > 0.0);
-    const u64 equal_before =
-        equal_to - (c0 + lane < chunks && !chunked ? work.equal[c0 + lane] : 0);
-    if (any != 0) {
-      const int l = hit != 0 ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
-      last = c0 + l;
-      last_before = __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, to - mine), l));
-      last_need = need - min(need, Lane64(equal_before, l));
-    }
-    done = hit != 0;
-    before = __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, to), kWave - 1));
-    need -= min(need, Lane64(equal_to, kWave - 1));
+  __syncthreads();
+  const Weigher w = WeigherOf(powers, best, s.temperature);
+  const Steps steps = StepsOf(w);
+  const bool share = s.top_p < 1.0F;
+  const int first = (blockIdx.x - row * groups) * kStepChunks;
+  const int last = min(first + kStepChunks, chunks);
+  for (int c = first + static_cast<int>(threadIdx.x / kWave); c < last; c += kWaves) {
+    float z[kQuarters][kRun];
+#pragma unroll
+    for (int q = 0; q < kQuarters; ++q)
+      LoadLogits<T>(p, row, c * kQuarters + q, z[q]);
+#pragma unroll
+    for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        const unsigned key = KeyOf(z[q][i]);
+        const int step = steps(key);
+        if (key != 0 && step < kList) {
+          atomicAdd(&counts[step], 1u);
+          if (share)
+            atomicAdd(&weights[step], UnitsOf(w(key), shift));
+        }
+      }
   }
-  left -= last_before;
-  need = last_need;
-  int token = -1, most = -1;  // the last kept one, where rounding leaves none
-  for (int q = 0; q < kQuarters && token < 0; ++q) {
-    const int d = last * kChunk + (q * kWave + lane) * kRun;
-    unsigned key[kRun];
-    LoadKeys<T>(p, row, d, key);
-    unsigned equal = 0;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i)
-      equal += !chunked && key[i] == kept.t;
-    const unsigned equal_to = WaveScan(equal);
-    u64 seen = equal_to - equal;
-    double weight[kRun], mine = 0.0;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      const bool in = chunked || key[i] > kept.t || (key[i] == kept.t && seen++ < need);
-      weight[i] = in ? w(key[i]) : 0.0;
-      mine += weight[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kList; i += kThreads)
+    if (counts[i] != 0) {
+      atomicAdd(&state->counts[i], counts[i]);
+      if (share)
+        atomicAdd(&state->weights[i], weights[i]);
     }
-    const double to = WaveScan(mine);
-    const u64 hit = __ballot(mine > 0.0 && to > left);
-    const u64 any = __ballot(mine > 0.0);
-    const int owner = hit != 0 ? __builtin_ctzll(hit) : any != 0 ? 63 - __builtin_clzll(any) : -1;
-    int place = -1, end = -1;
-    double sum = to - mine;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      sum += weight[i];
-      end = weight[i] > 0.0 ? i : end;
-      place = place < 0 && weight[i] > 0.0 && sum > left ? i : place;
-    }
-    place = RunStart(d, p.vocab) + (place < 0 ? end : place);
-    if (owner >= 0) {
-      most = __builtin_amdgcn_readlane(place, owner);
-      if (hit != 0)
-        token = most;
-    }
-    left -= __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, to), kWave - 1));
-    need -= min(need, static_cast<u64>(__builtin_amdgcn_readlane(equal_to, kWave - 1)));
-  }
-  if (lane == 0)
-    p.tokens[row] = token >= 0 ? token : most;
+}
+
+// The chunks' kept weights of the rows that have their threshold.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void KeptKernel(SampleParams p, int chunks, int quarters,
+                                                       int groups) {
+  __shared__ double powers[kTable];
+  __builtin_assume(p.vocab > kChunk);
+  const int row = blockIdx.x / groups;
+  const RowState* const state = StateOf(p, row, chunks);
+  if (state->status != RowState::kPick)
+    return;
+  const Settings s = SettingsOf(p, row);
+  const Work work = WorkOf(p, row, chunks);
+  FillTable(powers);
+  __syncthreads();
+  const int c = (blockIdx.x - row * groups) * kWaves + threadIdx.x / kWave;
+  if (c < chunks)
+    KeptOfChunk<T>(p, row, c, state->t, WeigherOf(powers, BestOf(work, quarters), s.temperature),
+                   work.weight + c, work.equal + c);
+}
+
+// Whether the rows' passes are launches of their own: where the rows do not fill the
+// device by themselves.
+bool SplitRows(std::int64_t rows, std::int64_t chunks) {
+  return rows <= kSplitRows && chunks <= kList;
 }
 
 int ChunksOf(int vocab) { return vocab <= kChunk ? 0 : (vocab - 1) / kChunk + 1; }
@@ -941,9 +1387,11 @@ int ChunksOf(int vocab) { return vocab <= kChunk ? 0 : (vocab - 1) / kChunk + 1;
 }  // namespace
 
 std::int64_t SampleWorkBytes(std::int64_t rows, std::int64_t vocab) {
-  std::int64_t each = ChunksOf(static_cast<int>(vocab)) * std::int64_t{2 + 1 + kQuarters};
-  each += each & 1;
-  return rows * each * static_cast<std::int64_t>(sizeof(unsigned));
+  const std::int64_t chunks = ChunksOf(static_cast<int>(vocab));
+  if (chunks == 0)
+    return 0;
+  return rows * (WorkWords(chunks) * static_cast<std::int64_t>(sizeof(unsigned)) +
+                 (SplitRows(rows, chunks) ? static_cast<std::int64_t>(sizeof(RowState)) : 0));
 }
 
 void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
@@ -966,13 +1414,33 @@ void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
       small(std::integral_constant<int, 1>());
     } else if (quarters == 2) {
       small(std::integral_constant<int, 2>());
+    } else if (quarters == 3) {
+      small(std::integral_constant<int, 3>());
     } else if (quarters <= kQuarters && chunks == 0) {
       small(std::integral_constant<int, kQuarters>());
     } else {
+      // A row may need a threshold where any setting may ask for one.
+      const bool filtered = p.top_ks != nullptr || p.top_ps != nullptr || p.min_ps != nullptr ||
+                            p.top_k > 0 || p.top_p < 1.0F || p.min_p > 0.0F;
+      const bool split = filtered && SplitRows(p.rows, chunks);
       Dispatch(ChunkKernel<T>, dim3(p.rows * groups), dim3(kThreads), 0, stream, true, false, p,
                chunks, groups);
-      Dispatch(RowKernel<T>, dim3(p.rows), dim3(kRowThreads), 0, stream, false, true, p, chunks,
-               quarters, shift);
+      const auto rows = [&](auto kernel, bool last) {
+        Dispatch(kernel, dim3(p.rows), dim3(kRowThreads), 0, stream, false, last, p, chunks,
+                 quarters, shift);
+      };
+      if (!split) {
+        rows(RowKernel<T, Phase::kWhole>, true);
+      } else {
+        const int step_groups = (chunks + kStepChunks - 1) / kStepChunks;
+        rows(RowKernel<T, Phase::kFirst>, false);
+        Dispatch(StepKernel<T>, dim3(p.rows * step_groups), dim3(kThreads), 0, stream, false,
+                 false, p, chunks, quarters, shift, step_groups);
+        rows(RowKernel<T, Phase::kSearch>, false);
+        Dispatch(KeptKernel<T>, dim3(p.rows * groups), dim3(kThreads), 0, stream, false, false, p,
+                 chunks, quarters, groups);
+        rows(RowKernel<T, Phase::kPick>, true);
+      }
     }
   });
   Check(hipGetLastError(), "sample launch");
