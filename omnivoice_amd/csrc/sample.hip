@@ -40,7 +40,7 @@ constexpr int kQuarters = 4;
 constexpr int kChunk = kQuarter * kQuarters;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kRowThreads = 512;            // of a row's work-group in the second launch
+constexpr int kRowThreads = 1024;           // of a row's work-group in the second launch
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kMostQuarters = 2048;         // that are ranked
 constexpr int kMostOpened = 256;            // quarters that are read for a list
@@ -247,6 +247,11 @@ struct Settings {
   int top_k;  // 0: all
   bool lost, greedy;
   __device__ __forceinline__ bool Whole() const { return !greedy && top_k == 0; }
+  // Whether the sums of the row's steps may be asked for.
+  __device__ __forceinline__ bool Searches(int quarters) const {
+    return !lost && !greedy &&
+           (top_k > min(kMostOpened, quarters) || (top_k == 0 && top_p < 1.0F));
+  }
 };
 __device__ __forceinline__ Settings SettingsOf(const SampleParams& p, int row) {
   Settings s;
@@ -562,7 +567,7 @@ struct Work {
 // What a row goes on with in the launches of its own passes, and their sums.
 struct RowState {
   enum : unsigned { kDone, kSearch, kPick };
-  unsigned status, t;
+  unsigned status, t, best, spare;
   u64 need;
   unsigned counts[kList];
   u64 weights[kList];
@@ -583,7 +588,8 @@ __device__ __forceinline__ Work WorkOf(const SampleParams& p, int row, int chunk
 // The largest key of every quarter of a chunk, and the chunk's weight beside the
 // chunk's own largest.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void ChunkKernel(SampleParams p, int chunks, int groups) {
+__global__ __launch_bounds__(kThreads) void ChunkKernel(SampleParams p, int chunks, int groups,
+                                                        bool split) {
   __shared__ double powers[kTable];
   __builtin_assume(p.vocab > kChunk);
   FillTable(powers);
@@ -597,6 +603,14 @@ __global__ __launch_bounds__(kThreads) void ChunkKernel(SampleParams p, int chun
 #pragma unroll
     for (int q = 0; q < kQuarters; ++q)
       LoadLogits<T>(p, row, chunk * kQuarters + q, z[q]);
+  }
+  if (split && s.Searches((p.vocab - 1) / kQuarter + 1)) {  // the sums that the next launch adds to
+    RowState* const state = StateOf(p, row, chunks);
+    const int part = blockIdx.x - row * groups;
+    for (int i = part * kThreads + threadIdx.x; i < kList; i += groups * kThreads) {
+      state->counts[i] = 0;
+      state->weights[i] = 0;
+    }
   }
   __syncthreads();
   if (chunk >= chunks)
@@ -644,24 +658,27 @@ struct RowShared {
   unsigned counts[kList];
   unsigned most[kMostQuarters];
   u64 list[kList];     // key, index
+  unsigned short open[kMostQuarters];
+  u64 unit[kShortList];    // the list's weights
   u64 before[kShortList];
   int rank[kShortList];
-  u64 slots[kRowWaves];
-  unsigned listed, t;
+  u64 slots[kRowWaves], count_slots[kRowWaves];
+  unsigned listed, opened, t;
   int bin;
   u64 above_weight, above_count;
 };
 
-template <typename V, typename F>
+// v is the same in every lane of a wave.
+template <int WAVES = kRowWaves, typename V, typename F>
 __device__ __forceinline__ V RowJoin(V v, u64* scratch, F&& join) {
-  // v is the same in every lane of a wave
   V* const slots = reinterpret_cast<V*>(scratch);
   __syncthreads();
   if (threadIdx.x % kWave == 0)
     slots[threadIdx.x / kWave] = v;
   __syncthreads();
   v = slots[0];
-  for (int i = 1; i < kRowWaves; ++i)
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i)
     v = join(v, slots[i]);
   return v;
 }
@@ -702,44 +719,47 @@ template <typename T>
 __device__ __forceinline__ bool Gather(const SampleParams& p, int row, int quarters,
                                        RowShared& sh, const unsigned* most, unsigned floor,
                                        unsigned high) {
+  constexpr int kAtOnce = 4;  // quarters' loads of a wave
+  const int wave = threadIdx.x / kWave;
   __syncthreads();
   if (threadIdx.x == 0)
     sh.listed = 0;
-  __syncthreads();
-  const auto take = [&](int q, const float (&z)[kRun]) {
-    const int start = RunStart(q, p.vocab);
+  for (int first = 0; first < quarters; first += kMostQuarters) {
+    if (threadIdx.x == 0)
+      sh.opened = 0;
+    __syncthreads();
+    const int count = min(quarters - first, kMostQuarters);
+    for (int q = threadIdx.x; q < count; q += kRowThreads)
+      if (most[first + q] >= floor)
+        sh.open[atomicAdd(&sh.opened, 1u)] = static_cast<unsigned short>(q);
+    __syncthreads();
+    const int opened = static_cast<int>(sh.opened);
+    for (int o = wave; o < opened; o += kAtOnce * kRowWaves) {
+      float z[kAtOnce][kRun];
+      int q[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      const unsigned key = KeyOf(z[i]);
-      if (key >= floor && key <= high) {
-        const unsigned at = atomicAdd(&sh.listed, 1u);
-        if (at < kList)
-          sh.list[at] = static_cast<u64>(key) << 32 | static_cast<unsigned>(start + i);
+      for (int i = 0; i < kAtOnce; ++i) {
+        q[i] = first + sh.open[min(o + i * kRowWaves, opened - 1)];
+        LoadLogits<T>(p, row, q[i], z[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (o + i * kRowWaves >= opened)
+          break;
+        const int start = RunStart(q[i], p.vocab);
+#pragma unroll
+        for (int e = 0; e < kRun; ++e) {
+          const unsigned key = KeyOf(z[i][e]);
+          if (key >= floor && key <= high) {
+            const unsigned at = atomicAdd(&sh.listed, 1u);
+            if (at < kList)
+              sh.list[at] = static_cast<u64>(key) << 32 | static_cast<unsigned>(start + e);
+          }
+        }
       }
     }
-  };
-  // Two quarters' loads at once.
-  int held = -1;
-  for (int q = threadIdx.x / kWave; q < quarters; q += kRowWaves) {
-    if (most[q] < floor)
-      continue;
-    if (held < 0) {
-      held = q;
-      continue;
-    }
-    float z[2][kRun];
-    LoadLogits<T>(p, row, held, z[0]);
-    LoadLogits<T>(p, row, q, z[1]);
-    take(held, z[0]);
-    take(q, z[1]);
-    held = -1;
+    __syncthreads();
   }
-  if (held >= 0) {
-    float z[kRun];
-    LoadLogits<T>(p, row, held, z);
-    take(held, z);
-  }
-  __syncthreads();
   return sh.listed <= kList;
 }
 
@@ -783,33 +803,35 @@ __device__ __forceinline__ void RowSearch(const SampleParams& p, int row, int ch
   constexpr int kBins = kList;
   const int tid = threadIdx.x, lane = tid % kWave;
   u64 above_weight = 0, above_count = 0;
-  // The bin in which the sums of the bins (0 is the top one) reach.
+  // The bin in which the sums of the bins (0 is the top one) reach: two bins a thread.
   const auto find = [&] {
+    static_assert(kBins == 2 * kRowThreads, "two bins a thread");
     __syncthreads();
-    if (tid < kWave) {
-      constexpr int kEach = kBins / kWave;
-      u64 weight = 0, count = 0;
-      for (int i = 0; i < kEach; ++i) {
-        weight += sh.weights[lane * kEach + i];
-        count += sh.counts[lane * kEach + i];
-      }
-      const u64 weight_to = WaveScan(weight), count_to = WaveScan(count);
-      const u64 hit =
-          __ballot((WEIGHT ? above_weight + weight_to : above_count + count_to) >= want);
-      // The last bin takes what fewer keys or the sums' rounding leave.
-      if (lane == (hit != 0 ? __builtin_ctzll(hit) : kWave - 1)) {
-        u64 aw = above_weight + weight_to - weight, ac = above_count + count_to - count;
-        int bin = lane * kEach;
-        for (int i = 0; i < kEach - 1; ++i, ++bin) {
-          if ((WEIGHT ? aw + sh.weights[bin] : ac + sh.counts[bin]) >= want)
-            break;
-          aw += sh.weights[bin];
-          ac += sh.counts[bin];
-        }
-        sh.bin = bin;
-        sh.above_weight = aw;
-        sh.above_count = ac;
-      }
+    const u64 w0 = sh.weights[2 * tid], w1 = sh.weights[2 * tid + 1];
+    const unsigned c0 = sh.counts[2 * tid], c1 = sh.counts[2 * tid + 1];
+    u64 weight_to = WaveScan(w0 + w1);
+    u64 count_to = WaveScan(static_cast<unsigned>(c0 + c1));
+    if (lane == kWave - 1) {
+      sh.slots[tid / kWave] = weight_to;
+      sh.count_slots[tid / kWave] = count_to;
+    }
+    __syncthreads();
+    weight_to += above_weight;
+    count_to += above_count;
+#pragma unroll
+    for (int i = 0; i < kRowWaves; ++i) {
+      const bool before = i < tid / kWave;
+      weight_to += before ? sh.slots[i] : 0;
+      count_to += before ? sh.count_slots[i] : 0;
+    }
+    const u64 weight = weight_to - w0 - w1, count = count_to - c0 - c1;
+    const u64 to = WEIGHT ? weight_to : count_to, from_here = WEIGHT ? weight : count;
+    // The last bin takes what fewer keys or the sums' rounding leave.
+    if ((to >= want && (from_here < want || tid == 0)) || (tid == kRowThreads - 1 && to < want)) {
+      const bool second = (WEIGHT ? weight + w0 : count + c0) < want;
+      sh.bin = 2 * tid + second;
+      sh.above_weight = weight + (second ? w0 : 0);
+      sh.above_count = count + (second ? c0 : 0);
     }
     __syncthreads();
     above_weight = sh.above_weight;
@@ -871,85 +893,79 @@ __device__ __forceinline__ void RowSearch(const SampleParams& p, int row, int ch
   __syncthreads();
 }
 
-// The draw from a short list, whose elements are ranked by the waves, an element at a
-// time against all; false where the list does not hold the share. The whole work-group
-// calls this.
+// For every element of a list, what `ahead` of it others count and weigh, added to
+// sh.rank and sh.before: a wave has 64 elements and a part of the others.
+template <typename F>
+__device__ __forceinline__ void RankList(RowShared& sh, int listed, F&& ahead) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int groups = (listed + kWave - 1) / kWave, parts = kRowWaves / groups;
+  const int part = wave / groups, e = wave % groups * kWave + lane;
+  if (part >= parts)
+    return;
+  const u64 mine = sh.list[min(e, listed - 1)];
+  int rank = 0;
+  u64 before = 0;
+  for (int i = part; i < listed; i += parts) {
+    const bool in = ahead(sh.list[i], mine);
+    rank += in;
+    before += in ? sh.unit[i] : 0;
+  }
+  if (e < listed) {
+    atomicAdd(&sh.rank[e], rank);
+    atomicAdd(&sh.before[e], before);
+  }
+}
+
+// The draw from a short list, an element a thread; false where the list does not hold the
+// share. The whole work-group calls this.
 __device__ __forceinline__ bool DrawFromList(const SampleParams& p, int row, RowShared& sh,
                                              int listed, const Settings& s, const Weigher& w,
                                              int shift, double all) {
-  constexpr int N = kShortList / kWave;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const bool share = s.top_p < 1.0F;
+  static_assert(kShortList <= kRowThreads && kShortList <= kRowWaves * kWave, "elements");
+  const int e = threadIdx.x;
+  const bool there = e < listed, share = s.top_p < 1.0F;
+  const auto total = [&](u64 v) {
+    return RowJoin(WaveSum64(v), sh.slots, [](u64 a, u64 b) { return a + b; });
+  };
   u64 whole = static_cast<u64>(ldexp(all, shift));
   if (s.top_k > 0)  // few elements take finer units, where they are all that counts
     shift = 51;
-  const int used = (listed + kWave - 1) / kWave;
-  unsigned key[N], index[N];
-  u64 weight[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int at = i * kWave + lane;
-    const u64 e = at < listed ? sh.list[at] : 0;
-    key[i] = static_cast<unsigned>(e >> 32);
-    index[i] = static_cast<unsigned>(e);
-    weight[i] = UnitsOf(w(key[i]), shift);
-  }
-  const auto sum = [&](auto&& value) {
-    u64 n = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (i >= used)
-        break;
-      n += value(i);
-    }
-    return WaveSum64(n);
-  };
-  if (share && s.top_k == 0 && sum([&](int i) { return weight[i]; }) < ShareOf(s.top_p, whole))
+  const u64 element = there ? sh.list[e] : 0;
+  const double weight = w(static_cast<unsigned>(element >> 32));
+  const u64 unit = UnitsOf(weight, shift);
+  if (share && s.top_k == 0 && total(unit) < ShareOf(s.top_p, whole))
     return false;
-  for (int e = wave; e < listed; e += kRowWaves) {
-    const u64 mine = sh.list[e];
-    const unsigned k = static_cast<unsigned>(mine >> 32), at = static_cast<unsigned>(mine);
-    int rank = 0;
-    u64 before = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (i >= used)
-        break;
-      const bool ahead = key[i] > k || (key[i] == k && index[i] < at);
-      rank += __popcll(__ballot(ahead));
-      before += ahead ? weight[i] : 0;
-    }
-    if (share)
-      before = WaveSum64(before);
-    if (lane == 0) {
-      sh.rank[e] = rank;
-      sh.before[e] = before;
-    }
+  if (e < kShortList) {
+    sh.unit[e] = unit;
+    sh.rank[e] = 0;
+    sh.before[e] = 0;
   }
   __syncthreads();
+  // Ahead are larger keys and equal ones of smaller index.
+  RankList(sh, listed, [](u64 other, u64 mine) {
+    return (other ^ 0xFFFFFFFFu) > (mine ^ 0xFFFFFFFFu);
+  });
+  __syncthreads();
+  const int rank = there ? sh.rank[e] : kList;
+  const u64 before = there ? sh.before[e] : 0;
   const int most = s.top_k > 0 ? s.top_k : listed;
-  if (s.top_k > 0)
-    whole = sum([&](int i) {
-      const int at = i * kWave + lane;
-      return at < listed && sh.rank[at] < most ? weight[i] : 0;
-    });
-  const u64 want = share ? ShareOf(s.top_p, whole) : kAll;
+  if (s.top_k > 0 && share)
+    whole = total(rank < most ? unit : 0);
   const double least = fmin(static_cast<double>(s.min_p), 1.0);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int at = i * kWave + lane;
-    const int rank = at < listed ? sh.rank[at] : kList;
-    const bool in = rank < most && sh.before[min(at, kShortList - 1)] < want && w(key[i]) >= least;
-    weight[i] = in || rank == 0 ? weight[i] : 0;
+  const bool in = rank < most && (!share || before < ShareOf(s.top_p, whole)) && weight >= least;
+  const u64 kept = in || rank == 0 ? unit : 0;
+  const u64 target = TargetOf(s.u, total(kept));
+  if (there) {
+    sh.unit[e] = kept;
+    sh.before[e] = 0;
   }
-  const u64 target = TargetOf(s.u, sum([&](int i) { return weight[i]; }));
-  for (int e = wave; e < listed; e += kRowWaves) {
-    const unsigned at = static_cast<unsigned>(sh.list[e]);
-    const u64 to = sum([&](int i) { return index[i] <= at ? weight[i] : 0; });
-    const u64 to_before = sum([&](int i) { return index[i] < at ? weight[i] : 0; });
-    if (to > target && to_before <= target && lane == 0)
-      p.tokens[row] = static_cast<int>(at);
-  }
+  __syncthreads();
+  RankList(sh, listed, [](u64 other, u64 mine) {
+    return static_cast<unsigned>(other) < static_cast<unsigned>(mine);
+  });
+  __syncthreads();
+  if (there && sh.before[e] <= target && target < sh.before[e] + kept)
+    p.tokens[row] = static_cast<int>(element);
   return true;
 }
 
@@ -1084,19 +1100,84 @@ __device__ __forceinline__ void Pick(const SampleParams& p, int row, int chunks,
     p.tokens[row] = token >= 0 ? token : most_of;
 }
 
-// kWhole: a row from the chunks' numbers to its token. Else the row's passes are launches
-// of their own: kFirst does what needs none, kSearch finds the threshold from their sums,
-// kPick draws from the chunks' kept weights.
-enum class Phase { kWhole, kFirst, kSearch, kPick };
+// The sums of the logit's steps of `row`'s chunks from `first` on, by a work-group.
+constexpr int kStepChunks = 16;  // of a work-group
+template <typename T>
+__device__ __forceinline__ void AddSteps(const SampleParams& p, int row, int chunks, int quarters,
+                                         int shift, int first, const Settings& s, RowShared& sh) {
+  RowState* const state = StateOf(p, row, chunks);
+  const Work work = WorkOf(p, row, chunks);
+  unsigned best = 0;
+  for (int i = threadIdx.x; i < quarters; i += kRowThreads)
+    best = max(best, work.most[i]);
+  for (int i = threadIdx.x; i < kList; i += kRowThreads) {
+    sh.counts[i] = 0;
+    sh.weights[i] = 0;
+  }
+  best = RowJoin(WaveMaxKey(best), sh.slots, [](unsigned a, unsigned b) { return max(a, b); });
+  if (best == 0 || best >= kKeyOfInf)
+    return;
+  const Weigher w = WeigherOf(sh.powers, best, s.temperature);
+  const Steps steps = StepsOf(w);
+  const bool share = s.top_p < 1.0F;
+  const int c = first + static_cast<int>(threadIdx.x / kWave);
+  static_assert(kStepChunks == kRowWaves, "a wave a chunk");
+  if (c < chunks) {
+    float z[kQuarters][kRun];
+#pragma unroll
+    for (int q = 0; q < kQuarters; ++q)
+      LoadLogits<T>(p, row, c * kQuarters + q, z[q]);
+#pragma unroll
+    for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        const unsigned key = KeyOf(z[q][i]);
+        const int step = steps(key);
+        if (key != 0 && step < kList) {
+          atomicAdd(&sh.counts[step], 1u);
+          if (share)
+            atomicAdd(&sh.weights[step], UnitsOf(w(key), shift));
+        }
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kList; i += kRowThreads)
+    if (sh.counts[i] != 0) {
+      atomicAdd(&state->counts[i], sh.counts[i]);
+      if (share)
+        atomicAdd(&state->weights[i], sh.weights[i]);
+    }
+}
+
+// kWhole: a row from the chunks' numbers to its token. Else the row's passes are spread
+// over work-groups and launches of their own: kFirst does what needs none, while other
+// work-groups sum the steps of rows that may search, kSearch finds the threshold from
+// the sums, kPick draws from the chunks' kept weights.
+// kPlain: rows of which none has a filter.
+enum class Phase { kPlain, kWhole, kFirst, kSearch, kPick };
+constexpr int ThreadsOf(Phase phase) {
+  return phase == Phase::kPlain ? kThreads : phase == Phase::kPick ? kWave : kRowThreads;
+}
 
 template <typename T, Phase PHASE>
-__global__ __launch_bounds__(kRowThreads) void RowKernel(SampleParams p, int chunks, int quarters,
+__global__ __launch_bounds__(ThreadsOf(PHASE)) void RowKernel(SampleParams p, int chunks, int quarters,
                                                          int shift) {
   __shared__ RowShared sh;
   __builtin_assume(p.vocab > kChunk);
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int row = blockIdx.x;
-  RowState* const state = PHASE == Phase::kWhole ? nullptr : StateOf(p, row, chunks);
+  const int row = blockIdx.x % p.rows;
+  if (PHASE == Phase::kFirst && static_cast<int>(blockIdx.x) >= p.rows) {
+    const Settings s = SettingsOf(p, row);
+    if (!s.Searches(quarters))
+      return;
+    FillTable(sh.powers);
+    AddSteps<T>(p, row, chunks, quarters, shift,
+                (static_cast<int>(blockIdx.x) / p.rows - 1) * kStepChunks, s, sh);
+    return;
+  }
+  constexpr int kGroup = ThreadsOf(PHASE), kGroupWaves = kGroup / kWave;
+  constexpr bool kOwn = PHASE == Phase::kPlain || PHASE == Phase::kWhole;
+  RowState* const state = kOwn ? nullptr : StateOf(p, row, chunks);
   if (PHASE == Phase::kSearch && state->status != RowState::kSearch)
     return;
   if (PHASE == Phase::kPick && state->status != RowState::kPick)
@@ -1113,14 +1194,21 @@ __global__ __launch_bounds__(kRowThreads) void RowKernel(SampleParams p, int chu
   if (PHASE == Phase::kFirst && tid == 0)
     state->status = RowState::kDone;
 
+  if constexpr (PHASE == Phase::kPick) {
+    __syncthreads();
+    if (wave == 0)
+      Pick<T>(p, row, chunks, work.weight, work.equal, s,
+              WeigherOf(sh.powers, state->best, s.temperature), state->t, state->need, 0.0);
+    return;
+  }
   unsigned best = 0;
-  for (int i = tid; i < quarters; i += kRowThreads) {
+  for (int i = tid; i < quarters; i += kGroup) {
     const unsigned m = work.most[i];
     if (ranked)
       sh.most[i] = m;
     best = max(best, m);
   }
-  best = RowJoin(WaveMaxKey(best), sh.slots, [](unsigned a, unsigned b) { return max(a, b); });
+  best = RowJoin<kGroupWaves>(WaveMaxKey(best), sh.slots, [](unsigned a, unsigned b) { return max(a, b); });
   if (best == 0 || best >= kKeyOfInf || s.lost) {
     if (tid == 0)
       p.tokens[row] = -1;
@@ -1128,10 +1216,10 @@ __global__ __launch_bounds__(kRowThreads) void RowKernel(SampleParams p, int chu
   }
   if (s.greedy) {
     unsigned first = ~0u;
-    for (int i = tid; i < quarters && first == ~0u; i += kRowThreads)
+    for (int i = tid; i < quarters && first == ~0u; i += kGroup)
       if (most[i] == best)
         first = i;
-    first = RowJoin(WaveMinKey(first), sh.slots,
+    first = RowJoin<kGroupWaves>(WaveMinKey(first), sh.slots,
                     [](unsigned a, unsigned b) { return min(a, b); });
     if (wave == 0) {
       unsigned key[kRun];
@@ -1148,16 +1236,11 @@ __global__ __launch_bounds__(kRowThreads) void RowKernel(SampleParams p, int chu
   }
 
   const Weigher w = WeigherOf(sh.powers, best, s.temperature);
-  if constexpr (PHASE == Phase::kPick) {
-    if (wave == 0)
-      Pick<T>(p, row, chunks, work.weight, work.equal, s, w, state->t, state->need, 0.0);
-    return;
-  }
   const bool share = s.top_p < 1.0F;
   // The whole row's weight, where the first launch left the chunks'.
   double all = 0.0;
   if (s.top_k == 0) {
-    for (int i = tid; i < chunks; i += kRowThreads) {
+    for (int i = tid; i < chunks; i += kGroup) {
       unsigned top = 0;
       for (int q = i * kQuarters; q < min((i + 1) * kQuarters, quarters); ++q)
         top = max(top, most[q]);
@@ -1165,9 +1248,9 @@ __global__ __launch_bounds__(kRowThreads) void RowKernel(SampleParams p, int chu
       weights[i] = sum;
       all += sum;
     }
-    all = RowJoin(WaveSum64(all), sh.slots, [](double a, double b) { return a + b; });
+    all = RowJoin<kGroupWaves>(WaveSum64(all), sh.slots, [](double a, double b) { return a + b; });
   }
-  if (s.top_k == 0 && !share && !(s.min_p > 0.0F)) {
+  if (PHASE == Phase::kPlain || (s.top_k == 0 && !share && !(s.min_p > 0.0F))) {
     __threadfence_block();
     __syncthreads();
     if (wave == 0)
@@ -1175,191 +1258,129 @@ __global__ __launch_bounds__(kRowThreads) void RowKernel(SampleParams p, int chu
     return;
   }
 
-  Kept kept{1, kAll, 0};
-  Source from{false, 0};
-  bool known = s.top_k == 0 && !share;  // min_p says the threshold itself
-  if (known)
-    kept.t = KeyOfShare(w, best, s.min_p);
-  const int opened = s.top_k > 0 ? s.top_k : kShareOpened;
-  if (PHASE != Phase::kSearch && ranked && (known || (opened <= kMostOpened && opened <= quarters))) {
-    unsigned floor = kept.t;
-    if (!known) {
-      // What reaches the last of the loudest quarters.
-      Held<8> loud;  // of up to 262144 tokens; every wave by itself
-      loud.used = min((quarters + kWave - 1) / kWave, 8);
+  if constexpr (PHASE != Phase::kPlain && PHASE != Phase::kPick) {
+    Kept kept{1, kAll, 0};
+    Source from{false, 0};
+    bool known = s.top_k == 0 && !share;  // min_p says the threshold itself
+    if (known)
+      kept.t = KeyOfShare(w, best, s.min_p);
+    const int opened = s.top_k > 0 ? s.top_k : kShareOpened;
+    if (PHASE != Phase::kSearch && ranked && (known || (opened <= kMostOpened && opened <= quarters))) {
+      unsigned floor = kept.t;
+      if (!known) {
+        // What reaches the last of the loudest quarters.
+        Held<8> loud;  // of up to 262144 tokens; every wave by itself
+        loud.used = min((quarters + kWave - 1) / kWave, 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        loud.key[i] = i * kWave + lane < quarters ? sh.most[i * kWave + lane] : 0;
-      floor = Held<8>::Search(1, best, [&](unsigned t) {
-        int n = loud.Count(t);
-        for (int i = 8 * kWave; i < quarters; i += kWave)
-          n += __popcll(__ballot(i + lane < quarters && sh.most[i + lane] >= t));
-        return n >= opened;
-      });
-    }
-    const bool fits = Gather<T>(p, row, quarters, sh, most, floor, best);
-    const int listed = static_cast<int>(sh.listed);
-    if (listed <= kShortList && DrawFromList(p, row, sh, listed, s, w, shift, all))
-      return;
-    if (fits && (known || s.top_k > 0))
-      from = Source{true, listed};
-  }
-  if (PHASE == Phase::kFirst && !from.list) {
-    // The row's passes are the next launches.
-    for (int i = tid; i < kList; i += kRowThreads) {
-      state->counts[i] = 0;
-      state->weights[i] = 0;
-    }
-    if (tid == 0) {
-      state->status = known ? RowState::kPick : RowState::kSearch;
-      state->t = kept.t;
-      state->need = kept.need;
-    }
-    return;
-  }
-
-  if (!known) {
-    const RowState* const sums = PHASE == Phase::kSearch ? state : nullptr;
-    u64 whole = s.top_k == 0 ? static_cast<u64>(ldexp(all, shift)) : 0;
-    if (s.top_k > 0) {
-      RowSearch<T, false>(p, row, chunks, quarters, most, sh, &from, sums, w, shift, best, 1,
-                          s.top_k);
-      kept.t = sh.t;
-      kept.need = s.top_k - sh.above_count;  // of those that there are
-      if (share) {
-        // The weight of what top_k keeps.
-        u64 sum = 0, equal = 0;
-        EachKey<T>(p, row, chunks, sh, from, [&](unsigned key, int) {
-          if (key > kept.t)
-            sum += UnitsOf(w(key), shift);
-          equal += key == kept.t;
+        for (int i = 0; i < 8; ++i)
+          loud.key[i] = i * kWave + lane < quarters ? sh.most[i * kWave + lane] : 0;
+        floor = Held<8>::Search(1, best, [&](unsigned t) {
+          int n = loud.Count(t);
+          for (int i = 8 * kWave; i < quarters; i += kWave)
+            n += __popcll(__ballot(i + lane < quarters && sh.most[i + lane] >= t));
+          return n >= opened;
         });
-        const auto add = [](u64 a, u64 b) { return a + b; };
-        whole = RowJoin(WaveSum64(sum), sh.slots, add);
-        kept.need = min(kept.need, RowJoin(WaveSum64(equal), sh.slots, add));
-        whole += kept.need * UnitsOf(w(kept.t), shift);
       }
+      const bool fits = Gather<T>(p, row, quarters, sh, most, floor, best);
+      const int listed = static_cast<int>(sh.listed);
+      if (listed <= kShortList && DrawFromList(p, row, sh, listed, s, w, shift, all))
+        return;
+      if (fits && (known || s.top_k > 0))
+        from = Source{true, listed};
     }
-    if (share) {
-      const u64 want = ShareOf(s.top_p, whole);
-      RowSearch<T, true>(p, row, chunks, quarters, most, sh, &from, sums, w, shift, best, kept.t,
-                         want);
-      const u64 each = UnitsOf(w(sh.t), shift);
-      const u64 need = each > 0 && want > sh.above_weight
-                           ? (want - sh.above_weight + each - 1) / each
-                           : kAll;
-      kept.need = sh.t > kept.t ? need : min(kept.need, need);
-      kept.t = max(sh.t, kept.t);
-    }
-    if (s.min_p > 0.0F) {
-      const unsigned t = KeyOfShare(w, best, s.min_p);
-      if (t > kept.t) {
-        kept.t = t;
-        kept.need = kAll;
+    if (PHASE == Phase::kFirst && !from.list) {
+      // The row's passes are the next launches.
+      if (tid == 0) {
+        state->status = known ? RowState::kPick : RowState::kSearch;
+        state->best = best;
+        state->t = kept.t;
+        state->need = kept.need;
       }
+      return;
     }
-  }
-  // The chunks' kept weights.
-  __syncthreads();
-  if (from.list && chunks <= kList) {
-    for (int i = tid; i < chunks; i += kRowThreads) {
-      sh.weights[i] = 0;
-      equals[i] = 0;
-    }
-    __syncthreads();
-    EachKey<T>(p, row, chunks, sh, from, [&](unsigned key, int index) {
-      if (key > kept.t)
-        atomicAdd(&sh.weights[index / kChunk], UnitsOf(w(key), shift));
-      else if (key == kept.t)
-        atomicAdd(&equals[index / kChunk], 1u);
-    });
-    __syncthreads();
-    for (int i = tid; i < chunks; i += kRowThreads)
-      weights[i] = ldexp(static_cast<double>(sh.weights[i]), -shift);
-  } else if (PHASE == Phase::kSearch) {
-    if (tid == 0) {
-      state->status = RowState::kPick;
-      state->t = kept.t;
-      state->need = kept.need;
-    }
-    return;
-  } else {
-    for (int c = wave; c < chunks; c += kRowWaves)
-      KeptOfChunk<T>(p, row, c, kept.t, w, weights + c, equals + c);
-  }
-  if (PHASE == Phase::kSearch && tid == 0)
-    state->status = RowState::kDone;
-  __threadfence_block();
-  __syncthreads();
-  if (wave == 0)
-    Pick<T>(p, row, chunks, weights, equals, s, w, kept.t, kept.need, 0.0);
-}
 
-// The best key of a row, by one wave.
-__device__ __forceinline__ unsigned BestOf(const Work& work, int quarters) {
-  unsigned best = 0;
-  for (int i = threadIdx.x % kWave; i < quarters; i += kWave)
-    best = max(best, work.most[i]);
-  return WaveMaxKey(best);
-}
-
-// The sums of the logit's steps of the rows that search a threshold.
-constexpr int kStepChunks = 8;  // of a work-group
-template <typename T>
-__global__ __launch_bounds__(kThreads) void StepKernel(SampleParams p, int chunks, int quarters,
-                                                       int shift, int groups) {
-  __shared__ double powers[kTable];
-  __shared__ unsigned counts[kList];
-  __shared__ u64 weights[kList];
-  __builtin_assume(p.vocab > kChunk);
-  const int row = blockIdx.x / groups;
-  RowState* const state = StateOf(p, row, chunks);
-  if (state->status != RowState::kSearch)
-    return;
-  const Settings s = SettingsOf(p, row);
-  const unsigned best = BestOf(WorkOf(p, row, chunks), quarters);
-  FillTable(powers);
-  for (int i = threadIdx.x; i < kList; i += kThreads) {
-    counts[i] = 0;
-    weights[i] = 0;
-  }
-  __syncthreads();
-  const Weigher w = WeigherOf(powers, best, s.temperature);
-  const Steps steps = StepsOf(w);
-  const bool share = s.top_p < 1.0F;
-  const int first = (blockIdx.x - row * groups) * kStepChunks;
-  const int last = min(first + kStepChunks, chunks);
-  for (int c = first + static_cast<int>(threadIdx.x / kWave); c < last; c += kWaves) {
-    float z[kQuarters][kRun];
-#pragma unroll
-    for (int q = 0; q < kQuarters; ++q)
-      LoadLogits<T>(p, row, c * kQuarters + q, z[q]);
-#pragma unroll
-    for (int q = 0; q < kQuarters; ++q)
-#pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        const unsigned key = KeyOf(z[q][i]);
-        const int step = steps(key);
-        if (key != 0 && step < kList) {
-          atomicAdd(&counts[step], 1u);
-          if (share)
-            atomicAdd(&weights[step], UnitsOf(w(key), shift));
+    if (!known) {
+      const RowState* const sums =
+          PHASE == Phase::kSearch && s.Searches(quarters) ? state : nullptr;
+      u64 whole = s.top_k == 0 ? static_cast<u64>(ldexp(all, shift)) : 0;
+      if (s.top_k > 0) {
+        RowSearch<T, false>(p, row, chunks, quarters, most, sh, &from, sums, w, shift, best, 1,
+                            s.top_k);
+        kept.t = sh.t;
+        kept.need = s.top_k - sh.above_count;  // of those that there are
+        if (share) {
+          // The weight of what top_k keeps.
+          u64 sum = 0, equal = 0;
+          EachKey<T>(p, row, chunks, sh, from, [&](unsigned key, int) {
+            if (key > kept.t)
+              sum += UnitsOf(w(key), shift);
+            equal += key == kept.t;
+          });
+          const auto add = [](u64 a, u64 b) { return a + b; };
+          whole = RowJoin(WaveSum64(sum), sh.slots, add);
+          kept.need = min(kept.need, RowJoin(WaveSum64(equal), sh.slots, add));
+          whole += kept.need * UnitsOf(w(kept.t), shift);
         }
       }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kList; i += kThreads)
-    if (counts[i] != 0) {
-      atomicAdd(&state->counts[i], counts[i]);
-      if (share)
-        atomicAdd(&state->weights[i], weights[i]);
+      if (share) {
+        const u64 want = ShareOf(s.top_p, whole);
+        RowSearch<T, true>(p, row, chunks, quarters, most, sh, &from, sums, w, shift, best, kept.t,
+                           want);
+        const u64 each = UnitsOf(w(sh.t), shift);
+        const u64 need = each > 0 && want > sh.above_weight
+                             ? (want - sh.above_weight + each - 1) / each
+                             : kAll;
+        kept.need = sh.t > kept.t ? need : min(kept.need, need);
+        kept.t = max(sh.t, kept.t);
+      }
+      if (s.min_p > 0.0F) {
+        const unsigned t = KeyOfShare(w, best, s.min_p);
+        if (t > kept.t) {
+          kept.t = t;
+          kept.need = kAll;
+        }
+      }
     }
+    // The chunks' kept weights.
+    __syncthreads();
+    if (from.list && chunks <= kList) {
+      for (int i = tid; i < chunks; i += kRowThreads) {
+        sh.weights[i] = 0;
+        equals[i] = 0;
+      }
+      __syncthreads();
+      EachKey<T>(p, row, chunks, sh, from, [&](unsigned key, int index) {
+        if (key > kept.t)
+          atomicAdd(&sh.weights[index / kChunk], UnitsOf(w(key), shift));
+        else if (key == kept.t)
+          atomicAdd(&equals[index / kChunk], 1u);
+      });
+      __syncthreads();
+      for (int i = tid; i < chunks; i += kRowThreads)
+        weights[i] = ldexp(static_cast<double>(sh.weights[i]), -shift);
+    } else if (PHASE == Phase::kSearch) {
+      if (tid == 0) {
+        state->status = RowState::kPick;
+        state->t = kept.t;
+        state->need = kept.need;
+      }
+      return;
+    } else {
+      for (int c = wave; c < chunks; c += kRowWaves)
+        KeptOfChunk<T>(p, row, c, kept.t, w, weights + c, equals + c);
+    }
+    if (PHASE == Phase::kSearch && tid == 0)
+      state->status = RowState::kDone;
+    __threadfence_block();
+    __syncthreads();
+    if (wave == 0)
+      Pick<T>(p, row, chunks, weights, equals, s, w, kept.t, kept.need, 0.0);
+  }
 }
 
 // The chunks' kept weights of the rows that have their threshold.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void KeptKernel(SampleParams p, int chunks, int quarters,
-                                                       int groups) {
+__global__ __launch_bounds__(kThreads) void KeptKernel(SampleParams p, int chunks, int groups) {
   __shared__ double powers[kTable];
   __builtin_assume(p.vocab > kChunk);
   const int row = blockIdx.x / groups;
@@ -1372,7 +1393,7 @@ __global__ __launch_bounds__(kThreads) void KeptKernel(SampleParams p, int chunk
   __syncthreads();
   const int c = (blockIdx.x - row * groups) * kWaves + threadIdx.x / kWave;
   if (c < chunks)
-    KeptOfChunk<T>(p, row, c, state->t, WeigherOf(powers, BestOf(work, quarters), s.temperature),
+    KeptOfChunk<T>(p, row, c, state->t, WeigherOf(powers, state->best, s.temperature),
                    work.weight + c, work.equal + c);
 }
 
@@ -1422,24 +1443,27 @@ void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
       // A row may need a threshold where any setting may ask for one.
       const bool filtered = p.top_ks != nullptr || p.top_ps != nullptr || p.min_ps != nullptr ||
                             p.top_k > 0 || p.top_p < 1.0F || p.min_p > 0.0F;
-      const bool split = filtered && SplitRows(p.rows, chunks);
+      // Where every row has one small k its list is short, but for many equals.
+      const bool listed = p.top_ks == nullptr && p.top_k > 0 && p.top_k <= kMostOpened &&
+                          p.top_k <= quarters;
+      const bool split = filtered && !listed && SplitRows(p.rows, chunks);
       Dispatch(ChunkKernel<T>, dim3(p.rows * groups), dim3(kThreads), 0, stream, true, false, p,
-               chunks, groups);
-      const auto rows = [&](auto kernel, bool last) {
-        Dispatch(kernel, dim3(p.rows), dim3(kRowThreads), 0, stream, false, last, p, chunks,
-                 quarters, shift);
+               chunks, groups, split);
+      const auto rows = [&](auto kernel, int groups_each, int threads, bool last) {
+        Dispatch(kernel, dim3(p.rows * groups_each), dim3(threads), 0, stream, false, last, p,
+                 chunks, quarters, shift);
       };
-      if (!split) {
-        rows(RowKernel<T, Phase::kWhole>, true);
+      if (!filtered) {
+        rows(RowKernel<T, Phase::kPlain>, 1, kThreads, true);
+      } else if (!split) {
+        rows(RowKernel<T, Phase::kWhole>, 1, kRowThreads, true);
       } else {
-        const int step_groups = (chunks + kStepChunks - 1) / kStepChunks;
-        rows(RowKernel<T, Phase::kFirst>, false);
-        Dispatch(StepKernel<T>, dim3(p.rows * step_groups), dim3(kThreads), 0, stream, false,
-                 false, p, chunks, quarters, shift, step_groups);
-        rows(RowKernel<T, Phase::kSearch>, false);
+        rows(RowKernel<T, Phase::kFirst>, 1 + (chunks + kStepChunks - 1) / kStepChunks,
+             kRowThreads, false);
+        rows(RowKernel<T, Phase::kSearch>, 1, kRowThreads, false);
         Dispatch(KeptKernel<T>, dim3(p.rows * groups), dim3(kThreads), 0, stream, false, false, p,
-                 chunks, quarters, groups);
-        rows(RowKernel<T, Phase::kPick>, true);
+                 chunks, groups);
+        rows(RowKernel<T, Phase::kPick>, 1, kWave, true);
       }
     }
   });
