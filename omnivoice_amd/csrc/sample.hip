@@ -26,6 +26,8 @@
 // 2^x in 64 bits from a table of 256 powers and three terms. Sums that several lanes
 // form in any order are whole numbers of 2^-shift; the others are 64-bit numbers in a
 // fixed order. No result depends on the order of the work.
+#include <algorithm>
+
 #include "step.hpp"
 
 #pragma clang fp contract(off)
@@ -51,6 +53,10 @@ constexpr int kOctaves = 50;                // weights below 2^-50 do not count
 constexpr int kTable = 256;
 
 // ---------------------------------------------------------------- lanes
+// The wave's number, which the compiler then knows to be the same in all lanes.
+__device__ __forceinline__ int WaveIndex() {
+  return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave));
+}
 template <int CTRL>
 __device__ __forceinline__ u64 Dpp64(u64 v) {
   const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false);
@@ -183,16 +189,6 @@ __device__ __forceinline__ void LoadLogits(const SampleParams& p, std::int64_t r
     }
   }
 }
-template <typename T>
-__device__ __forceinline__ void LoadKeys(const SampleParams& p, std::int64_t row, int q,
-                                         unsigned (&key)[kRun]) {
-  float z[kRun];
-  LoadLogits<T>(p, row, q, z);
-#pragma unroll
-  for (int i = 0; i < kRun; ++i)
-    key[i] = KeyOf(z[i]);
-}
-
 // ---------------------------------------------------------------- weights
 // 2^(j / 256), by the series of e^x.
 struct Powers {
@@ -231,9 +227,13 @@ struct Weigher {
     e = __fma_rn(r, e, 1.0);
     return ldexp(e * powers[k & (kTable - 1)], k >> 8);
   }
+  // None where it is below 2^-50.
+  __device__ __forceinline__ double Of(float z) const {
+    const double w = Raw(z);
+    return w >= 0x1p-50 ? w : 0.0;
+  }
   __device__ __forceinline__ double operator()(unsigned key) const {
-    const double w = Raw(LogitOf(key));
-    return (key != 0) & (w >= 0x1p-50) ? w : 0.0;
+    return key != 0 ? Of(LogitOf(key)) : 0.0;
   }
 };
 // In whole units of 2^-shift, shift <= 51: the last bits of a sum with 2^(52 - shift).
@@ -247,11 +247,6 @@ struct Settings {
   int top_k;  // 0: all
   bool lost, greedy;
   __device__ __forceinline__ bool Whole() const { return !greedy && top_k == 0; }
-  // Whether the sums of the row's steps may be asked for.
-  __device__ __forceinline__ bool Searches(int quarters) const {
-    return !lost && !greedy &&
-           (top_k > min(kMostOpened, quarters) || (top_k == 0 && top_p < 1.0F));
-  }
 };
 __device__ __forceinline__ Settings SettingsOf(const SampleParams& p, int row) {
   Settings s;
@@ -305,18 +300,15 @@ struct Kept {
 };
 constexpr u64 kAll = ~u64{0};
 
-// N elements a lane, of which `used` registers are in use in some lane.
+// N elements a lane.
 template <int N>
 struct Held {
   unsigned key[N];
   u64 weight[N];
-  int used;
   __device__ __forceinline__ int Count(unsigned t) const {
     int n = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (i >= used)
-        break;
       n += __popcll(__ballot(key[i] >= t));
     }
     return n;
@@ -325,8 +317,6 @@ struct Held {
     u64 n = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (i >= used)
-        break;
       n += key[i] >= t ? weight[i] : 0;
     }
     return WaveSum64(n);
@@ -335,8 +325,6 @@ struct Held {
     unsigned n = ~0u;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (i >= used)
-        break;
       n = key[i] != 0 ? min(n, key[i]) : n;
     }
     return WaveMinKey(n);
@@ -353,47 +341,41 @@ struct Held {
     }
     return low;
   }
-  // Of all that is held, or the prefix of weight ShareOf(top_p, *whole) of it where the
-  // row holds more; false where that does not reach.
-  __device__ __forceinline__ bool Select(const Settings& s, const Weigher& w, unsigned best,
-                                         int shift, const u64* whole, Kept* kept) const {
+  __device__ __forceinline__ Kept Select(const Settings& s, const Weigher& w, unsigned best,
+                                         int shift) const {
     const unsigned least = Least();
-    kept->t = least;
-    kept->need = kAll;
-    kept->weight = Weight(1);
+    Kept kept{least, kAll, Weight(1)};
     if (s.top_k > 0 && Count(1) > s.top_k) {
-      kept->t = Search(least, best, [&](unsigned t) { return Count(t) >= s.top_k; });
-      const unsigned above = kept->t + 1;
-      kept->need = s.top_k - Count(above);
-      kept->weight = Weight(above) + kept->need * UnitsOf(w(kept->t), shift);
+      kept.t = Search(least, best, [&](unsigned t) { return Count(t) >= s.top_k; });
+      const unsigned above = kept.t + 1;
+      kept.need = s.top_k - Count(above);
+      kept.weight = Weight(above) + kept.need * UnitsOf(w(kept.t), shift);
     }
     if (s.top_p < 1.0F) {
-      const u64 want = ShareOf(s.top_p, whole != nullptr ? *whole : kept->weight);
-      if (kept->weight < want)
-        return false;
-      const unsigned low = kept->t;
+      const u64 want = ShareOf(s.top_p, kept.weight);
+      const unsigned low = kept.t;
       u64 above = Weight(low + 1);
       if (above >= want) {
-        kept->t = Search(low + 1, best, [&](unsigned t) { return Weight(t) >= want; });
-        kept->need = kAll;
-        above = Weight(kept->t + 1);
+        kept.t = Search(low + 1, best, [&](unsigned t) { return Weight(t) >= want; });
+        kept.need = kAll;
+        above = Weight(kept.t + 1);
       }
-      const u64 each = UnitsOf(w(kept->t), shift);
+      const u64 each = UnitsOf(w(kept.t), shift);
       if (each > 0) {
-        kept->need = min(kept->need, (want - above + each - 1) / each);
-        kept->need = min(kept->need, static_cast<u64>(Count(kept->t) - Count(kept->t + 1)));
-        kept->weight = above + kept->need * each;
+        kept.need = min(kept.need, (want - above + each - 1) / each);
+        kept.need = min(kept.need, static_cast<u64>(Count(kept.t) - Count(kept.t + 1)));
+        kept.weight = above + kept.need * each;
       }
     }
     if (s.min_p > 0.0F) {
       const unsigned t = KeyOfShare(w, best, s.min_p);
-      if (t > kept->t) {
-        kept->t = t;
-        kept->need = kAll;
-        kept->weight = Weight(t);
+      if (t > kept.t) {
+        kept.t = t;
+        kept.need = kAll;
+        kept.weight = Weight(t);
       }
     }
-    return true;
+    return kept;
   }
 };
 
@@ -434,10 +416,38 @@ __device__ __forceinline__ bool DrawOf(const unsigned (&key)[R], const u64 (&wei
 }
 
 // ---------------------------------------------------------------- small rows
-// A wave a row of up to 512 Q tokens. With a top_k of 64 or less, the lanes' largest keys
-// give a floor that the k best reach, and the few elements that do go through LDS, in the
-// row's order, to two a lane.
-constexpr int kFew = 2 * kWave;
+// A wave a row of up to 512 Q tokens. With a top_k of 128 or less, the largest keys of the
+// lanes' halves give a floor that the k best reach, and the few elements that do go
+// through LDS, in the row's order, to two or four a lane.
+constexpr int kFew = 4 * kWave;
+
+// The draw from `listed` elements in the row's order, R a lane.
+template <int R>
+__device__ __forceinline__ void DrawFew(const SampleParams& p, int row, const u64* few,
+                                        int listed, const Settings& s, const Weigher& w,
+                                        unsigned best, int shift) {
+  const int lane = threadIdx.x % kWave;
+  Held<R> held;
+  int index[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const u64 e = R * lane + i < listed ? few[R * lane + i] : 0;
+    held.key[i] = static_cast<unsigned>(e >> 32);
+    index[i] = static_cast<int>(e);
+    held.weight[i] = UnitsOf(w(held.key[i]), shift);
+  }
+  const Kept kept = held.Select(s, w, best, shift);
+  u64 left = TargetOf(s.u, kept.weight), need = kept.need;
+  int of, place;
+  if (DrawOf(held.key, held.weight, kept.t, &need, &left, &of, &place)) {
+    int token = index[0];
+#pragma unroll
+    for (int i = 1; i < R; ++i)
+      token = place == i ? index[i] : token;
+    if (lane == of)
+      p.tokens[row] = token;
+  }
+}
 
 template <typename T, int Q>
 __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shift) {
@@ -445,30 +455,29 @@ __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shif
   __shared__ double powers[kTable];
   __shared__ u64 few[kWaves][kFew];  // key, index
   FillTable(powers);
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = WaveIndex();
   const int row = blockIdx.x * kWaves + wave;
   Held<N> held;
-  held.used = N;
   Settings s{};
   if (row < p.rows) {
     s = SettingsOf(p, row);
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      unsigned key[kRun];
-      LoadKeys<T>(p, row, q, key);
+      float z[kRun];
+      LoadLogits<T>(p, row, q, z);
 #pragma unroll
       for (int i = 0; i < kRun; ++i)
-        held.key[q * kRun + i] = key[i];
+        held.key[q * kRun + i] = KeyOf(z[i]);
     }
   }
   __syncthreads();
   if (row >= p.rows)
     return;
-  unsigned most = 0;
+  unsigned most[2] = {0, 0};  // of the lane's halves
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    most = max(most, held.key[i]);
-  const unsigned best = WaveMaxKey(most);
+    most[i < N / 2] = max(most[i < N / 2], held.key[i]);
+  const unsigned best = WaveMaxKey(max(most[0], most[1]));
   if (best == 0 || best >= kKeyOfInf || s.lost) {
     if (lane == 0)
       p.tokens[row] = -1;
@@ -478,10 +487,15 @@ __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shif
   Kept kept{best, 1, 1};
   u64 left, need;
   int of, place;
-  if (!s.greedy && s.top_k > 0 && s.top_k <= kWave) {
-    const unsigned floor = Held<1>::Search(1, best, [&](unsigned t) {
-      return __popcll(__ballot(most >= t)) >= s.top_k;
-    });
+  if (!s.greedy && s.top_k > 0 && s.top_k <= 2 * kWave) {
+    unsigned floor = 1, high = best;
+    while (floor < high) {
+      const unsigned mid = floor + (high - floor + 1) / 2;
+      if (__popcll(__ballot(most[0] >= mid)) + __popcll(__ballot(most[1] >= mid)) >= s.top_k)
+        floor = mid;
+      else
+        high = mid - 1;
+    }
     unsigned from[Q];  // where the lane's elements go
     int listed = 0;
 #pragma unroll
@@ -506,49 +520,30 @@ __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shif
       }
       // The wave's own part of LDS: its writes are done before its reads.
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      Held<2> best_few;
-      best_few.used = 2;
-      int index[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const u64 e = 2 * lane + i < listed ? few[wave][2 * lane + i] : 0;
-        best_few.key[i] = static_cast<unsigned>(e >> 32);
-        index[i] = static_cast<int>(e);
-        best_few.weight[i] = UnitsOf(w(best_few.key[i]), shift);
-      }
-      best_few.Select(s, w, best, shift, nullptr, &kept);
-      left = TargetOf(s.u, kept.weight);
-      need = kept.need;
-      if (DrawOf(best_few.key, best_few.weight, kept.t, &need, &left, &of, &place)) {
-        const int token = place == 0 ? index[0] : index[1];
-        if (lane == of)
-          p.tokens[row] = token;
-      }
+      if (listed <= kFew / 2)
+        DrawFew<2>(p, row, few[wave], listed, s, w, best, shift);
+      else
+        DrawFew<4>(p, row, few[wave], listed, s, w, best, shift);
       return;
     }
   }
-  if (s.greedy) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      held.weight[i] = held.key[i] == best;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      held.weight[i] = UnitsOf(w(held.key[i]), shift);
-    held.Select(s, w, best, shift, nullptr, &kept);
-  }
+  for (int i = 0; i < N; ++i)
+    held.weight[i] = s.greedy ? held.key[i] == best : UnitsOf(w(held.key[i]), shift);
+  if (!s.greedy)
+    kept = held.Select(s, w, best, shift);
   left = TargetOf(s.greedy ? 0.0F : s.u, kept.weight);
   need = kept.need;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
-    unsigned key[kRun];
-    u64 weight[kRun];
+    unsigned run_key[kRun];
+    u64 run_weight[kRun];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      key[i] = held.key[q * kRun + i];
-      weight[i] = held.weight[q * kRun + i];
+      run_key[i] = held.key[q * kRun + i];
+      run_weight[i] = held.weight[q * kRun + i];
     }
-    if (DrawOf(key, weight, kept.t, &need, &left, &of, &place)) {
+    if (DrawOf(run_key, run_weight, kept.t, &need, &left, &of, &place)) {
       if (lane == of)
         p.tokens[row] = RunStart(q, p.vocab) + place;
       return;
@@ -557,45 +552,93 @@ __global__ __launch_bounds__(kThreads) void SmallKernel(SampleParams p, int shif
 }
 
 // ---------------------------------------------------------------- large rows
-// A row's part of the workspace: the chunks' weights, their equals of a threshold, the
-// quarters' largest keys.
+// A row's part of the workspace: the chunks' weights, the quarters' largest keys.
 struct Work {
   double* weight;
-  unsigned* equal;
   unsigned* most;
 };
-// What a row goes on with in the launches of its own passes, and their sums.
+// What a row that needs its threshold goes on with, and its sums.
 struct RowState {
-  enum : unsigned { kDone, kSearch, kPick };
-  unsigned status, t, best, spare;
-  u64 need;
+  enum : unsigned { kDone, kCollect, kKnown, kSlow };
+  unsigned status, best;
+  unsigned t;       // kKnown: all from it on is kept
+  unsigned raised;  // where min_p's key is above the steps below: all from it on is kept
+  unsigned listed;  // elements of the list
+  u64 whole;        // the row's weight in units, without a top_k
+  // The steps whose elements are listed: the one in which top_k ends, and low .. high, in
+  // which the share does; what is above them.
+  int k_step, low_step, high_step;
+  u64 k_count, k_weight, low_count, low_weight;
   unsigned counts[kList];
   u64 weights[kList];
+  u64 list[kList];  // key, index
 };
-constexpr int kSplitRows = 256;
+constexpr int kBatch = 512;  // rows that have a state at once
+
+struct RowCall {
+  SampleParams p;
+  int first, rows;  // of the launch
+  int chunks, quarters, shift;
+};
 __host__ __device__ constexpr std::int64_t WorkWords(std::int64_t chunks) {
-  return (chunks * (2 + 1 + kQuarters) + 3) / 4 * 4;
-}
-__device__ __forceinline__ RowState* StateOf(const SampleParams& p, int row, int chunks) {
-  return reinterpret_cast<RowState*>(p.work + WorkWords(chunks) * p.rows) + row;
+  return (chunks * (2 + kQuarters) + 3) / 4 * 4;
 }
 __device__ __forceinline__ Work WorkOf(const SampleParams& p, int row, int chunks) {
   double* const base = reinterpret_cast<double*>(p.work + WorkWords(chunks) * row);
-  unsigned* const equal = reinterpret_cast<unsigned*>(base + chunks);
-  return {base, equal, equal + chunks};
+  return {base, reinterpret_cast<unsigned*>(base + chunks)};
+}
+__device__ __forceinline__ RowState* StateOf(const RowCall& c, int i) {
+  return reinterpret_cast<RowState*>(c.p.work + WorkWords(c.chunks) * c.p.rows) + i;
+}
+
+// A wave's four quarters of a chunk, all loads on their way at once; then f(first element
+// of the lane's run, logits) for one after the other, in a loop that stays one.
+template <typename T, typename F>
+__device__ __forceinline__ void EachQuarter(const SampleParams& p, int row, int chunk, F&& f) {
+  float z[kQuarters][kRun];
+#pragma unroll
+  for (int q = 0; q < kQuarters; ++q)
+    LoadLogits<T>(p, row, chunk * kQuarters + q, z[q]);
+#pragma unroll 1
+  for (int q = 0; q < kQuarters; ++q) {
+    float v[kRun];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const float front = q == 0 ? z[0][i] : z[1][i], back = q == 2 ? z[2][i] : z[3][i];
+      v[i] = q < 2 ? front : back;
+    }
+    f(RunStart(chunk * kQuarters + q, p.vocab), v);
+  }
+}
+
+// Clears what the launches behind add to; `part` of `parts` work-groups.
+__device__ __forceinline__ void ClearState(RowState* state, int part, int parts) {
+  for (int i = part * kThreads + threadIdx.x; i < kList; i += parts * kThreads) {
+    state->counts[i] = 0;
+    state->weights[i] = 0;
+  }
+  if (part == 0 && threadIdx.x == 0) {
+    state->status = RowState::kDone;
+    state->listed = 0;
+    state->raised = 0;
+  }
+}
+__global__ __launch_bounds__(kThreads) void ClearKernel(RowCall c) {
+  ClearState(StateOf(c, blockIdx.x), 0, 1);
 }
 
 // The largest key of every quarter of a chunk, and the chunk's weight beside the
 // chunk's own largest.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void ChunkKernel(SampleParams p, int chunks, int groups,
-                                                        bool split) {
+__global__ __launch_bounds__(kThreads) void ChunkKernel(RowCall c, int groups, bool clear) {
   __shared__ double powers[kTable];
+  const SampleParams& p = c.p;
+  const int chunks = c.chunks;
   __builtin_assume(p.vocab > kChunk);
   FillTable(powers);
   const int lane = threadIdx.x % kWave;
   const int row = blockIdx.x / groups;
-  const int chunk = (blockIdx.x - row * groups) * kWaves + threadIdx.x / kWave;
+  const int chunk = (blockIdx.x - row * groups) * kWaves + WaveIndex();
   float z[kQuarters][kRun];
   Settings s{};
   if (chunk < chunks) {
@@ -604,14 +647,8 @@ __global__ __launch_bounds__(kThreads) void ChunkKernel(SampleParams p, int chun
     for (int q = 0; q < kQuarters; ++q)
       LoadLogits<T>(p, row, chunk * kQuarters + q, z[q]);
   }
-  if (split && s.Searches((p.vocab - 1) / kQuarter + 1)) {  // the sums that the next launch adds to
-    RowState* const state = StateOf(p, row, chunks);
-    const int part = blockIdx.x - row * groups;
-    for (int i = part * kThreads + threadIdx.x; i < kList; i += groups * kThreads) {
-      state->counts[i] = 0;
-      state->weights[i] = 0;
-    }
-  }
+  if (clear)
+    ClearState(StateOf(c, row), blockIdx.x - row * groups, groups);
   __syncthreads();
   if (chunk >= chunks)
     return;
@@ -652,24 +689,8 @@ __global__ __launch_bounds__(kThreads) void ChunkKernel(SampleParams p, int chun
     work.weight[chunk] = all;
 }
 
-struct RowShared {
-  double powers[kTable];
-  u64 weights[kList];  // of a pass's bins; as 64-bit numbers, the chunks'
-  unsigned counts[kList];
-  unsigned most[kMostQuarters];
-  u64 list[kList];     // key, index
-  unsigned short open[kMostQuarters];
-  u64 unit[kShortList];    // the list's weights
-  u64 before[kShortList];
-  int rank[kShortList];
-  u64 slots[kRowWaves], count_slots[kRowWaves];
-  unsigned listed, opened, t;
-  int bin;
-  u64 above_weight, above_count;
-};
-
 // v is the same in every lane of a wave.
-template <int WAVES = kRowWaves, typename V, typename F>
+template <int WAVES, typename V, typename F>
 __device__ __forceinline__ V RowJoin(V v, u64* scratch, F&& join) {
   V* const slots = reinterpret_cast<V*>(scratch);
   __syncthreads();
@@ -682,105 +703,213 @@ __device__ __forceinline__ V RowJoin(V v, u64* scratch, F&& join) {
     v = join(v, slots[i]);
   return v;
 }
+template <int WAVES, typename V>
+__device__ __forceinline__ V RowSum(V v, u64* scratch) {
+  return RowJoin<WAVES>(WaveSum64(v), scratch, [](V a, V b) { return a + b; });
+}
 
-// What a search goes over: the row, or the list of all its keys from some key on.
-struct Source {
-  bool list;
-  int count;
-};
+// The largest key of the row; also in sh_most, where the quarters fit.
+template <int WAVES>
+__device__ __forceinline__ unsigned BestOf(const Work& work, int quarters, unsigned* sh_most,
+                                           u64* slots) {
+  unsigned best = 0;
+  for (int i = threadIdx.x; i < quarters; i += WAVES * kWave) {
+    const unsigned m = work.most[i];
+    if (i < kMostQuarters)
+      sh_most[i] = m;
+    best = max(best, m);
+  }
+  return RowJoin<WAVES>(WaveMaxKey(best), slots, [](unsigned a, unsigned b) { return max(a, b); });
+}
 
-// Calls f(key, index) for the elements, a wave a chunk of the row.
-template <typename T, typename F>
-__device__ __forceinline__ void EachKey(const SampleParams& p, int row, int chunks,
-                                        const RowShared& sh, const Source& from, F&& f) {
-  if (from.list) {
-    for (int i = threadIdx.x; i < from.count; i += kRowThreads)
-      f(static_cast<unsigned>(sh.list[i] >> 32), static_cast<int>(sh.list[i]));
+// The first token of the largest key.
+template <typename T, int WAVES>
+__device__ __forceinline__ void DrawBest(const RowCall& c, int row, const Work& work, unsigned best,
+                                         u64* slots) {
+  unsigned first = ~0u;
+  for (int i = threadIdx.x; i < c.quarters && first == ~0u; i += WAVES * kWave)
+    if (work.most[i] == best)
+      first = i;
+  first = RowJoin<WAVES>(WaveMinKey(first), slots,
+                         [](unsigned a, unsigned b) { return min(a, b); });
+  if (threadIdx.x >= kWave)
+    return;
+  float z[kRun];
+  LoadLogits<T>(c.p, row, static_cast<int>(first), z);
+  unsigned token = ~0u;
+#pragma unroll
+  for (int i = kRun - 1; i >= 0; --i)
+    token = KeyOf(z[i]) == best ? RunStart(static_cast<int>(first), c.p.vocab) + i : token;
+  token = WaveMinKey(token);
+  if (threadIdx.x == 0)
+    c.p.tokens[row] = static_cast<int>(token);
+}
+
+// The chunks' weights beside the row's best, and their sum.
+template <int WAVES>
+__device__ __forceinline__ double WholeOf(const RowCall& c, const Work& work, const Weigher& w,
+                                          u64* slots) {
+  double all = 0.0;
+  for (int i = threadIdx.x; i < c.chunks; i += WAVES * kWave) {
+    unsigned top = 0;
+    for (int q = i * kQuarters; q < min((i + 1) * kQuarters, c.quarters); ++q)
+      top = max(top, work.most[q]);
+    const double sum = work.weight[i] * w(top);
+    work.weight[i] = sum;
+    all += sum;
+  }
+  return RowSum<WAVES>(all, slots);
+}
+
+// The draw by the chunks' kept weights, by one wave: the chunk, 64 at a time, then the
+// place in it. Kept is what is above t (0: all) and of what equals it the first `need`,
+// which `equals` counts by chunk (null: none).
+template <typename T>
+__device__ __forceinline__ void Pick(const RowCall& c, int row, const double* weights,
+                                     const unsigned* equals, const Settings& s, const Weigher& w,
+                                     unsigned t, u64 need0) {
+  const SampleParams& p = c.p;
+  const int lane = threadIdx.x % kWave;
+  const bool bounded = t != 0;
+  const double each = bounded ? w(t) : 0.0;
+  const auto last_lane = [](double v) {
+    return __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, v), kWave - 1));
+  };
+  // Twice over the chunks: their sum, then the place.
+  double total = 0.0, left = __builtin_inf(), last_before = 0.0;
+  int last = 0;  // the chunk; the last one that keeps any where rounding leaves none
+  u64 last_need = 0;
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {
+    u64 need = need0;
+    double before = 0.0;
+    bool done = false;
+#pragma unroll 1
+    for (int c0 = 0; c0 < c.chunks && !done; c0 += kWave) {
+      const bool there = c0 + lane < c.chunks;
+      const unsigned equal = there && equals != nullptr ? equals[c0 + lane] : 0;
+      const u64 equal_to = equals != nullptr ? WaveScan(static_cast<u64>(equal)) : 0;
+      const u64 equal_before = equal_to - equal;
+      const u64 in = need > equal_before ? min(need - equal_before, static_cast<u64>(equal)) : 0;
+      const double mine = (there ? weights[c0 + lane] : 0.0) + static_cast<double>(in) * each;
+      const double to = before + WaveScan(mine);
+      const u64 hit = __ballot(mine > 0.0 && to > left), any = __ballot(mine > 0.0);
+      if (any != 0) {
+        const int l = hit != 0 ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
+        last = c0 + l;
+        last_before = __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, to - mine), l));
+        last_need = need - min(need, Lane64(equal_before, l));
+      }
+      done = hit != 0;
+      before = last_lane(to);
+      need -= min(need, Lane64(equal_to, kWave - 1));
+    }
+    if (turn == 0) {
+      total = before;
+      left = static_cast<double>(fminf(fmaxf(s.u, 0.0F), 1.0F)) * total;
+      if (!(left < total))
+        left = total * (1.0 - 0x1p-53);
+    }
+  }
+  left -= last_before;
+  u64 need = last_need;
+  int token = -1;  // the last kept one, where rounding leaves none
+  bool done = false;
+  EachQuarter<T>(p, row, last, [&](int start, const float (&z)[kRun]) {
+    if (done)
+      return;
+    unsigned equal = 0;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i)
+      equal += bounded && KeyOf(z[i]) == t;
+    const unsigned equal_to = WaveScan(equal);
+    u64 seen = equal_to - equal;
+    double to_place[kRun], mine = 0.0;
+    int end = -1;  // the lane's last kept one
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const unsigned key = KeyOf(z[i]);
+      const bool in = !bounded || key > t || (key == t && seen++ < need);
+      const double weight = in ? w(key) : 0.0;
+      end = weight > 0.0 ? i : end;
+      mine += weight;
+      to_place[i] = mine;
+    }
+    const double to = WaveScan(mine);
+    const u64 hit = __ballot(mine > 0.0 && to > left), any = __ballot(mine > 0.0);
+    int place = end;
+#pragma unroll
+    for (int i = kRun - 1; i >= 0; --i) {
+      const double before = i > 0 ? to_place[i - 1] : 0.0;
+      place = to_place[i] > before && (to - mine) + to_place[i] > left ? i : place;
+    }
+    done = hit != 0;
+    if (any != 0)
+      token = __builtin_amdgcn_readlane(
+          start + place, done ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any));
+    left -= last_lane(to);
+    need -= min(need, static_cast<u64>(__builtin_amdgcn_readlane(equal_to, kWave - 1)));
+  });
+  if (lane == 0)
+    p.tokens[row] = token;
+}
+
+// Rows of which none has a filter, or that are decided by the chunks' numbers.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void PlainKernel(RowCall c) {
+  __shared__ double powers[kTable];
+  __shared__ unsigned most[kMostQuarters];
+  __shared__ u64 slots[kWaves];
+  const int row = c.first + blockIdx.x;
+  const Settings s = SettingsOf(c.p, row);
+  const Work work = WorkOf(c.p, row, c.chunks);
+  FillTable(powers);
+  const unsigned best = BestOf<kWaves>(work, c.quarters, most, slots);
+  if (best == 0 || best >= kKeyOfInf || s.lost) {
+    if (threadIdx.x == 0)
+      c.p.tokens[row] = -1;
     return;
   }
-  for (int c = threadIdx.x / kWave; c < chunks; c += kRowWaves) {
-    float z[kQuarters][kRun];
-#pragma unroll
-    for (int q = 0; q < kQuarters; ++q)
-      LoadLogits<T>(p, row, c * kQuarters + q, z[q]);
-#pragma unroll
-    for (int q = 0; q < kQuarters; ++q) {
-      const int start = RunStart(c * kQuarters + q, p.vocab);
-#pragma unroll
-      for (int i = 0; i < kRun; ++i)
-        f(KeyOf(z[q][i]), start + i);
-    }
+  if (s.greedy) {
+    DrawBest<T, kWaves>(c, row, work, best, slots);
+    return;
   }
+  const Weigher w = WeigherOf(powers, best, s.temperature);
+  WholeOf<kWaves>(c, work, w, slots);
+  __syncthreads();
+  if (threadIdx.x < kWave)
+    Pick<T>(c, row, work.weight, nullptr, s, w, 0, 0);
 }
 
-// The list of the row's keys from `floor` to `high`; false where it does not hold them.
-// Quarters without any are not read. The whole work-group calls this.
-template <typename T>
-__device__ __forceinline__ bool Gather(const SampleParams& p, int row, int quarters,
-                                       RowShared& sh, const unsigned* most, unsigned floor,
-                                       unsigned high) {
-  constexpr int kAtOnce = 4;  // quarters' loads of a wave
-  const int wave = threadIdx.x / kWave;
-  __syncthreads();
-  if (threadIdx.x == 0)
-    sh.listed = 0;
-  for (int first = 0; first < quarters; first += kMostQuarters) {
-    if (threadIdx.x == 0)
-      sh.opened = 0;
-    __syncthreads();
-    const int count = min(quarters - first, kMostQuarters);
-    for (int q = threadIdx.x; q < count; q += kRowThreads)
-      if (most[first + q] >= floor)
-        sh.open[atomicAdd(&sh.opened, 1u)] = static_cast<unsigned short>(q);
-    __syncthreads();
-    const int opened = static_cast<int>(sh.opened);
-    for (int o = wave; o < opened; o += kAtOnce * kRowWaves) {
-      float z[kAtOnce][kRun];
-      int q[kAtOnce];
-#pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        q[i] = first + sh.open[min(o + i * kRowWaves, opened - 1)];
-        LoadLogits<T>(p, row, q[i], z[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        if (o + i * kRowWaves >= opened)
-          break;
-        const int start = RunStart(q[i], p.vocab);
-#pragma unroll
-        for (int e = 0; e < kRun; ++e) {
-          const unsigned key = KeyOf(z[i][e]);
-          if (key >= floor && key <= high) {
-            const unsigned at = atomicAdd(&sh.listed, 1u);
-            if (at < kList)
-              sh.list[at] = static_cast<u64>(key) << 32 | static_cast<unsigned>(start + e);
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-  return sh.listed <= kList;
-}
+// ---------------------------------------------------------------- rows with filters
+struct RowShared {
+  double powers[kTable];
+  u64 weights[kList];   // of bins; as 64-bit numbers, the chunks'
+  unsigned counts[kList];
+  u64 list[kList];      // key, index
+  union {
+    struct {
+      unsigned most[kMostQuarters];
+      unsigned short open[kMostQuarters];
+    };
+    struct {
+      u64 unit[kShortList], before[kShortList];  // of the list's elements
+      int rank[kShortList];
+    };
+  };
+  u64 slots[kRowWaves], count_slots[kRowWaves];
+  unsigned listed, opened;
+  int bin;
+  u64 above_weight, above_count;
+};
 
 // 2048 equal steps of the logit from the best down to the smallest weight that counts.
 struct Steps {
   float top, scale;
-  __device__ __forceinline__ int operator()(unsigned key) const {
-    const float at = fminf(top - LogitOf(key), 3e38F) * scale;
-    return at < static_cast<float>(kList) ? static_cast<int>(at) : kList;
-  }
-  // The smallest key of a step up to `last`; 64 keys at once.
-  __device__ __forceinline__ unsigned Least(unsigned best, int last) const {
-    unsigned low = kKeyOfMinusInf, high = best;
-    while (high - low > 1) {
-      const unsigned step = (high - low + kWave - 1) / kWave;
-      const unsigned key = min(low + step * (threadIdx.x % kWave + 1), high);
-      const int at = __builtin_ctzll(__ballot(key == high || (*this)(key) <= last));
-      high = min(low + step * (at + 1), high);
-      low += step * at;
-    }
-    return high;
+  // kList where the element is none of them.
+  __device__ __forceinline__ int operator()(float z) const {
+    const float at = fminf(top - z, 3e38F) * scale;
+    return at < static_cast<float>(kList) && z > -__builtin_inff() ? static_cast<int>(at) : kList;
   }
 };
 __device__ __forceinline__ Steps StepsOf(const Weigher& w) {
@@ -789,115 +918,95 @@ __device__ __forceinline__ Steps StepsOf(const Weigher& w) {
                 1e30F)};
 }
 
-// The key at which the count of keys (or their weight) reaches `want`, from the top: sums
-// of the logit's steps (from `state`, or a pass over the elements), then of equal ranges
-// of the keys in the step that was found, until that is one key. Where the first sums
-// leave few elements the passes go over a list, of all from that step up if it holds
-// them. Below `floor` nothing counts. The whole work-group calls this; the result is in
-// sh.t, sh.above_count and sh.above_weight.
-template <typename T, bool WEIGHT>
-__device__ __forceinline__ void RowSearch(const SampleParams& p, int row, int chunks,
-                                          int quarters, const unsigned* most, RowShared& sh,
-                                          Source* from, const RowState* state, const Weigher& w,
-                                          int shift, unsigned best, unsigned floor, u64 want) {
-  constexpr int kBins = kList;
-  const int tid = threadIdx.x, lane = tid % kWave;
-  u64 above_weight = 0, above_count = 0;
-  // The bin in which the sums of the bins (0 is the top one) reach: two bins a thread.
-  const auto find = [&] {
-    static_assert(kBins == 2 * kRowThreads, "two bins a thread");
-    __syncthreads();
-    const u64 w0 = sh.weights[2 * tid], w1 = sh.weights[2 * tid + 1];
-    const unsigned c0 = sh.counts[2 * tid], c1 = sh.counts[2 * tid + 1];
-    u64 weight_to = WaveScan(w0 + w1);
-    u64 count_to = WaveScan(static_cast<unsigned>(c0 + c1));
-    if (lane == kWave - 1) {
-      sh.slots[tid / kWave] = weight_to;
-      sh.count_slots[tid / kWave] = count_to;
-    }
-    __syncthreads();
-    weight_to += above_weight;
-    count_to += above_count;
+// The bin (0 is the top one) in which the sums of sh.counts, or of sh.weights, reach
+// `want` from what is above them; sh.bin, and what is above it in sh.above_count and
+// sh.above_weight. Two bins a thread; the whole work-group calls this.
+__device__ __forceinline__ void FindBin(RowShared& sh, bool by_weight, u64 want, u64 above_count,
+                                        u64 above_weight) {
+  static_assert(kList == 2 * kRowThreads, "two bins a thread");
+  const int tid = threadIdx.x, wave = WaveIndex();
+  __syncthreads();
+  const u64 w0 = sh.weights[2 * tid], w1 = sh.weights[2 * tid + 1];
+  const unsigned c0 = sh.counts[2 * tid], c1 = sh.counts[2 * tid + 1];
+  u64 weight_to = WaveScan(w0 + w1), count_to = WaveScan(c0 + c1);
+  if (tid % kWave == kWave - 1) {
+    sh.slots[wave] = weight_to;
+    sh.count_slots[wave] = count_to;
+  }
+  __syncthreads();
+  weight_to += above_weight;
+  count_to += above_count;
+  for (int i = 0; i < wave; ++i) {
+    weight_to += sh.slots[i];
+    count_to += sh.count_slots[i];
+  }
+  const u64 weight = weight_to - w0 - w1, count = count_to - c0 - c1;
+  const u64 to = by_weight ? weight_to : count_to, from = by_weight ? weight : count;
+  // The last bin takes what fewer keys or the sums' rounding leave.
+  if ((to >= want && (from < want || tid == 0)) || (tid == kRowThreads - 1 && to < want)) {
+    const bool second = (by_weight ? weight + w0 : count + c0) < want;
+    sh.bin = 2 * tid + second;
+    sh.above_weight = weight + (second ? w0 : 0);
+    sh.above_count = count + (second ? c0 : 0);
+  }
+  __syncthreads();
+}
+
+// The list of the row's keys from `floor` on, of the quarters that have any; false where
+// it does not hold them. The whole work-group calls this.
+template <typename T>
+__device__ __forceinline__ bool Gather(const RowCall& c, int row, RowShared& sh, unsigned floor) {
+  const int wave = WaveIndex();
+  const float from = LogitOf(max(floor, kKeyOfMinusInf + 1));
+  if (threadIdx.x == 0) {
+    sh.listed = 0;
+    sh.opened = 0;
+  }
+  __syncthreads();
+  for (int q = threadIdx.x; q < c.quarters; q += kRowThreads)
+    if (sh.most[q] >= floor)
+      sh.open[atomicAdd(&sh.opened, 1u)] = static_cast<unsigned short>(q);
+  __syncthreads();
+  const int opened = static_cast<int>(sh.opened);
+  constexpr int kAtOnce = 4;  // quarters' loads of a wave
+#pragma unroll 1
+  for (int o = wave; o < opened; o += kAtOnce * kRowWaves) {
+    float z[kAtOnce][kRun];
 #pragma unroll
-    for (int i = 0; i < kRowWaves; ++i) {
-      const bool before = i < tid / kWave;
-      weight_to += before ? sh.slots[i] : 0;
-      count_to += before ? sh.count_slots[i] : 0;
-    }
-    const u64 weight = weight_to - w0 - w1, count = count_to - c0 - c1;
-    const u64 to = WEIGHT ? weight_to : count_to, from_here = WEIGHT ? weight : count;
-    // The last bin takes what fewer keys or the sums' rounding leave.
-    if ((to >= want && (from_here < want || tid == 0)) || (tid == kRowThreads - 1 && to < want)) {
-      const bool second = (WEIGHT ? weight + w0 : count + c0) < want;
-      sh.bin = 2 * tid + second;
-      sh.above_weight = weight + (second ? w0 : 0);
-      sh.above_count = count + (second ? c0 : 0);
-    }
-    __syncthreads();
-    above_weight = sh.above_weight;
-    above_count = sh.above_count;
-    return sh.bin;
-  };
-  const auto pass = [&](const Source& source, auto&& bin_of) {
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kRowThreads) {
-      sh.weights[i] = 0;
-      sh.counts[i] = 0;
-    }
-    __syncthreads();
-    EachKey<T>(p, row, chunks, sh, source, [&](unsigned key, int) {
-      const int bin = bin_of(key);
-      if (key >= floor && bin < kBins) {
-        atomicAdd(&sh.counts[bin], 1u);
-        if constexpr (WEIGHT)
-          atomicAdd(&sh.weights[bin], UnitsOf(w(key), shift));
+    for (int i = 0; i < kAtOnce; ++i)
+      LoadLogits<T>(c.p, row, sh.open[min(o + i * kRowWaves, opened - 1)], z[i]);
+#pragma unroll 1
+    for (int i = 0; i < kAtOnce && o + i * kRowWaves < opened; ++i) {
+      float v[kRun];
+      unsigned mine = 0;
+#pragma unroll
+      for (int e = 0; e < kRun; ++e) {
+        const float front = i == 0 ? z[0][e] : z[1][e], back = i == 2 ? z[2][e] : z[3][e];
+        v[e] = i < 2 ? front : back;
+        mine += v[e] >= from;
       }
-    });
-    return find();
-  };
-  const Steps steps = StepsOf(w);
-  int first;
-  if (state != nullptr && !from->list) {
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kRowThreads) {
-      sh.weights[i] = state->weights[i];
-      sh.counts[i] = state->counts[i];
+      if (__ballot(mine != 0) == 0)
+        continue;
+      const int start = RunStart(sh.open[o + i * kRowWaves], c.p.vocab);
+      unsigned at = mine != 0 ? atomicAdd(&sh.listed, mine) : 0;
+#pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        if (v[e] >= from) {
+          if (at < kList)
+            sh.list[at] = static_cast<u64>(KeyOf(v[e])) << 32 | static_cast<unsigned>(start + e);
+          ++at;
+        }
     }
-    first = find();
-  } else {
-    first = pass(*from, steps);
-  }
-  const unsigned held = sh.counts[first];
-  unsigned low = max(steps.Least(best, first), floor);
-  unsigned high = first == 0 ? best : steps.Least(best, first - 1) - 1;
-  Source source = *from;
-  if (!from->list && held <= kList && low < high) {
-    const bool all = above_count + held <= kList;
-    source.list = Gather<T>(p, row, quarters, sh, most, low, all ? best : high);
-    source.count = static_cast<int>(sh.listed);
-    if (all)
-      *from = source;
-  }
-  while (low < high) {
-    const int bits = 32 - __builtin_clz(high - low);
-    const int down = bits > 11 ? bits - 11 : 0;
-    const int bin = pass(source, [&](unsigned key) {
-      return key >= low && key <= high ? static_cast<int>((high - key) >> down) : kBins;
-    });
-    high -= min(static_cast<unsigned>(bin) << down, high - low);
-    low = max(low, down == 0 ? high : high - min(high, (1u << down) - 1));
   }
   __syncthreads();
-  if (tid == 0)
-    sh.t = high;
-  __syncthreads();
+  return sh.listed <= kList;
 }
 
 // For every element of a list, what `ahead` of it others count and weigh, added to
 // sh.rank and sh.before: a wave has 64 elements and a part of the others.
 template <typename F>
 __device__ __forceinline__ void RankList(RowShared& sh, int listed, F&& ahead) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = WaveIndex();
   const int groups = (listed + kWave - 1) / kWave, parts = kRowWaves / groups;
   const int part = wave / groups, e = wave % groups * kWave + lane;
   if (part >= parts)
@@ -905,6 +1014,7 @@ __device__ __forceinline__ void RankList(RowShared& sh, int listed, F&& ahead) {
   const u64 mine = sh.list[min(e, listed - 1)];
   int rank = 0;
   u64 before = 0;
+#pragma unroll 2
   for (int i = part; i < listed; i += parts) {
     const bool in = ahead(sh.list[i], mine);
     rank += in;
@@ -917,229 +1027,84 @@ __device__ __forceinline__ void RankList(RowShared& sh, int listed, F&& ahead) {
 }
 
 // The draw from a short list, an element a thread; false where the list does not hold the
-// share. The whole work-group calls this.
+// share of `whole` (0: of itself). The whole work-group calls this.
 __device__ __forceinline__ bool DrawFromList(const SampleParams& p, int row, RowShared& sh,
                                              int listed, const Settings& s, const Weigher& w,
-                                             int shift, double all) {
+                                             int shift, double whole_row) {
   static_assert(kShortList <= kRowThreads && kShortList <= kRowWaves * kWave, "elements");
   const int e = threadIdx.x;
   const bool there = e < listed, share = s.top_p < 1.0F;
-  const auto total = [&](u64 v) {
-    return RowJoin(WaveSum64(v), sh.slots, [](u64 a, u64 b) { return a + b; });
-  };
-  u64 whole = static_cast<u64>(ldexp(all, shift));
+  u64 whole = static_cast<u64>(ldexp(whole_row, shift));
   if (s.top_k > 0)  // few elements take finer units, where they are all that counts
     shift = 51;
   const u64 element = there ? sh.list[e] : 0;
   const double weight = w(static_cast<unsigned>(element >> 32));
   const u64 unit = UnitsOf(weight, shift);
-  if (share && s.top_k == 0 && total(unit) < ShareOf(s.top_p, whole))
-    return false;
-  if (e < kShortList) {
-    sh.unit[e] = unit;
-    sh.rank[e] = 0;
-    sh.before[e] = 0;
+  // What is kept: first the elements' ranks by key, then the weights before them by index.
+  u64 kept = unit, target = 0;
+  int rank = 0;
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {
+    const u64 all = RowSum<kRowWaves>(kept, sh.slots);
+    if (turn == 0) {
+      if (share && s.top_k == 0 && all < ShareOf(s.top_p, whole))
+        return false;
+    } else {
+      target = TargetOf(s.u, all);
+    }
+    if (e < kShortList) {
+      sh.unit[e] = kept;
+      sh.rank[e] = 0;
+      sh.before[e] = 0;
+    }
+    __syncthreads();
+    // Ahead are larger keys and equal ones of smaller index; then smaller indices.
+    RankList(sh, listed, [&](u64 other, u64 mine) {
+      return turn == 0 ? (other ^ 0xFFFFFFFFu) > (mine ^ 0xFFFFFFFFu)
+                       : static_cast<unsigned>(other) < static_cast<unsigned>(mine);
+    });
+    __syncthreads();
+    const u64 before = there ? sh.before[e] : 0;
+    if (turn == 0) {
+      rank = there ? sh.rank[e] : kList;
+      const int most = s.top_k > 0 ? s.top_k : listed;
+      if (s.top_k > 0 && share)
+        whole = RowSum<kRowWaves>(rank < most ? unit : 0, sh.slots);
+      const bool in = rank < most && (!share || before < ShareOf(s.top_p, whole)) &&
+                      weight >= fmin(static_cast<double>(s.min_p), 1.0);
+      kept = in || rank == 0 ? unit : 0;
+    } else if (there && before <= target && target < before + kept) {
+      p.tokens[row] = static_cast<int>(element);
+    }
   }
-  __syncthreads();
-  // Ahead are larger keys and equal ones of smaller index.
-  RankList(sh, listed, [](u64 other, u64 mine) {
-    return (other ^ 0xFFFFFFFFu) > (mine ^ 0xFFFFFFFFu);
-  });
-  __syncthreads();
-  const int rank = there ? sh.rank[e] : kList;
-  const u64 before = there ? sh.before[e] : 0;
-  const int most = s.top_k > 0 ? s.top_k : listed;
-  if (s.top_k > 0 && share)
-    whole = total(rank < most ? unit : 0);
-  const double least = fmin(static_cast<double>(s.min_p), 1.0);
-  const bool in = rank < most && (!share || before < ShareOf(s.top_p, whole)) && weight >= least;
-  const u64 kept = in || rank == 0 ? unit : 0;
-  const u64 target = TargetOf(s.u, total(kept));
-  if (there) {
-    sh.unit[e] = kept;
-    sh.before[e] = 0;
-  }
-  __syncthreads();
-  RankList(sh, listed, [](u64 other, u64 mine) {
-    return static_cast<unsigned>(other) < static_cast<unsigned>(mine);
-  });
-  __syncthreads();
-  if (there && sh.before[e] <= target && target < sh.before[e] + kept)
-    p.tokens[row] = static_cast<int>(element);
   return true;
 }
 
-// The chunk's kept weight: above the threshold, and how many equal it. A wave's.
+// The sums of the logit's steps of the row's chunks from `first` on, added to its state
+// by a work-group.
 template <typename T>
-__device__ __forceinline__ void KeptOfChunk(const SampleParams& p, int row, int c, unsigned t,
-                                            const Weigher& w, double* weight, unsigned* equals) {
-  double sum = 0.0;
-  unsigned equal = 0;
-  float z[kQuarters][kRun];
-#pragma unroll
-  for (int q = 0; q < kQuarters; ++q)
-    LoadLogits<T>(p, row, c * kQuarters + q, z[q]);
-#pragma unroll
-  for (int q = 0; q < kQuarters; ++q)
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      const unsigned key = KeyOf(z[q][i]);
-      if (key > t)
-        sum += w(key);
-      equal += key == t;
-    }
-  sum = WaveSum64(sum);
-  const u64 n = WaveSum64(static_cast<u64>(equal));
-  if (threadIdx.x % kWave == 0) {
-    *weight = sum;
-    *equals = static_cast<unsigned>(n);
-  }
-}
-
-// The draw by the chunks' kept weights: one wave finds the chunk, 64 at a time, then the
-// place in it. Without a threshold (t is 0) `all` is what is kept.
-template <typename T>
-__device__ __forceinline__ void Pick(const SampleParams& p, int row, int chunks,
-                                     const double* weights, const unsigned* equals,
-                                     const Settings& s, const Weigher& w, unsigned t, u64 need0,
-                                     double all) {
-  const int lane = threadIdx.x % kWave;
-  const bool chunked = t == 0;
-  const double each = chunked ? 0.0 : w(t);
-  // The kept weight of the lane's chunk and the equals before it, of 64 chunks with `need`
-  // equals left.
-  const auto chunk_weight = [&](int c, u64 need, u64* equal_to, u64* equal_before) {
-    const unsigned equal = c < chunks && !chunked ? equals[c] : 0;
-    *equal_to = chunked ? 0 : WaveScan(static_cast<u64>(equal));
-    *equal_before = *equal_to - equal;
-    const u64 in = need > *equal_before ? min(need - *equal_before, static_cast<u64>(equal)) : 0;
-    return (c < chunks ? weights[c] : 0.0) + static_cast<double>(in) * each;
-  };
-  const auto last_lane = [](double v) {
-    return __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, v), kWave - 1));
-  };
-  u64 need = need0, equal_to, equal_before;
-  double total = all;
-  if (!chunked) {
-    total = 0.0;
-    for (int c0 = 0; c0 < chunks; c0 += kWave) {
-      total += WaveSum64(chunk_weight(c0 + lane, need, &equal_to, &equal_before));
-      need -= min(need, Lane64(equal_to, kWave - 1));
-    }
-  }
-  double left = static_cast<double>(fminf(fmaxf(s.u, 0.0F), 1.0F)) * total;
-  if (!(left < total))
-    left = total * (1.0 - 0x1p-53);
-  need = need0;
-  bool done = false;
-  double before = 0.0;
-  int last = 0;  // the chunk; the last one that keeps any where rounding leaves none
-  double last_before = 0.0;
-  u64 last_need = 0;
-  for (int c0 = 0; c0 < chunks && !done; c0 += kWave) {
-    const double mine = chunk_weight(c0 + lane, need, &equal_to, &equal_before);
-    const double to = before + WaveScan(mine);
-    const u64 hit = __ballot(mine > 0.0 && to > left);
-    const u64 any = __ballot(mine > 0.0);
-    if (any != 0) {
-      const int l = hit != 0 ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
-      last = c0 + l;
-      last_before = __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, to - mine), l));
-      last_need = need - min(need, Lane64(equal_before, l));
-    }
-    done = hit != 0;
-    before = last_lane(to);
-    need -= min(need, Lane64(equal_to, kWave - 1));
-  }
-  left -= last_before;
-  need = last_need;
-  unsigned key[kQuarters][kRun];
-#pragma unroll
-  for (int q = 0; q < kQuarters; ++q)
-    LoadKeys<T>(p, row, last * kQuarters + q, key[q]);
-  int token = -1, most_of = -1;  // the last kept one, where rounding leaves none
-#pragma unroll
-  for (int q = 0; q < kQuarters; ++q) {
-    if (token >= 0)
-      break;
-    unsigned equal = 0;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i)
-      equal += !chunked && key[q][i] == t;
-    const unsigned equals_to = __ballot(equal != 0) != 0 ? WaveScan(equal) : 0;
-    u64 seen = equals_to - equal;
-    double to_place[kRun], mine = 0.0;
-    int end = -1;  // the lane's last kept one
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      const bool in = chunked || key[q][i] > t || (key[q][i] == t && seen++ < need);
-      const double weight = in ? w(key[q][i]) : 0.0;
-      end = weight > 0.0 ? i : end;
-      mine += weight;
-      to_place[i] = mine;
-    }
-    const double to = WaveScan(mine);
-    const u64 hit = __ballot(mine > 0.0 && to > left);
-    const u64 any = __ballot(mine > 0.0);
-    int place = end;
-#pragma unroll
-    for (int i = kRun - 1; i >= 0; --i) {
-      const double before_it = i > 0 ? to_place[i - 1] : 0.0;
-      place = to_place[i] > before_it && (to - mine) + to_place[i] > left ? i : place;
-    }
-    place += RunStart(last * kQuarters + q, p.vocab);
-    if (any != 0) {
-      most_of = __builtin_amdgcn_readlane(place, hit != 0 ? __builtin_ctzll(hit)
-                                                          : 63 - __builtin_clzll(any));
-      token = hit != 0 ? most_of : -1;
-    }
-    left -= last_lane(to);
-    need -= min(need, static_cast<u64>(__builtin_amdgcn_readlane(equals_to, kWave - 1)));
-  }
-  if (lane == 0)
-    p.tokens[row] = token >= 0 ? token : most_of;
-}
-
-// The sums of the logit's steps of `row`'s chunks from `first` on, by a work-group.
-constexpr int kStepChunks = 16;  // of a work-group
-template <typename T>
-__device__ __forceinline__ void AddSteps(const SampleParams& p, int row, int chunks, int quarters,
-                                         int shift, int first, const Settings& s, RowShared& sh) {
-  RowState* const state = StateOf(p, row, chunks);
-  const Work work = WorkOf(p, row, chunks);
-  unsigned best = 0;
-  for (int i = threadIdx.x; i < quarters; i += kRowThreads)
-    best = max(best, work.most[i]);
+__device__ __forceinline__ void AddSteps(const RowCall& c, int row, RowState* state, int first,
+                                         const Settings& s, const Weigher& w, RowShared& sh) {
   for (int i = threadIdx.x; i < kList; i += kRowThreads) {
     sh.counts[i] = 0;
     sh.weights[i] = 0;
   }
-  best = RowJoin(WaveMaxKey(best), sh.slots, [](unsigned a, unsigned b) { return max(a, b); });
-  if (best == 0 || best >= kKeyOfInf)
-    return;
-  const Weigher w = WeigherOf(sh.powers, best, s.temperature);
+  __syncthreads();
   const Steps steps = StepsOf(w);
   const bool share = s.top_p < 1.0F;
-  const int c = first + static_cast<int>(threadIdx.x / kWave);
-  static_assert(kStepChunks == kRowWaves, "a wave a chunk");
-  if (c < chunks) {
-    float z[kQuarters][kRun];
-#pragma unroll
-    for (int q = 0; q < kQuarters; ++q)
-      LoadLogits<T>(p, row, c * kQuarters + q, z[q]);
-#pragma unroll
-    for (int q = 0; q < kQuarters; ++q)
+  const int chunk = first + WaveIndex();
+  if (chunk < c.chunks)
+    EachQuarter<T>(c.p, row, chunk, [&](int, const float (&z)[kRun]) {
 #pragma unroll
       for (int i = 0; i < kRun; ++i) {
-        const unsigned key = KeyOf(z[q][i]);
-        const int step = steps(key);
-        if (key != 0 && step < kList) {
+        const int step = steps(z[i]);
+        if (step < kList) {
           atomicAdd(&sh.counts[step], 1u);
           if (share)
-            atomicAdd(&sh.weights[step], UnitsOf(w(key), shift));
+            atomicAdd(&sh.weights[step], UnitsOf(w.Of(z[i]), c.shift));
         }
       }
-  }
+    });
   __syncthreads();
   for (int i = threadIdx.x; i < kList; i += kRowThreads)
     if (sh.counts[i] != 0) {
@@ -1149,258 +1114,363 @@ __device__ __forceinline__ void AddSteps(const SampleParams& p, int row, int chu
     }
 }
 
-// kWhole: a row from the chunks' numbers to its token. Else the row's passes are spread
-// over work-groups and launches of their own: kFirst does what needs none, while other
-// work-groups sum the steps of rows that may search, kSearch finds the threshold from
-// the sums, kPick draws from the chunks' kept weights.
-// kPlain: rows of which none has a filter.
-enum class Phase { kPlain, kWhole, kFirst, kSearch, kPick };
-constexpr int ThreadsOf(Phase phase) {
-  return phase == Phase::kPlain ? kThreads : phase == Phase::kPick ? kWave : kRowThreads;
-}
-
-template <typename T, Phase PHASE>
-__global__ __launch_bounds__(ThreadsOf(PHASE)) void RowKernel(SampleParams p, int chunks, int quarters,
-                                                         int shift) {
+// A row's first work-group draws what needs no threshold, or from a short list; the
+// others sum the steps of rows that will need it.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void FirstKernel(RowCall c) {
   __shared__ RowShared sh;
-  __builtin_assume(p.vocab > kChunk);
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int row = blockIdx.x % p.rows;
-  if (PHASE == Phase::kFirst && static_cast<int>(blockIdx.x) >= p.rows) {
-    const Settings s = SettingsOf(p, row);
-    if (!s.Searches(quarters))
-      return;
-    FillTable(sh.powers);
-    AddSteps<T>(p, row, chunks, quarters, shift,
-                (static_cast<int>(blockIdx.x) / p.rows - 1) * kStepChunks, s, sh);
+  __builtin_assume(c.p.vocab > kChunk);
+  const int tid = threadIdx.x, lane = tid % kWave, wave = WaveIndex();
+  const int at = blockIdx.x % c.rows, row = c.first + at, part = blockIdx.x / c.rows;
+  const Settings s = SettingsOf(c.p, row);
+  const bool share = s.top_p < 1.0F, ranked = c.quarters <= kMostQuarters;
+  const int opened = s.top_k > 0 ? s.top_k : kShareOpened;
+  const bool short_list = ranked && opened <= min(kMostOpened, c.quarters);
+  const bool searches = (s.top_k > 0 && !short_list) || (s.top_k == 0 && share);
+  if (part > 0 && (s.lost || s.greedy || !searches))
     return;
-  }
-  constexpr int kGroup = ThreadsOf(PHASE), kGroupWaves = kGroup / kWave;
-  constexpr bool kOwn = PHASE == Phase::kPlain || PHASE == Phase::kWhole;
-  RowState* const state = kOwn ? nullptr : StateOf(p, row, chunks);
-  if (PHASE == Phase::kSearch && state->status != RowState::kSearch)
-    return;
-  if (PHASE == Phase::kPick && state->status != RowState::kPick)
-    return;
-  const Settings s = SettingsOf(p, row);
-  const Work work = WorkOf(p, row, chunks);
+  RowState* const state = StateOf(c, at);
+  const Work work = WorkOf(c.p, row, c.chunks);
   FillTable(sh.powers);
-  // The chunks' and quarters' numbers, in LDS where they fit.
-  double* const weights =
-      chunks <= kList ? reinterpret_cast<double*>(sh.weights) : work.weight;
-  unsigned* const equals = chunks <= kList ? sh.counts : work.equal;
-  const bool ranked = quarters <= kMostQuarters;
-  const unsigned* const most = ranked ? sh.most : work.most;
-  if (PHASE == Phase::kFirst && tid == 0)
-    state->status = RowState::kDone;
-
-  if constexpr (PHASE == Phase::kPick) {
-    __syncthreads();
-    if (wave == 0)
-      Pick<T>(p, row, chunks, work.weight, work.equal, s,
-              WeigherOf(sh.powers, state->best, s.temperature), state->t, state->need, 0.0);
+  const unsigned best = BestOf<kRowWaves>(work, c.quarters, sh.most, sh.slots);
+  if (best == 0 || best >= kKeyOfInf || s.lost) {
+    if (part == 0 && tid == 0)
+      c.p.tokens[row] = -1;
     return;
   }
-  unsigned best = 0;
-  for (int i = tid; i < quarters; i += kGroup) {
-    const unsigned m = work.most[i];
-    if (ranked)
-      sh.most[i] = m;
-    best = max(best, m);
-  }
-  best = RowJoin<kGroupWaves>(WaveMaxKey(best), sh.slots, [](unsigned a, unsigned b) { return max(a, b); });
-  if (best == 0 || best >= kKeyOfInf || s.lost) {
-    if (tid == 0)
-      p.tokens[row] = -1;
+  const Weigher w = WeigherOf(sh.powers, best, s.greedy ? 1.0F : s.temperature);
+  if (part > 0) {
+    AddSteps<T>(c, row, state, (part - 1) * kRowWaves, s, w, sh);
     return;
   }
   if (s.greedy) {
-    unsigned first = ~0u;
-    for (int i = tid; i < quarters && first == ~0u; i += kGroup)
-      if (most[i] == best)
-        first = i;
-    first = RowJoin<kGroupWaves>(WaveMinKey(first), sh.slots,
-                    [](unsigned a, unsigned b) { return min(a, b); });
-    if (wave == 0) {
-      unsigned key[kRun];
-      LoadKeys<T>(p, row, static_cast<int>(first), key);
-      unsigned token = ~0u;
-#pragma unroll
-      for (int i = kRun - 1; i >= 0; --i)
-        token = key[i] == best ? RunStart(static_cast<int>(first), p.vocab) + i : token;
-      token = WaveMinKey(token);
-      if (lane == 0)
-        p.tokens[row] = static_cast<int>(token);
-    }
+    DrawBest<T, kRowWaves>(c, row, work, best, sh.slots);
     return;
   }
-
-  const Weigher w = WeigherOf(sh.powers, best, s.temperature);
-  const bool share = s.top_p < 1.0F;
-  // The whole row's weight, where the first launch left the chunks'.
-  double all = 0.0;
+  double whole = 0.0;
   if (s.top_k == 0) {
-    for (int i = tid; i < chunks; i += kGroup) {
-      unsigned top = 0;
-      for (int q = i * kQuarters; q < min((i + 1) * kQuarters, quarters); ++q)
-        top = max(top, most[q]);
-      const double sum = work.weight[i] * w(top);
-      weights[i] = sum;
-      all += sum;
-    }
-    all = RowJoin<kGroupWaves>(WaveSum64(all), sh.slots, [](double a, double b) { return a + b; });
-  }
-  if (PHASE == Phase::kPlain || (s.top_k == 0 && !share && !(s.min_p > 0.0F))) {
-    __threadfence_block();
-    __syncthreads();
-    if (wave == 0)
-      Pick<T>(p, row, chunks, weights, equals, s, w, 0, 0, all);
-    return;
-  }
-
-  if constexpr (PHASE != Phase::kPlain && PHASE != Phase::kPick) {
-    Kept kept{1, kAll, 0};
-    Source from{false, 0};
-    bool known = s.top_k == 0 && !share;  // min_p says the threshold itself
-    if (known)
-      kept.t = KeyOfShare(w, best, s.min_p);
-    const int opened = s.top_k > 0 ? s.top_k : kShareOpened;
-    if (PHASE != Phase::kSearch && ranked && (known || (opened <= kMostOpened && opened <= quarters))) {
-      unsigned floor = kept.t;
-      if (!known) {
-        // What reaches the last of the loudest quarters.
-        Held<8> loud;  // of up to 262144 tokens; every wave by itself
-        loud.used = min((quarters + kWave - 1) / kWave, 8);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          loud.key[i] = i * kWave + lane < quarters ? sh.most[i * kWave + lane] : 0;
-        floor = Held<8>::Search(1, best, [&](unsigned t) {
-          int n = loud.Count(t);
-          for (int i = 8 * kWave; i < quarters; i += kWave)
-            n += __popcll(__ballot(i + lane < quarters && sh.most[i + lane] >= t));
-          return n >= opened;
-        });
-      }
-      const bool fits = Gather<T>(p, row, quarters, sh, most, floor, best);
-      const int listed = static_cast<int>(sh.listed);
-      if (listed <= kShortList && DrawFromList(p, row, sh, listed, s, w, shift, all))
-        return;
-      if (fits && (known || s.top_k > 0))
-        from = Source{true, listed};
-    }
-    if (PHASE == Phase::kFirst && !from.list) {
-      // The row's passes are the next launches.
-      if (tid == 0) {
-        state->status = known ? RowState::kPick : RowState::kSearch;
-        state->best = best;
-        state->t = kept.t;
-        state->need = kept.need;
-      }
+    whole = WholeOf<kRowWaves>(c, work, w, sh.slots);
+    if (!share && !(s.min_p > 0.0F)) {
+      __syncthreads();
+      if (wave == 0)
+        Pick<T>(c, row, work.weight, nullptr, s, w, 0, 0);
       return;
     }
-
+  }
+  const bool known = s.top_k == 0 && !share;  // min_p says the threshold itself
+  unsigned floor = known ? KeyOfShare(w, best, s.min_p) : 1;
+  if (ranked && (known || short_list)) {
     if (!known) {
-      const RowState* const sums =
-          PHASE == Phase::kSearch && s.Searches(quarters) ? state : nullptr;
-      u64 whole = s.top_k == 0 ? static_cast<u64>(ldexp(all, shift)) : 0;
-      if (s.top_k > 0) {
-        RowSearch<T, false>(p, row, chunks, quarters, most, sh, &from, sums, w, shift, best, 1,
-                            s.top_k);
-        kept.t = sh.t;
-        kept.need = s.top_k - sh.above_count;  // of those that there are
-        if (share) {
-          // The weight of what top_k keeps.
-          u64 sum = 0, equal = 0;
-          EachKey<T>(p, row, chunks, sh, from, [&](unsigned key, int) {
-            if (key > kept.t)
-              sum += UnitsOf(w(key), shift);
-            equal += key == kept.t;
-          });
-          const auto add = [](u64 a, u64 b) { return a + b; };
-          whole = RowJoin(WaveSum64(sum), sh.slots, add);
-          kept.need = min(kept.need, RowJoin(WaveSum64(equal), sh.slots, add));
-          whole += kept.need * UnitsOf(w(kept.t), shift);
-        }
-      }
-      if (share) {
-        const u64 want = ShareOf(s.top_p, whole);
-        RowSearch<T, true>(p, row, chunks, quarters, most, sh, &from, sums, w, shift, best, kept.t,
-                           want);
-        const u64 each = UnitsOf(w(sh.t), shift);
-        const u64 need = each > 0 && want > sh.above_weight
-                             ? (want - sh.above_weight + each - 1) / each
-                             : kAll;
-        kept.need = sh.t > kept.t ? need : min(kept.need, need);
-        kept.t = max(sh.t, kept.t);
-      }
-      if (s.min_p > 0.0F) {
-        const unsigned t = KeyOfShare(w, best, s.min_p);
-        if (t > kept.t) {
-          kept.t = t;
-          kept.need = kAll;
-        }
+      // What reaches the last of the loudest quarters: the largest key that `opened` of
+      // them reach, between ever closer borders, of which every wave counts one.
+      unsigned high = best;
+#pragma unroll 1
+      while (floor < high) {
+        const unsigned step = (high - floor + kRowWaves - 1) / kRowWaves;
+        const unsigned border = min(floor + step * (wave + 1), high);
+        int n = 0;
+        for (int i = lane; i < c.quarters; i += kWave)
+          n += sh.most[i] >= border;
+        n = static_cast<int>(WaveSum64(static_cast<u64>(n)));
+        if (lane == 0)
+          sh.count_slots[wave] = n;
+        __syncthreads();
+        unsigned reached = 0;
+#pragma unroll
+        for (int i = 0; i < kRowWaves; ++i)
+          reached += static_cast<int>(sh.count_slots[i]) >= opened;
+        __syncthreads();
+        // `reached` borders are; the one behind them, if any, is not.
+        const unsigned above =
+            reached == kRowWaves ? high : min(floor + step * (reached + 1), high) - 1;
+        floor = min(floor + step * reached, high);
+        high = max(above, floor);
       }
     }
-    // The chunks' kept weights.
-    __syncthreads();
-    if (from.list && chunks <= kList) {
-      for (int i = tid; i < chunks; i += kRowThreads) {
-        sh.weights[i] = 0;
-        equals[i] = 0;
-      }
-      __syncthreads();
-      EachKey<T>(p, row, chunks, sh, from, [&](unsigned key, int index) {
-        if (key > kept.t)
-          atomicAdd(&sh.weights[index / kChunk], UnitsOf(w(key), shift));
-        else if (key == kept.t)
-          atomicAdd(&equals[index / kChunk], 1u);
-      });
-      __syncthreads();
-      for (int i = tid; i < chunks; i += kRowThreads)
-        weights[i] = ldexp(static_cast<double>(sh.weights[i]), -shift);
-    } else if (PHASE == Phase::kSearch) {
-      if (tid == 0) {
-        state->status = RowState::kPick;
-        state->t = kept.t;
-        state->need = kept.need;
-      }
+    Gather<T>(c, row, sh, floor);
+    const int listed = static_cast<int>(sh.listed);
+    if (listed <= kShortList && DrawFromList(c.p, row, sh, listed, s, w, c.shift, whole))
       return;
-    } else {
-      for (int c = wave; c < chunks; c += kRowWaves)
-        KeptOfChunk<T>(p, row, c, kept.t, w, weights + c, equals + c);
-    }
-    if (PHASE == Phase::kSearch && tid == 0)
-      state->status = RowState::kDone;
-    __threadfence_block();
-    __syncthreads();
-    if (wave == 0)
-      Pick<T>(p, row, chunks, weights, equals, s, w, kept.t, kept.need, 0.0);
+  }
+  if (tid == 0) {
+    state->status = known ? RowState::kKnown : searches ? RowState::kCollect : RowState::kSlow;
+    state->best = best;
+    state->t = floor;
+    state->whole = static_cast<u64>(ldexp(whole, c.shift));
   }
 }
 
-// The chunks' kept weights of the rows that have their threshold.
+// Every chunk's weight above the steps in which the threshold is, and the list of the
+// elements in them. Each work-group finds the steps from the row's sums by itself.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void KeptKernel(SampleParams p, int chunks, int groups) {
-  __shared__ double powers[kTable];
-  __builtin_assume(p.vocab > kChunk);
-  const int row = blockIdx.x / groups;
-  const RowState* const state = StateOf(p, row, chunks);
-  if (state->status != RowState::kPick)
+__global__ __launch_bounds__(kRowThreads) void CollectKernel(RowCall c) {
+  __shared__ RowShared sh;
+  __builtin_assume(c.p.vocab > kChunk);
+  const int tid = threadIdx.x;
+  const int at = blockIdx.x % c.rows, row = c.first + at, part = blockIdx.x / c.rows;
+  RowState* const state = StateOf(c, at);
+  const unsigned status = state->status;
+  if (status != RowState::kCollect && status != RowState::kKnown)
     return;
-  const Settings s = SettingsOf(p, row);
-  const Work work = WorkOf(p, row, chunks);
-  FillTable(powers);
+  const Settings s = SettingsOf(c.p, row);
+  const bool share = s.top_p < 1.0F;
+  FillTable(sh.powers);
   __syncthreads();
-  const int c = (blockIdx.x - row * groups) * kWaves + threadIdx.x / kWave;
-  if (c < chunks)
-    KeptOfChunk<T>(p, row, c, state->t, WeigherOf(powers, state->best, s.temperature),
-                   work.weight + c, work.equal + c);
+  const Weigher w = WeigherOf(sh.powers, state->best, s.temperature);
+  const Steps steps = StepsOf(w);
+  int k_step = kList, low_step = kList, high_step = -1;
+  bool raised = false;  // to what is kept from `from` on
+  float from = 0.0F;
+  if (status == RowState::kKnown) {
+    raised = true;
+    from = LogitOf(state->t);
+  } else {
+    for (int i = tid; i < kList; i += kRowThreads) {
+      sh.counts[i] = state->counts[i];
+      sh.weights[i] = state->weights[i];
+    }
+    u64 least = state->whole, most = state->whole;  // of what the share is of
+    u64 k_count = 0, k_weight = 0;
+    if (s.top_k > 0) {
+      FindBin(sh, false, s.top_k, 0, 0);
+      k_step = low_step = high_step = sh.bin;
+      k_count = sh.above_count;
+      k_weight = least = sh.above_weight;
+      most = k_weight + sh.weights[k_step];
+    }
+    if (share) {
+      FindBin(sh, true, ShareOf(s.top_p, most), 0, 0);
+      high_step = min(sh.bin, k_step);
+      FindBin(sh, true, ShareOf(s.top_p, max(least, u64{1})), 0, 0);
+      low_step = min(sh.bin, high_step);
+    }
+    unsigned elements = k_step < kList && (k_step < low_step || k_step > high_step)
+                            ? sh.counts[k_step] : 0;
+    u64 low_count = 0, low_weight = 0;
+    for (int i = tid; i < low_step; i += kRowThreads) {
+      low_count += sh.counts[i];
+      low_weight += sh.weights[i];
+    }
+    low_count = RowSum<kRowWaves>(low_count, sh.slots);
+    low_weight = RowSum<kRowWaves>(low_weight, sh.slots);
+    for (int i = low_step; i <= high_step; ++i)
+      elements += sh.counts[i];
+    if (part == 0 && tid == 0) {
+      state->k_step = k_step;
+      state->low_step = low_step;
+      state->high_step = high_step;
+      state->k_count = k_count;
+      state->k_weight = k_weight;
+      state->low_count = low_count;
+      state->low_weight = low_weight;
+    }
+    // The row's work-groups all see the same; the first one tells the next launch.
+    if (s.min_p > 0.0F) {
+      const unsigned t = KeyOfShare(w, state->best, s.min_p);
+      raised = steps(LogitOf(t)) < low_step;
+      from = LogitOf(t);
+      if (raised && part == 0 && tid == 0)
+        state->raised = t;
+    }
+    if (!raised && elements > kList) {
+      if (part == 0 && tid == 0)
+        state->listed = kList + 1;
+      return;
+    }
+  }
+  const int chunk = part * kRowWaves + WaveIndex();
+  if (chunk >= c.chunks)
+    return;
+  double sum = 0.0;
+  EachQuarter<T>(c.p, row, chunk, [&](int start, const float (&z)[kRun]) {
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int step = steps(z[i]);
+      if (raised ? z[i] >= from : step < low_step)
+        sum += w.Of(z[i]);
+      if (!raised && step < kList && ((step >= low_step && step <= high_step) || step == k_step)) {
+        const unsigned to = atomicAdd(&state->listed, 1u);
+        state->list[min(to, kList - 1u)] =
+            static_cast<u64>(KeyOf(z[i])) << 32 | static_cast<unsigned>(start + i);
+      }
+    }
+  });
+  sum = WaveSum64(sum);
+  if (tid % kWave == 0)
+    WorkOf(c.p, row, c.chunks).weight[chunk] = sum;
 }
 
-// Whether the rows' passes are launches of their own: where the rows do not fill the
-// device by themselves.
-bool SplitRows(std::int64_t rows, std::int64_t chunks) {
-  return rows <= kSplitRows && chunks <= kList;
+// The threshold from the list of the steps that hold it, or from passes over the row, and
+// the draw.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
+  __shared__ RowShared sh;
+  __builtin_assume(c.p.vocab > kChunk);
+  const int tid = threadIdx.x, lane = tid % kWave, wave = WaveIndex();
+  const int row = c.first + blockIdx.x;
+  RowState* const state = StateOf(c, blockIdx.x);
+  const unsigned status = state->status;
+  if (status == RowState::kDone)
+    return;
+  const Settings s = SettingsOf(c.p, row);
+  const unsigned best = state->best;
+  const Work work = WorkOf(c.p, row, c.chunks);
+  FillTable(sh.powers);
+  __syncthreads();
+  const Weigher w = WeigherOf(sh.powers, best, s.temperature);
+  const unsigned from = status == RowState::kKnown ? state->t : state->raised;
+  if (from != 0) {
+    if (wave == 0)
+      Pick<T>(c, row, work.weight, nullptr, s, w, from - 1, 0);
+    return;
+  }
+  const Steps steps = StepsOf(w);
+  const unsigned listed = state->listed;
+  const bool slow = status == RowState::kSlow || listed > kList;
+  const bool share = s.top_p < 1.0F;
+  if (!slow)
+    for (unsigned i = tid; i < listed; i += kRowThreads)
+      sh.list[i] = state->list[i];
+  __syncthreads();
+  // Calls f(key, index) for the listed elements, or the row's.
+  const auto each_key = [&](auto&& f) {
+    if (!slow) {
+      for (unsigned i = tid; i < listed; i += kRowThreads)
+        f(static_cast<unsigned>(sh.list[i] >> 32), static_cast<int>(sh.list[i]));
+      return;
+    }
+#pragma unroll 1
+    for (int q = wave; q < c.quarters; q += kRowWaves) {
+      float z[kRun];
+      LoadLogits<T>(c.p, row, q, z);
+      const int start = RunStart(q, c.p.vocab);
+#pragma unroll
+      for (int i = 0; i < kRun; ++i)
+        f(KeyOf(z[i]), start + i);
+    }
+  };
+  Kept kept{1, kAll, 0};
+  u64 whole = state->whole;
+  // First where top_k ends, then where the share does: sums of 2048 ranges of the keys
+  // that may hold the threshold, then of the range that does, until that is one key.
+#pragma unroll 1
+  for (int turn = s.top_k > 0 ? 0 : 1; turn < (share ? 2 : 1); ++turn) {
+    const bool by_weight = turn == 1;
+    const u64 want = by_weight ? ShareOf(s.top_p, whole) : s.top_k;
+    const int first_step = slow ? 0 : by_weight ? state->low_step : state->k_step;
+    const int last_step = slow ? kList : by_weight ? state->high_step : state->k_step;
+    u64 above_count = slow ? 0 : by_weight ? state->low_count : state->k_count;
+    u64 above_weight = slow ? 0 : by_weight ? state->low_weight : state->k_weight;
+    const unsigned floor = kept.t;
+    unsigned low = ~0u, high = 0;
+    each_key([&](unsigned key, int) {
+      const int step = steps(LogitOf(key));
+      if (key >= floor && step >= first_step && step <= last_step) {
+        low = min(low, key);
+        high = max(high, key);
+      }
+    });
+    low = RowJoin<kRowWaves>(WaveMinKey(low), sh.slots,
+                             [](unsigned a, unsigned b) { return min(a, b); });
+    high = RowJoin<kRowWaves>(WaveMaxKey(high), sh.slots,
+                              [](unsigned a, unsigned b) { return max(a, b); });
+    low = min(low, high);
+    bool one = false;
+#pragma unroll 1
+    while (!one) {
+      const int bits = high == low ? 0 : 32 - __builtin_clz(high - low);
+      const int down = bits > 11 ? bits - 11 : 0;
+      __syncthreads();
+      for (int i = tid; i < kList; i += kRowThreads) {
+        sh.weights[i] = 0;
+        sh.counts[i] = 0;
+      }
+      __syncthreads();
+      each_key([&](unsigned key, int) {
+        if (key >= low && key <= high && key != 0) {
+          const unsigned bin = (high - key) >> down;
+          atomicAdd(&sh.counts[bin], 1u);
+          atomicAdd(&sh.weights[bin], UnitsOf(w(key), c.shift));
+        }
+      });
+      FindBin(sh, by_weight, want, above_count, above_weight);
+      const unsigned bin = sh.bin;
+      above_count = sh.above_count;
+      above_weight = sh.above_weight;
+      high -= min(bin << down, high - low);
+      low = max(low, high - min(high, (1u << down) - 1));
+      one = down == 0;
+    }
+    const u64 equal = sh.counts[sh.bin], each = UnitsOf(w(high), c.shift);
+    u64 need = equal;
+    if (!by_weight)
+      need = min(need, want - min(want, above_count));
+    else if (each > 0)
+      need = min(need, (want - min(want, above_weight) + each - 1) / each);
+    if (by_weight && high == kept.t)
+      need = min(need, kept.need);
+    kept = Kept{high, need, 0};
+    whole = above_weight + need * each;  // what top_k keeps
+    __syncthreads();
+  }
+  if (s.min_p > 0.0F) {
+    const unsigned t = KeyOfShare(w, best, s.min_p);
+    if (t > kept.t)
+      kept = Kept{t, kAll, 0};
+  }
+  // The chunks' kept weights: above the listed steps by the launch before, and the list's.
+  const bool held = c.chunks <= kList;  // in LDS
+  double* const weights = reinterpret_cast<double*>(sh.weights);
+  if (!slow && held) {
+    __syncthreads();
+    for (int i = tid; i < c.chunks; i += kRowThreads) {
+      sh.weights[i] = 0;
+      sh.counts[i] = 0;
+    }
+    __syncthreads();
+    const int first_step = state->low_step;
+    each_key([&](unsigned key, int index) {
+      if (steps(LogitOf(key)) < first_step)
+        return;
+      if (key > kept.t)
+        atomicAdd(&sh.weights[index / kChunk], UnitsOf(w(key), c.shift));
+      else if (key == kept.t)
+        atomicAdd(&sh.counts[index / kChunk], 1u);
+    });
+    __syncthreads();
+    for (int i = tid; i < c.chunks; i += kRowThreads)
+      weights[i] = work.weight[i] + ldexp(static_cast<double>(sh.weights[i]), -c.shift);
+    __syncthreads();
+    if (wave == 0)
+      Pick<T>(c, row, weights, sh.counts, s, w, kept.t, kept.need);
+    return;
+  }
+  // The whole row once more, for its chunks above the threshold and the equals. The equals
+  // take the place of the quarters' largest keys, which are no longer needed.
+  unsigned* const equals = work.most;
+  const float border = LogitOf(kept.t);
+#pragma unroll 1
+  for (int chunk = wave; chunk < c.chunks; chunk += kRowWaves) {
+    double sum = 0.0;
+    unsigned equal = 0;
+    EachQuarter<T>(c.p, row, chunk, [&](int, const float (&z)[kRun]) {
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        if (z[i] > border)
+          sum += w.Of(z[i]);
+        equal += z[i] == border;
+      }
+    });
+    sum = WaveSum64(sum);
+    equal = static_cast<unsigned>(WaveSum64(static_cast<u64>(equal)));
+    if (lane == 0) {
+      work.weight[chunk] = sum;
+      equals[chunk] = equal;
+    }
+  }
+  __syncthreads();
+  if (wave == 0)
+    Pick<T>(c, row, work.weight, equals, s, w, kept.t, kept.need);
 }
 
 int ChunksOf(int vocab) { return vocab <= kChunk ? 0 : (vocab - 1) / kChunk + 1; }
@@ -1411,8 +1481,8 @@ std::int64_t SampleWorkBytes(std::int64_t rows, std::int64_t vocab) {
   const std::int64_t chunks = ChunksOf(static_cast<int>(vocab));
   if (chunks == 0)
     return 0;
-  return rows * (WorkWords(chunks) * static_cast<std::int64_t>(sizeof(unsigned)) +
-                 (SplitRows(rows, chunks) ? static_cast<std::int64_t>(sizeof(RowState)) : 0));
+  return rows * WorkWords(chunks) * static_cast<std::int64_t>(sizeof(unsigned)) +
+         std::min<std::int64_t>(rows, kBatch) * static_cast<std::int64_t>(sizeof(RowState));
 }
 
 void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
@@ -1420,51 +1490,48 @@ void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
   int bits = 0;
   while ((std::int64_t{1} << bits) < p.vocab)
     ++bits;
-  const int shift = 62 - bits < 51 ? 62 - bits : 51;
-  const int chunks = ChunksOf(p.vocab);
-  const int groups = (chunks + kWaves - 1) / kWaves;
-  Require(static_cast<std::int64_t>(p.rows) * groups < (1 << 23), "rows times vocab too large");
-  const int quarters = (p.vocab + kQuarter - 1) / kQuarter;
+  RowCall c{p, 0, p.rows, ChunksOf(p.vocab), (p.vocab - 1) / kQuarter + 1, std::min(62 - bits, 51)};
+  const int groups = (c.chunks + kWaves - 1) / kWaves;
+  const int row_groups = (c.chunks + kRowWaves - 1) / kRowWaves;
+  Require(static_cast<std::int64_t>(p.rows) * groups < (1 << 23) &&
+              std::int64_t{kBatch} * (row_groups + 1) < (1 << 21),
+          "rows times vocab too large");
   WithType(type, [&](auto t) {
     using T = decltype(t);
     const auto small = [&](auto q) {
       Dispatch(SmallKernel<T, q()>, dim3((p.rows + kWaves - 1) / kWaves), dim3(kThreads), 0,
-               stream, true, true, p, shift);
+               stream, true, true, p, c.shift);
     };
-    if (quarters == 1) {
-      small(std::integral_constant<int, 1>());
-    } else if (quarters == 2) {
-      small(std::integral_constant<int, 2>());
-    } else if (quarters == 3) {
-      small(std::integral_constant<int, 3>());
-    } else if (quarters <= kQuarters && chunks == 0) {
-      small(std::integral_constant<int, kQuarters>());
-    } else {
-      // A row may need a threshold where any setting may ask for one.
-      const bool filtered = p.top_ks != nullptr || p.top_ps != nullptr || p.min_ps != nullptr ||
-                            p.top_k > 0 || p.top_p < 1.0F || p.min_p > 0.0F;
-      // Where every row has one small k its list is short, but for many equals.
-      const bool listed = p.top_ks == nullptr && p.top_k > 0 && p.top_k <= kMostOpened &&
-                          p.top_k <= quarters;
-      const bool split = filtered && !listed && SplitRows(p.rows, chunks);
-      Dispatch(ChunkKernel<T>, dim3(p.rows * groups), dim3(kThreads), 0, stream, true, false, p,
-               chunks, groups, split);
-      const auto rows = [&](auto kernel, int groups_each, int threads, bool last) {
-        Dispatch(kernel, dim3(p.rows * groups_each), dim3(threads), 0, stream, false, last, p,
-                 chunks, quarters, shift);
-      };
-      if (!filtered) {
-        rows(RowKernel<T, Phase::kPlain>, 1, kThreads, true);
-      } else if (!split) {
-        rows(RowKernel<T, Phase::kWhole>, 1, kRowThreads, true);
-      } else {
-        rows(RowKernel<T, Phase::kFirst>, 1 + (chunks + kStepChunks - 1) / kStepChunks,
-             kRowThreads, false);
-        rows(RowKernel<T, Phase::kSearch>, 1, kRowThreads, false);
-        Dispatch(KeptKernel<T>, dim3(p.rows * groups), dim3(kThreads), 0, stream, false, false, p,
-                 chunks, groups);
-        rows(RowKernel<T, Phase::kPick>, 1, kWave, true);
-      }
+    if (c.chunks == 0) {
+      if (c.quarters == 1)
+        small(std::integral_constant<int, 1>());
+      else if (c.quarters == 2)
+        small(std::integral_constant<int, 2>());
+      else if (c.quarters == 3)
+        small(std::integral_constant<int, 3>());
+      else
+        small(std::integral_constant<int, kQuarters>());
+      return;
+    }
+    const bool filters = p.top_ks != nullptr || p.top_ps != nullptr || p.min_ps != nullptr ||
+                         p.top_k > 0 || p.top_p < 1.0F || p.min_p > 0.0F;
+    const bool clear = filters && p.rows <= kBatch;  // else batch by batch
+    Dispatch(ChunkKernel<T>, dim3(p.rows * groups), dim3(kThreads), 0, stream, true, false, c,
+             groups, clear);
+    if (!filters) {
+      Dispatch(PlainKernel<T>, dim3(p.rows), dim3(kThreads), 0, stream, false, true, c);
+      return;
+    }
+    for (c.first = 0; c.first < p.rows; c.first += kBatch) {
+      c.rows = std::min(p.rows - c.first, kBatch);
+      const bool last = c.first + kBatch >= p.rows;
+      if (!clear)
+        Dispatch(ClearKernel, dim3(c.rows), dim3(kThreads), 0, stream, false, false, c);
+      Dispatch(FirstKernel<T>, dim3(c.rows * (1 + row_groups)), dim3(kRowThreads), 0, stream, false,
+               false, c);
+      Dispatch(CollectKernel<T>, dim3(c.rows * row_groups), dim3(kRowThreads), 0, stream, false,
+               false, c);
+      Dispatch(FinishKernel<T>, dim3(c.rows), dim3(kRowThreads), 0, stream, false, last, c);
     }
   });
   Check(hipGetLastError(), "sample launch");
