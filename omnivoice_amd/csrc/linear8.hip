@@ -140,7 +140,9 @@ struct Tile {
   static constexpr int kWaveCount = WM * WN;
   static constexpr int kThreads = kWaveCount * kWave;
   static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  static constexpr int kStageBytes = (BM + BN) * kStep;
+  // x has STAGES stages, w one more: its loads have a step more to arrive.
+  static constexpr int kXBytes = BM * kStep, kWBytes = BN * kStep;
+  static constexpr int kBytes = STAGES * kXBytes + (STAGES + 1) * kWBytes;
   static constexpr int kXLoads = BM / 8 / kWaveCount, kWLoads = BN / 8 / kWaveCount;
   static constexpr int kLoads = kXLoads + kWLoads;
   static_assert(BM % (8 * kWaveCount) == 0 && BN % (8 * kWaveCount) == 0, "whole loads a wave");
@@ -150,164 +152,240 @@ struct Tile {
   }
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(WM* WN* kWave) void TileKernel(Linear8Params p, int row_tiles,
-                                                            int col_tiles) {
-  using S = Tile<T, BM, BN, WM, WN, STAGES>;
-  constexpr int FM = S::FM, FN = S::FN;
-  __shared__ __align__(16) unsigned char lds[STAGES * S::kStageBytes];
-  const int lane = threadIdx.x % kWave;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int wm = wave / WN, wn = wave % WN;
-
-  // Work-groups go to the XCDs in turn: each XCD takes a run of tiles, ordered down
-  // columns of eight row tiles.
-  const int tiles = row_tiles * col_tiles;
-  int tile = blockIdx.x;
-  {
-    const int each = tiles / kXcds, rest = tiles % kXcds;
-    const int xcd = tile % kXcds, at = tile / kXcds;
-    tile = xcd * each + min(xcd, rest) + at;
+// A block of ROWS rows by COLS columns of a wave's results goes through the wave's part of
+// LDS, so that every store writes whole runs of a row: 16 bytes a lane, next to each other.
+// (Stores of a lane's own columns, 16 bytes of every 64, took 23 us of a tile of 256 by 256,
+// these 4.) `staged` is what the lanes wrote; rows are kRowBytes apart.
+template <typename T, int ROWS, int COLS>
+struct Staged {
+  static constexpr int kVec = 16 / sizeof(T);
+  static constexpr int kLanes = COLS / kVec;  // of a row
+  static constexpr int kRowBytes = COLS * sizeof(T) + 16;
+  static constexpr int kBytes = ROWS * kRowBytes;
+  static __device__ __forceinline__ void Store(const unsigned char* staged, T* y,
+                                               std::int64_t stride, int row0, int rows, int col0,
+                                               int cols) {
+    const int lane = threadIdx.x % kWave;
+    const int col = col0 + lane % kLanes * kVec;
+#pragma unroll
+    for (int i = 0; i < ROWS; i += kWave / kLanes) {
+      const int r = i + lane / kLanes;
+      const unsigned char* const from = staged + r * kRowBytes + lane % kLanes * 16;
+      T* const to = y + (row0 + r) * stride + col;
+      if (row0 + r < rows && col + kVec <= cols)
+        __builtin_memcpy(to, from, 16);
+      else if (row0 + r < rows)
+#pragma unroll 1
+        for (int e = 0; col + e < cols; ++e)
+          to[e] = reinterpret_cast<const T*>(from)[e];
+    }
   }
+};
+// Between a wave's own writes and reads of LDS.
+__device__ __forceinline__ void WaitLds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// A work-group's tile. Work-groups go to the XCDs in turn: each XCD takes a run of tiles,
+// ordered down columns of eight row tiles.
+__device__ __forceinline__ void TileOf(int row_tiles, int col_tiles, int bm, int bn, int* row0,
+                                       int* col0) {
+  const int tiles = row_tiles * col_tiles;
+  const int each = tiles / kXcds, rest = tiles % kXcds;
+  const int xcd = blockIdx.x % kXcds, at = blockIdx.x / kXcds;
+  const int tile = xcd * each + min(xcd, rest) + at;
   const int band = tile / (8 * col_tiles);
   const int high = min(8, row_tiles - 8 * band);
   const int in_band = tile - band * 8 * col_tiles;
-  const int row0 = (band * 8 + in_band % high) * BM;
-  const int col0 = in_band / high * BN;
+  *row0 = (band * 8 + in_band % high) * bm;
+  *col0 = in_band / high * bn;
+}
 
-  // This lane's chunk of the eight rows that one load brings.
-  const int sub = lane / 8, chunk = lane % 8;
-  std::uint32_t x_at[S::kXLoads], w_at[S::kWLoads];
-#pragma unroll
-  for (int i = 0; i < S::kXLoads; ++i) {
-    const int r = (wave * S::kXLoads + i) * 8 + sub;
-    x_at[i] = static_cast<std::uint32_t>(min(r, p.rows - 1 - row0)) *
-                  static_cast<std::uint32_t>(p.x_stride) +
-              (chunk ^ S::SwizzleX(r)) * 16;
-  }
-#pragma unroll
-  for (int i = 0; i < S::kWLoads; ++i) {
-    const int r = (wave * S::kWLoads + i) * 8 + sub;
-    w_at[i] = static_cast<std::uint32_t>(min(r, p.out - 1 - col0)) *
-                  static_cast<std::uint32_t>(p.in) +
-              (chunk ^ S::SwizzleW(r)) * 16;
-  }
-  const unsigned char* const x = p.x + row0 * p.x_stride;
-  const unsigned char* const w = p.w + static_cast<std::size_t>(col0) * p.in;
-  const std::uint32_t lds0 = LdsAddress(lds);
-  const auto fetch = [&](int step, int stage) {
-    const std::uint32_t to = lds0 + stage * S::kStageBytes;
-#pragma unroll
-    for (int i = 0; i < S::kXLoads; ++i)
-      DmaToLds(x + step * kStep, x_at[i], to + (wave * S::kXLoads + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < S::kWLoads; ++i)
-      DmaToLds(w + step * kStep, w_at[i],
-               to + BM * kStep + (wave * S::kWLoads + i) * 1024);
-  };
-
-  // Operand m of x: rows 16 m + lane % 16 of the wave's; operand n of w: rows dealt.
-  const int part = lane / 16, i16 = lane % 16;
+// Where a wave's part of the tile lies, and how it is fetched and read.
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool WHOLE>
+struct TileWork {
+  using S = Tile<T, BM, BN, WM, WN, STAGES>;
+  static constexpr int FM = S::FM, FN = S::FN;
+  int wave, row0, col0, part, i16, first_row, first_col;
+  std::uint32_t x_at[S::kXLoads], w_at[S::kWLoads], lds0;
+  const unsigned char* x;
+  const unsigned char* w;
   int x_read[2], w_read[2];
-  {
+
+  __device__ __forceinline__ TileWork(const Linear8Params& p, int row_tiles, int col_tiles,
+                                      const unsigned char* lds) {
+    const int lane = threadIdx.x % kWave;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wm = wave / WN, wn = wave % WN;
+    TileOf(row_tiles, col_tiles, BM, BN, &row0, &col0);
+    // This lane's chunk of the eight rows that one load brings.
+    const int sub = lane / 8, chunk = lane % 8;
+#pragma unroll
+    for (int i = 0; i < S::kXLoads; ++i) {
+      const int r = (wave * S::kXLoads + i) * 8 + sub;
+      x_at[i] = static_cast<std::uint32_t>(min(r, p.rows - 1 - row0)) *
+                    static_cast<std::uint32_t>(p.x_stride) +
+                (chunk ^ S::SwizzleX(r)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < S::kWLoads; ++i) {
+      const int r = (wave * S::kWLoads + i) * 8 + sub;
+      w_at[i] = static_cast<std::uint32_t>(min(r, p.out - 1 - col0)) *
+                    static_cast<std::uint32_t>(p.in) +
+                (chunk ^ S::SwizzleW(r)) * 16;
+    }
+    x = p.x + row0 * p.x_stride;
+    w = p.w + static_cast<std::size_t>(col0) * p.in;
+    lds0 = LdsAddress(lds);
+    // Operand m of x: rows 16 m + lane % 16 of the wave's; operand n of w: rows dealt.
+    part = lane / 16;
+    i16 = lane % 16;
     const int r = wm * FM * 16 + i16;
     const int c = wn * FN * 16 + (i16 / 4) * 4 * FN + i16 % 4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      x_read[h] = r * kStep + ((2 * part + h) ^ S::SwizzleX(r)) * 16;
-      w_read[h] = BM * kStep + c * kStep + ((2 * part + h) ^ S::SwizzleW(c)) * 16;
+      x_read[h] = r * kStep + ((part + 4 * h) ^ S::SwizzleX(r)) * 16;
+      w_read[h] = c * kStep + ((part + 4 * h) ^ S::SwizzleW(c)) * 16;
+    }
+    first_row = row0 + r;
+    first_col = col0 + wn * FN * 16 + part * 4 * FN;
+  }
+
+  // Load i of this wave's of a step into a stage.
+  __device__ __forceinline__ void LoadX(int step, int stage, int i) const {
+    DmaToLds(x + step * kStep, x_at[i],
+             lds0 + stage * S::kXBytes + (wave * S::kXLoads + i) * 1024);
+  }
+  __device__ __forceinline__ void LoadW(int step, int stage, int i) const {
+    DmaToLds(w + step * kStep, w_at[i],
+             lds0 + STAGES * S::kXBytes + stage * S::kWBytes + (wave * S::kWLoads + i) * 1024);
+  }
+  __device__ __forceinline__ void ReadX(const unsigned char* from, int m,
+                                        Operand<S::kHalf>* to) const {
+    to->Set(*reinterpret_cast<const intx4*>(from + x_read[0] + m * 16 * kStep),
+            *reinterpret_cast<const intx4*>(from + x_read[1] + m * 16 * kStep));
+  }
+  __device__ __forceinline__ void ReadW(const unsigned char* from, int n,
+                                        Operand<S::kHalf>* to) const {
+    to->Set(*reinterpret_cast<const intx4*>(from + w_read[0] + n * 4 * kStep),
+            *reinterpret_cast<const intx4*>(from + w_read[1] + n * 4 * kStep));
+  }
+
+  // The last, partial step, which comes straight from memory, and the results.
+  __device__ __forceinline__ void Finish(const Linear8Params& p, floatx4 (&acc)[FM][FN],
+                                         unsigned char* lds) const {
+    const int steps = p.in / kStep;
+    if (!WHOLE && p.in % kStep != 0) {
+      Operand<S::kHalf> a, b[FN];
+      const int k = steps * kStep + part * 32;
+#pragma unroll
+      for (int n = 0; n < FN; ++n) {
+        const int c = first_col - part * 4 * FN + (i16 / 4) * 4 * FN + n * 4 + i16 % 4;
+        LoadOperand(p.w + static_cast<std::size_t>(min(c, p.out - 1)) * p.in, k, p.in, &b[n]);
+      }
+#pragma unroll
+      for (int m = 0; m < FM; ++m) {
+        LoadOperand(p.x + min(first_row + 16 * m, p.rows - 1) * p.x_stride, k, p.in, &a);
+#pragma unroll
+        for (int n = 0; n < FN; ++n)
+          acc[m][n] = Multiply(b[n], a, acc[m][n]);
+      }
+    }
+    constexpr int kCols = 4 * FN;  // of a lane
+    using Out = Staged<T, 16, 16 * FN>;
+    // All scales at once, before the first store.
+    float ws[kCols], xs[FM];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      ws[c] = p.w_scales[min(first_col + c, p.out - 1)];
+#pragma unroll
+    for (int m = 0; m < FM; ++m)
+      xs[m] = p.x_scales[min(first_row + 16 * m, p.rows - 1)];
+    __syncthreads();  // the stages are read
+    unsigned char* const staged = lds + wave * Out::kBytes;
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+      T v[kCols];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+        v[c] = static_cast<T>(acc[m][c / 4][c % 4] * xs[m] * ws[c]);
+      WaitLds();
+      __builtin_memcpy(staged + i16 * Out::kRowBytes + part * kCols * sizeof(T), v, sizeof(v));
+      WaitLds();
+      Out::Store(staged, static_cast<T*>(p.y), p.y_stride, first_row - i16 + 16 * m, p.rows,
+                 first_col - part * kCols, p.out);
     }
   }
+};
+
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool WHOLE>
+__global__ __launch_bounds__(WM* WN* kWave) void TileKernel(Linear8Params p, int row_tiles,
+                                                            int col_tiles) {
+  using S = Tile<T, BM, BN, WM, WN, STAGES>;
+  constexpr int FM = S::FM, FN = S::FN;
+  __shared__ __align__(16) unsigned char lds[S::kBytes];
+  const TileWork<T, BM, BN, WM, WN, STAGES, WHOLE> t(p, row_tiles, col_tiles, lds);
   floatx4 acc[FM][FN];
 #pragma unroll
   for (int m = 0; m < FM; ++m)
 #pragma unroll
     for (int n = 0; n < FN; ++n)
       acc[m][n] = floatx4{0, 0, 0, 0};
-
   const int steps = p.in / kStep;
+  // Loads in the order in which the loop goes on with them.
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
+  for (int s = 0; s < STAGES; ++s) {
+    if (s > 0 && s - 1 < steps)
+#pragma unroll
+      for (int i = 0; i < S::kXLoads; ++i)
+        t.LoadX(s - 1, s - 1, i);
     if (s < steps)
-      fetch(s, s);
-  int stage = 0;
+#pragma unroll
+      for (int i = 0; i < S::kWLoads; ++i)
+        t.LoadW(s, s, i);
+  }
+  int x_stage = 0, w_stage = 0;
+#pragma unroll 1
   for (int step = 0; step < steps; ++step) {
-    if (step + STAGES - 1 <= steps)
-      WaitLoads<S::kLoads*(STAGES - 2)>();
+    if (step + STAGES - 1 < steps)
+      WaitLoads<S::kWLoads + (STAGES - 2) * S::kLoads>();
     else
       WaitLoads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (step + STAGES - 1 < steps)
-      fetch(step + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-    const unsigned char* const from = lds + stage * S::kStageBytes;
-    Operand<S::kHalf> b[FN];
+    const unsigned char* const x_from = lds + x_stage * S::kXBytes;
+    const unsigned char* const w_from = lds + STAGES * S::kXBytes + w_stage * S::kWBytes;
+    const int x_to = x_stage == 0 ? STAGES - 1 : x_stage - 1;
+    const int w_to = w_stage == 0 ? STAGES : w_stage - 1;
+    Operand<S::kHalf> b[FN], a[2];
 #pragma unroll
     for (int n = 0; n < FN; ++n)
-      b[n].Set(*reinterpret_cast<const intx4*>(from + w_read[0] + n * 4 * kStep),
-               *reinterpret_cast<const intx4*>(from + w_read[1] + n * 4 * kStep));
+      t.ReadW(w_from, n, &b[n]);
+    t.ReadX(x_from, 0, &a[0]);
+    // The loads go out a few at a time between the products: all at once they hold every
+    // wave up until the address unit has taken them.
 #pragma unroll
     for (int m = 0; m < FM; ++m) {
-      Operand<S::kHalf> a;
-      a.Set(*reinterpret_cast<const intx4*>(from + x_read[0] + m * 16 * kStep),
-            *reinterpret_cast<const intx4*>(from + x_read[1] + m * 16 * kStep));
+      if (m + 1 < FM)
+        t.ReadX(x_from, m + 1, &a[(m + 1) & 1]);
 #pragma unroll
       for (int n = 0; n < FN; ++n)
-        acc[m][n] = Multiply(b[n], a, acc[m][n]);
+        acc[m][n] = Multiply(b[n], a[m & 1], acc[m][n]);
+      constexpr int kEach = (S::kLoads + FM - 1) / FM;
+#pragma unroll
+      for (int i = m * kEach; i < (m + 1) * kEach && i < S::kLoads; ++i) {
+        if (i < S::kXLoads) {
+          if (step + STAGES - 1 < steps)
+            t.LoadX(step + STAGES - 1, x_to, i);
+        } else if (step + STAGES < steps) {
+          t.LoadW(step + STAGES, w_to, i - S::kXLoads);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("" ::: "memory");
-    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    x_stage = x_stage == STAGES - 1 ? 0 : x_stage + 1;
+    w_stage = w_stage == STAGES ? 0 : w_stage + 1;
   }
-
-  const int first_row = row0 + wm * FM * 16 + i16;
-  const int first_col = col0 + wn * FN * 16 + part * 4 * FN;
-  if (p.in % kStep != 0) {  // the last, partial step comes straight from memory
-    Operand<S::kHalf> a, b[FN];
-    const int k = steps * kStep + part * 32;
-#pragma unroll
-    for (int n = 0; n < FN; ++n) {
-      const int c = min(col0 + wn * FN * 16 + (i16 / 4) * 4 * FN + n * 4 + i16 % 4, p.out - 1);
-      LoadOperand(p.w + static_cast<std::size_t>(c) * p.in, k, p.in, &b[n]);
-    }
-#pragma unroll
-    for (int m = 0; m < FM; ++m) {
-      LoadOperand(p.x + min(first_row + 16 * m, p.rows - 1) * p.x_stride, k, p.in, &a);
-#pragma unroll
-      for (int n = 0; n < FN; ++n)
-        acc[m][n] = Multiply(b[n], a, acc[m][n]);
-    }
-  }
-
-  constexpr int kCols = 4 * FN;  // of a lane
-  constexpr int kVec = 16 / sizeof(T);
-  const bool whole = first_col + kCols <= p.out;
-  float ws[kCols];
-#pragma unroll
-  for (int c = 0; c < kCols; ++c)
-    ws[c] = p.w_scales[min(first_col + c, p.out - 1)];
-  T* const y = static_cast<T*>(p.y);
-#pragma unroll
-  for (int m = 0; m < FM; ++m) {
-    const int row = first_row + 16 * m;
-    if (row >= p.rows)
-      break;
-    const float xs = p.x_scales[row];
-    T* const to = y + row * p.y_stride + first_col;
-    T v[kCols];
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-      v[c] = static_cast<T>(acc[m][c / 4][c % 4] * xs * ws[c]);
-    if (whole) {
-#pragma unroll
-      for (int c = 0; c < kCols; c += kVec)
-        __builtin_memcpy(to + c, v + c, 16);
-    } else {
-#pragma unroll
-      for (int c = 0; c < kCols; ++c)
-        if (first_col + c < p.out)
-          to[c] = v[c];
-    }
-  }
+  t.Finish(p, acc, lds);
 }
 
 template <typename T>
@@ -317,11 +395,11 @@ void Launch(const Linear8Params& p, hipStream_t s) {
     Dispatch(SkinnyKernel<T, mb()>, dim3((p.out + 15) / 16, (p.rows + kRows - 1) / kRows),
              dim3(kWaves * kWave), 0, s, true, true, p);
   };
-  const auto tiled = [&](auto bm, auto bn, auto wm, auto wn, auto stages) {
+  const auto tiled = [&](auto bm, auto bn, auto wm, auto wn, auto stages, auto whole) {
     const int row_tiles = (p.rows + bm() - 1) / bm(), col_tiles = (p.out + bn() - 1) / bn();
     Require(static_cast<std::int64_t>(row_tiles) * col_tiles < (1 << 23),
             "linear: too many tiles");
-    Dispatch(TileKernel<T, bm(), bn(), wm(), wn(), stages()>, dim3(row_tiles * col_tiles),
+    Dispatch(TileKernel<T, bm(), bn(), wm(), wn(), stages(), whole()>, dim3(row_tiles * col_tiles),
              dim3(wm() * wn() * kWave), 0, s, true, true, p, row_tiles, col_tiles);
   };
   using std::integral_constant;
@@ -332,15 +410,18 @@ void Launch(const Linear8Params& p, hipStream_t s) {
     skinny(integral_constant<int, 1>());
   else if (p.rows <= 64 || p.x_stride > kTileStride)
     skinny(integral_constant<int, 4>());
-  else if (groups(256, 256) >= 2 * kCus)
+  else if (!std::is_same_v<T, float> && p.in % kStep == 0 && groups(256, 256) >= kCus / 2)
     tiled(integral_constant<int, 256>(), integral_constant<int, 256>(),
-          integral_constant<int, 2>(), integral_constant<int, 4>(), integral_constant<int, 2>());
+          integral_constant<int, 2>(), integral_constant<int, 4>(), integral_constant<int, 2>(),
+          std::true_type());
   else if (groups(128, 128) >= kCus)
     tiled(integral_constant<int, 128>(), integral_constant<int, 128>(),
-          integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 2>());
+          integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 2>(),
+          std::false_type());
   else
     tiled(integral_constant<int, 64>(), integral_constant<int, 64>(),
-          integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 4>());
+          integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 4>(),
+          std::false_type());
 }
 
 }  // namespace
