@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+import threading
 from dataclasses import dataclass, field
 from typing import Callable, List, Optional, Sequence, Tuple
 
@@ -682,17 +683,23 @@ def op_attention(qkv, out, heads: int, kv_heads: int,
 
 # --------------------------------------------------------------- 8-bit key/value cache
 
+_KINDS: dict = {}  # torch's types, once they are needed
+
+
+def _kinds() -> dict:
+    if not _KINDS:
+        import torch
+        _KINDS.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2,
+                       torch.float8_e4m3fn: 3, torch.uint8: 3})
+    return _KINDS
+
+
 def _type_of(t, name: str, with_f32: bool = True) -> int:
     """OVG_F16, OVG_BF16 or OVG_F32 of a tensor."""
-    import torch
-    dtype = t.dtype
-    if dtype is torch.float16:
-        return 0
-    if dtype is torch.bfloat16:
-        return 1
-    if with_f32 and dtype is torch.float32:
-        return 2
-    raise GeneratorError(f"{name}: {dtype} is not supported")
+    kind = _kinds().get(t.dtype, 3)
+    if kind < (3 if with_f32 else 2):
+        return kind
+    raise GeneratorError(f"{name}: {t.dtype} is not supported")
 
 
 def _expect(t, name: str, dtype, shape: Tuple[int, ...], device) -> None:
@@ -726,19 +733,37 @@ def _raw_stream(index: int) -> int:
         return torch.cuda.current_stream(index).cuda_stream
 
 
+def _current_device() -> int:
+    import torch
+    try:
+        return torch._C._cuda_getDevice()  # a tensor of a GPU is there: no need to look for one
+    except AttributeError:
+        return torch.cuda.current_device()
+
+
+class _Local(threading.local):
+    """What a thread's calls use one after the other."""
+
+    def __init__(self):
+        self.err = _buf()
+
+
+_LOCAL = _Local()
+
+
 def _enqueue(fn, device, stream, *args) -> None:
     """fn(*args, stream, ...) with the tensors' device current; without a
     stream, on that device's current one."""
-    import torch
     if device.type != "cuda":
         raise GeneratorError(f"needs tensors of a GPU, got {device}")
     index = device.index
     if stream is None:
         stream = _raw_stream(index)
-    err = _buf()
-    if index == torch.cuda.current_device():
+    err = _LOCAL.err
+    if index == _current_device():
         status = fn(*args, stream, err, 1024)
     else:
+        import torch
         with torch.cuda.device(index):
             status = fn(*args, stream, err, 1024)
     if status != OVG_OK:
@@ -973,8 +998,18 @@ def _matrix_stride(t, name: str, rows: int, width: int, device) -> int:
 
 
 def _is_e4m3(t) -> bool:
-    import torch
-    return t.dtype is torch.float8_e4m3fn or t.dtype is torch.uint8
+    return _kinds().get(t.dtype) == 3
+
+
+def _matrix(t, name: str) -> Tuple[int, int, int, object]:
+    """(rows, width, row stride, device) of a [rows][width] tensor whose rows are
+    contiguous."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (shape[1] > 1 and strides[1] != 1):
+        raise GeneratorError(f"{name}: needs [rows][width] with contiguous rows, got "
+                             f"{tuple(shape)} with strides {strides}")
+    rows, width = shape
+    return rows, width, strides[0] if rows > 1 else width, t.device
 
 
 def op_add_rmsnorm(x, weight, out, eps: float = 1e-6, residual=None, total=None, scales=None,
@@ -984,12 +1019,8 @@ def op_add_rmsnorm(x, weight, out, eps: float = 1e-6, residual=None, total=None,
     weight (float32 [width]) into out [rows][width]: fp16, bf16, float32, or e4m3 codes
     (float8_e4m3fn or uint8) with scales (float32 [rows]). Enqueued on `stream`."""
     import torch
-    if x.dim() != 2:
-        raise GeneratorError(f"x: needs [rows][width], got {tuple(x.shape)}")
-    rows, width = x.shape
-    device = x.device
+    rows, width, stride, device = _matrix(x, "x")
     kind = _type_of(x, "x")
-    stride = _matrix_stride(x, "x", rows, width, device)
     out_stride = _matrix_stride(out, "out", rows, width, device)
     _expect(weight, "weight", torch.float32, (width,), device)
     r_ptr = t_ptr = s_ptr = None
@@ -1023,12 +1054,8 @@ def op_quantize8(x, codes, scales, gate=None, stream=None) -> None:
     codes [rows][width] (float8_e4m3fn or uint8) and power-of-two scales (float32
     [rows]). Enqueued on `stream`."""
     import torch
-    if x.dim() != 2:
-        raise GeneratorError(f"x: needs [rows][width], got {tuple(x.shape)}")
-    rows, width = x.shape
-    device = x.device
+    rows, width, stride, device = _matrix(x, "x")
     kind = _type_of(x, "x")
-    stride = _matrix_stride(x, "x", rows, width, device)
     codes_stride = _matrix_stride(codes, "codes", rows, width, device)
     if not _is_e4m3(codes):
         raise GeneratorError(f"codes: {codes.dtype} is not supported")
@@ -1048,16 +1075,13 @@ def op_linear8(x, x_scales, w, w_scales, y, stream=None) -> None:
     (float8_e4m3fn or uint8) with the rows' scales (float32 [rows], [out]), as
     op_quantize8 gives them. `in` is a multiple of 16. Enqueued on `stream`."""
     import torch
-    if x.dim() != 2 or w.dim() != 2:
-        raise GeneratorError(f"x, w: need [rows][in] and [out][in], got {tuple(x.shape)} and "
-                             f"{tuple(w.shape)}")
-    rows, width = x.shape
-    out = w.shape[0]
-    device = x.device
+    rows, width, stride, device = _matrix(x, "x")
+    out, w_width, w_stride, w_device = _matrix(w, "w")
     if not _is_e4m3(x) or not _is_e4m3(w):
         raise GeneratorError(f"x, w: {x.dtype}, {w.dtype} are not supported")
-    stride = _matrix_stride(x, "x", rows, width, device)
-    _expect(w, "w", w.dtype, (out, width), device)
+    if w_width != width or w_stride != width or w_device != device:
+        raise GeneratorError(f"w: needs a contiguous [out][{width}] on {device}, got "
+                             f"{tuple(w.shape)} with strides {w.stride()} on {w.device}")
     _expect(x_scales, "x_scales", torch.float32, (rows,), device)
     _expect(w_scales, "w_scales", torch.float32, (out,), device)
     y_stride = _matrix_stride(y, "y", rows, out, device)

@@ -77,50 +77,85 @@ __device__ __forceinline__ void LoadOperand(const unsigned char* row, int k, int
 }
 
 // ---------------------------------------------------------------- few rows
-// 16 MB rows by 16 columns; the waves take every fourth step of K and join in LDS.
+// 16 MB rows by 16 NB columns; the waves take every fourth step of K and join in LDS.
 constexpr int kWaves = 4;
 
-template <typename T, int MB>
+template <typename T, int MB, int NB>
 __global__ __launch_bounds__(kWaves* kWave) void SkinnyKernel(Linear8Params p) {
   constexpr bool kHalf = std::is_same_v<T, float>;
-  __shared__ floatx4 parts[kWaves][MB][kWave];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int row0 = blockIdx.y * 16 * MB, col0 = blockIdx.x * 16;
-  const int part = (lane / 16) * 32;
-  const unsigned char* const w =
-      p.w + static_cast<std::size_t>(min(col0 + lane % 16, p.out - 1)) * p.in;
-  const unsigned char* x[MB];
-  floatx4 acc[MB];
+  __shared__ floatx4 parts[kWaves][MB * NB][kWave];
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int row0 = blockIdx.y * 16 * MB, col0 = blockIdx.x * 16 * NB;
+  const int part = lane / 16;
+  const unsigned char *x[MB], *w[NB];
+  floatx4 acc[MB][NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+    w[n] = p.w + static_cast<std::size_t>(min(col0 + 16 * n + lane % 16, p.out - 1)) * p.in;
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
     x[m] = p.x + min(row0 + 16 * m + lane % 16, p.rows - 1) * p.x_stride;
-    acc[m] = floatx4{0, 0, 0, 0};
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+      acc[m][n] = floatx4{0, 0, 0, 0};
   }
-  for (int k = wave * kStep; k < p.in; k += kWaves * kStep) {
-    Operand<kHalf> b, a;
-    LoadOperand(w, k + part, p.in, &b);
+  // Whole steps without a question, two in flight, each load of 64 bytes in a row; the
+  // last, partial one with it.
+  const int whole = p.in / kStep * kStep;
+  int k = wave * kStep;
+  const auto load = [&](const unsigned char* row, Operand<kHalf>* to) {
+    to->Set(*reinterpret_cast<const intx4*>(row + k + part * 16),
+            *reinterpret_cast<const intx4*>(row + k + part * 16 + 64));
+  };
+#pragma unroll 2
+  for (; k < whole; k += kWaves * kStep) {
+    Operand<kHalf> a[MB], b[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+      load(w[n], &b[n]);
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+      load(x[m], &a[m]);
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        acc[m][n] = Multiply(a[m], b[n], acc[m][n]);
+  }
+  if (k < p.in) {
+    Operand<kHalf> a, b[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+      LoadOperand(w[n], k + part * 32, p.in, &b[n]);
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-      LoadOperand(x[m], k + part, p.in, &a);
-      acc[m] = Multiply(a, b, acc[m]);
+      LoadOperand(x[m], k + part * 32, p.in, &a);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        acc[m][n] = Multiply(a, b[n], acc[m][n]);
     }
   }
 #pragma unroll
   for (int m = 0; m < MB; ++m)
-    parts[wave][m][lane] = acc[m];
-  __syncthreads();
-  const int col = col0 + lane % 16;
-  for (int m = wave; m < MB; m += kWaves) {
-    floatx4 sum = parts[0][m][lane];
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i)
-      sum += parts[i][m][lane];
+    for (int n = 0; n < NB; ++n)
+      parts[wave][m * NB + n][lane] = acc[m][n];
+  __syncthreads();
+  for (int i = wave; i < MB * NB; i += kWaves) {
+    floatx4 sum = parts[0][i][lane];
+#pragma unroll
+    for (int v = 1; v < kWaves; ++v)
+      sum += parts[v][i][lane];
+    const int col = col0 + i % NB * 16 + lane % 16;
+    const int first = row0 + i / NB * 16 + 4 * part;
+    const float ws = p.w_scales[min(col, p.out - 1)];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = row0 + 16 * m + 4 * (lane / 16) + r;
+      const int row = first + r;
+      const float xs = p.x_scales[min(row, p.rows - 1)];
       if (row < p.rows && col < p.out)
-        static_cast<T*>(p.y)[row * p.y_stride + col] =
-            static_cast<T>(sum[r] * p.x_scales[row] * p.w_scales[col]);
+        static_cast<T*>(p.y)[row * p.y_stride + col] = static_cast<T>(sum[r] * xs * ws);
     }
   }
 }
@@ -390,10 +425,21 @@ __global__ __launch_bounds__(WM* WN* kWave) void TileKernel(Linear8Params p, int
 
 template <typename T>
 void Launch(const Linear8Params& p, hipStream_t s) {
-  const auto skinny = [&](auto mb) {
-    constexpr int kRows = 16 * mb();
-    Dispatch(SkinnyKernel<T, mb()>, dim3((p.out + 15) / 16, (p.rows + kRows - 1) / kRows),
+  const auto groups = [&](int bm, int bn) {
+    return static_cast<std::int64_t>((p.rows + bm - 1) / bm) * ((p.out + bn - 1) / bn);
+  };
+  // Twice the columns where a work-group is left to every CU: what is read of x halves.
+  const auto skinny_of = [&](auto mb, auto nb) {
+    constexpr int kRows = 16 * mb(), kCols = 16 * nb();
+    Dispatch(SkinnyKernel<T, mb(), nb()>,
+             dim3((p.out + kCols - 1) / kCols, (p.rows + kRows - 1) / kRows),
              dim3(kWaves * kWave), 0, s, true, true, p);
+  };
+  const auto skinny = [&](auto mb) {
+    if (groups(16 * mb(), 32) >= kCus)
+      skinny_of(mb, std::integral_constant<int, 2>());
+    else
+      skinny_of(mb, std::integral_constant<int, 1>());
   };
   const auto tiled = [&](auto bm, auto bn, auto wm, auto wn, auto stages, auto whole) {
     const int row_tiles = (p.rows + bm() - 1) / bm(), col_tiles = (p.out + bn() - 1) / bn();
@@ -403,14 +449,15 @@ void Launch(const Linear8Params& p, hipStream_t s) {
              dim3(wm() * wn() * kWave), 0, s, true, true, p, row_tiles, col_tiles);
   };
   using std::integral_constant;
-  const auto groups = [&](int bm, int bn) {
-    return static_cast<std::int64_t>((p.rows + bm - 1) / bm) * ((p.out + bn - 1) / bn);
-  };
-  if (p.rows <= 16)
-    skinny(integral_constant<int, 1>());
-  else if (p.rows <= 64 || p.x_stride > kTileStride)
-    skinny(integral_constant<int, 4>());
-  else if (!std::is_same_v<T, float> && p.in % kStep == 0 && groups(256, 256) >= kCus / 2)
+  if (p.rows <= 64 || p.x_stride > kTileStride) {
+    // As many rows to a work-group as leave one to every CU.
+    if (p.rows > 32 && groups(64, 16) >= kCus)
+      skinny(integral_constant<int, 4>());
+    else if (p.rows > 16 && groups(32, 16) >= kCus)
+      skinny(integral_constant<int, 2>());
+    else
+      skinny(integral_constant<int, 1>());
+  } else if (p.in % kStep == 0 && groups(256, 256) >= kCus / 2)
     tiled(integral_constant<int, 256>(), integral_constant<int, 256>(),
           integral_constant<int, 2>(), integral_constant<int, 4>(), integral_constant<int, 2>(),
           std::true_type());
