@@ -485,7 +485,7 @@ int ovg_op_token_logprobs(const void* logits, const void* uncond, int64_t rows, 
  * residual_type is x's or float32. total may be residual, or x where the types are
  * the same; out may be x or residual where its type is the same and it is not total.
  * x_type and out_type fp16, bf16 or float32, weight float32 [width]; width <= 65536,
- * rows <= 2^22, epsilon > 0. */
+ * rows < 2^22, epsilon > 0. */
 int ovg_op_add_rmsnorm(const void* x, int64_t x_stride, int x_type, const void* residual,
                        int64_t residual_stride, void* total, int64_t total_stride,
                        int residual_type, const float* weight, void* out, int64_t out_stride,
@@ -493,7 +493,7 @@ int ovg_op_add_rmsnorm(const void* x, int64_t x_stride, int x_type, const void* 
                        void* stream, char* error, size_t error_len);
 
 /* x, or x * silu(gate) with a gate of x's type, in 8 bits: weights that are prepared
- * once, activations before a product. width <= 65536, rows <= 2^22. */
+ * once, activations before a product. width <= 65536, rows < 2^22. */
 int ovg_op_quantize8(const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
                     int type, void* codes, int64_t codes_stride, float* scales, int64_t rows,
                     int64_t width, void* stream, char* error, size_t error_len);
@@ -501,7 +501,11 @@ int ovg_op_quantize8(const void* x, int64_t x_stride, const void* gate, int64_t 
 /* y[rows][out] = x[rows][in] w[out][in]^T of 8-bit rows in float32 sums, each times its
  * row's and its column's scale (in this order; any scales), rounded to `type`. `in` is a
  * multiple of 16 up to 65536; x and w are 16-byte aligned, x_stride a multiple of 16;
- * rows and out up to 2^22. The order of a sum goes by the call's shape. */
+ * rows and out below 2^22. The order of a sum goes by the call's shape. float32 results
+ * have sums right to float32's rounding. 16-bit results come from sums in which, of eight
+ * codes' products next to each other, the bits below 2^-13 of the largest one's power of
+ * two are cut off: under 2^-10 of the products' magnitudes, 1.5e-5 of a sum of random ones,
+ * beside their own rounding of 2^-9 or 2^-12. */
 int ovg_op_linear8(const void* x, int64_t x_stride, const float* x_scales, const void* w,
                    const float* w_scales, void* y, int64_t y_stride, int type, int64_t rows,
                    int64_t in, int64_t out, void* stream, char* error, size_t error_len);
@@ -534,7 +538,7 @@ int ovg_rotary_frequencies(int64_t rotary, double theta, int scaling, double fac
  * or with `sequences` those of the rows' tokens, as ovg_op_cache_write places them
  * (tables are not read; rows of nobody are left as they were). Angles are formed in 64
  * bits: right to 2^-22 for positions up to 2^30 of frequencies up to 1. head_dim up to 512, rows
- * up to 2^24. */
+ * below 2^24. */
 int ovg_op_rotary(const void* q, void* q_out, int64_t q_stride, int64_t q_out_stride,
                   int64_t heads, const void* k, void* k_out, int64_t k_stride,
                   int64_t k_out_stride, int64_t kv_heads, int type, int64_t rows,
@@ -566,7 +570,8 @@ typedef struct ovg_sampling {
  * than 2^-50 of the best counts as none. Weights and sums are right to 2^-40 of the sum and
  * do not depend on the order of the work. A row with a NaN or +infinity among its logits,
  * without a token to draw, or with a NaN among its numbers has the token -1; random numbers
- * outside [0, 1) count as the nearest inside. rows up to 2^22. `workspace` as above. */
+ * outside [0, 1) count as the nearest inside. rows below 2^22, rows times
+ * vocab up to 6e10. `workspace` as above. */
 int64_t ovg_op_sample_workspace(int64_t rows, int64_t vocab);
 int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
                   int64_t stride, int64_t uncond_stride, float guidance, int64_t mask_id,

@@ -11,7 +11,7 @@
 // or of sixteen, eight elements in a row to a lane, so that it is read once; the
 // sums are joined over the lanes by DPP and over the waves through LDS, in a fixed
 // order. Sums are float32. Where the largest magnitude is within 2^-18 of a power's
-// border, or the squares' sum is not finite, the row is summed and its maximum found
+// border, or the squares leave float32's range, the row is summed and its maximum found
 // again in 64 bits, so that the scale is the one that the formulas give.
 #include "step.hpp"
 
@@ -217,8 +217,9 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
       squares += part;
     }
     squares = Lanes::Sum(squares, scratch);
-    factor = rsqrtf(squares / static_cast<float>(width) + p.eps);
-    careful = !(squares < __builtin_inff());
+    const float mean = squares / static_cast<float>(width) + p.eps;
+    factor = rsqrtf(mean);
+    careful = !(mean > 1e-30F && mean < __builtin_inff());
     if (careful)
       factor = static_cast<float>(total64());
     if constexpr (kSecond) {

@@ -20,8 +20,7 @@ namespace ovg {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPairs = 8;     // of a lane
-constexpr int kMostRowsOf = 4;  // rows of a work-group, one wave's search each
+constexpr int kPairs = 8;  // of a lane
 
 // cos and sin of position * f.
 __device__ __forceinline__ float2 Turn(int position, float f) {
@@ -54,104 +53,118 @@ __device__ __forceinline__ void ElementsOf(int s, int half, int dim, int* lo, in
 }
 
 template <typename T, bool INTERLEAVED, bool VECTOR>
-__global__ __launch_bounds__(kThreads) void RotaryKernel(RotaryParams p, int lanes,
-                                                         int rows_of) {
-  __shared__ float2 turns[kMostRowsOf * kMostRotaryDim / 2];
-  __shared__ int held[kMostRowsOf];
-  const int tid = threadIdx.x, row0 = blockIdx.x * rows_of;
+__global__ __launch_bounds__(kThreads) void RotaryKernel(RotaryParams p, int lanes) {
+  __shared__ float2 turns[kMostRotaryDim / 2];
+  __shared__ int held;
+  const int tid = threadIdx.x, row = blockIdx.x;
   const int half = p.rotary / 2, slots = p.dim / 2;
-  if (tid / kWave < rows_of) {
-    const int row = row0 + tid / kWave;
-    int position = 0, valid = row < p.rows;
-    if (p.positions != nullptr) {
-      position = valid ? p.positions[row] : 0;
-    } else {
-      const Found f = FindItem(p.sequences, 1, 0, 0, row);
-      valid = valid && f.item >= 0 && f.item < f.span.count;
-      position = f.span.start + f.item;
-    }
-    for (int i = tid % kWave; i < half; i += kWave) {
-      const float2 t = Turn(position, p.frequencies[i]);
-      turns[(tid / kWave) * half + i] = float2{t.x * p.magnitude, t.y * p.magnitude};
-    }
-    if (tid % kWave == 0)
-      held[tid / kWave] = valid;
-  }
-  __syncthreads();
-
-  // A group of lanes a head; whole waves stay together for the sums.
-  const int groups = kThreads / lanes, group = tid / lanes, lane = tid % lanes;
+  // A group of lanes a head.
+  const int groups = kThreads / lanes, lane = tid % lanes;
   const int heads = p.heads[0] + p.heads[1];
   const int s0 = lane * kPairs;
-  for (int at = group; at < (rows_of * heads + groups - 1) / groups * groups; at += groups) {
-    const int r = at / heads, head = at % heads, row = row0 + r;
-    const bool on = r < rows_of && s0 < slots && held[min(r, rows_of - 1)];
+  const bool there = s0 < slots;
+  int lo, hi;
+  ElementsOf<INTERLEAVED>(s0, half, p.dim, &lo, &hi);
+  float a[kPairs], b[kPairs];
+  const auto load = [&](int head) {
     const int which = head >= p.heads[0];
-    const int of = head - (which ? p.heads[0] : 0);
     const T* x = static_cast<const T*>(p.x[which]) + row * p.x_stride[which] +
-                 static_cast<std::int64_t>(of) * p.dim;
-    float a[kPairs], b[kPairs];
-    int lo, hi;
-    ElementsOf<INTERLEAVED>(s0, half, p.dim, &lo, &hi);
+                 static_cast<std::int64_t>(head - (which ? p.heads[0] : 0)) * p.dim;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i)
       a[i] = b[i] = 0.0F;
-    if (on) {
-      if (VECTOR && INTERLEAVED) {
-        float v[2 * kPairs];
-        LoadFloats<2 * kPairs>(x + lo, v);
+    if (!there)
+      return;
+    if (VECTOR && INTERLEAVED) {
+      float v[2 * kPairs];
+      LoadFloats<2 * kPairs>(x + lo, v);
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          a[i] = v[2 * i];
-          b[i] = v[2 * i + 1];
-        }
-      } else if (VECTOR) {
-        LoadFloats<kPairs>(x + lo, a);
-        LoadFloats<kPairs>(x + hi, b);
-      } else {
-        for (int i = 0; i < kPairs; ++i) {
-          if (s0 + i >= slots)
-            break;
+      for (int i = 0; i < kPairs; ++i) {
+        a[i] = v[2 * i];
+        b[i] = v[2 * i + 1];
+      }
+    } else if (VECTOR) {
+      LoadFloats<kPairs>(x + lo, a);
+      LoadFloats<kPairs>(x + hi, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+        if (s0 + i < slots) {
           int l, h;
           ElementsOf<INTERLEAVED>(s0 + i, half, p.dim, &l, &h);
           a[i] = static_cast<float>(x[l]);
           b[i] = static_cast<float>(x[h]);
         }
-      }
     }
-    if (p.norm[which] != nullptr || p.norm[0] != nullptr || p.norm[1] != nullptr) {
+  };
+
+  // The first head's loads are on their way while the first wave forms the turns.
+  int head = tid / lanes;
+  if (head < heads)
+    load(head);
+  if (tid < kWave) {
+    int position = 0;
+    bool valid = true;
+    if (p.positions != nullptr) {
+      position = p.positions[row];
+    } else {
+      const Found f = FindItem(p.sequences, 1, 0, 0, row);
+      valid = f.item >= 0 && f.item < f.span.count;
+      position = f.span.start + f.item;
+    }
+    for (int i = tid; i < half; i += kWave) {
+      const float2 t = Turn(position, p.frequencies[i]);
+      turns[i] = float2{t.x * p.magnitude, t.y * p.magnitude};
+    }
+    if (tid == 0)
+      held = valid;
+  }
+  __syncthreads();
+  if (!held)
+    return;
+
+  while (head < heads) {
+    const int which = head >= p.heads[0];
+    const float* const norm = p.norm[which];
+    if (norm != nullptr) {
       float squares = 0.0F;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i)
         squares += a[i] * a[i] + b[i] * b[i];
       for (int offset = lanes / 2; offset > 0; offset /= 2)
         squares += __shfl_xor(squares, offset);
-      if (on && p.norm[which] != nullptr) {
-        const float factor = rsqrtf(squares / static_cast<float>(p.dim) + p.eps);
+      const float mean = squares / static_cast<float>(p.dim) + p.eps;
+      float factor = rsqrtf(mean);
+      if (!(mean > 1e-30F && mean < __builtin_inff())) {  // the same in the head's lanes
+        double wide = 0.0;
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          if (s0 + i >= slots)
-            break;
+        for (int i = 0; i < kPairs; ++i)
+          wide += static_cast<double>(a[i]) * a[i] + static_cast<double>(b[i]) * b[i];
+        for (int offset = lanes / 2; offset > 0; offset /= 2)
+          wide += __shfl_xor(wide, offset);
+        factor = static_cast<float>(1.0 / sqrt(wide / p.dim + static_cast<double>(p.eps)));
+      }
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+        if (s0 + i < slots) {
           int l, h;
           ElementsOf<INTERLEAVED>(s0 + i, half, p.dim, &l, &h);
-          a[i] = p.norm[which][l] * (a[i] * factor);
-          b[i] = p.norm[which][h] * (b[i] * factor);
+          a[i] = norm[l] * (a[i] * factor);
+          b[i] = norm[h] * (b[i] * factor);
         }
-      }
     }
-    if (!on)
-      continue;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i)
       if (s0 + i < half) {
-        const float2 t = turns[r * half + s0 + i];
+        const float2 t = turns[s0 + i];
         const float x0 = a[i], x1 = b[i];
         a[i] = x0 * t.x - x1 * t.y;
         b[i] = x1 * t.x + x0 * t.y;
       }
     T* out = static_cast<T*>(p.out[which]) + row * p.out_stride[which] +
-             static_cast<std::int64_t>(of) * p.dim;
-    if (VECTOR && INTERLEAVED) {
+             static_cast<std::int64_t>(head - (which ? p.heads[0] : 0)) * p.dim;
+    if (!there) {
+    } else if (VECTOR && INTERLEAVED) {
       float v[2 * kPairs];
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
@@ -163,15 +176,18 @@ __global__ __launch_bounds__(kThreads) void RotaryKernel(RotaryParams p, int lan
       StoreFloats<kPairs>(out + lo, a);
       StoreFloats<kPairs>(out + hi, b);
     } else {
-      for (int i = 0; i < kPairs; ++i) {
-        if (s0 + i >= slots)
-          break;
-        int l, h;
-        ElementsOf<INTERLEAVED>(s0 + i, half, p.dim, &l, &h);
-        out[l] = static_cast<T>(a[i]);
-        out[h] = static_cast<T>(b[i]);
-      }
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+        if (s0 + i < slots) {
+          int l, h;
+          ElementsOf<INTERLEAVED>(s0 + i, half, p.dim, &l, &h);
+          out[l] = static_cast<T>(a[i]);
+          out[h] = static_cast<T>(b[i]);
+        }
     }
+    head += groups;
+    if (head < heads)
+      load(head);
   }
 }
 
@@ -185,13 +201,11 @@ void LaunchRotary(const RotaryParams& p, bool interleaved, DType type, hipStream
   while (lanes * kPairs < p.dim / 2)
     lanes *= 2;
   const bool vector = p.dim % (2 * kPairs) == 0 && (interleaved || p.rotary % (2 * kPairs) == 0);
-  const int rows_of = 1;
-  const dim3 grid((p.rows + rows_of - 1) / rows_of);
   WithType(type, [&](auto t) {
     using T = decltype(t);
     const auto launch = [&](auto i, auto v) {
-      Dispatch(RotaryKernel<T, i(), v()>, grid, dim3(kThreads), 0, stream, true, true, p, lanes,
-               rows_of);
+      Dispatch(RotaryKernel<T, i(), v()>, dim3(p.rows), dim3(kThreads), 0, stream, true, true, p,
+               lanes);
     };
     if (interleaved && vector)
       launch(std::true_type(), std::true_type());

@@ -1473,12 +1473,18 @@ __global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
     Pick<T>(c, row, work.weight, equals, s, w, kept.t, kept.need);
 }
 
+// Work-groups of the first launch. A batch's others have a fourth of them and two for a
+// row at most; lanes of a launch count under 2^32.
+constexpr std::int64_t kMostGroups = 1 << 23;
+static_assert((kMostGroups / 4 + 2 * kBatch) * kRowThreads < (std::int64_t{1} << 32), "lanes");
 int ChunksOf(int vocab) { return vocab <= kChunk ? 0 : (vocab - 1) / kChunk + 1; }
 
 }  // namespace
 
 std::int64_t SampleWorkBytes(std::int64_t rows, std::int64_t vocab) {
   const std::int64_t chunks = ChunksOf(static_cast<int>(vocab));
+  if (rows * ((chunks + kWaves - 1) / kWaves) >= kMostGroups)
+    return -1;
   if (chunks == 0)
     return 0;
   return rows * WorkWords(chunks) * static_cast<std::int64_t>(sizeof(unsigned)) +
@@ -1493,9 +1499,6 @@ void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
   RowCall c{p, 0, p.rows, ChunksOf(p.vocab), (p.vocab - 1) / kQuarter + 1, std::min(62 - bits, 51)};
   const int groups = (c.chunks + kWaves - 1) / kWaves;
   const int row_groups = (c.chunks + kRowWaves - 1) / kRowWaves;
-  Require(static_cast<std::int64_t>(p.rows) * groups < (1 << 23) &&
-              std::int64_t{kBatch} * (row_groups + 1) < (1 << 21),
-          "rows times vocab too large");
   WithType(type, [&](auto t) {
     using T = decltype(t);
     const auto small = [&](auto q) {

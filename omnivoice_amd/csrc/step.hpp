@@ -29,7 +29,7 @@ struct RowParams {
   int rows, width;
   float eps;
 };
-constexpr int kMostRows = 1 << 22;
+constexpr int kMostRows = (1 << 22) - 1;  // a launch of 1024 lanes a row counts under 2^32
 constexpr int kMostWidth = 1 << 16;
 // second: the residual's type, kE4m3 for none.
 void LaunchAddNorm(const RowParams& p, DType x, DType second, DType out, hipStream_t stream);
@@ -61,6 +61,7 @@ struct RotaryParams {
   float magnitude, eps;
 };
 constexpr int kMostRotaryDim = 512;
+constexpr int kMostRotaryRows = (1 << 24) - 1;  // of 256 lanes
 void LaunchRotary(const RotaryParams& p, bool interleaved, DType type, hipStream_t stream);
 
 // ---------------------------------------------------------------- sampling
@@ -81,6 +82,7 @@ struct SampleParams {
   const float* min_ps;
   unsigned* work;  // SampleWorkBytes
 };
+// -1 for more rows and tokens than a launch covers.
 std::int64_t SampleWorkBytes(std::int64_t rows, std::int64_t vocab);
 void LaunchSample(const SampleParams& p, DType type, hipStream_t stream);
 

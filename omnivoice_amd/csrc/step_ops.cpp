@@ -12,7 +12,7 @@ namespace {
 using namespace ovg::ops;
 
 void RequireRows(int64_t rows, int64_t width) {
-  ovg::Require(rows >= 0 && rows <= ovg::kMostRows, "rows outside [0, 2^22]");
+  ovg::Require(rows >= 0 && rows <= ovg::kMostRows, "rows outside [0, 2^22)");
   ovg::Require(width >= 1 && width <= ovg::kMostWidth, "width outside [1, 65536]");
 }
 
@@ -101,10 +101,10 @@ int ovg_op_linear8(const void* x, int64_t x_stride, const float* x_scales, const
                    const float* w_scales, void* y, int64_t y_stride, int type, int64_t rows,
                    int64_t in, int64_t out, void* stream, char* error, size_t error_len) {
   return Guard("linear8: ", error, error_len, [&] {
-    ovg::Require(rows >= 0 && rows <= ovg::kMostRows, "rows outside [0, 2^22]");
+    ovg::Require(rows >= 0 && rows <= ovg::kMostRows, "rows outside [0, 2^22)");
     ovg::Require(in >= 16 && in % 16 == 0 && in <= ovg::kMostWidth,
                  "in must be a multiple of 16 in [16, 65536]");
-    ovg::Require(out >= 0 && out <= ovg::kMostRows, "out outside [0, 2^22]");
+    ovg::Require(out >= 0 && out <= ovg::kMostRows, "out outside [0, 2^22)");
     const ovg::DType to = TypeOf(type, true);
     RequireStride(x_stride, in);
     ovg::Require(x_stride % 16 == 0, "x's rows must be a multiple of 16 codes apart");
@@ -181,7 +181,7 @@ int ovg_op_rotary(const void* q, void* q_out, int64_t q_stride, int64_t q_out_st
                   const float* q_norm, const float* k_norm, float epsilon, void* stream,
                   char* error, size_t error_len) {
   return Guard("rotary: ", error, error_len, [&] {
-    ovg::Require(rows >= 0 && rows <= (1 << 24), "rows outside [0, 2^24]");
+    ovg::Require(rows >= 0 && rows <= ovg::kMostRotaryRows, "rows outside [0, 2^24)");
     ovg::Require(head_dim >= 2 && head_dim % 2 == 0 && head_dim <= ovg::kMostRotaryDim,
                  "head_dim must be even in [2, 512]");
     ovg::Require(rotary >= 2 && rotary % 2 == 0 && rotary <= head_dim,
@@ -255,7 +255,7 @@ int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t 
                   size_t error_len) {
   return Guard("sample: ", error, error_len, [&] {
     const ovg::DType t = TypeOf(type, true);
-    ovg::Require(rows >= 0 && rows <= ovg::kMostRows, "rows outside [0, 2^22]");
+    ovg::Require(rows >= 0 && rows <= ovg::kMostRows, "rows outside [0, 2^22)");
     ovg::Require(vocab >= 1 && FitsInt(vocab), "vocab outside [1, 2^30]");
     ovg::Require(mask_id >= -1 && mask_id < (int64_t{1} << 31), "mask_id must be -1 or a token");
     ovg::Require(Finite(guidance), "guidance must be finite");
@@ -269,12 +269,13 @@ int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t 
     number(sampling->temperatures, sampling->temperature, "temperature");
     number(sampling->top_ps, sampling->top_p, "top_p");
     number(sampling->min_ps, sampling->min_p, "min_p");
+    const int64_t bytes = ovg::SampleWorkBytes(rows, vocab);
+    ovg::Require(bytes >= 0, "rows times vocab too large");
     if (rows == 0)
       return;
     ovg::Require(logits && random && tokens, "null pointer");
     auto s = static_cast<hipStream_t>(stream);
     RequireCurrentDevice(s);
-    const int64_t bytes = ovg::SampleWorkBytes(rows, vocab);
     ovg::Require(bytes == 0 || (workspace && workspace_bytes >= bytes && Aligned16(workspace)),
                  "workspace of " + std::to_string(bytes) + " bytes needed, 16-byte aligned");
     ovg::SampleParams p{};

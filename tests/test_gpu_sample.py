@@ -231,3 +231,134 @@ def test_rows_past_32_bit_offsets():
     tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
     ov.op_sample(c, torch.rand(rows, device="cuda"), tokens, top_k=1)
     assert torch.equal(tokens.cpu().long(), torch.arange(rows) * 7 % vocab)
+
+
+LONG = [dict(), dict(top_p=0.9), dict(top_k=40), dict(top_k=2000), dict(top_k=9000, top_p=0.95),
+        dict(min_p=0.1), dict(top_p=0.999, min_p=0.3), dict(top_k=3000, min_p=0.5),
+        dict(top_k=300, top_p=0.5, temperature=2.0), dict(temperature=3.0, top_p=0.99)]
+
+
+@pytest.mark.parametrize("settings", LONG)
+@pytest.mark.parametrize("rows,vocab,kind", [(3, 151936, "f32"), (2, 1100001, "bf16"),
+                                             (1, 4300000, "f32")])
+def test_many_kept_and_long_rows(settings, rows, vocab, kind):
+    """Thresholds far down a row, a min_p above the one that top_p would set, rows of more
+    parts than a work-group holds."""
+    c, random = logits_of(vocab + 1, rows, vocab, kind)
+    check(c, random, **settings)
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=300), dict(top_p=0.9), dict(top_k=30),
+                                      dict(min_p=0.01)])
+def test_more_rows_than_hold_a_state(settings):
+    c, random = logits_of(11, 1100, 2600, "f16")
+    check(c, random, **settings)
+
+
+def test_settings_of_many_rows():
+    rows = 700
+    c, random = logits_of(12, rows, 4100, "bf16")
+    g = torch.Generator().manual_seed(13)
+
+    def pick(values, dtype):
+        return torch.tensor(values, dtype=dtype)[torch.randint(0, len(values), (rows,),
+                                                               generator=g)]
+    check(c, random, pick([0.0, 0.6, 1.0, 2.0], torch.float32),
+          pick([0, 3, 600, 5000], torch.int32), pick([1.0, 0.9, 0.4], torch.float32),
+          pick([0.0, 0.05], torch.float32))
+
+
+@pytest.mark.parametrize("top_k", [0, 10, 700, 3000])
+def test_more_equals_than_a_list_holds(top_k):
+    """Thousands of equal logits around the threshold, some above and below, in 8 rows."""
+    c = torch.zeros(8, 40000)
+    c[:, ::7] = 1.0
+    c[:, 5::9] = -4.0
+    c[1:, 100] = 9.0
+    c[2, :] = 0.5
+    random = torch.linspace(0, 1, 9)[:-1].contiguous()
+    check(c, random, top_k=top_k)
+    check(c, random, top_k=top_k, temperature=0.5, min_p=0.2)
+    # Shares that end inside the equals, away from a token's border.
+    check(c[:2], random[:2], top_k=top_k, top_p=0.61803)
+
+
+def test_the_callers_workspace():
+    """Nothing behind it is written, what is in it does not matter."""
+    c, random = logits_of(14, 6, 30000, "bf16")
+    need = ov.op_sample_workspace(6, 30000)
+    for fill in (0, 255):
+        space = torch.full((need + 4096,), fill, dtype=torch.uint8, device="cuda")
+        for settings in (dict(), dict(top_k=20), dict(top_p=0.9), dict(top_k=900, min_p=0.01)):
+            want = check(c, random, **settings)
+            tokens = torch.zeros(6, dtype=torch.int32, device="cuda")
+            ov.op_sample(c.cuda(), random.cuda(), tokens, workspace=space[:need], **settings)
+            np.testing.assert_array_equal(tokens.cpu(), want)
+        assert (space[need:] == fill).all()
+    with pytest.raises(ov.GeneratorError, match="workspace"):
+        ov.op_sample(c.cuda(), random.cuda(), tokens, workspace=space[:need - 16])
+
+
+def test_two_captured_draws_at_once():
+    """Two graphs with workspaces of their own, replayed on two streams at once, with eager
+    draws between; each follows its logits."""
+    rows, vocab = 40, 30000
+    settings = [dict(top_p=0.9, temperature=0.8), dict(top_k=700, min_p=0.001)]
+    draws = []
+    for i, s in enumerate(settings):
+        d = dict(c=torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda"),
+                 random=torch.zeros(rows, device="cuda"),
+                 tokens=torch.zeros(rows, dtype=torch.int32, device="cuda"),
+                 space=torch.zeros(ov.op_sample_workspace(rows, vocab), dtype=torch.uint8,
+                                   device="cuda"),
+                 stream=torch.cuda.Stream(), graph=torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(d["graph"], stream=d["stream"]):
+            ov.op_sample(d["c"], d["random"], d["tokens"], workspace=d["space"], **s)
+        draws.append(d)
+    for t in range(4):
+        inputs = [logits_of(20 + 2 * t + i, rows, vocab, "bf16") for i in range(2)]
+        for d, (c, random) in zip(draws, inputs):
+            d["c"].copy_(c)
+            d["random"].copy_(random)
+            d["tokens"].fill_(-9)
+        torch.cuda.synchronize()
+        for d in draws:
+            with torch.cuda.stream(d["stream"]):
+                d["graph"].replay()
+        want = [check(c, random, **s) for (c, random), s in zip(inputs, settings)]
+        torch.cuda.synchronize()
+        for d, w in zip(draws, want):
+            np.testing.assert_array_equal(d["tokens"].cpu(), w)
+
+
+def test_threads():
+    """Calls of several host threads, each on a stream of its own."""
+    import threading
+    rows, vocab = 20, 9000
+    c, random = logits_of(30, rows, vocab)
+    want = check(c, random, top_p=0.8)
+    dev, u = c.cuda(), random.cuda()
+    got = [torch.zeros(rows, dtype=torch.int32, device="cuda") for _ in range(4)]
+    wrong = []
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        try:
+            for _ in range(20):
+                ov.op_sample(dev, u, got[i], top_p=0.8, stream=stream)
+                if i % 2:  # refused calls of one thread leave the others' alone
+                    with pytest.raises(ov.GeneratorError, match="top_p"):
+                        ov.op_sample(dev, u, got[i], top_p=float("nan"), stream=stream)
+            stream.synchronize()
+        except BaseException as e:
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+    for g in got:
+        np.testing.assert_array_equal(g.cpu(), want)

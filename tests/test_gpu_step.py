@@ -648,3 +648,86 @@ def test_streams():
     for o in got:
         assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
         assert torch.equal(o[2], tokens)
+
+
+# ------------------------------------------------------------------ far sizes and values
+
+@pytest.mark.parametrize("eps", [1e-45, 1e-38, 1e-20])
+@pytest.mark.parametrize("scale", [1e-22, 1e-12, 1.0])
+def test_norm_of_a_tiny_epsilon(eps, scale):
+    """Means under float32's smallest numbers."""
+    x = normal(31, 5, 300) * scale
+    w = 1 + 0.1 * normal(32, 300)
+    eps = float(np.float32(eps))
+    check_norm(x, w, None, "f32", eps)
+    check_norm(x, w, None, "e4m3", eps)
+
+
+@pytest.mark.parametrize("scale", [1e-22, 1.0, 1e25])
+def test_rotary_norms_of_any_loudness(scale):
+    x = normal(33, 6, 5, 96) * scale
+    positions = torch.arange(6, dtype=torch.int32) * 1000
+    f = torch.tensor(ov.rotary_frequencies(96)[0])
+    w = 1 + 0.2 * normal(34, 96)
+    eps = float(np.float32(1e-45)) if scale < 1 else 1e-6
+    for interleaved in (False, True):
+        out = torch.zeros(6, 5, 96, device="cuda")
+        ov.op_rotary(x.cuda(), out, None, None, f.cuda(), positions=positions.cuda(),
+                     q_norm=w.cuda(), eps=eps, interleaved=interleaved)
+        check_rotary(out, x, positions, f, interleaved, 1.0, w, eps, "f32")
+
+
+def test_rotary_of_the_most_rows():
+    rows = (1 << 24) - 1
+    q = torch.ones(rows, 1, 2, dtype=torch.float16, device="cuda")
+    positions = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    positions[-3:] = torch.tensor([1, 2, 3], dtype=torch.int32)
+    ov.op_rotary(q, q, None, None, torch.ones(1, device="cuda"), positions=positions)
+    assert (q[:-3] == 1).all()
+    check_rotary(q[-3:], torch.ones(3, 1, 2, dtype=torch.float16),
+                 torch.tensor([1, 2, 3]), torch.ones(1), False, 1.0, None, 0, "f16")
+
+
+@pytest.mark.parametrize("rows,width,out", [(2100, 2064, 2100), (4100, 128, 2300),
+                                            (3900, 384, 2500), (2300, 1152, 4100),
+                                            (4096, 256, 4096), (33000, 128, 250),
+                                            (100, 128, 70000)])
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+def test_product_of_whole_numbers_in_large_tiles(rows, width, out, kind):
+    test_product_of_whole_numbers(rows, width, out, kind)
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_product_of_rows_far_apart(rows):
+    stride = (1 << 23) + 16
+    a, x = whole_codes(41, rows, 272)
+    b, w = whole_codes(42, 130, 272)
+    wide = torch.zeros(rows, stride, dtype=torch.uint8, device="cuda")
+    wide[:, :272] = x.view(torch.uint8).cuda()
+    y = torch.zeros(rows, 130, device="cuda")
+    one = torch.ones(130, device="cuda")
+    ov.op_linear8(wide[:, :272], one[:rows], w.cuda(), one, y)
+    assert torch.equal(y.cpu().double(), a.double() @ b.double().t())
+
+
+@pytest.mark.parametrize("rows,out", [(16, 64), (64, 9000), (300, 200), (4100, 2300)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_product_of_loud_codes_in_16_bits(rows, out, kind):
+    """One loud code in eight, quiet ones of one sign around it: what the sums of eight
+    products cut off is under 7 * 2^-13 of the products' magnitudes; the additions of the
+    256 / 8 sums and the scales' products are 2^-18 more."""
+    width = 256
+    g = torch.Generator().manual_seed(43)
+    x = torch.rand(rows, width, generator=g) * 0.02 + 0.01
+    x[:, ::8] = 448.0 * torch.sign(normal(44, rows, width // 8))
+    x = x.to(torch.float8_e4m3fn)
+    w = (torch.rand(out, width, generator=g) * 2 + 0.5).to(torch.float8_e4m3fn)
+    one = torch.ones(max(rows, out), device="cuda")
+    y = torch.zeros(rows, out, dtype=TYPES[kind], device="cuda")
+    scale = one[:rows] * 2.0 ** -6
+    ov.op_linear8(x.cuda(), scale, w.cuda(), one[:out], y)
+    a = x.float().double() * 2.0 ** -6
+    want, size = a @ w.float().double().t(), a.abs() @ w.float().double().t()
+    bound = size * (7 * 2.0 ** -13 + 2.0 ** -18) * (1 + HALF_STEP[kind]) + \
+        want.abs() * HALF_STEP[kind] + TINY[kind]
+    assert ((y.cpu().double() - want).abs() <= bound).all()

@@ -278,3 +278,27 @@ def test_frequencies_refuse():
                  (128, 1e6, "yarn", 2.0)):
         with pytest.raises(ov.GeneratorError):
             ov.rotary_frequencies(*args)
+
+
+def test_the_most_rows():
+    """What a launch cannot count is refused before any device work."""
+    assert "rows" in norm(rows=2 ** 22)
+    assert "rows" in quantize(rows=2 ** 22)
+    assert "rows" in linear(rows=2 ** 22)
+    assert "out" in linear(out=2 ** 22, ys=2 ** 22)
+    assert "rows" in rotary(rows=2 ** 24)
+    assert "rows" in sample(rows=2 ** 22)
+    assert "rows times vocab" in sample(rows=2 ** 21, vocab=40000, stride=40000)
+    assert ov.op_sample_workspace(2 ** 21, 40000) == -1
+    assert ov.op_sample_workspace(2 ** 21, 2048) == 0
+    assert ov.op_sample_workspace(2 ** 20, 40000) > 0
+    assert ov.op_sample_workspace(63, 2 ** 30) > 0
+    assert ov.op_sample_workspace(64, 2 ** 30) == -1
+
+
+def test_a_workspace_that_does_not_fit():
+    need = ov.op_sample_workspace(4, 9000)
+    for space, size in ((None, need), (HERE, need - 1), (HERE, 0)):
+        assert f"workspace of {need} bytes" in sample(vocab=9000, stride=9000, space=space,
+                                                      size=size)
+    assert "16-byte aligned" in sample(vocab=9000, stride=9000, space=HERE + 8, size=need)
