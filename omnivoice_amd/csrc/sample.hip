@@ -952,6 +952,38 @@ __device__ __forceinline__ void FindBin(RowShared& sh, bool by_weight, u64 want,
   __syncthreads();
 }
 
+// The largest key, up to best, that `opened` of the quarters' largest reach (1: fewer do):
+// 64 borders at once, a lane each, every wave a part of the quarters. The whole work-group
+// calls this.
+__device__ __forceinline__ unsigned ReachedBy(RowShared& sh, int quarters, int opened,
+                                              unsigned best) {
+  static_assert(kList == 2 * kRowWaves * kWave, "two rounds' counts");
+  const int lane = threadIdx.x % kWave, wave = WaveIndex();
+  unsigned low = 1, high = best;
+#pragma unroll 1
+  for (int round = 0; low < high; round ^= 1) {
+    const unsigned step = (high - low + kWave - 1) / kWave;
+    const unsigned border = min(low + step * (lane + 1), high);
+    unsigned n = 0;
+#pragma unroll 4
+    for (int i = wave; i < quarters; i += kRowWaves)
+      n += sh.most[i] >= border;
+    unsigned* const counts = sh.counts + round * kRowWaves * kWave;
+    counts[wave * kWave + lane] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < kRowWaves; ++i)
+      n += counts[i * kWave + lane];
+    // The first `reached` borders are; the one behind them, if any, is not.
+    const int reached = __popcll(__ballot(static_cast<int>(n) >= opened));
+    const unsigned above = reached == kWave ? high : min(low + step * (reached + 1), high) - 1;
+    low = min(low + step * reached, high);
+    high = max(above, low);
+  }
+  return low;
+}
+
 // The list of the row's keys from `floor` on, of the quarters that have any; false where
 // it does not hold them. The whole work-group calls this.
 template <typename T>
@@ -968,35 +1000,36 @@ __device__ __forceinline__ bool Gather(const RowCall& c, int row, RowShared& sh,
       sh.open[atomicAdd(&sh.opened, 1u)] = static_cast<unsigned short>(q);
   __syncthreads();
   const int opened = static_cast<int>(sh.opened);
-  constexpr int kAtOnce = 4;  // quarters' loads of a wave
+  constexpr int kAtOnce = 8;  // quarters' loads of a wave
 #pragma unroll 1
   for (int o = wave; o < opened; o += kAtOnce * kRowWaves) {
     float z[kAtOnce][kRun];
+    int start[kAtOnce];
+    unsigned mine = 0;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int q = sh.open[min(o + i * kRowWaves, opened - 1)];
+      LoadLogits<T>(c.p, row, q, z[i]);
+      start[i] = RunStart(q, c.p.vocab);
+    }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
-      LoadLogits<T>(c.p, row, sh.open[min(o + i * kRowWaves, opened - 1)], z[i]);
-#pragma unroll 1
-    for (int i = 0; i < kAtOnce && o + i * kRowWaves < opened; ++i) {
-      float v[kRun];
-      unsigned mine = 0;
 #pragma unroll
       for (int e = 0; e < kRun; ++e) {
-        const float front = i == 0 ? z[0][e] : z[1][e], back = i == 2 ? z[2][e] : z[3][e];
-        v[e] = i < 2 ? front : back;
-        mine += v[e] >= from;
+        z[i][e] = o + i * kRowWaves < opened ? z[i][e] : -__builtin_inff();
+        mine += z[i][e] >= from;
       }
-      if (__ballot(mine != 0) == 0)
-        continue;
-      const int start = RunStart(sh.open[o + i * kRowWaves], c.p.vocab);
-      unsigned at = mine != 0 ? atomicAdd(&sh.listed, mine) : 0;
+    unsigned at = mine != 0 ? atomicAdd(&sh.listed, mine) : 0;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
       for (int e = 0; e < kRun; ++e)
-        if (v[e] >= from) {
+        if (z[i][e] >= from) {
           if (at < kList)
-            sh.list[at] = static_cast<u64>(KeyOf(v[e])) << 32 | static_cast<unsigned>(start + e);
+            sh.list[at] =
+                static_cast<u64>(KeyOf(z[i][e])) << 32 | static_cast<unsigned>(start[i] + e);
           ++at;
         }
-    }
   }
   __syncthreads();
   return sh.listed <= kList;
@@ -1080,11 +1113,45 @@ __device__ __forceinline__ bool DrawFromList(const SampleParams& p, int row, Row
   return true;
 }
 
-// The sums of the logit's steps of the row's chunks from `first` on, added to its state
-// by a work-group.
+// What is to be done of a batch by work-groups that take items of it in turn: of the rows
+// in sh.open, parts of 16 waves with `per` quarters each, as few as leave each work-group
+// one item, else whole chunks.
+struct Items {
+  int count, parts, per;
+};
+template <typename F>
+__device__ __forceinline__ Items ItemsOf(const RowCall& c, RowShared& sh, int groups, F&& in) {
+  static_assert(kBatch <= kRowThreads, "a thread a row");
+  const int tid = threadIdx.x, wave = WaveIndex();
+  const bool mine = tid < c.rows && in(tid);
+  const u64 lanes = __ballot(mine);
+  if (tid % kWave == 0)
+    sh.slots[wave] = lanes;
+  __syncthreads();
+  int before = 0, rows = 0;
+  for (int i = 0; i < kRowWaves; ++i) {
+    const int n = __popcll(sh.slots[i]);
+    before += i < wave ? n : 0;
+    rows += n;
+  }
+  if (mine)
+    sh.open[before + __popcll(lanes & ((u64{1} << tid % kWave) - 1))] =
+        static_cast<unsigned short>(tid);
+  Items items{0, 0, 0};
+  for (int per = 1; per <= kQuarters; per *= 2)
+    if (items.count == 0 || items.count > groups) {
+      items.per = per;
+      items.parts = (c.quarters + per * kRowWaves - 1) / (per * kRowWaves);
+      items.count = rows * items.parts;
+    }
+  return items;  // the caller's next barrier is sh.open's too
+}
+
+// The sums of the logit's steps of a part of a row, added to its state.
 template <typename T>
-__device__ __forceinline__ void AddSteps(const RowCall& c, int row, RowState* state, int first,
-                                         const Settings& s, const Weigher& w, RowShared& sh) {
+__device__ __forceinline__ void AddSteps(const RowCall& c, int row, RowState* state, int part,
+                                         int per, const Settings& s, const Weigher& w,
+                                         RowShared& sh) {
   for (int i = threadIdx.x; i < kList; i += kRowThreads) {
     sh.counts[i] = 0;
     sh.weights[i] = 0;
@@ -1092,19 +1159,21 @@ __device__ __forceinline__ void AddSteps(const RowCall& c, int row, RowState* st
   __syncthreads();
   const Steps steps = StepsOf(w);
   const bool share = s.top_p < 1.0F;
-  const int chunk = first + WaveIndex();
-  if (chunk < c.chunks)
-    EachQuarter<T>(c.p, row, chunk, [&](int, const float (&z)[kRun]) {
+  const int first = (part * kRowWaves + WaveIndex()) * per;
+#pragma unroll 1
+  for (int q = first; q < min(first + per, c.quarters); ++q) {
+    float z[kRun];
+    LoadLogits<T>(c.p, row, q, z);
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        const int step = steps(z[i]);
-        if (step < kList) {
-          atomicAdd(&sh.counts[step], 1u);
-          if (share)
-            atomicAdd(&sh.weights[step], UnitsOf(w.Of(z[i]), c.shift));
-        }
+    for (int i = 0; i < kRun; ++i) {
+      const int step = steps(z[i]);
+      if (step < kList) {
+        atomicAdd(&sh.counts[step], 1u);
+        if (share)
+          atomicAdd(&sh.weights[step], UnitsOf(w.Of(z[i]), c.shift));
       }
-    });
+    }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < kList; i += kRowThreads)
     if (sh.counts[i] != 0) {
@@ -1114,35 +1183,57 @@ __device__ __forceinline__ void AddSteps(const RowCall& c, int row, RowState* st
     }
 }
 
-// A row's first work-group draws what needs no threshold, or from a short list; the
-// others sum the steps of rows that will need it.
+// Whether a list of the quarters' loudest may do, and whether the row's sums of steps are
+// formed meanwhile.
+__device__ __forceinline__ int OpenedOf(const Settings& s) {
+  return s.top_k > 0 ? s.top_k : kShareOpened;
+}
+__device__ __forceinline__ bool ShortList(const RowCall& c, const Settings& s) {
+  return c.quarters <= kMostQuarters && OpenedOf(s) <= min(kMostOpened, c.quarters);
+}
+__device__ __forceinline__ bool Searches(const RowCall& c, const Settings& s) {
+  return !s.lost && !s.greedy && (s.top_k > 0 ? !ShortList(c, s) : s.top_p < 1.0F);
+}
+
+// A work-group a row draws what needs no threshold, or from a short list; those behind
+// sum the steps of rows that will need them.
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void FirstKernel(RowCall c) {
   __shared__ RowShared sh;
   __builtin_assume(c.p.vocab > kChunk);
-  const int tid = threadIdx.x, lane = tid % kWave, wave = WaveIndex();
-  const int at = blockIdx.x % c.rows, row = c.first + at, part = blockIdx.x / c.rows;
+  const int tid = threadIdx.x, wave = WaveIndex();
+  FillTable(sh.powers);
+  if (static_cast<int>(blockIdx.x) >= c.rows) {
+    const int helpers = gridDim.x - c.rows;
+    const Items items = ItemsOf(c, sh, helpers, [&](int at) {
+      return Searches(c, SettingsOf(c.p, c.first + at));
+    });
+#pragma unroll 1
+    for (int item = blockIdx.x - c.rows; item < items.count; item += helpers) {
+      __syncthreads();  // the last item's sums are read
+      const int at = sh.open[item / items.parts], row = c.first + at;
+      const Settings s = SettingsOf(c.p, row);
+      const unsigned best =
+          BestOf<kRowWaves>(WorkOf(c.p, row, c.chunks), c.quarters, sh.most, sh.slots);
+      if (best == 0 || best >= kKeyOfInf)
+        continue;
+      const Weigher w = WeigherOf(sh.powers, best, s.temperature);
+      AddSteps<T>(c, row, StateOf(c, at), item % items.parts, items.per, s, w, sh);
+    }
+    return;
+  }
+  const int at = blockIdx.x, row = c.first + at;
   const Settings s = SettingsOf(c.p, row);
   const bool share = s.top_p < 1.0F, ranked = c.quarters <= kMostQuarters;
-  const int opened = s.top_k > 0 ? s.top_k : kShareOpened;
-  const bool short_list = ranked && opened <= min(kMostOpened, c.quarters);
-  const bool searches = (s.top_k > 0 && !short_list) || (s.top_k == 0 && share);
-  if (part > 0 && (s.lost || s.greedy || !searches))
-    return;
   RowState* const state = StateOf(c, at);
   const Work work = WorkOf(c.p, row, c.chunks);
-  FillTable(sh.powers);
   const unsigned best = BestOf<kRowWaves>(work, c.quarters, sh.most, sh.slots);
   if (best == 0 || best >= kKeyOfInf || s.lost) {
-    if (part == 0 && tid == 0)
+    if (tid == 0)
       c.p.tokens[row] = -1;
     return;
   }
   const Weigher w = WeigherOf(sh.powers, best, s.greedy ? 1.0F : s.temperature);
-  if (part > 0) {
-    AddSteps<T>(c, row, state, (part - 1) * kRowWaves, s, w, sh);
-    return;
-  }
   if (s.greedy) {
     DrawBest<T, kRowWaves>(c, row, work, best, sh.slots);
     return;
@@ -1159,41 +1250,18 @@ __global__ __launch_bounds__(kRowThreads) void FirstKernel(RowCall c) {
   }
   const bool known = s.top_k == 0 && !share;  // min_p says the threshold itself
   unsigned floor = known ? KeyOfShare(w, best, s.min_p) : 1;
-  if (ranked && (known || short_list)) {
-    if (!known) {
-      // What reaches the last of the loudest quarters: the largest key that `opened` of
-      // them reach, between ever closer borders, of which every wave counts one.
-      unsigned high = best;
-#pragma unroll 1
-      while (floor < high) {
-        const unsigned step = (high - floor + kRowWaves - 1) / kRowWaves;
-        const unsigned border = min(floor + step * (wave + 1), high);
-        int n = 0;
-        for (int i = lane; i < c.quarters; i += kWave)
-          n += sh.most[i] >= border;
-        n = static_cast<int>(WaveSum64(static_cast<u64>(n)));
-        if (lane == 0)
-          sh.count_slots[wave] = n;
-        __syncthreads();
-        unsigned reached = 0;
-#pragma unroll
-        for (int i = 0; i < kRowWaves; ++i)
-          reached += static_cast<int>(sh.count_slots[i]) >= opened;
-        __syncthreads();
-        // `reached` borders are; the one behind them, if any, is not.
-        const unsigned above =
-            reached == kRowWaves ? high : min(floor + step * (reached + 1), high) - 1;
-        floor = min(floor + step * reached, high);
-        high = max(above, floor);
-      }
-    }
+  if (known ? ranked : ShortList(c, s)) {
+    if (!known)
+      floor = ReachedBy(sh, c.quarters, OpenedOf(s), best);
     Gather<T>(c, row, sh, floor);
     const int listed = static_cast<int>(sh.listed);
     if (listed <= kShortList && DrawFromList(c.p, row, sh, listed, s, w, c.shift, whole))
       return;
   }
   if (tid == 0) {
-    state->status = known ? RowState::kKnown : searches ? RowState::kCollect : RowState::kSlow;
+    state->status = known              ? RowState::kKnown
+                    : Searches(c, s) ? RowState::kCollect
+                                     : RowState::kSlow;
     state->best = best;
     state->t = floor;
     state->whole = static_cast<u64>(ldexp(whole, c.shift));
@@ -1201,21 +1269,16 @@ __global__ __launch_bounds__(kRowThreads) void FirstKernel(RowCall c) {
 }
 
 // Every chunk's weight above the steps in which the threshold is, and the list of the
-// elements in them. Each work-group finds the steps from the row's sums by itself.
+// elements in them, of a part of a row. Each work-group finds the steps from the row's sums
+// by itself.
 template <typename T>
-__global__ __launch_bounds__(kRowThreads) void CollectKernel(RowCall c) {
-  __shared__ RowShared sh;
-  __builtin_assume(c.p.vocab > kChunk);
-  const int tid = threadIdx.x;
-  const int at = blockIdx.x % c.rows, row = c.first + at, part = blockIdx.x / c.rows;
+__device__ __forceinline__ void Collect(const RowCall& c, int at, int part, int per,
+                                        RowShared& sh) {
+  const int tid = threadIdx.x, row = c.first + at;
   RowState* const state = StateOf(c, at);
   const unsigned status = state->status;
-  if (status != RowState::kCollect && status != RowState::kKnown)
-    return;
   const Settings s = SettingsOf(c.p, row);
   const bool share = s.top_p < 1.0F;
-  FillTable(sh.powers);
-  __syncthreads();
   const Weigher w = WeigherOf(sh.powers, state->best, s.temperature);
   const Steps steps = StepsOf(w);
   int k_step = kList, low_step = kList, high_step = -1;
@@ -1278,26 +1341,55 @@ __global__ __launch_bounds__(kRowThreads) void CollectKernel(RowCall c) {
       return;
     }
   }
-  const int chunk = part * kRowWaves + WaveIndex();
-  if (chunk >= c.chunks)
-    return;
-  double sum = 0.0;
-  EachQuarter<T>(c.p, row, chunk, [&](int start, const float (&z)[kRun]) {
+  double* const weights = WorkOf(c.p, row, c.chunks).weight;
+  const int first = (part * kRowWaves + WaveIndex()) * per;
+  double* const sums = reinterpret_cast<double*>(sh.weights);  // of the quarters
+  __syncthreads();  // the bins are read
+#pragma unroll 1
+  for (int i = 0; i < per; ++i) {
+    double sum = 0.0;
+    if (first + i < c.quarters) {
+      float z[kRun];
+      LoadLogits<T>(c.p, row, first + i, z);
+      const int start = RunStart(first + i, c.p.vocab);
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      const int step = steps(z[i]);
-      if (raised ? z[i] >= from : step < low_step)
-        sum += w.Of(z[i]);
-      if (!raised && step < kList && ((step >= low_step && step <= high_step) || step == k_step)) {
-        const unsigned to = atomicAdd(&state->listed, 1u);
-        state->list[min(to, kList - 1u)] =
-            static_cast<u64>(KeyOf(z[i])) << 32 | static_cast<unsigned>(start + i);
+      for (int e = 0; e < kRun; ++e) {
+        const int step = steps(z[e]);
+        if (raised ? z[e] >= from : step < low_step)
+          sum += w.Of(z[e]);
+        if (!raised && step < kList &&
+            ((step >= low_step && step <= high_step) || step == k_step)) {
+          const unsigned to = atomicAdd(&state->listed, 1u);
+          state->list[min(to, kList - 1u)] =
+              static_cast<u64>(KeyOf(z[e])) << 32 | static_cast<unsigned>(start + e);
+        }
       }
     }
+    sum = WaveSum64(sum);
+    if (tid % kWave == 0)
+      sums[WaveIndex() * per + i] = sum;
+  }
+  __syncthreads();
+  const int of_part = kRowWaves * per / kQuarters, chunk = part * of_part + tid;
+  if (tid < of_part && chunk < c.chunks) {
+    const double* const of = sums + tid * kQuarters;
+    weights[chunk] = (of[0] + of[1]) + (of[2] + of[3]);
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void CollectKernel(RowCall c) {
+  __shared__ RowShared sh;
+  __builtin_assume(c.p.vocab > kChunk);
+  FillTable(sh.powers);
+  const Items items = ItemsOf(c, sh, gridDim.x, [&](int at) {
+    const unsigned status = StateOf(c, at)->status;
+    return status == RowState::kCollect || status == RowState::kKnown;
   });
-  sum = WaveSum64(sum);
-  if (tid % kWave == 0)
-    WorkOf(c.p, row, c.chunks).weight[chunk] = sum;
+#pragma unroll 1
+  for (int item = blockIdx.x; item < items.count; item += gridDim.x) {
+    __syncthreads();  // the last item's sums are read
+    Collect<T>(c, sh.open[item / items.parts], item % items.parts, items.per, sh);
+  }
 }
 
 // The threshold from the list of the steps that hold it, or from passes over the row, and
@@ -1473,10 +1565,7 @@ __global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
     Pick<T>(c, row, work.weight, equals, s, w, kept.t, kept.need);
 }
 
-// Work-groups of the first launch. A batch's others have a fourth of them and two for a
-// row at most; lanes of a launch count under 2^32.
-constexpr std::int64_t kMostGroups = 1 << 23;
-static_assert((kMostGroups / 4 + 2 * kBatch) * kRowThreads < (std::int64_t{1} << 32), "lanes");
+constexpr std::int64_t kMostGroups = 1 << 23;  // of the first launch: lanes count under 2^32
 int ChunksOf(int vocab) { return vocab <= kChunk ? 0 : (vocab - 1) / kChunk + 1; }
 
 }  // namespace
@@ -1498,7 +1587,6 @@ void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
     ++bits;
   RowCall c{p, 0, p.rows, ChunksOf(p.vocab), (p.vocab - 1) / kQuarter + 1, std::min(62 - bits, 51)};
   const int groups = (c.chunks + kWaves - 1) / kWaves;
-  const int row_groups = (c.chunks + kRowWaves - 1) / kRowWaves;
   WithType(type, [&](auto t) {
     using T = decltype(t);
     const auto small = [&](auto q) {
@@ -1530,10 +1618,13 @@ void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
       const bool last = c.first + kBatch >= p.rows;
       if (!clear)
         Dispatch(ClearKernel, dim3(c.rows), dim3(kThreads), 0, stream, false, false, c);
-      Dispatch(FirstKernel<T>, dim3(c.rows * (1 + row_groups)), dim3(kRowThreads), 0, stream, false,
-               false, c);
-      Dispatch(CollectKernel<T>, dim3(c.rows * row_groups), dim3(kRowThreads), 0, stream, false,
-               false, c);
+      // A work-group fills a CU.
+      const int parts = static_cast<int>(std::min<std::int64_t>(
+          std::int64_t{c.rows} * ((c.quarters + kRowWaves - 1) / kRowWaves), kCus));
+      const int helpers = std::min(parts, std::max(kCus - c.rows, kCus / 2));
+      Dispatch(FirstKernel<T>, dim3(c.rows + helpers), dim3(kRowThreads), 0, stream, false, false,
+               c);
+      Dispatch(CollectKernel<T>, dim3(parts), dim3(kRowThreads), 0, stream, false, false, c);
       Dispatch(FinishKernel<T>, dim3(c.rows), dim3(kRowThreads), 0, stream, false, last, c);
     }
   });
