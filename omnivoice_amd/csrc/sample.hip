@@ -46,7 +46,7 @@ constexpr int kRowThreads = 1024;           // of a row's work-group in the seco
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kMostQuarters = 2048;         // that are ranked
 constexpr int kMostOpened = 256;            // quarters that are read for a list
-constexpr int kShortList = 512;             // of which every element is ranked
+constexpr int kShortList = 512;             // elements of a list that one wave holds
 constexpr int kList = 2048;                 // elements of a list
 constexpr int kShareOpened = 64;            // opened for a share alone
 constexpr int kOctaves = 50;                // weights below 2^-50 do not count
@@ -341,8 +341,9 @@ struct Held {
     }
     return low;
   }
+  // top_p's share is of `whole`, or of what top_k keeps.
   __device__ __forceinline__ Kept Select(const Settings& s, const Weigher& w, unsigned best,
-                                         int shift) const {
+                                         int shift, u64 whole = 0) const {
     const unsigned least = Least();
     Kept kept{least, kAll, Weight(1)};
     if (s.top_k > 0 && Count(1) > s.top_k) {
@@ -352,7 +353,7 @@ struct Held {
       kept.weight = Weight(above) + kept.need * UnitsOf(w(kept.t), shift);
     }
     if (s.top_p < 1.0F) {
-      const u64 want = ShareOf(s.top_p, kept.weight);
+      const u64 want = ShareOf(s.top_p, whole != 0 ? whole : kept.weight);
       const unsigned low = kept.t;
       u64 above = Weight(low + 1);
       if (above >= want) {
@@ -421,11 +422,12 @@ __device__ __forceinline__ bool DrawOf(const unsigned (&key)[R], const u64 (&wei
 // through LDS, in the row's order, to two or four a lane.
 constexpr int kFew = 4 * kWave;
 
-// The draw from `listed` elements in the row's order, R a lane.
+// The draw from `listed` elements in the row's order, R a lane; top_p's share is of `whole`,
+// or of what top_k keeps. False where the list does not hold the share.
 template <int R>
-__device__ __forceinline__ void DrawFew(const SampleParams& p, int row, const u64* few,
+__device__ __forceinline__ bool DrawFew(const SampleParams& p, int row, const u64* few,
                                         int listed, const Settings& s, const Weigher& w,
-                                        unsigned best, int shift) {
+                                        unsigned best, int shift, u64 whole = 0) {
   const int lane = threadIdx.x % kWave;
   Held<R> held;
   int index[R];
@@ -436,7 +438,9 @@ __device__ __forceinline__ void DrawFew(const SampleParams& p, int row, const u6
     index[i] = static_cast<int>(e);
     held.weight[i] = UnitsOf(w(held.key[i]), shift);
   }
-  const Kept kept = held.Select(s, w, best, shift);
+  if (whole != 0 && held.Weight(1) < ShareOf(s.top_p, whole))
+    return false;
+  const Kept kept = held.Select(s, w, best, shift, whole);
   u64 left = TargetOf(s.u, kept.weight), need = kept.need;
   int of, place;
   if (DrawOf(held.key, held.weight, kept.t, &need, &left, &of, &place)) {
@@ -447,6 +451,7 @@ __device__ __forceinline__ void DrawFew(const SampleParams& p, int row, const u6
     if (lane == of)
       p.tokens[row] = token;
   }
+  return true;
 }
 
 template <typename T, int Q>
@@ -887,18 +892,9 @@ struct RowShared {
   u64 weights[kList];   // of bins; as 64-bit numbers, the chunks'
   unsigned counts[kList];
   u64 list[kList];      // key, index
-  union {
-    struct {
-      unsigned most[kMostQuarters];
-      unsigned short open[kMostQuarters];
-    };
-    struct {
-      u64 unit[kShortList], before[kShortList];  // of the list's elements
-      int rank[kShortList];
-    };
-  };
+  unsigned most[kMostQuarters];
+  unsigned short open[kMostQuarters];
   u64 slots[kRowWaves], count_slots[kRowWaves];
-  unsigned listed, opened;
   int bin;
   u64 above_weight, above_count;
 };
@@ -984,133 +980,84 @@ __device__ __forceinline__ unsigned ReachedBy(RowShared& sh, int quarters, int o
   return low;
 }
 
-// The list of the row's keys from `floor` on, of the quarters that have any; false where
-// it does not hold them. The whole work-group calls this.
+// The list of the row's keys from `floor` on in the row's order; the number of them, or
+// kShortList + 1 where it does not hold them. The whole work-group calls this.
 template <typename T>
-__device__ __forceinline__ bool Gather(const RowCall& c, int row, RowShared& sh, unsigned floor) {
-  const int wave = WaveIndex();
+__device__ __forceinline__ int Gather(const RowCall& c, int row, RowShared& sh, unsigned floor) {
+  const int tid = threadIdx.x, lane = tid % kWave, wave = WaveIndex();
   const float from = LogitOf(max(floor, kKeyOfMinusInf + 1));
-  if (threadIdx.x == 0) {
-    sh.listed = 0;
-    sh.opened = 0;
+  // A sum over the waves before this one, and over all.
+  const auto before_wave = [&](int n, int* all) {
+    if (lane == 0)
+      sh.count_slots[wave] = n;
+    __syncthreads();
+    int before = 0;
+    *all = 0;
+#pragma unroll
+    for (int i = 0; i < kRowWaves; ++i) {
+      const int m = static_cast<int>(sh.count_slots[i]);
+      before += i < wave ? m : 0;
+      *all += m;
+    }
+    __syncthreads();
+    return before;
+  };
+  int opened = 0;  // quarters that have any
+  for (int q0 = 0; q0 < c.quarters; q0 += kRowThreads) {
+    const bool open = q0 + tid < c.quarters && sh.most[q0 + tid] >= floor;
+    const u64 lanes = __ballot(open);
+    int all;
+    const int at = opened + before_wave(__popcll(lanes), &all);
+    if (open)
+      sh.open[at + __popcll(lanes & ((u64{1} << lane) - 1))] =
+          static_cast<unsigned short>(q0 + tid);
+    opened += all;
   }
+  if (opened > kShortList)
+    return kShortList + 1;
   __syncthreads();
-  for (int q = threadIdx.x; q < c.quarters; q += kRowThreads)
-    if (sh.most[q] >= floor)
-      sh.open[atomicAdd(&sh.opened, 1u)] = static_cast<unsigned short>(q);
-  __syncthreads();
-  const int opened = static_cast<int>(sh.opened);
   constexpr int kAtOnce = 8;  // quarters' loads of a wave
+  int listed = 0;
 #pragma unroll 1
-  for (int o = wave; o < opened; o += kAtOnce * kRowWaves) {
+  for (int o = 0; o < opened; o += kAtOnce * kRowWaves) {
+    const int each = min((opened - o + kRowWaves - 1) / kRowWaves, kAtOnce);
+    const int first = o + wave * each, last = min(first + each, opened);
     float z[kAtOnce][kRun];
-    int start[kAtOnce];
-    unsigned mine = 0;
+    int to[kAtOnce], start[kAtOnce], mine = 0;
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const int q = sh.open[min(o + i * kRowWaves, opened - 1)];
-      LoadLogits<T>(c.p, row, q, z[i]);
+      const int q = sh.open[min(first + i, opened - 1)];
       start[i] = RunStart(q, c.p.vocab);
+      if (i < each)
+        LoadLogits<T>(c.p, row, q, z[i]);
     }
 #pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      unsigned n = 0;
+      if (first + i < last)
+#pragma unroll
+        for (int e = 0; e < kRun; ++e)
+          n += z[i][e] >= from;
+      const unsigned scan = WaveScan(n);
+      to[i] = mine + static_cast<int>(scan - n);
+      mine += __builtin_amdgcn_readlane(scan, kWave - 1);
+    }
+    int all;
+    const int at = listed + before_wave(mine, &all);
+    listed += all;
+    if (listed > kShortList)
+      return kShortList + 1;
+#pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
+      if (first + i < last)
 #pragma unroll
-      for (int e = 0; e < kRun; ++e) {
-        z[i][e] = o + i * kRowWaves < opened ? z[i][e] : -__builtin_inff();
-        mine += z[i][e] >= from;
-      }
-    unsigned at = mine != 0 ? atomicAdd(&sh.listed, mine) : 0;
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i)
-#pragma unroll
-      for (int e = 0; e < kRun; ++e)
-        if (z[i][e] >= from) {
-          if (at < kList)
-            sh.list[at] =
+        for (int e = 0; e < kRun; ++e)
+          if (z[i][e] >= from)
+            sh.list[at + to[i]++] =
                 static_cast<u64>(KeyOf(z[i][e])) << 32 | static_cast<unsigned>(start[i] + e);
-          ++at;
-        }
   }
   __syncthreads();
-  return sh.listed <= kList;
-}
-
-// For every element of a list, what `ahead` of it others count and weigh, added to
-// sh.rank and sh.before: a wave has 64 elements and a part of the others.
-template <typename F>
-__device__ __forceinline__ void RankList(RowShared& sh, int listed, F&& ahead) {
-  const int lane = threadIdx.x % kWave, wave = WaveIndex();
-  const int groups = (listed + kWave - 1) / kWave, parts = kRowWaves / groups;
-  const int part = wave / groups, e = wave % groups * kWave + lane;
-  if (part >= parts)
-    return;
-  const u64 mine = sh.list[min(e, listed - 1)];
-  int rank = 0;
-  u64 before = 0;
-#pragma unroll 2
-  for (int i = part; i < listed; i += parts) {
-    const bool in = ahead(sh.list[i], mine);
-    rank += in;
-    before += in ? sh.unit[i] : 0;
-  }
-  if (e < listed) {
-    atomicAdd(&sh.rank[e], rank);
-    atomicAdd(&sh.before[e], before);
-  }
-}
-
-// The draw from a short list, an element a thread; false where the list does not hold the
-// share of `whole` (0: of itself). The whole work-group calls this.
-__device__ __forceinline__ bool DrawFromList(const SampleParams& p, int row, RowShared& sh,
-                                             int listed, const Settings& s, const Weigher& w,
-                                             int shift, double whole_row) {
-  static_assert(kShortList <= kRowThreads && kShortList <= kRowWaves * kWave, "elements");
-  const int e = threadIdx.x;
-  const bool there = e < listed, share = s.top_p < 1.0F;
-  u64 whole = static_cast<u64>(ldexp(whole_row, shift));
-  if (s.top_k > 0)  // few elements take finer units, where they are all that counts
-    shift = 51;
-  const u64 element = there ? sh.list[e] : 0;
-  const double weight = w(static_cast<unsigned>(element >> 32));
-  const u64 unit = UnitsOf(weight, shift);
-  // What is kept: first the elements' ranks by key, then the weights before them by index.
-  u64 kept = unit, target = 0;
-  int rank = 0;
-#pragma unroll 1
-  for (int turn = 0; turn < 2; ++turn) {
-    const u64 all = RowSum<kRowWaves>(kept, sh.slots);
-    if (turn == 0) {
-      if (share && s.top_k == 0 && all < ShareOf(s.top_p, whole))
-        return false;
-    } else {
-      target = TargetOf(s.u, all);
-    }
-    if (e < kShortList) {
-      sh.unit[e] = kept;
-      sh.rank[e] = 0;
-      sh.before[e] = 0;
-    }
-    __syncthreads();
-    // Ahead are larger keys and equal ones of smaller index; then smaller indices.
-    RankList(sh, listed, [&](u64 other, u64 mine) {
-      return turn == 0 ? (other ^ 0xFFFFFFFFu) > (mine ^ 0xFFFFFFFFu)
-                       : static_cast<unsigned>(other) < static_cast<unsigned>(mine);
-    });
-    __syncthreads();
-    const u64 before = there ? sh.before[e] : 0;
-    if (turn == 0) {
-      rank = there ? sh.rank[e] : kList;
-      const int most = s.top_k > 0 ? s.top_k : listed;
-      if (s.top_k > 0 && share)
-        whole = RowSum<kRowWaves>(rank < most ? unit : 0, sh.slots);
-      const bool in = rank < most && (!share || before < ShareOf(s.top_p, whole)) &&
-                      weight >= fmin(static_cast<double>(s.min_p), 1.0);
-      kept = in || rank == 0 ? unit : 0;
-    } else if (there && before <= target && target < before + kept) {
-      p.tokens[row] = static_cast<int>(element);
-    }
-  }
-  return true;
+  return listed;
 }
 
 // What is to be done of a batch by work-groups that take items of it in turn: of the rows
@@ -1253,10 +1200,20 @@ __global__ __launch_bounds__(kRowThreads) void FirstKernel(RowCall c) {
   if (known ? ranked : ShortList(c, s)) {
     if (!known)
       floor = ReachedBy(sh, c.quarters, OpenedOf(s), best);
-    Gather<T>(c, row, sh, floor);
-    const int listed = static_cast<int>(sh.listed);
-    if (listed <= kShortList && DrawFromList(c.p, row, sh, listed, s, w, c.shift, whole))
-      return;
+    const int listed = Gather<T>(c, row, sh, floor);
+    if (listed <= kShortList) {
+      if (wave != 0)
+        return;
+      const u64 of = s.top_k == 0 && share ? static_cast<u64>(ldexp(whole, c.shift)) : 0;
+      const auto draw = [&](auto each) {
+        return DrawFew<each()>(c.p, row, sh.list, listed, s, w, best, c.shift, of);
+      };
+      using std::integral_constant;
+      if (listed <= 2 * kWave    ? draw(integral_constant<int, 2>())
+          : listed <= 4 * kWave  ? draw(integral_constant<int, 4>())
+                                 : draw(integral_constant<int, kShortList / kWave>()))
+        return;
+    }
   }
   if (tid == 0) {
     state->status = known              ? RowState::kKnown
