@@ -766,15 +766,22 @@ __device__ __forceinline__ double WholeOf(const RowCall& c, const Work& work, co
   return RowSum<WAVES>(all, slots);
 }
 
-// The draw by the chunks' kept weights, by one wave: the chunk, 64 at a time, then the
-// place in it. Kept is what is above t (0: all) and of what equals it the first `need`,
-// which `equals` counts by chunk (null: none).
+struct PickShared {
+  unsigned equal[kQuarters];
+  int hit[kQuarters], token[kQuarters];
+  double total[kQuarters];
+};
+// The draw by the chunks' kept weights: the chunk, 64 at a time, then the place in it. The
+// whole work-group calls this, behind a barrier; four waves of it work. Kept is what is
+// above t (0: all) and of what equals it the first `need`, which `equals` counts by chunk
+// (null: none).
 template <typename T>
 __device__ __forceinline__ void Pick(const RowCall& c, int row, const double* weights,
                                      const unsigned* equals, const Settings& s, const Weigher& w,
-                                     unsigned t, u64 need0) {
+                                     unsigned t, u64 need0, PickShared& sh) {
   const SampleParams& p = c.p;
-  const int lane = threadIdx.x % kWave;
+  const int lane = threadIdx.x % kWave, wave = WaveIndex();
+  const bool mine = wave < kQuarters;
   const bool bounded = t != 0;
   const double each = bounded ? w(t) : 0.0;
   const auto last_lane = [](double v) {
@@ -785,7 +792,7 @@ __device__ __forceinline__ void Pick(const RowCall& c, int row, const double* we
   int last = 0;  // the chunk; the last one that keeps any where rounding leaves none
   u64 last_need = 0;
 #pragma unroll 1
-  for (int turn = 0; turn < 2; ++turn) {
+  for (int turn = mine ? 0 : 2; turn < 2; ++turn) {
     u64 need = need0;
     double before = 0.0;
     bool done = false;
@@ -796,13 +803,13 @@ __device__ __forceinline__ void Pick(const RowCall& c, int row, const double* we
       const u64 equal_to = equals != nullptr ? WaveScan(static_cast<u64>(equal)) : 0;
       const u64 equal_before = equal_to - equal;
       const u64 in = need > equal_before ? min(need - equal_before, static_cast<u64>(equal)) : 0;
-      const double mine = (there ? weights[c0 + lane] : 0.0) + static_cast<double>(in) * each;
-      const double to = before + WaveScan(mine);
-      const u64 hit = __ballot(mine > 0.0 && to > left), any = __ballot(mine > 0.0);
+      const double kept = (there ? weights[c0 + lane] : 0.0) + static_cast<double>(in) * each;
+      const double to = before + WaveScan(kept);
+      const u64 hit = __ballot(kept > 0.0 && to > left), any = __ballot(kept > 0.0);
       if (any != 0) {
         const int l = hit != 0 ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
         last = c0 + l;
-        last_before = __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, to - mine), l));
+        last_before = __builtin_bit_cast(double, Lane64(__builtin_bit_cast(u64, to - kept), l));
         last_need = need - min(need, Lane64(equal_before, l));
       }
       done = hit != 0;
@@ -817,46 +824,68 @@ __device__ __forceinline__ void Pick(const RowCall& c, int row, const double* we
     }
   }
   left -= last_before;
-  u64 need = last_need;
-  int token = -1;  // the last kept one, where rounding leaves none
-  bool done = false;
-  EachQuarter<T>(p, row, last, [&](int start, const float (&z)[kRun]) {
-    if (done)
-      return;
-    unsigned equal = 0;
+  // A wave a quarter: the equals, then the kept weights before it, then the place.
+  const int q = last * kQuarters + wave;
+  float z[kRun];
+  unsigned equal = 0, equal_to = 0;
+  if (mine) {
+    LoadLogits<T>(p, row, q, z);
 #pragma unroll
     for (int i = 0; i < kRun; ++i)
       equal += bounded && KeyOf(z[i]) == t;
-    const unsigned equal_to = WaveScan(equal);
+    equal_to = WaveScan(equal);
+    if (lane == kWave - 1)
+      sh.equal[wave] = equal_to;
+  }
+  __syncthreads();
+  u64 need = last_need;
+  double to_place[kRun], weight_of = 0.0, to = 0.0;
+  int end = -1;  // the lane's last kept one
+  if (mine) {
+    for (int i = 0; i < wave; ++i)
+      need -= min(need, static_cast<u64>(sh.equal[i]));
     u64 seen = equal_to - equal;
-    double to_place[kRun], mine = 0.0;
-    int end = -1;  // the lane's last kept one
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
       const unsigned key = KeyOf(z[i]);
       const bool in = !bounded || key > t || (key == t && seen++ < need);
       const double weight = in ? w(key) : 0.0;
       end = weight > 0.0 ? i : end;
-      mine += weight;
-      to_place[i] = mine;
+      weight_of += weight;
+      to_place[i] = weight_of;
     }
-    const double to = WaveScan(mine);
-    const u64 hit = __ballot(mine > 0.0 && to > left), any = __ballot(mine > 0.0);
+    to = WaveScan(weight_of);
+    if (lane == kWave - 1)
+      sh.total[wave] = to;
+  }
+  __syncthreads();
+  if (mine) {
+    for (int i = 0; i < wave; ++i)
+      left -= sh.total[i];
+    const u64 hit = __ballot(weight_of > 0.0 && to > left), any = __ballot(weight_of > 0.0);
     int place = end;
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i) {
       const double before = i > 0 ? to_place[i - 1] : 0.0;
-      place = to_place[i] > before && (to - mine) + to_place[i] > left ? i : place;
+      place = to_place[i] > before && (to - weight_of) + to_place[i] > left ? i : place;
     }
-    done = hit != 0;
-    if (any != 0)
-      token = __builtin_amdgcn_readlane(
-          start + place, done ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any));
-    left -= last_lane(to);
-    need -= min(need, static_cast<u64>(__builtin_amdgcn_readlane(equal_to, kWave - 1)));
-  });
-  if (lane == 0)
+    const int token = RunStart(q, p.vocab) + place;
+    if (lane == 0)
+      sh.hit[wave] = hit != 0;
+    const int of = hit != 0 ? __builtin_ctzll(hit) : any != 0 ? 63 - __builtin_clzll(any) : 0;
+    if (lane == of)
+      sh.token[wave] = any != 0 ? token : -1;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int token = -1;  // the last kept one, where rounding leaves none
+    for (int i = 0; i < kQuarters; ++i) {
+      token = sh.token[i] >= 0 ? sh.token[i] : token;
+      if (sh.hit[i])
+        break;
+    }
     p.tokens[row] = token;
+  }
 }
 
 // Rows of which none has a filter, or that are decided by the chunks' numbers.
@@ -865,6 +894,7 @@ __global__ __launch_bounds__(kThreads) void PlainKernel(RowCall c) {
   __shared__ double powers[kTable];
   __shared__ unsigned most[kMostQuarters];
   __shared__ u64 slots[kWaves];
+  __shared__ PickShared pick;
   const int row = c.first + blockIdx.x;
   const Settings s = SettingsOf(c.p, row);
   const Work work = WorkOf(c.p, row, c.chunks);
@@ -882,8 +912,7 @@ __global__ __launch_bounds__(kThreads) void PlainKernel(RowCall c) {
   const Weigher w = WeigherOf(powers, best, s.temperature);
   WholeOf<kWaves>(c, work, w, slots);
   __syncthreads();
-  if (threadIdx.x < kWave)
-    Pick<T>(c, row, work.weight, nullptr, s, w, 0, 0);
+  Pick<T>(c, row, work.weight, nullptr, s, w, 0, 0, pick);
 }
 
 // ---------------------------------------------------------------- rows with filters
@@ -895,6 +924,7 @@ struct RowShared {
   unsigned most[kMostQuarters];
   unsigned short open[kMostQuarters];
   u64 slots[kRowWaves], count_slots[kRowWaves];
+  PickShared pick;
   int bin;
   u64 above_weight, above_count;
 };
@@ -1190,8 +1220,7 @@ __global__ __launch_bounds__(kRowThreads) void FirstKernel(RowCall c) {
     whole = WholeOf<kRowWaves>(c, work, w, sh.slots);
     if (!share && !(s.min_p > 0.0F)) {
       __syncthreads();
-      if (wave == 0)
-        Pick<T>(c, row, work.weight, nullptr, s, w, 0, 0);
+      Pick<T>(c, row, work.weight, nullptr, s, w, 0, 0, sh.pick);
       return;
     }
   }
@@ -1369,8 +1398,7 @@ __global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
   const Weigher w = WeigherOf(sh.powers, best, s.temperature);
   const unsigned from = status == RowState::kKnown ? state->t : state->raised;
   if (from != 0) {
-    if (wave == 0)
-      Pick<T>(c, row, work.weight, nullptr, s, w, from - 1, 0);
+    Pick<T>(c, row, work.weight, nullptr, s, w, from - 1, 0, sh.pick);
     return;
   }
   const Steps steps = StepsOf(w);
@@ -1490,8 +1518,7 @@ __global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
     for (int i = tid; i < c.chunks; i += kRowThreads)
       weights[i] = work.weight[i] + ldexp(static_cast<double>(sh.weights[i]), -c.shift);
     __syncthreads();
-    if (wave == 0)
-      Pick<T>(c, row, weights, sh.counts, s, w, kept.t, kept.need);
+    Pick<T>(c, row, weights, sh.counts, s, w, kept.t, kept.need, sh.pick);
     return;
   }
   // The whole row once more, for its chunks above the threshold and the equals. The equals
@@ -1518,8 +1545,7 @@ __global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
     }
   }
   __syncthreads();
-  if (wave == 0)
-    Pick<T>(c, row, work.weight, equals, s, w, kept.t, kept.need);
+  Pick<T>(c, row, work.weight, equals, s, w, kept.t, kept.need, sh.pick);
 }
 
 constexpr std::int64_t kMostGroups = 1 << 23;  // of the first launch: lanes count under 2^32
