@@ -189,6 +189,16 @@ __device__ __forceinline__ void LoadLogits(const SampleParams& p, std::int64_t r
     }
   }
 }
+// One that is not masked.
+template <typename T>
+__device__ __forceinline__ float LogitAt(const SampleParams& p, std::int64_t row, int token) {
+  const float z = static_cast<float>(static_cast<const T*>(p.logits)[row * p.stride + token]);
+  if (p.uncond == nullptr)
+    return z;
+  const float u =
+      static_cast<float>(static_cast<const T*>(p.uncond)[row * p.uncond_stride + token]);
+  return z == -__builtin_inff() ? z : z + p.guidance * (z - u);
+}
 // ---------------------------------------------------------------- weights
 // 2^(j / 256), by the series of e^x.
 struct Powers {
@@ -926,6 +936,7 @@ struct RowShared {
   u64 slots[kRowWaves], count_slots[kRowWaves];
   PickShared pick;
   int bin;
+  unsigned floor;
   u64 above_weight, above_count;
 };
 
@@ -978,36 +989,38 @@ __device__ __forceinline__ void FindBin(RowShared& sh, bool by_weight, u64 want,
   __syncthreads();
 }
 
-// The largest key, up to best, that `opened` of the quarters' largest reach (1: fewer do):
-// 64 borders at once, a lane each, every wave a part of the quarters. The whole work-group
-// calls this.
+// The largest key, up to best, that `opened` of the quarters' largest reach (1: fewer do),
+// by halves. The first wave searches, which has 512 of them in registers; the whole
+// work-group calls this.
 __device__ __forceinline__ unsigned ReachedBy(RowShared& sh, int quarters, int opened,
                                               unsigned best) {
-  static_assert(kList == 2 * kRowWaves * kWave, "two rounds' counts");
-  const int lane = threadIdx.x % kWave, wave = WaveIndex();
-  unsigned low = 1, high = best;
-#pragma unroll 1
-  for (int round = 0; low < high; round ^= 1) {
-    const unsigned step = (high - low + kWave - 1) / kWave;
-    const unsigned border = min(low + step * (lane + 1), high);
-    unsigned n = 0;
-#pragma unroll 4
-    for (int i = wave; i < quarters; i += kRowWaves)
-      n += sh.most[i] >= border;
-    unsigned* const counts = sh.counts + round * kRowWaves * kWave;
-    counts[wave * kWave + lane] = n;
-    __syncthreads();
-    n = 0;
+  const int lane = threadIdx.x % kWave;
+  if (threadIdx.x < kWave) {
+    constexpr int kHeld = 8;
+    unsigned held[kHeld];
 #pragma unroll
-    for (int i = 0; i < kRowWaves; ++i)
-      n += counts[i * kWave + lane];
-    // The first `reached` borders are; the one behind them, if any, is not.
-    const int reached = __popcll(__ballot(static_cast<int>(n) >= opened));
-    const unsigned above = reached == kWave ? high : min(low + step * (reached + 1), high) - 1;
-    low = min(low + step * reached, high);
-    high = max(above, low);
+    for (int i = 0; i < kHeld; ++i)
+      held[i] = i * kWave + lane < quarters ? sh.most[i * kWave + lane] : 0;
+    unsigned low = 1, high = best;
+#pragma unroll 1
+    while (low < high) {
+      const unsigned mid = low + (high - low + 1) / 2;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        n += __popcll(__ballot(held[i] >= mid));
+      for (int i = kHeld * kWave; i < quarters; i += kWave)
+        n += __popcll(__ballot(i + lane < quarters && sh.most[i + lane] >= mid));
+      if (n >= opened)
+        low = mid;
+      else
+        high = mid - 1;
+    }
+    if (lane == 0)
+      sh.floor = low;
   }
-  return low;
+  __syncthreads();
+  return sh.floor;
 }
 
 // The list of the row's keys from `floor` on in the row's order; the number of them, or
@@ -1046,45 +1059,42 @@ __device__ __forceinline__ int Gather(const RowCall& c, int row, RowShared& sh, 
   if (opened > kShortList)
     return kShortList + 1;
   __syncthreads();
-  constexpr int kAtOnce = 8;  // quarters' loads of a wave
+  constexpr int kAtOnce = 4;  // quarters' loads of a wave
   int listed = 0;
 #pragma unroll 1
   for (int o = 0; o < opened; o += kAtOnce * kRowWaves) {
     const int each = min((opened - o + kRowWaves - 1) / kRowWaves, kAtOnce);
-    const int first = o + wave * each, last = min(first + each, opened);
+    const int first = o + wave * each, count = min(each, opened - first);
     float z[kAtOnce][kRun];
-    int to[kAtOnce], start[kAtOnce], mine = 0;
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int q = sh.open[min(first + i, opened - 1)];
-      start[i] = RunStart(q, c.p.vocab);
-      if (i < each)
-        LoadLogits<T>(c.p, row, q, z[i]);
-    }
+    for (int i = 0; i < kAtOnce; ++i)
+      if (i < count)
+        LoadLogits<T>(c.p, row, sh.open[first + i], z[i]);
+    unsigned in = 0;  // a bit an element
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      unsigned n = 0;
-      if (first + i < last)
+    for (int i = 0; i < kAtOnce; ++i)
+      if (i < count)
 #pragma unroll
         for (int e = 0; e < kRun; ++e)
-          n += z[i][e] >= from;
-      const unsigned scan = WaveScan(n);
-      to[i] = mine + static_cast<int>(scan - n);
-      mine += __builtin_amdgcn_readlane(scan, kWave - 1);
-    }
+          in |= z[i][e] >= from ? 1u << (i * kRun + e) : 0;
     int all;
-    const int at = listed + before_wave(mine, &all);
+    int at = listed + before_wave(static_cast<int>(WaveSum64(static_cast<u64>(__popc(in)))), &all);
     listed += all;
     if (listed > kShortList)
       return kShortList + 1;
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i)
-      if (first + i < last)
-#pragma unroll
-        for (int e = 0; e < kRun; ++e)
-          if (z[i][e] >= from)
-            sh.list[at + to[i]++] =
-                static_cast<u64>(KeyOf(z[i][e])) << 32 | static_cast<unsigned>(start[i] + e);
+    // The few elements' logits come from memory again: a loop instead of a store for each.
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      unsigned mine = in >> (i * kRun) & ((1u << kRun) - 1);
+      const unsigned n = __popc(mine), scan = WaveScan(n);
+      const int start = RunStart(sh.open[first + i], c.p.vocab);
+      for (int to = at + static_cast<int>(scan - n); mine != 0; ++to, mine &= mine - 1) {
+        const int token = start + __builtin_ctz(mine);
+        sh.list[to] = static_cast<u64>(KeyOf(LogitAt<T>(c.p, row, token))) << 32 |
+                      static_cast<unsigned>(token);
+      }
+      at += __builtin_amdgcn_readlane(scan, kWave - 1);
+    }
   }
   __syncthreads();
   return listed;
