@@ -78,7 +78,11 @@ __device__ __forceinline__ void LoadOperand(const unsigned char* row, int k, int
 }
 
 // ---------------------------------------------------------------- few rows
-// 16 MB rows by 16 NB columns; the waves take every fourth step of K and join in LDS.
+// 16 MB rows by 16 NB columns; the waves take every fourth step of K and join in LDS, in a
+// fixed order. Operands come straight from memory: a weight is used once, and 16 lines of
+// 64 bytes in flight a wave, two steps of them, are what the latency asks for. Bound by
+// reading the weights: 16 x 1024 x 4096 (4 MiB) 3.4 us, of which an empty launch is 2; 16 x
+// 4096 x 8192 (32 MiB) 9.3 us, 3.6 TB/s; 32 x 8192 x 8192 18 us, 3.7 TB/s.
 constexpr int kWaves = 4;
 
 template <typename T, int MB, int NB>
@@ -165,11 +169,17 @@ __global__ __launch_bounds__(kWaves* kWave) void SkinnyKernel(Linear8Params p) {
 // BM rows by BN columns of a work-group, WM by WN waves, a ring of STAGES steps of both
 // operands in LDS, filled by loads that go there directly. A row's 128 codes lie in LDS
 // in 16-byte chunks, chunk c of row r at c ^ Swizzle(r), so that the 16 rows that a
-// wave's operand reads at one c are in 16 different groups of banks.
+// wave's operand reads at one c are in 16 different groups of banks (no conflicts by the
+// counters; a third of the reads' time without).
 //
 // The weights are the left operand, so that a lane holds neighbouring columns of one
 // row: their rows are dealt to the wave's FN operands such that a lane's 4 FN columns
 // are next to each other.
+//
+// Bound by the matrix cores and the reads from LDS that feed them: 4096 x 4096 x 8192 takes
+// 102 us in bf16, 2690 TFLOP/s, beside 97 us of the card's library at 8 bits; float32, at
+// half the products' rate, 207. Small products are bound by their steps' latency: 580 x 2048
+// x 1024 in float32 9.7 us, of which 16 steps, a launch and the results' stores.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 struct Tile {
   static constexpr bool kHalf = std::is_same_v<T, float>;
@@ -429,7 +439,8 @@ void Launch(const Linear8Params& p, hipStream_t s) {
   const auto groups = [&](int bm, int bn) {
     return static_cast<std::int64_t>((p.rows + bm - 1) / bm) * ((p.out + bn - 1) / bn);
   };
-  // Twice the columns where a work-group is left to every CU: what is read of x halves.
+  // Twice the columns, which halves what is read of x, where a work-group is left to every
+  // CU (32 x 8192 x 8192: 18.2 us, so 24.1; 32 x 4096 x 4096, 128 work-groups: 10.1, so 8.3).
   const auto skinny_of = [&](auto mb, auto nb) {
     constexpr int kRows = 16 * mb(), kCols = 16 * nb();
     Dispatch(SkinnyKernel<T, mb(), nb()>,
@@ -450,26 +461,34 @@ void Launch(const Linear8Params& p, hipStream_t s) {
              dim3(wm() * wn() * kWave), 0, s, true, true, p, row_tiles, col_tiles);
   };
   using std::integral_constant;
-  if (p.rows <= 64 || p.x_stride > kTileStride) {
-    // As many rows to a work-group as leave one to every CU.
-    if (p.rows > 32 && groups(64, 16) >= kCus)
-      skinny(integral_constant<int, 4>());
-    else if (p.rows > 16 && groups(32, 16) >= kCus)
+  if (p.rows <= 32 || groups(64, 64) < kCus / 6 || p.x_stride > kTileStride) {
+    // Few rows, or few tiles: 64 x 4096 x 2048 (32 tiles) takes 8.2 us, 10.7 with tiles, 64 x
+    // 4096 x 3000 (47) 13.5 and 10.8, 64 x 8192 x 8192 30 and 21; 32 x 4096 x 4096, half of
+    // whose tiles' rows are none, 8.3 and 10.7. 32 rows to a work-group where that leaves one
+    // to every CU: 32 x 8192 x 8192 24 us, 31 with 16; 64 x 4096 x 1024, 128 work-groups of
+    // 32, 8.0 and 6.1.
+    if (p.rows > 16 && groups(32, 16) >= kCus)
       skinny(integral_constant<int, 2>());
     else
       skinny(integral_constant<int, 1>());
-  } else if (p.in % kStep == 0 && groups(256, 256) >= kCus / 2)
+  } else if (p.in % kStep == 0 && groups(256, 256) >= kCus) {
+    // A tile for every CU: 4096 x 4096 x 4096 takes 56 us, 67 in tiles of 128, 4096 x 4096 x
+    // 2048, half as many, 44 and 33; float32 104 and 119, 90 and 60. Without the partial step
+    // the kernel's code is as long as its registers reach.
     tiled(integral_constant<int, 256>(), integral_constant<int, 256>(),
           integral_constant<int, 2>(), integral_constant<int, 4>(), integral_constant<int, 2>(),
           std::true_type());
-  else if (groups(128, 128) >= kCus)
+  } else if (groups(128, 128) >= kCus * 3 / 4) {
+    // 1900 x 2048 x 2048 (240 tiles) takes 14.4 us, 16.6 in tiles of 64, 1024 x 1024 x 2048
+    // (128) 9.2 and 6.8; float32 1500 x 2048 x 2048 (192) 22.0 and 21.6.
     tiled(integral_constant<int, 128>(), integral_constant<int, 128>(),
           integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 2>(),
           std::false_type());
-  else
+  } else {
     tiled(integral_constant<int, 64>(), integral_constant<int, 64>(),
           integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 4>(),
           std::false_type());
+  }
 }
 
 }  // namespace

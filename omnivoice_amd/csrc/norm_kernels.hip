@@ -158,23 +158,35 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
   const int width = p.width;
   const In* const x = static_cast<const In*>(p.x) + row * p.x_stride;
 
+  // The weights, or gates, and the results stay in registers where there is room. The
+  // lanes of 1024 have 128 registers: from 32 elements a lane on weights and gates are read
+  // again from the caches, a run after the other.
+  constexpr bool kHeld = THREADS < 1024 || CHUNKS <= 2;
+  const auto one_by_one = [] {
+    if constexpr (!kHeld)
+      __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr int kHolds = kHeld && MODE != Mode::kPlain ? CHUNKS : 1;
   float v[CHUNKS][kVec];
-  float g[MODE == Mode::kPlain ? 1 : CHUNKS][kVec];  // weights, or gates
+  float g[kHolds][kVec];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c)
     LoadRun(x, (c * THREADS + tid) * kVec, width, v[c]);
-  if constexpr (MODE == Mode::kNorm) {
+  const auto load_g = [&](int c, float (&to)[kVec]) {
+    if constexpr (MODE == Mode::kNorm)
+      LoadRun(p.weight, (c * THREADS + tid) * kVec, width, to);
+    else if constexpr (MODE == Mode::kGate)
+      LoadRun(static_cast<const Second*>(p.second) + row * p.second_stride,
+              (c * THREADS + tid) * kVec, width, to);
+  };
+  if constexpr (kHeld && MODE != Mode::kPlain) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
-      LoadRun(p.weight, (c * THREADS + tid) * kVec, width, g[c]);
+      load_g(c, g[c]);
   }
   if constexpr (kSecond) {
     const Second* const second = static_cast<const Second*>(p.second) + row * p.second_stride;
-    if constexpr (MODE == Mode::kGate) {
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c)
-        LoadRun(second, (c * THREADS + tid) * kVec, width, g[c]);
-    } else {
+    if constexpr (MODE != Mode::kGate) {
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
         float s[kVec];
@@ -182,6 +194,7 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
           v[c][i] = static_cast<float>(static_cast<Second>(v[c][i] + s[i]));
+        one_by_one();
       }
     }
   }
@@ -200,10 +213,12 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
   const auto total64 = [&] {
     double t = 0.0;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
+    for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
         t += static_cast<double>(v[c][i]) * static_cast<double>(v[c][i]);
+      one_by_one();
+    }
     return 1.0 / sqrt(Lanes::Sum(t, scratch) / width + static_cast<double>(p.eps));
   };
   if constexpr (MODE == Mode::kNorm) {
@@ -229,13 +244,28 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
         StoreRun(total, (c * THREADS + tid) * kVec, width, v[c]);
     }
   }
-  const auto value = [&](int c, int i) {
-    if constexpr (MODE == Mode::kNorm)
-      return g[c][i] * (v[c][i] * factor);
-    else if constexpr (MODE == Mode::kGate)
-      return Gated(v[c][i], g[c][i]);
-    else
-      return v[c][i];
+  // The weights or gates of a run, and its results.
+  const auto g_of = [&](int c, float (&to)[kVec]) {
+    if constexpr (kHeld && MODE != Mode::kPlain) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        to[i] = g[c][i];
+    } else {
+      load_g(c, to);
+    }
+  };
+  const auto values = [&](int c, float (&to)[kVec]) {
+    float by[kVec];
+    g_of(c, by);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      if constexpr (MODE == Mode::kNorm)
+        to[i] = by[i] * (v[c][i] * factor);
+      else if constexpr (MODE == Mode::kGate)
+        to[i] = Gated(v[c][i], by[i]);
+      else
+        to[i] = v[c][i];
+    }
   };
 
   if constexpr (!kCodes) {
@@ -243,24 +273,24 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       float y[kVec];
-#pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        y[i] = value(c, i);
+      values(c, y);
       StoreRun(out, (c * THREADS + tid) * kVec, width, y);
+      one_by_one();
     }
   } else {
     // The order of magnitudes' bits is the magnitudes' own, infinities and NaN
-    // behind every number.
-    float y[CHUNKS][kVec];
+    // behind every number. A run's elements of other lanes are zeros times the row's own
+    // weights or gates: a NaN there is the row's, too.
+    float held[kHeld ? CHUNKS : 1][kVec];
     unsigned amax = 0;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const int d = (c * THREADS + tid) * kVec, start = RunStart(d, width);
+      auto& y = held[kHeld ? c : 0];
+      values(c, y);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        y[c][i] = Owned(start + i, d, width) ? value(c, i) : 0.0F;
-        amax = max(amax, __float_as_uint(y[c][i]) & 0x7FFFFFFFu);
-      }
+      for (int i = 0; i < kVec; ++i)
+        amax = max(amax, __float_as_uint(y[i]) & 0x7FFFFFFFu);
+      one_by_one();
     }
     amax = Lanes::Max(amax, scratch);
     const bool lost = amax >= 0x7F800000u;
@@ -271,15 +301,22 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
         double most = 0.0;
         const double r = MODE == Mode::kNorm ? total64() : 1.0;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
+        for (int c = 0; c < CHUNKS; ++c) {
+          auto& y = held[kHeld ? c : 0];
+          if (!kHeld)
+            values(c, y);
+          float by[kVec];
+          g_of(c, by);
 #pragma unroll
           for (int i = 0; i < kVec; ++i) {
             // Far from the largest they cannot be it.
-            if (!(fabsf(y[c][i]) >= __uint_as_float(amax) * 0.999F))
+            if (!(fabsf(y[i]) >= __uint_as_float(amax) * 0.999F))
               continue;
-            const double a = v[c][i], b = g[c][i];
+            const double a = v[c][i], b = by[i];
             most = fmax(most, fabs(MODE == Mode::kNorm ? b * a * r : a * (b / (1.0 + exp(-b)))));
           }
+          one_by_one();
+        }
         e = ScaleExponent(Lanes::Max(most, scratch));
       }
     }
@@ -287,10 +324,14 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
     unsigned char* const out = static_cast<unsigned char*>(p.out) + row * p.out_stride;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
+      auto& y = held[kHeld ? c : 0];
+      if (!kHeld)
+        values(c, y);
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
-        y[c][i] = lost ? 0.0F : y[c][i] * inverse;
-      StoreCodes(out, (c * THREADS + tid) * kVec, width, y[c]);
+        y[i] = lost ? 0.0F : y[i] * inverse;
+      StoreCodes(out, (c * THREADS + tid) * kVec, width, y);
+      one_by_one();
     }
     if (tid == 0)
       p.scales[row] = lost ? __builtin_nanf("") : PowerOf(e);
@@ -310,8 +351,14 @@ void LaunchRows(const RowParams& p, hipStream_t s) {
     launch(integral_constant<int, 64>(), integral_constant<int, 2>());
   else if (p.width <= 4 * kVec * kWave)
     launch(integral_constant<int, 64>(), integral_constant<int, 4>());
+  else if (p.width <= 2 * kVec * 256)
+    launch(integral_constant<int, 256>(), integral_constant<int, 2>());
   else if (p.width <= 4 * kVec * 256)
     launch(integral_constant<int, 256>(), integral_constant<int, 4>());
+  else if (p.width <= 2 * kVec * 1024)
+    launch(integral_constant<int, 1024>(), integral_constant<int, 2>());
+  else if (p.width <= 4 * kVec * 1024)
+    launch(integral_constant<int, 1024>(), integral_constant<int, 4>());
   else
     launch(integral_constant<int, 1024>(), integral_constant<int, 8>());
 }

@@ -691,7 +691,9 @@ def test_rotary_of_the_most_rows():
 @pytest.mark.parametrize("rows,width,out", [(2100, 2064, 2100), (4100, 128, 2300),
                                             (3900, 384, 2500), (2300, 1152, 4100),
                                             (4096, 256, 4096), (33000, 128, 250),
-                                            (100, 128, 70000)])
+                                            (4300, 384, 4200), (9000, 128, 2100),
+                                            (100, 128, 70000), (64, 256, 9000), (50, 2064, 2500),
+                                            (1000, 528, 130), (32, 400, 9000)])
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
 def test_product_of_whole_numbers_in_large_tiles(rows, width, out, kind):
     test_product_of_whole_numbers(rows, width, out, kind)
