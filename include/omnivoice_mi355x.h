@@ -567,11 +567,12 @@ typedef struct ovg_sampling {
  * w = exp((z - max z) / temperature); top_k keeps the first of them, top_p a prefix of
  * what top_k keeps, min_p what weighs enough, and the best always stays. The token is the
  * first, by index, at which the kept weights pass random * their sum; one that weighs less
- * than 2^-50 of the best counts as none. Weights and sums are right to 2^-40 of the sum and
- * do not depend on the order of the work. A row with a NaN or +infinity among its logits,
- * without a token to draw, or with a NaN among its numbers has the token -1; random numbers
- * outside [0, 1) count as the nearest inside. rows below 2^22, rows times
- * vocab up to 6e10. `workspace` as above. */
+ * than 2^-50 of the best counts as none. Weights are right to 2^-42 and sums to 2^-40; with
+ * filters, among n > 2048 tokens, sums are to n 2^-50 and top_p's border to n^2 2^-61 of the
+ * sum (2^-32 and 2^-26 for 151936). Nothing depends on the order of the work. A row with a
+ * NaN or +infinity among its logits, without a token to draw, or with a NaN among its
+ * numbers has the token -1; random numbers outside [0, 1) count as the nearest inside. rows
+ * below 2^22, rows times vocab up to 6e10. `workspace` as above, for this call alone. */
 int64_t ovg_op_sample_workspace(int64_t rows, int64_t vocab);
 int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
                   int64_t stride, int64_t uncond_stride, float guidance, int64_t mask_id,

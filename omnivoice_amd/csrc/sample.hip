@@ -10,22 +10,32 @@
 // What is kept is a prefix of the order: the keys (logits as ordered numbers) above a
 // threshold and the first `need` of those equal to it.
 //
-// Up to 2048 tokens a wave has its row in registers and searches thresholds by halves.
-// Larger vocabularies take two launches. The first has a wave for every chunk of 2048
-// tokens, which leaves the largest key of each quarter and, where the row needs it, the
-// chunk's weight beside its own largest. The second has a work-group for every row.
-// Without filters it finds the chunk by the chunks' weights and reads only that one. The
-// k best lie in the k quarters with the largest keys, so with filters it reads those (64
-// for top_p alone) and ranks the few elements that reach the last one's. Where that is
-// not enough (a large k, a share that needs more) it reads the row again: sums of 2048
-// steps of the logit, passes over what the step that was found holds, and one for the
-// chunks' kept weights. With few rows these take launches of their own, in which all CUs
-// share the rows, and which end at once where no row needs them.
+// Up to 2048 tokens a wave has its row in registers and searches thresholds by halves
+// (2000 guided rows of 1025 float32, the best 50: 11 us, 16 MB). Larger vocabularies take
+// two launches, or four with filters:
+//   1  A wave for every chunk of 2048 tokens leaves the largest key of each quarter and,
+//      where the row needs it, the chunk's weight beside its own largest.
+//   2  Rows without filters: a work-group a row finds the chunk by the chunks' weights and
+//      reads only that one. Rows with filters: the k best lie in the k quarters with the
+//      largest keys, so a work-group a row reads those (64 for top_p alone) and lists the
+//      few elements that reach the last one's, from which a wave draws. Where that will not
+//      do, or may not (a large k, a share that may need more), other work-groups meanwhile
+//      form the row's sums of 2048 steps of the logit.
+//   3  For rows that were not drawn: the steps that hold the threshold by those sums, the
+//      list of the elements in them, and the chunks' weights above them.
+//   4  The threshold from the list, or from passes over the row where the list does not hold
+//      it (thousands of equals), and the draw.
+// Bound by the arithmetic of the weights, 16 operations in 64 bits and a table's value for
+// each: 300 rows of 151936 bf16 without filters 43 us (40 + 8 with the launches overlapped;
+// their 91 MB are 18 us), 64 rows with settings of all kinds 69 us (10 + 24 + 19 + 18), of
+// which the bytes are 4: there the chain of short, dependent searches of launches 2 to 4 is
+// what bounds.
 //
 // A draw lands where sums of up to 2^17 weights say, so weights have 2^-42 and better:
-// 2^x in 64 bits from a table of 256 powers and three terms. Sums that several lanes
-// form in any order are whole numbers of 2^-shift; the others are 64-bit numbers in a
-// fixed order. No result depends on the order of the work.
+// 2^x in 64 bits from a table of 256 powers and three terms (ten terms without a table: 47
+// us for launch 1 of the 300 rows, so 40). Sums that several lanes form in any order are
+// whole numbers of 2^-shift; the others are 64-bit numbers in a fixed order. No result
+// depends on the order of the work, nor on the rows beside.
 #include <algorithm>
 
 #include "step.hpp"
@@ -588,7 +598,9 @@ struct RowState {
   u64 weights[kList];
   u64 list[kList];  // key, index
 };
-constexpr int kBatch = 512;  // rows that have a state at once
+// Rows that have a state at once: 41 KB each, so that the workspace of 4096 rows is 28 MB and
+// not 175; 1024 rows take launches 2 to 4 twice.
+constexpr int kBatch = 512;
 
 struct RowCall {
   SampleParams p;
