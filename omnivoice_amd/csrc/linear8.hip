@@ -478,10 +478,18 @@ void Launch(const Linear8Params& p, hipStream_t s) {
     tiled(integral_constant<int, 256>(), integral_constant<int, 256>(),
           integral_constant<int, 2>(), integral_constant<int, 4>(), integral_constant<int, 2>(),
           std::true_type());
-  } else if (groups(128, 128) >= kCus * 3 / 4) {
-    // 1900 x 2048 x 2048 (240 tiles) takes 14.4 us, 16.6 in tiles of 64, 1024 x 1024 x 2048
-    // (128) 9.2 and 6.8; float32 1500 x 2048 x 2048 (192) 22.0 and 21.6.
+  } else if (groups(128, 128) > kCus) {
+    // 4096 x 4096 x 2048 (512 tiles) takes 33 us, 45 in tiles of 64, 3000 x 2048 x 2048 (384)
+    // 18.4 and 21.7, 2048 x 2048 x 2048 (256) 14.6 both, 1500 x 2048 x 2048 (192) 14.1 and
+    // 12.1; float32 61 and 76, 34 and 31, 24 and 23, 23 and 19.
     tiled(integral_constant<int, 128>(), integral_constant<int, 128>(),
+          integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 2>(),
+          std::false_type());
+  } else if (groups(64, 64) > 2 * kCus) {
+    // Four stages leave two work-groups to a CU, two four: 1400 x 2048 x 2048 (704 tiles)
+    // takes 11.5 us with two stages, 13.7 with four, 1000 x 1024 x 2048 (512) 7.0 and 6.6, 580
+    // x 2048 x 1024 (160) 10.4 and 7.3; float32 17.5 and 21.2, 9.1 and 10.2, 12.3 and 10.5.
+    tiled(integral_constant<int, 64>(), integral_constant<int, 64>(),
           integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 2>(),
           std::false_type());
   } else {

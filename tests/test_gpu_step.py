@@ -693,7 +693,8 @@ def test_rotary_of_the_most_rows():
                                             (4096, 256, 4096), (33000, 128, 250),
                                             (4300, 384, 4200), (9000, 128, 2100),
                                             (100, 128, 70000), (64, 256, 9000), (50, 2064, 2500),
-                                            (1000, 528, 130), (32, 400, 9000)])
+                                            (1000, 528, 130), (32, 400, 9000), (1300, 528, 2000),
+                                            (4000, 128, 1030), (1025, 272, 2100)])
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
 def test_product_of_whole_numbers_in_large_tiles(rows, width, out, kind):
     test_product_of_whole_numbers(rows, width, out, kind)
@@ -733,3 +734,42 @@ def test_product_of_loud_codes_in_16_bits(rows, out, kind):
     bound = size * (7 * 2.0 ** -13 + 2.0 ** -18) * (1 + HALF_STEP[kind]) + \
         want.abs() * HALF_STEP[kind] + TINY[kind]
     assert ((y.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("rows,width", [(2, 4096), (3, 4100), (2, 16384), (2, 16390), (3, 20001),
+                                        (1, 32768), (2, 33000), (2, 65530)])
+def test_wide_rows(rows, width):
+    """Every width's number of lanes and runs, loud rows and gates among them."""
+    x = normal(51, rows, width)
+    r = normal(52, rows, width)
+    w = 1 + 0.2 * normal(53, width)
+    for out in ("e4m3", "bf16"):
+        check_norm(x.half(), w, r.half(), out, 1e-6, extra=3)
+        check_norm(x * 1e25, w, None, out, 1e-6)
+    gate = (normal(54, rows, width) * 4).half()
+    codes = torch.zeros(rows, width, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(rows, device="cuda")
+    ov.op_quantize8(x.half().cuda(), codes, scales, gate=gate.cuda())
+    g = gate.double()
+    check_codes(codes, scales, x.half().double() * g * torch.sigmoid(g), GATE)
+    ov.op_quantize8(x.cuda(), codes, scales)
+    check_codes(codes, scales, x, 0.0)
+    lost = x.clone()
+    lost[0, width - 1], w2 = np.nan, w.clone()
+    ov.op_quantize8(lost.cuda(), codes, scales)
+    assert torch.isnan(scales[0]) and (codes[0] == 0).all() and torch.isfinite(scales[1:]).all()
+    w2[width // 2] = np.inf
+    ov.op_add_rmsnorm(x.cuda(), w2.cuda(), codes, 1e-6, scales=scales)
+    assert torch.isnan(scales).all() and (codes == 0).all()
+
+
+def test_wide_rows_beside_a_scale_border():
+    """As test_norm_beside_a_scale_border, in rows whose weights are read twice."""
+    for width in (20000, 40000):
+        x = normal(55, 12, width)
+        x[:, 17] = 30.0
+        y = norm_of(x, None, torch.ones(width), 1e-6)[1]
+        weight = torch.ones(width)
+        for r in range(12):
+            weight[17] = float(1.75 * 2.0 ** 4 * (1 + (r - 6) * 2.0 ** -25) / y[r, 17])
+            check_norm(x[r:r + 1], weight, None, "e4m3", 1e-6)
