@@ -991,7 +991,7 @@ __device__ __forceinline__ void FindBin(RowShared& sh, bool by_weight, u64 want,
   }
   const u64 weight = weight_to - w0 - w1, count = count_to - c0 - c1;
   const u64 to = by_weight ? weight_to : count_to, from = by_weight ? weight : count;
-  // The last bin takes what fewer keys or the sums' rounding leave.
+  // The last bin stands for sums that do not reach it.
   if ((to >= want && (from < want || tid == 0)) || (tid == kRowThreads - 1 && to < want)) {
     const bool second = (by_weight ? weight + w0 : count + c0) < want;
     sh.bin = 2 * tid + second;
@@ -1474,7 +1474,9 @@ __global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
     high = RowJoin<kRowWaves>(WaveMaxKey(high), sh.slots,
                               [](unsigned a, unsigned b) { return max(a, b); });
     low = min(low, high);
-    bool one = false;
+    // A top_k that all tokens fit into, or a share that the sums' rounding leaves above all of
+    // them, cuts nothing off; the first sums, which are of every key, say so.
+    bool one = false, fewer = false;
 #pragma unroll 1
     while (!one) {
       const int bits = high == low ? 0 : 32 - __builtin_clz(high - low);
@@ -1494,12 +1496,20 @@ __global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
       });
       FindBin(sh, by_weight, want, above_count, above_weight);
       const unsigned bin = sh.bin;
+      fewer = (by_weight ? sh.above_weight + sh.weights[bin]
+                         : sh.above_count + sh.counts[bin]) < want;
+      if (fewer) {
+        whole = sh.above_weight + sh.weights[bin];
+        break;
+      }
       above_count = sh.above_count;
       above_weight = sh.above_weight;
       high -= min(bin << down, high - low);
       low = max(low, high - min(high, (1u << down) - 1));
       one = down == 0;
     }
+    if (fewer)
+      continue;
     const u64 equal = sh.counts[sh.bin], each = UnitsOf(w(high), c.shift);
     u64 need = equal;
     if (!by_weight)

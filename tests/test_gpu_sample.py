@@ -283,6 +283,32 @@ def test_more_equals_than_a_list_holds(top_k):
     check(c[:2], random[:2], top_k=top_k, top_p=0.61803)
 
 
+def few_allowed(rows, vocab, allowed, values, seed=40):
+    """Rows of -infinities with `allowed` tokens of so many different values, far enough
+    apart in the row to lie in every part of it; 0: any values."""
+    g = torch.Generator().manual_seed(seed)
+    c = torch.full((rows, vocab), -np.inf)
+    for r in range(rows):
+        at = torch.randperm(vocab, generator=g)[:allowed]
+        c[r, at] = -torch.randint(0, values, (allowed,), generator=g).float() if values else \
+            torch.randn(allowed, generator=g)
+    return c, torch.rand(rows, generator=g)
+
+
+@pytest.mark.parametrize("values", [1, 2, 5, 0])
+@pytest.mark.parametrize("vocab,allowed", [(20000, 3000), (20000, 6000), (151936, 3000)])
+def test_fewer_tokens_than_top_k(vocab, allowed, values):
+    """A top_k that all of the tokens fit into cuts nothing off: shares are of all of them,
+    the last ones and their equals too. 3000 equal tokens with a share of 0.9: 2700."""
+    c, random = few_allowed(6, vocab, allowed, values)
+    for top_k in (allowed + 1, 9000):
+        for settings in (dict(top_p=0.9), dict(top_p=0.95), dict(top_p=0.95, min_p=0.001),
+                         dict(), dict(top_p=0.9, temperature=1e30), dict(temperature=3e38)):
+            check(c, random, top_k=top_k, **settings)
+    each_k = torch.tensor([allowed - 1, allowed, allowed + 1, 19999, 0, 5], dtype=torch.int32)
+    check(c, random, top_k=each_k, top_p=torch.tensor([0.9, 1.0, 0.9, 0.97, 0.9, 0.8]))
+
+
 def test_the_callers_workspace():
     """Nothing behind it is written, what is in it does not matter."""
     c, random = logits_of(14, 6, 30000, "bf16")
