@@ -1448,7 +1448,8 @@ __global__ __launch_bounds__(kRowThreads) void FinishKernel(RowCall c) {
         f(KeyOf(z[i]), start + i);
     }
   };
-  Kept kept{1, kAll, 0};
+  // Of all that can be drawn -infinity is a border that a comparison of logits knows too.
+  Kept kept{kKeyOfMinusInf, kAll, 0};
   u64 whole = state->whole;
   // First where top_k ends, then where the share does: sums of 2048 ranges of the keys
   // that may hold the threshold, then of the range that does, until that is one key.

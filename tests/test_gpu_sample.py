@@ -309,6 +309,33 @@ def test_fewer_tokens_than_top_k(vocab, allowed, values):
     check(c, random, top_k=each_k, top_p=torch.tensor([0.9, 1.0, 0.9, 0.97, 0.9, 0.8]))
 
 
+LONG_ROW = 4300000  # more parts than a work-group holds in LDS
+
+
+def test_long_rows_with_few_tokens():
+    c, random = few_allowed(2, LONG_ROW, 10, 0)
+    for settings in (dict(top_k=50), dict(top_k=9), dict(top_k=50, top_p=0.9),
+                     dict(top_k=11, min_p=0.1)):
+        check(c, random, **settings)
+
+
+@pytest.mark.parametrize("settings", [dict(top_k=50, temperature=0.2),
+                                      dict(top_k=2000, temperature=0.05),
+                                      dict(top_k=3000, temperature=0.01, top_p=0.999)])
+def test_long_rows_of_few_that_weigh(settings):
+    """Fewer than top_k tokens weigh 2^-50 of the best."""
+    c, random = logits_of(41, 2, LONG_ROW)
+    check(c, random, **settings)
+
+
+def test_long_rows_of_a_share_past_the_sums():
+    """A best token, a share of nearly all, and millions that weigh less than a unit of the
+    sums does: together 2^-19 of the row, whose parts the sums do not see."""
+    c = torch.full((3, LONG_ROW), -28.5)
+    c[:, 2000001] = 0.0
+    check(c, torch.tensor([0.3, 0.5, 0.7]), top_p=1.0 - 2.0 ** -24)
+
+
 def test_the_callers_workspace():
     """Nothing behind it is written, what is in it does not matter."""
     c, random = logits_of(14, 6, 30000, "bf16")
