@@ -13,8 +13,9 @@
 // order. Bound by memory: 16384 rows of 1024 bf16 with a bf16 residual to 8 bits, 118
 // MB, take 22.5 us from inputs in the caches and 27 from memory (4.4 TB/s; a copy
 // reaches 5.0 to 5.3), 580 rows of 4096 gated in fp16 6 us, of which 2.4 are their
-// bytes' and the rest a launch and the latency of load, sum and store. Sums are float32. Where the largest magnitude is within 2^-18 of a power's
-// border, or the squares leave float32's range, the row is summed and its maximum found
+// bytes' and the rest a launch and the latency of load, sum and store. Sums are float32. Where
+// the largest magnitude is so near to a power's border that float32 may have taken it over
+// (kBeside), or the squares leave float32's range, the row is summed and its maximum found
 // again in 64 bits, so that the scale is the one that the formulas give.
 #include "step.hpp"
 
@@ -93,6 +94,13 @@ __device__ __forceinline__ float PowerOf(int e) {  // -126 .. 127
 }
 
 __device__ __forceinline__ float Gated(float x, float g) { return x * (g / (1.0F + __expf(-g))); }
+
+// How many steps of 2^-23 from a power's border, 1.75, float32 may take a row's largest
+// value over it. A norm is off by 26 * 2^-24: 23 steps. e^-g is off by 1.5 |g| 2^-24, the
+// product's and the constant's roundings, and 2^-23 of its own, the rest by 6 * 2^-24; gates
+// from -88.8 down, whose power is infinite, give 0: 124 steps.
+template <Mode MODE>
+constexpr int kBeside = MODE == Mode::kGate ? 128 : 32;
 
 // Eight elements of a row, those before `d` and behind the row not among them: a
 // row's last, partial run is loaded from its end backwards, so that no load is
@@ -300,7 +308,7 @@ __global__ __launch_bounds__(THREADS < kRowThreads ? kRowThreads : THREADS) void
     int e = ScaleExponent(amax);
     if constexpr (MODE != Mode::kPlain) {
       const int off = static_cast<int>(amax & 0x7FFFFFu) - 0x600000;
-      if (!lost && (careful || (off <= 32 && off >= -32))) {
+      if (!lost && (careful || (off <= kBeside<MODE> && off >= -kBeside<MODE>))) {
         double most = 0.0;
         const double r = MODE == Mode::kNorm ? total64() : 1.0;
 #pragma unroll

@@ -247,6 +247,28 @@ def test_gate_of_any_size():
     assert torch.isnan(scales).all()  # -inf * 0
 
 
+# Gates down to -88 and so the error of their power, which is the product's: (1.5 |g| + 8) 2^-24.
+DEEP_GATE = (1.5 * 88 + 8) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("low,high", [(-24.0, -8.0), (-64.0, -24.0), (-87.0, -64.0)])
+def test_gates_beside_a_scale_border(low, high):
+    """Rows whose largest product is 448 times a power of two to a hundred parts in 2^24, by
+    gates that make its rounding that large: the scale is the formula's."""
+    rows, width = 20000, 24
+    gen = torch.Generator().manual_seed(50)
+    g = torch.zeros(rows, width)
+    g[:, 5] = low + (high - low) * torch.rand(rows, generator=gen)
+    x = torch.zeros(rows, width)
+    s = g[:, 5].double() * torch.sigmoid(g[:, 5].double())
+    aim = -1.75 * (1 + torch.randint(-100, 101, (rows,), generator=gen).double() * 2.0 ** -24)
+    x[:, 5] = (aim / s).float()
+    codes = torch.zeros(rows, width, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(rows, device="cuda")
+    ov.op_quantize8(x.cuda(), codes, scales, gate=g.cuda())
+    check_codes(codes, scales, x.double() * g.double() * torch.sigmoid(g.double()), DEEP_GATE)
+
+
 # ------------------------------------------------------------------ product
 
 def whole_codes(seed, rows, width, most=8):
