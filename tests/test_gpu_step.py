@@ -269,6 +269,36 @@ def test_gates_beside_a_scale_border(low, high):
     check_codes(codes, scales, x.double() * g.double() * torch.sigmoid(g.double()), DEEP_GATE)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+def test_deep_gates_of_loud_rows(kind):
+    """Gates whose power leaves float32's range beside values that bring the product back."""
+    g = torch.tensor([-64.0, -70.0, -80.0, -87.0, -88.5, -89.0, -95.0, -103.0, -104.0, -120.0,
+                      -150.0, -155.0, -160.0])
+    x = torch.tensor([1.0, 1e10, -1e20, 3e35, 1e38, 3.3e38, -3.3e38])
+    gate = g[:, None, None].expand(-1, len(x), 11).reshape(-1, 11).clone()
+    value = x[None, :, None].expand(len(g), -1, 11).reshape(-1, 11).clone()
+    gate[:, 3:] += normal(51, *gate[:, 3:].shape)
+    value[:, ::2] *= 0.9
+    value = value.clamp(-65504, 65504) if kind == "f16" else value
+    gate, value = gate.to(TYPES[kind]), value.to(TYPES[kind])
+    codes = torch.zeros(gate.shape, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(len(gate), device="cuda")
+    ov.op_quantize8(value.cuda(), codes, scales, gate=gate.cuda())
+    d = gate.double()
+    check_codes(codes, scales, value.double() * d * torch.exp(d) / (1 + torch.exp(d)), DEEP_GATE)
+
+
+def test_gates_past_every_power():
+    """Nothing is left of what is finite; an infinite value or gate is the row's."""
+    g = torch.tensor([[-200.0], [-299.0], [-301.0], [-3e38], [-100.0], [-np.inf], [-100.0]])
+    x = torch.tensor([[3e38], [-3e38], [3e38], [3e38], [np.inf], [1.0], [np.nan]])
+    codes = torch.full((7, 1), 9, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(7, device="cuda")
+    ov.op_quantize8(x.cuda(), codes, scales, gate=g.cuda())
+    assert (codes[:, 0].cpu() & 0x7F == 0).all()
+    assert (scales[:4].cpu() == 2.0 ** -100).all() and torch.isnan(scales[4:]).all()
+
+
 # ------------------------------------------------------------------ product
 
 def whole_codes(seed, rows, width, most=8):
