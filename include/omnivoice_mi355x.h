@@ -501,11 +501,11 @@ int ovg_op_quantize8(const void* x, int64_t x_stride, const void* gate, int64_t 
 /* y[rows][out] = x[rows][in] w[out][in]^T of 8-bit rows in float32 sums, each times its
  * row's and its column's scale (in this order; any scales), rounded to `type`. `in` is a
  * multiple of 16 up to 65536; x and w are 16-byte aligned, x_stride a multiple of 16;
- * rows and out below 2^22. The order of a sum goes by the call's shape. float32 results
- * have sums right to float32's rounding. 16-bit results come from sums in which, of eight
- * codes' products next to each other, the bits below 2^-13 of the largest one's power of
- * two are cut off: under 2^-10 of the products' magnitudes, 1.5e-5 of a sum of random ones,
- * beside their own rounding of 2^-9 or 2^-12. */
+ * rows and out below 2^22. The order of a sum goes by the call's shape. Results in float32,
+ * and 16-bit ones of up to 32 rows, have sums right to float32's rounding. 16-bit results of
+ * more rows may come from sums in which, of eight codes' products next to each other, the bits
+ * below 2^-13 of the largest one's power of two are cut off: under 2^-10 of the products'
+ * magnitudes, 1.5e-5 of a sum of random ones, beside their own rounding of 2^-8 or 2^-11. */
 int ovg_op_linear8(const void* x, int64_t x_stride, const float* x_scales, const void* w,
                    const float* w_scales, void* y, int64_t y_stride, int type, int64_t rows,
                    int64_t in, int64_t out, void* stream, char* error, size_t error_len);

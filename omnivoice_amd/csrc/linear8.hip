@@ -20,12 +20,15 @@ constexpr std::int64_t kTileStride = 1 << 23;  // 256 rows of it are 32-bit offs
 
 // D[4 (l / 16) + r][l % 16] in element r of lane l, rows of `a` by rows of `b`.
 //
-// The instruction adds the products of eight codes in a row at a time, aligned to the
+// The 8-bit instruction adds the products of eight codes in a row at a time, aligned to the
 // largest: bits below 2^-13 of that one's power of two are cut off, at most 7/8192 of the
-// products' magnitudes and 1.5e-5 of a sum of random ones. 16-bit results, which round by
-// 2^-9 or 2^-12, take it; float32 results go through fp16, which holds every e4m3 code, and
-// whose products are added as float32 (6e-8), at half the rate and with the conversions
-// (4096 x 4096 x 8192: 112 us with the codes' own products, 207 through fp16).
+// products' magnitudes and 1.5e-5 of a sum of random ones (the 8-bit one of 32 codes does the same).
+// fp16 holds every e4m3 code, and its products are added as float32 (6e-8), at half the rate
+// and with the conversions. Few rows and float32 results go through fp16, which costs few rows
+// 1 to 5 % (16 x 1024 x 4096 in bf16 3.5 us both ways, 32 x 8192 x 8192 18.9 and 18.1 by the
+// codes' own products); 16-bit results of tiles, which round by 2^-8 or 2^-11, take the codes'
+// own (on one card 4096 x 4096 x 8192 in bf16 101 us, 187 through fp16; 64 x 4096 x 3000 10.8
+// and 16.1).
 template <bool HALF>
 struct Operand {
   intx8 codes;
@@ -81,13 +84,13 @@ __device__ __forceinline__ void LoadOperand(const unsigned char* row, int k, int
 // 16 MB rows by 16 NB columns; the waves take every fourth step of K and join in LDS, in a
 // fixed order. Operands come straight from memory: a weight is used once, and 16 lines of
 // 64 bytes in flight a wave, two steps of them, are what the latency asks for. Bound by
-// reading the weights: 16 x 1024 x 4096 (4 MiB) 3.4 us, of which an empty launch is 2; 16 x
-// 4096 x 8192 (32 MiB) 9.3 us, 3.6 TB/s; 32 x 8192 x 8192 18 us, 3.7 TB/s.
+// reading the weights: 16 x 1024 x 4096 (4 MiB) 3.5 us, of which an empty launch is 2; 16 x
+// 4096 x 8192 (32 MiB) 9.4 us, 3.6 TB/s; 32 x 8192 x 8192 18.9 us, 3.6 TB/s.
 constexpr int kWaves = 4;
 
 template <typename T, int MB, int NB>
 __global__ __launch_bounds__(kWaves* kWave) void SkinnyKernel(Linear8Params p) {
-  constexpr bool kHalf = std::is_same_v<T, float>;
+  using Codes = Operand<true>;
   __shared__ floatx4 parts[kWaves][MB * NB][kWave];
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -109,13 +112,13 @@ __global__ __launch_bounds__(kWaves* kWave) void SkinnyKernel(Linear8Params p) {
   // last, partial one with it.
   const int whole = p.in / kStep * kStep;
   int k = wave * kStep;
-  const auto load = [&](const unsigned char* row, Operand<kHalf>* to) {
+  const auto load = [&](const unsigned char* row, Codes* to) {
     to->Set(*reinterpret_cast<const intx4*>(row + k + part * 16),
             *reinterpret_cast<const intx4*>(row + k + part * 16 + 64));
   };
 #pragma unroll 2
   for (; k < whole; k += kWaves * kStep) {
-    Operand<kHalf> a[MB], b[NB];
+    Codes a[MB], b[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
       load(w[n], &b[n]);
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(kWaves* kWave) void SkinnyKernel(Linear8Params p) {
         acc[m][n] = Multiply(a[m], b[n], acc[m][n]);
   }
   if (k < p.in) {
-    Operand<kHalf> a, b[NB];
+    Codes a, b[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
       LoadOperand(w[n], k + part * 32, p.in, &b[n]);
@@ -177,9 +180,10 @@ __global__ __launch_bounds__(kWaves* kWave) void SkinnyKernel(Linear8Params p) {
 // are next to each other.
 //
 // Bound by the matrix cores and the reads from LDS that feed them: 4096 x 4096 x 8192 takes
-// 102 us in bf16, 2690 TFLOP/s, beside 97 us of the card's library at 8 bits; float32, at
-// half the products' rate, 207. Small products are bound by their steps' latency: 580 x 2048
-// x 1024 in float32 9.7 us, of which 16 steps, a launch and the results' stores.
+// 99 to 107 us in bf16 by card and run, 2780 to 2570 TFLOP/s, beside 97 to 104 of the card's
+// library at 8 bits; float32, at half the products' rate, 198 to 203. Small products are bound
+// by their steps' latency: 580 x 2048 x 1024 in float32 10.3 us, of which 16 steps, a launch
+// and the results' stores.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 struct Tile {
   static constexpr bool kHalf = std::is_same_v<T, float>;
@@ -440,7 +444,8 @@ void Launch(const Linear8Params& p, hipStream_t s) {
     return static_cast<std::int64_t>((p.rows + bm - 1) / bm) * ((p.out + bn - 1) / bn);
   };
   // Twice the columns, which halves what is read of x, where a work-group is left to every
-  // CU (32 x 8192 x 8192: 18.2 us, so 24.1; 32 x 4096 x 4096, 128 work-groups: 10.1, so 8.3).
+  // CU (32 x 8192 x 8192: 18.9 us, 24.5 without; 32 x 4096 x 4096, 128 work-groups: 10.2, 8.4
+  // without).
   const auto skinny_of = [&](auto mb, auto nb) {
     constexpr int kRows = 16 * mb(), kCols = 16 * nb();
     Dispatch(SkinnyKernel<T, mb(), nb()>,
@@ -462,33 +467,33 @@ void Launch(const Linear8Params& p, hipStream_t s) {
   };
   using std::integral_constant;
   if (p.rows <= 32 || groups(64, 64) < kCus / 6 || p.x_stride > kTileStride) {
-    // Few rows, or few tiles: 64 x 4096 x 2048 (32 tiles) takes 8.2 us, 10.7 with tiles, 64 x
-    // 4096 x 3000 (47) 13.5 and 10.8, 64 x 8192 x 8192 30 and 21; 32 x 4096 x 4096, half of
-    // whose tiles' rows are none, 8.3 and 10.7. 32 rows to a work-group where that leaves one
-    // to every CU: 32 x 8192 x 8192 24 us, 31 with 16; 64 x 4096 x 1024, 128 work-groups of
-    // 32, 8.0 and 6.1.
+    // Few rows, or few tiles: 64 x 4096 x 2048 (32 tiles) takes 8.4 us, 10.8 with tiles, 64 x
+    // 4096 x 3000 (47) 13.6 and 10.9, 64 x 8192 x 8192 32 and 22; 32 x 4096 x 4096, half of
+    // whose tiles' rows are none, 8.4 and 10.8 (bf16; in float32 tiles take half as long again).
+    // 32 rows to a work-group where that leaves one to every CU: 32 x 8192 x 8192 24.5 us, 31
+    // with 16; 64 x 4096 x 1024, 128 work-groups of 32, 8.0 and 6.3.
     if (p.rows > 16 && groups(32, 16) >= kCus)
       skinny(integral_constant<int, 2>());
     else
       skinny(integral_constant<int, 1>());
   } else if (p.in % kStep == 0 && groups(256, 256) >= kCus) {
-    // A tile for every CU: 4096 x 4096 x 4096 takes 56 us, 67 in tiles of 128, 4096 x 4096 x
-    // 2048, half as many, 44 and 33; float32 104 and 119, 90 and 60. Without the partial step
+    // A tile for every CU: 4096 x 4096 x 4096 takes 54 us, 62 in tiles of 128, 4096 x 4096 x
+    // 2048, half as many, 46 and 34; float32 98 and 112, 90 and 61. Without the partial step
     // the kernel's code is as long as its registers reach.
     tiled(integral_constant<int, 256>(), integral_constant<int, 256>(),
           integral_constant<int, 2>(), integral_constant<int, 4>(), integral_constant<int, 2>(),
           std::true_type());
   } else if (groups(128, 128) > kCus) {
-    // 4096 x 4096 x 2048 (512 tiles) takes 33 us, 45 in tiles of 64, 3000 x 2048 x 2048 (384)
-    // 18.4 and 21.7, 2048 x 2048 x 2048 (256) 14.6 both, 1500 x 2048 x 2048 (192) 14.1 and
-    // 12.1; float32 61 and 76, 34 and 31, 24 and 23, 23 and 19.
+    // 4096 x 4096 x 2048 (512 tiles) takes 34 us, 49 in tiles of 64, 3000 x 2048 x 2048 (384)
+    // 18.8 and 21.7, 2048 x 2048 x 2048 (256) 14.2 and 14.0, 1500 x 2048 x 2048 (192) 13.9 and
+    // 11.8; float32 61 and 74, 31 and 32, 23 and 22, 22 and 18.
     tiled(integral_constant<int, 128>(), integral_constant<int, 128>(),
           integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 2>(),
           std::false_type());
   } else if (groups(64, 64) > 2 * kCus) {
     // Four stages leave two work-groups to a CU, two four: 1400 x 2048 x 2048 (704 tiles)
-    // takes 11.5 us with two stages, 13.7 with four, 1000 x 1024 x 2048 (512) 7.0 and 6.6, 580
-    // x 2048 x 1024 (160) 10.4 and 7.3; float32 17.5 and 21.2, 9.1 and 10.2, 12.3 and 10.5.
+    // takes 11.6 us with two stages, 13.9 with four, 1000 x 1024 x 2048 (512) 7.0 and 6.6, 580
+    // x 2048 x 1024 (160) 10.2 and 7.2; float32 18.1 and 20.8, 9.4 and 9.7, 12.2 and 10.3.
     tiled(integral_constant<int, 64>(), integral_constant<int, 64>(),
           integral_constant<int, 2>(), integral_constant<int, 2>(), integral_constant<int, 2>(),
           std::false_type());

@@ -353,6 +353,25 @@ def test_product_of_any_codes(rows, width, out):
     assert rel < 2.0 ** -16
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,width,out", [(1, 1024, 48), (16, 1024, 4096), (17, 1040, 33),
+                                            (32, 1040, 900), (64, 1024, 300)])
+def test_product_of_few_rows_keeps_small_products(rows, width, out, kind):
+    """Ones beside products of 448 * 448 that cancel one another, eight codes in a row: whole
+    numbers, whose sums stay under 2^24 (65 * 200704), so that nothing may be lost. 64 rows
+    of 300 columns are too few tiles for those, and go the same way."""
+    a, b = torch.ones(rows, width), torch.ones(out, width)
+    for r in range(rows):
+        a[r, r % 8::16], a[r, r % 8 + 8::16] = 448.0, -448.0
+    for k in range(8):
+        b[k::8, k::8] = 448.0
+    x, w = a.to(torch.float8_e4m3fn), b.to(torch.float8_e4m3fn)
+    y = torch.zeros(rows, out, dtype=TYPES[kind], device="cuda")
+    one = torch.ones(max(rows, out), device="cuda")
+    ov.op_linear8(x.cuda(), one[:rows].contiguous(), w.cuda(), one[:out].contiguous(), y)
+    assert torch.equal(y.cpu(), (a.double() @ b.double().t()).to(TYPES[kind]))
+
+
 @pytest.mark.parametrize("rows", [4, 40, 300])
 def test_product_of_lost_rows_and_far_scales(rows):
     """A NaN scale or code is its own row's, a far scale no overflow."""
