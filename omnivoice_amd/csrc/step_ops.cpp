@@ -163,7 +163,8 @@ int ovg_rotary_frequencies(int64_t rotary, double theta, int scaling, double fac
       f /= factor;
     if (scaling == OVG_ROTARY_PARTS) {
       const double at = (static_cast<double>(i) - low) / std::max(high - low, 1e-3);
-      const double slow = std::min(std::max(at, 0.0), 1.0);
+      // Also where no pair turns once, and `high` is below the first one.
+      const double slow = static_cast<double>(i) >= high ? 1.0 : std::min(std::max(at, 0.0), 1.0);
       f = f / factor * slow + f * (1.0 - slow);
     }
     frequencies[i] = static_cast<float>(f);

@@ -271,6 +271,16 @@ def test_frequencies_by_parts():
     assert m == 1.0
 
 
+@pytest.mark.parametrize("original", [1.0, 3.0, 6.0])
+def test_frequencies_by_parts_of_less_than_a_turn(original):
+    """Trained on fewer positions than the first pair turns in once (2 pi): every pair is
+    divided, the first one too."""
+    for rotary, theta in ((128, 1e6), (2, 1e4), (64, 2.0)):
+        f, _ = ov.rotary_frequencies(rotary, theta)
+        g, _ = ov.rotary_frequencies(rotary, theta, "parts", 8.0, original)
+        np.testing.assert_array_equal(g, f / 8)
+
+
 def test_frequencies_refuse():
     for args in ((0,), (3,), (-2,), (514,), (128, 1.0), (128, NAN), (128, INF),
                  (128, 1e6, "linear", 0.5), (128, 1e6, "base", NAN), (128, 1e6, "base", INF),
