@@ -514,7 +514,7 @@ int ovg_op_linear8(const void* x, int64_t x_stride, const float* x_scales, const
  * theta^(-2 i / rotary), for contexts `factor` times as long as the trained one
  *   OVG_ROTARY_LINEAR  all divided by factor
  *   OVG_ROTARY_BASE    of theta * factor^(rotary / (rotary - 2)): the last one divided
- *                      by factor, the first one kept
+ *                      by factor, the first one kept (a single one: kept)
  *   OVG_ROTARY_PARTS   those that turn less than once over original_positions divided by
  *                      factor, those that turn over 32 times kept, a ramp over the pairs
  *                      between; magnitude 0.1 ln(factor) + 1
@@ -552,8 +552,9 @@ int ovg_op_rotary(const void* q, void* q_out, int64_t q_stride, int64_t q_out_st
 typedef struct ovg_sampling {
   float temperature; /* 0 or less: the best token */
   int32_t top_k;     /* the first k tokens; 0 or less: all */
-  float top_p;       /* the shortest prefix with this share of their weight; 1: all */
-  float min_p;       /* what weighs at least this share of the best; 0: all */
+  float top_p;       /* the shortest prefix with this share of their weight; 1 or more: all */
+  float min_p;       /* what weighs at least this share of the best; 0 or less: all, above 1
+                        counts as 1: the best and its equals */
   const float* temperatures;
   const int32_t* top_ks;
   const float* top_ps;
@@ -564,15 +565,16 @@ typedef struct ovg_sampling {
  * by random[row] in [0, 1). With `uncond` the logits are z = c + guidance * (c - u) as in
  * ovg_op_token_logprobs; the token `mask_id` (-1: none) and those of -infinity are never
  * drawn. Tokens are ordered by z, equal ones by index, and weigh
- * w = exp((z - max z) / temperature); top_k keeps the first of them, top_p a prefix of
- * what top_k keeps, min_p what weighs enough, and the best always stays. The token is the
- * first, by index, at which the kept weights pass random * their sum; one that weighs less
- * than 2^-50 of the best counts as none. Weights are right to 2^-42 and sums to 2^-40; with
- * filters, among n > 2048 tokens, sums are to n 2^-50 and top_p's border to n^2 2^-61 of the
- * sum (2^-32 and 2^-26 for 151936). Nothing depends on the order of the work. A row with a
- * NaN or +infinity among its logits, without a token to draw, or with a NaN among its
- * numbers has the token -1; random numbers outside [0, 1) count as the nearest inside. rows
- * below 2^22, rows times vocab up to 6e10. `workspace` as above, for this call alone. */
+ * w = exp((z - max z) / temperature); top_k keeps the first of them (all where there are
+ * fewer), top_p a prefix of what top_k keeps, min_p what weighs enough, and the best always
+ * stays. The token is the first, by index, at which the kept weights pass random * their sum;
+ * one that weighs less than 2^-50 of the best counts as none. Weights are right to 2^-42 and
+ * sums to 2^-40; with filters, among n > 2048 tokens, sums are to n 2^-50 and top_p's border
+ * to n^2 2^-61 of the sum (2^-32 and 2^-26 for 151936). Nothing depends on the order of the
+ * work. A row with a NaN or +infinity among its logits, without a token to draw, or with a NaN
+ * among its numbers has the token -1; random numbers outside [0, 1) count as the nearest
+ * inside. rows below 2^22, rows times vocab up to 6e10. `workspace` as above, for this call
+ * alone. */
 int64_t ovg_op_sample_workspace(int64_t rows, int64_t vocab);
 int ovg_op_sample(const void* logits, const void* uncond, int64_t rows, int64_t vocab,
                   int64_t stride, int64_t uncond_stride, float guidance, int64_t mask_id,

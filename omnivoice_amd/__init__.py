@@ -1177,8 +1177,8 @@ def op_sample(logits, random, tokens, temperature=1.0, top_k=0, top_p=1.0, min_p
     """Draws tokens [rows] (int32) from logits [rows][vocab] (fp16, bf16 or float32,
     contiguous rows) by the numbers random [rows] (float32 in [0, 1)), at a temperature (0:
     the best) among the top_k best, of these the shortest prefix that holds top_p of their
-    weight, and what weighs min_p of the best or more. Each setting is a number or a device
-    tensor [rows] (float32, top_k int32). With `uncond` the logits are
+    weight, and what weighs min_p of the best or more (above 1: 1). Each setting is a number
+    or a device tensor [rows] (float32, top_k int32). With `uncond` the logits are
     c + guidance * (c - u); mask_id is never drawn. `workspace`: a device tensor of
     op_sample_workspace bytes (one is allocated without it). Enqueued on `stream`."""
     import torch

@@ -214,6 +214,16 @@ def test_numbers_that_are_none():
     np.testing.assert_array_equal(tokens.cpu(), np.floor(random.numpy().astype(np.float64) * 100))
 
 
+@pytest.mark.parametrize("vocab", [7, 1500, 30000])
+@pytest.mark.parametrize("min_p", [1.0, 1.5, np.inf])
+def test_min_p_from_one_on(vocab, min_p):
+    """The best and its equals, whichever of them is first."""
+    c = torch.zeros(6, vocab)
+    c[:, [1, vocab // 2, vocab - 1]] = 3.0
+    got = check(c, torch.tensor([0.0, 0.3, 0.4, 0.6, 0.7, 0.99]), min_p=min_p)
+    assert got.tolist() == [1, 1, vocab // 2, vocab // 2, vocab - 1, vocab - 1]
+
+
 def test_no_rows_and_one_draw_many_times():
     tokens = torch.zeros(0, dtype=torch.int32, device="cuda")
     ov.op_sample(torch.zeros(0, 50, device="cuda"), torch.zeros(0, device="cuda"), tokens)
