@@ -24,7 +24,7 @@
 //   3  For rows that were not drawn: the steps that hold the threshold by those sums, the
 //      list of the elements in them, and the chunks' weights above them.
 //   4  The threshold from the list, or from passes over the row where the list does not hold
-//      it (thousands of equals), and the draw.
+//      it (thousands of equals, or of near ones at a high temperature), and the draw.
 // Bound by the arithmetic of the weights, 16 operations in 64 bits and a table's value for
 // each: 300 rows of 151936 bf16 without filters 43 us (40 + 8 with the launches overlapped;
 // their 91 MB are 18 us), 64 rows with settings of all kinds 69 us (10 + 24 + 19 + 18), of
@@ -58,7 +58,10 @@ constexpr int kMostQuarters = 2048;         // that are ranked
 constexpr int kMostOpened = 256;            // quarters that are read for a list
 constexpr int kShortList = 512;             // elements of a list that one wave holds
 constexpr int kList = 2048;                 // elements of a list
-constexpr int kShareOpened = 64;            // opened for a share alone
+// Opened for a share alone, of which the loudest quarters hold most: 512 rows of 32000 bf16
+// with top_p 0.9 take 140 us, 159 with 32 and 140 with 128; a row of 151936, whose share they
+// do not hold, 49, 46 and 52.
+constexpr int kShareOpened = 64;
 constexpr int kOctaves = 50;                // weights below 2^-50 do not count
 constexpr int kTable = 256;
 
@@ -1637,6 +1640,9 @@ void LaunchSample(const SampleParams& p, DType type, hipStream_t stream) {
       // A work-group fills a CU.
       const int parts = static_cast<int>(std::min<std::int64_t>(
           std::int64_t{c.rows} * ((c.quarters + kRowWaves - 1) / kRowWaves), kCus));
+      // What the rows leave of the CUs, or half of them where they leave less: with an eighth
+      // 300 rows of 151936 with top_p 0.9 take 685 us, with half 328, 512 of 32000 265 and
+      // 140 (with all 280 and 121); 64 rows of 151936 97 with what is left, 106 with half.
       const int helpers = std::min(parts, std::max(kCus - c.rows, kCus / 2));
       Dispatch(FirstKernel<T>, dim3(c.rows + helpers), dim3(kRowThreads), 0, stream, false, false,
                c);
