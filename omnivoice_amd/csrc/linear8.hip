@@ -182,8 +182,8 @@ __global__ __launch_bounds__(kWaves* kWave) void SkinnyKernel(Linear8Params p) {
 // Bound by the matrix cores and the reads from LDS that feed them: 4096 x 4096 x 8192 takes
 // 99 to 107 us in bf16 by card and run, 2780 to 2570 TFLOP/s, beside 97 to 104 of the card's
 // library at 8 bits; float32, at half the products' rate, 198 to 203. Small products are bound
-// by their steps' latency: 580 x 2048 x 1024 in float32 10.3 us, of which 16 steps, a launch
-// and the results' stores.
+// by their steps' latency: 580 x 2048 x 1024 in float32 9.7 to 10.4 us, of which 16 steps, a
+// launch and the results' stores.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 struct Tile {
   static constexpr bool kHalf = std::is_same_v<T, float>;
